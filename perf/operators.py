@@ -163,7 +163,7 @@ def _plain_loss(s):
     counted = s["targets"] >= 0
     t = s["targets"].long().clamp(min=0)
     loss = torch.where(counted, lse - logits.gather(1, t[:, None])[:, 0], 0.0)
-    out = dict(loss=loss, lse=lse)
+    out = dict(loss=loss, lse=torch.where(counted, lse, 0.0))
     if c["grads"]:
         p = p / total
         p[torch.arange(c["rows"], device=p.device), t] -= 1.0
@@ -269,11 +269,12 @@ def _exact_loss(s):
         z = torch.mm(x, wt)
         if c["bias"]:
             z += s["bias"].double()
-        out["lse"][a:b] = torch.logsumexp(z, 1)
+        lse = torch.logsumexp(z, 1)
         picked = torch.nonzero(t >= 0)[:, 0]
-        out["loss"][a + picked] = out["lse"][a + picked] - z[picked, t[picked]]
+        out["lse"][a + picked] = lse[picked]
+        out["loss"][a + picked] = lse[picked] - z[picked, t[picked]]
         if c["grads"]:
-            dz = torch.exp(z - out["lse"][a:b, None])
+            dz = torch.exp(z - lse[:, None])
             dz[picked, t[picked]] -= 1.0
             dz *= torch.where(t >= 0, g, torch.zeros_like(g))[:, None]
             out["dx"][a:b] = torch.mm(dz, w)
