@@ -65,6 +65,18 @@ class AdnProfile(C.Structure):
                 ("total_ms", C.c_double)]
 
 
+ADN_T_F32 = 0
+ADN_T_BF16 = 1
+
+
+class AdnLmLossArgs(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("d", C.c_int32), ("vocab", C.c_int32), ("dtype", C.c_uint32),
+                ("x", C.c_void_p), ("x_stride", C.c_int64), ("w", C.c_void_p), ("w_stride", C.c_int64),
+                ("bias", C.c_void_p), ("targets", C.c_void_p), ("dloss", C.c_void_p), ("loss", C.c_void_p),
+                ("lse", C.c_void_p), ("dx", C.c_void_p), ("dx_stride", C.c_int64), ("dw", C.c_void_p),
+                ("dw_stride", C.c_int64), ("db", C.c_void_p)]
+
+
 class AdnError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"[{code}] {msg}")
@@ -139,6 +151,17 @@ def lib():
         "adn_embed_context_noalloc": (C.c_int, [ctx_p, C.c_int32, C.c_int32, I32P, C.c_int32, F32P]),
         "adn_noalloc_guard_set": (C.c_int, [ctx_p, C.c_uint32]),
         "adn_gemm_blocks": (C.c_int, [C.POINTER(AdnConfig), C.c_int32, C.c_int32, C.c_int32, I32P]),
+        "adn_context_device": (C.c_int, [ctx_p, I32P]),
+        "adn_lm_loss_async": (C.c_int, [ctx_p, C.POINTER(AdnLmLossArgs)]),
+        "adn_rms_norm_async": (C.c_int, [ctx_p, C.c_int32, C.c_int32, C.c_uint32, C.c_void_p, C.c_int64, C.c_void_p,
+                                         C.c_float, C.c_void_p, C.c_int64]),
+        "adn_rms_norm_backward_async": (C.c_int, [ctx_p, C.c_int32, C.c_int32, C.c_uint32, C.c_void_p, C.c_int64,
+                                                  C.c_void_p, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                                  C.c_void_p]),
+        "adn_embed_lookup_async": (C.c_int, [ctx_p, C.c_int32, C.c_int32, C.c_int32, C.c_uint32, C.c_void_p,
+                                             C.c_void_p, C.c_int64, C.c_float, C.c_void_p, C.c_int64]),
+        "adn_embed_grad_async": (C.c_int, [ctx_p, C.c_int32, C.c_int32, C.c_int32, C.c_uint32, C.c_void_p, C.c_void_p,
+                                           C.c_int64, C.c_float, C.c_void_p, C.c_int64]),
         "adn_profile_forward": (C.c_int, [ctx_p, C.POINTER(AdnRun), C.POINTER(AdnOutputs),
                                           C.POINTER(AdnProfile)]),
     }

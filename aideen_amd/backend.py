@@ -51,6 +51,13 @@ def _dev_i(t) -> Optional[C.POINTER(C.c_int32)]:
     return None if t is None else C.cast(C.c_void_p(t.data_ptr()), _I32P)
 
 
+_DTYPES = {"torch.float32": _lib.ADN_T_F32, "torch.bfloat16": _lib.ADN_T_BF16}
+
+
+def _invalid(msg: str) -> "_lib.AdnError":
+    return _lib.AdnError(_lib.ADN_E_INVALID, msg)
+
+
 def device_count() -> int:
     n = C.c_int32(0)
     check(lib().adn_device_count(C.byref(n)))
@@ -78,6 +85,7 @@ class GpuDeqBackend:
         check(lib().adn_create(C.byref(cfg), C.byref(self._ctx)))
         self.max_batch, self.max_seq = max_batch, max_seq
         self._weights_keepalive = None
+        self._device: Optional[int] = None
 
     @classmethod
     def new_blocking(cls, model, max_batch: int = 1, max_seq: int = 1) -> Optional["GpuDeqBackend"]:
@@ -252,6 +260,133 @@ class GpuDeqBackend:
                       h_star=None) -> None:
         check(lib().adn_adjoint_async(self._ctx, int(ntok), _dev_f(h_star), _dev_f(dl), int(iters), float(damping),
                                       _dev_f(v_out), _dev_f(src_out)))
+
+    # training operators (device memory, enqueue only) --------------------------------------
+    # Arguments are torch tensors on the context's GPU; matrices float32 or bfloat16 (all of one
+    # call alike) with adjacent elements in a row and any row stride, vectors float32, ids int32.
+    def _matrix(self, t, name: str, rows: int, d: int, dtype=None):
+        """(pointer, row stride) of a [rows][d] tensor."""
+        if tuple(t.shape) != (rows, d):
+            raise _invalid(f"{name} must have the shape ({rows}, {d}), got {tuple(t.shape)}")
+        if dtype is not None and t.dtype != dtype:
+            raise _invalid(f"{name} must be {dtype} as the call's other matrices, got {t.dtype}")
+        self._on_device(t, name)
+        if d > 1 and t.stride(1) != 1:
+            raise _invalid(f"{name}: the elements of a row must be adjacent")
+        return t.data_ptr(), (t.stride(0) if rows > 1 else d)
+
+    def _vector(self, t, name: str, n: int, dtype: str = "torch.float32"):
+        """Pointer of a contiguous [n] tensor; None for None."""
+        if t is None:
+            return None
+        if t.dim() != 1 or t.shape[0] != n or str(t.dtype) != dtype or (n > 1 and t.stride(0) != 1):
+            raise _invalid(f"{name} must be a contiguous {dtype} tensor of {n} elements")
+        self._on_device(t, name)
+        return t.data_ptr()
+
+    def _on_device(self, t, name: str) -> None:
+        if not t.is_cuda or t.device.index != self.device:
+            raise _invalid(f"{name} must be on the context's GPU (cuda:{self.device}), got {t.device}")
+
+    @property
+    def device(self) -> int:
+        """Ordinal of the GPU that the context was created on."""
+        if self._device is None:
+            n = C.c_int32(0)
+            check(lib().adn_context_device(self._ctx, C.byref(n)))
+            self._device = n.value
+        return self._device
+
+    @staticmethod
+    def _dtype(t) -> int:
+        code = _DTYPES.get(str(t.dtype))
+        if code is None:
+            raise _invalid(f"float32 or bfloat16 expected, got {t.dtype}")
+        return code
+
+    def lm_loss_async(self, x, targets, *, outputs: Dict[str, object], w=None, bias=None, dloss=None) -> None:
+        """Softmax cross entropy of the rows x [rows][d] against targets [rows] through the head w
+        [vocab][d] (+ bias [vocab]; w None: the uploaded lm_w and lm_b), with its gradients for the
+        upstream gradient dloss [rows] (None = 1).  ``outputs`` names the wanted results: loss [rows],
+        lse [rows], dx [rows][d], dw [vocab][d], db [vocab].  A target < 0 leaves its row out."""
+        unknown = set(outputs) - {"loss", "lse", "dx", "dw", "db"}
+        if unknown:
+            raise _invalid(f"unknown outputs {sorted(unknown)}")
+        if x.dim() != 2 or (w is not None and w.dim() != 2):
+            raise _invalid("x and w must be matrices")
+        rows, d = x.shape
+        V = self.model.V if w is None else w.shape[0]
+        a = _lib.AdnLmLossArgs(rows=rows, d=d, vocab=V, dtype=self._dtype(x))
+        a.x, a.x_stride = self._matrix(x, "x", rows, d)
+        if w is not None:
+            a.w, a.w_stride = self._matrix(w, "w", V, d, x.dtype)
+        a.bias = self._vector(bias, "bias", V)
+        a.targets = self._vector(targets, "targets", rows, "torch.int32")
+        a.dloss = self._vector(dloss, "dloss", rows)
+        a.loss = self._vector(outputs.get("loss"), "loss", rows)
+        a.lse = self._vector(outputs.get("lse"), "lse", rows)
+        a.db = self._vector(outputs.get("db"), "db", V)
+        if outputs.get("dx") is not None:
+            a.dx, a.dx_stride = self._matrix(outputs["dx"], "dx", rows, d, x.dtype)
+            if rows == 0:
+                a.dx = None
+        if outputs.get("dw") is not None:
+            a.dw, a.dw_stride = self._matrix(outputs["dw"], "dw", V, d, x.dtype)
+        if rows == 0 and not (a.dw or a.db):
+            return  # an empty batch, and only row outputs: nothing to write
+        check(lib().adn_lm_loss_async(self._ctx, C.byref(a)))
+
+    def rms_norm_async(self, x, y, *, gain=None, eps: float = 1e-5) -> None:
+        """y = x / sqrt(mean(x^2) + eps) * gain per row (the LM head's norm); gain [d] float32 or None."""
+        if x.dim() != 2:
+            raise _invalid("x must be a matrix")
+        rows, d = x.shape
+        xp, xs = self._matrix(x, "x", rows, d)
+        yp, ys = self._matrix(y, "y", rows, d, x.dtype)
+        check(lib().adn_rms_norm_async(self._ctx, rows, d, self._dtype(x), xp, xs, self._vector(gain, "gain", d), eps,
+                                       yp, ys))
+
+    def rms_norm_backward_async(self, x, dy, *, outputs: Dict[str, object], gain=None, eps: float = 1e-5) -> None:
+        """Gradients of rms_norm_async for the upstream gradient dy: ``outputs`` names dx [rows][d]
+        and/or dg [d] (float32)."""
+        unknown = set(outputs) - {"dx", "dg"}
+        if unknown:
+            raise _invalid(f"unknown outputs {sorted(unknown)}")
+        if x.dim() != 2:
+            raise _invalid("x must be a matrix")
+        rows, d = x.shape
+        xp, xs = self._matrix(x, "x", rows, d)
+        dyp, dys = self._matrix(dy, "dy", rows, d, x.dtype)
+        dxp, dxs = (None, d) if outputs.get("dx") is None else self._matrix(outputs["dx"], "dx", rows, d, x.dtype)
+        dgp = self._vector(outputs.get("dg"), "dg", d)
+        if rows == 0 and dgp is None:
+            return
+        check(lib().adn_rms_norm_backward_async(self._ctx, rows, d, self._dtype(x), xp, xs,
+                                                self._vector(gain, "gain", d), eps, dyp, dys, dxp, dxs, dgp))
+
+    def embed_lookup_async(self, tokens, out, *, table=None, scale: float = 1.0) -> None:
+        """out[i] = scale * table[tokens[i]] (``Tokenizer::embed_sequence``, tokenizer.rs:151-159, with a
+        factor); table None: the uploaded embedding.  A token < 0 gives a row of zeros."""
+        if out.dim() != 2 or (table is not None and table.dim() != 2):
+            raise _invalid("out and table must be matrices")
+        n, d = out.shape
+        V = self.model.V if table is None else table.shape[0]
+        tp, ts = (None, d) if table is None else self._matrix(table, "table", V, d, out.dtype)
+        op, os_ = self._matrix(out, "out", n, d)
+        check(lib().adn_embed_lookup_async(self._ctx, n, d, V, self._dtype(out),
+                                           self._vector(tokens, "tokens", n, "torch.int32"), tp, ts, scale, op, os_))
+
+    def embed_grad_async(self, dout, tokens, dtable, *, scale: float = 1.0) -> None:
+        """The table's gradient: dtable[v] = scale * sum of the rows dout[i] with tokens[i] = v, in the
+        order of i; every row of dtable is written."""
+        if dout.dim() != 2 or dtable.dim() != 2:
+            raise _invalid("dout and dtable must be matrices")
+        n, d = dout.shape
+        V = dtable.shape[0]
+        sp, ss = self._matrix(dout, "dout", n, d)
+        dp, ds = self._matrix(dtable, "dtable", V, d, dout.dtype)
+        check(lib().adn_embed_grad_async(self._ctx, n, d, V, self._dtype(dout),
+                                         self._vector(tokens, "tokens", n, "torch.int32"), sp, ss, scale, dp, ds))
 
     # reference-named conveniences ---------------------------------------------------------
     def run_forward_deq(self, batch, seq, max_iters, eps, damping, s_in):

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "train.h"
 
 using namespace adn;
 
@@ -65,6 +66,7 @@ struct adn_ctx {
     int last_ntok = 0;
     double *ctx_tot = nullptr;  // embed_context chunk totals (2 x ctx_tot_n doubles)
     long ctx_tot_n = 0;
+    DevBuf train_ws;            // the training operators' workspace (calls run in stream order)
 
     // split-precision copies of the GEMM weights (hi/lo halves of w * scale)
     struct Split {
@@ -1916,6 +1918,200 @@ int adn_profile_forward(adn_ctx *c, const adn_run *r, const adn_outputs *o, adn_
     } catch (const HipError &e) {
         return hip_fail(e);
     }
+}
+
+}  // extern "C"
+
+// =========================================================================================
+// training operators (device memory, enqueue only)
+// =========================================================================================
+namespace {
+
+// The context's GPU as the calling thread's current device, for the length of a call.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(int device) {
+        ADN_HIP(hipGetDevice(&before));
+        if (before != device)
+            ADN_HIP(hipSetDevice(device));
+        else
+            before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// A workspace of `bytes`; null (with the error set) where it would have to grow under capture.  Grows
+// by half at least; earlier blocks stay allocated, as graphs captured with them may be replayed.
+void *train_workspace(adn_ctx *c, size_t bytes) {
+    if (c->train_ws.bytes >= bytes && c->train_ws.p) return c->train_ws.p;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    ADN_HIP(hipStreamIsCapturing(c->stream, &cap));
+    if (cap != hipStreamCaptureStatusNone) {
+        set_error("the workspace would have to grow under stream capture: run the call once before capturing it");
+        return nullptr;
+    }
+    bytes = std::max(bytes, c->train_ws.bytes + c->train_ws.bytes / 2);
+    c->train_ws.p = dmalloc(c, bytes);
+    c->train_ws.bytes = bytes;
+    return c->train_ws.p;
+}
+
+std::string check_rows(const char *what, const void *p, int64_t stride, int32_t rows, int32_t d, uint32_t dtype) {
+    if (rows > 0 && !p) return std::string("null ") + what;
+    if (stride < d || stride > (1ll << 32))
+        return std::string("the stride of ") + what + " must be in [d, 2^32] elements";
+    if ((uintptr_t)p % elem_bytes(dtype)) return std::string(what) + " is not aligned to its elements";
+    return "";
+}
+
+std::string check_words(const char *what, const void *p) {
+    return (uintptr_t)p % 4 ? std::string(what) + " is not aligned to its elements" : "";
+}
+
+std::string check_sizes(int32_t rows, int32_t max_rows, int32_t d, int32_t vocab, uint32_t dtype) {
+    if (dtype != ADN_T_F32 && dtype != ADN_T_BF16) return "unknown dtype";
+    if (rows < 0 || rows > max_rows) return "the number of rows must be in [0, " + std::to_string(max_rows) + "]";
+    if (d < 1 || d > 8192) return "d must be in [1, 8192]";
+    if (vocab < 1 || vocab > (1 << 24)) return "vocab must be in [1, 2^24]";
+    return "";
+}
+
+// The first message of several checks.
+std::string first_of(std::initializer_list<std::string> msgs) {
+    for (const auto &m : msgs)
+        if (!m.empty()) return m;
+    return "";
+}
+
+constexpr int TRAIN_MAX_ROWS = 1 << 24, LOSS_MAX_ROWS = 1 << 20;
+
+// Runs f() (the launches) on the context's device with `bytes` of workspace.
+template <typename F>
+int train_launch(adn_ctx *c, size_t bytes, F &&f) {
+    try {
+        DeviceScope scope(c->device);
+        void *ws = nullptr;
+        if (bytes) {
+            ws = train_workspace(c, bytes);
+            if (!ws) return ADN_E_CAPACITY;
+        }
+        f(ws);
+        ADN_HIP(hipGetLastError());
+    } catch (const HipError &e) {
+        return hip_fail(e);
+    } catch (const std::exception &e) {
+        return fail(ADN_E_HIP, e.what());
+    }
+    return ADN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int adn_context_device(const adn_ctx *c, int32_t *device) {
+    if (!c || !device) return fail(ADN_E_INVALID, "null argument");
+    *device = c->device;
+    return ADN_OK;
+}
+
+int adn_lm_loss_async(adn_ctx *c, const adn_lm_loss_args *a) {
+    if (!c || !a) return fail(ADN_E_INVALID, "null argument");
+    std::string msg = check_sizes(a->rows, LOSS_MAX_ROWS, a->d, a->vocab, a->dtype);
+    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+    if (!a->loss && !a->lse && !a->dx && !a->dw && !a->db) return fail(ADN_E_INVALID, "no output is wanted");
+    LossParams p{};
+    p.rows = a->rows, p.d = a->d, p.vocab = a->vocab, p.dtype = a->dtype;
+    p.w = a->w, p.w_stride = a->w_stride, p.bias = a->bias;
+    if (!a->w) {
+        if (!c->has_weights) return fail(ADN_E_NO_WEIGHTS, "adn_lm_loss_async without w before adn_upload_weights");
+        if (a->dtype != ADN_T_F32 || a->d != c->D.d || a->vocab != c->D.V || a->bias)
+            return fail(ADN_E_INVALID, "w NULL is the context's head: ADN_T_F32, its d_r and vocab, bias NULL");
+        p.w = c->lm_w, p.w_stride = c->D.d, p.bias = c->lm_b;
+    }
+    msg = first_of({check_rows("x", a->x, a->x_stride, a->rows, a->d, a->dtype),
+                    check_rows("w", p.w, p.w_stride, a->vocab, a->d, a->dtype),
+                    a->dx ? check_rows("dx", a->dx, a->dx_stride, a->rows, a->d, a->dtype) : "",
+                    a->dw ? check_rows("dw", a->dw, a->dw_stride, a->vocab, a->d, a->dtype) : "",
+                    a->rows > 0 && !a->targets ? "null targets" : "", check_words("bias", p.bias),
+                    check_words("targets", a->targets), check_words("dloss", a->dloss), check_words("loss", a->loss),
+                    check_words("lse", a->lse), check_words("db", a->db)});
+    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+    p.x = a->x, p.x_stride = a->x_stride;
+    p.targets = a->targets, p.dloss = a->dloss;
+    p.loss = a->loss, p.lse = a->lse;
+    p.dx = a->dx, p.dx_stride = a->dx_stride;
+    p.dw = a->dw, p.dw_stride = a->dw_stride;
+    p.db = a->db;
+    p.err = c->d_err;
+    return train_launch(c, loss_workspace_bytes(p), [&](void *ws) { launch_loss(p, ws, c->stream); });
+}
+
+int adn_rms_norm_async(adn_ctx *c, int32_t rows, int32_t d, uint32_t dtype, const void *x, int64_t x_stride,
+                       const float *gain, float eps, void *y, int64_t y_stride) {
+    if (!c) return fail(ADN_E_INVALID, "null context");
+    std::string msg = check_sizes(rows, TRAIN_MAX_ROWS, d, 1, dtype);
+    if (msg.empty())
+        msg = first_of({check_rows("x", x, x_stride, rows, d, dtype), check_rows("y", y, y_stride, rows, d, dtype),
+                        check_words("gain", gain), eps >= 0.0f ? "" : "eps must be >= 0"});
+    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+    NormParams p{};
+    p.rows = rows, p.d = d, p.dtype = dtype;
+    p.x = x, p.x_stride = x_stride, p.gain = gain, p.eps = eps;
+    p.y = y, p.y_stride = y_stride;
+    return train_launch(c, 0, [&](void *) { launch_norm(p, c->stream); });
+}
+
+int adn_rms_norm_backward_async(adn_ctx *c, int32_t rows, int32_t d, uint32_t dtype, const void *x,
+                                int64_t x_stride, const float *gain, float eps, const void *dy, int64_t dy_stride,
+                                void *dx, int64_t dx_stride, float *dg) {
+    if (!c) return fail(ADN_E_INVALID, "null context");
+    std::string msg = check_sizes(rows, TRAIN_MAX_ROWS, d, 1, dtype);
+    if (msg.empty() && !dx && !dg) msg = "no output is wanted";
+    if (msg.empty())
+        msg = first_of({check_rows("x", x, x_stride, rows, d, dtype), check_rows("dy", dy, dy_stride, rows, d, dtype),
+                        dx ? check_rows("dx", dx, dx_stride, rows, d, dtype) : "", check_words("gain", gain),
+                        check_words("dg", dg), eps >= 0.0f ? "" : "eps must be >= 0"});
+    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+    NormParams p{};
+    p.rows = rows, p.d = d, p.dtype = dtype;
+    p.x = x, p.x_stride = x_stride, p.gain = gain, p.eps = eps;
+    p.dy = dy, p.dy_stride = dy_stride, p.dx = dx, p.dx_stride = dx_stride, p.dg = dg;
+    return train_launch(c, norm_backward_workspace_bytes(p), [&](void *ws) { launch_norm_backward(p, ws, c->stream); });
+}
+
+int adn_embed_lookup_async(adn_ctx *c, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,
+                           const void *table, int64_t table_stride, float scale, void *out, int64_t out_stride) {
+    if (!c) return fail(ADN_E_INVALID, "null context");
+    std::string msg = check_sizes(n, TRAIN_MAX_ROWS, d, vocab, dtype);
+    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+    if (!table) {
+        if (!c->has_weights) return fail(ADN_E_NO_WEIGHTS, "adn_embed_lookup_async without a table before adn_upload_weights");
+        if (dtype != ADN_T_F32 || d != c->D.d || vocab != c->D.V)
+            return fail(ADN_E_INVALID, "table NULL is the context's embedding: ADN_T_F32, its d_r and vocab");
+        table = c->embed, table_stride = c->D.d;
+    }
+    msg = first_of({check_rows("table", table, table_stride, vocab, d, dtype),
+                    check_rows("out", out, out_stride, n, d, dtype), n > 0 && !tokens ? "null tokens" : "",
+                    check_words("tokens", tokens)});
+    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+    TableParams p{n, d, vocab, dtype, tokens, scale, table, table_stride, out, out_stride, c->d_err};
+    return train_launch(c, 0, [&](void *) { launch_embed_lookup(p, c->stream); });
+}
+
+int adn_embed_grad_async(adn_ctx *c, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,
+                         const void *dout, int64_t dout_stride, float scale, void *dtable, int64_t dtable_stride) {
+    if (!c) return fail(ADN_E_INVALID, "null context");
+    std::string msg = check_sizes(n, TRAIN_MAX_ROWS, d, vocab, dtype);
+    if (msg.empty())
+        msg = first_of({check_rows("dout", dout, dout_stride, n, d, dtype),
+                        check_rows("dtable", dtable, dtable_stride, vocab, d, dtype),
+                        n > 0 && !tokens ? "null tokens" : "", check_words("tokens", tokens)});
+    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+    TableParams p{n, d, vocab, dtype, tokens, scale, dout, dout_stride, dtable, dtable_stride, c->d_err};
+    return train_launch(c, embed_grad_workspace_bytes(p), [&](void *ws) { launch_embed_grad(p, ws, c->stream); });
 }
 
 }  // extern "C"

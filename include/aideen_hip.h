@@ -306,6 +306,68 @@ int adn_adjoint(adn_ctx *ctx, int32_t ntok, const float *h_star, const float *dl
 int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const float *dl, int32_t iters,
                       float damping, float *v_out, float *src);
 
+/* --- training operators of the LM head and the embedding table --------------------------------
+ * What lies between a forward's pooled rows and adn_adjoint's dl, and behind its source gradient:
+ * the head's RMS norm (lm_head.rs:35-54), the softmax cross entropy over the whole vocabulary with
+ * its gradients, and the embedding rows (tokenizer.rs:117-119, 151-159) with the table's gradient.
+ * All take device memory of the context's GPU and only enqueue on the context's stream; the tensors
+ * must not overlap.  Sizes are the call's own (the context's configuration bounds them only where
+ * its weights are used).  Matrices are rows of d elements at a stride in elements (>= d) of the type
+ * dtype; any alignment of whole elements is served (16-byte aligned rows at the full rate).  Sums
+ * are taken in fp32 in an order that the sizes alone decide, so equal calls give equal bits; each
+ * output is rounded once to its type.  A token or target id < 0 marks a position without one (a
+ * padded batch); ids >= vocab are treated so too and reported by the next adn_synchronize().
+ * Workspaces belong to the context, grow to the largest request and are kept until it is destroyed:
+ * a call that would have to grow one is refused under stream capture (ADN_E_CAPACITY), so run a
+ * call once before capturing it, and do not replay graphs of one context side by side. */
+#define ADN_T_F32 0u
+#define ADN_T_BF16 1u
+
+/* loss_i = lse_i - z_i,t(i), z = x w^T + bias, lse_i = log sum_v exp(z_iv); with dz_iv = dloss_i
+ * (exp(z_iv - lse_i) - [v = t(i)]): dx = dz w, dw = dz^T x, db = sum_i dz_i.  The logits are formed
+ * a piece of the vocabulary at a time and never kept.  Rows without a target are left out: their x
+ * is not read, their loss, lse and dx are 0.  A bias of -inf or of the type's lowest value takes an
+ * entry out of the vocabulary; a row whose logits are all -inf, or not a number, has a loss, a dx
+ * and a share of dw that are not numbers. */
+typedef struct adn_lm_loss_args {
+    int32_t rows, d, vocab;     /* rows in [0, 2^20], d in [1, 8192], vocab in [1, 2^24] */
+    uint32_t dtype;             /* ADN_T_*: x, w, dx and dw                               */
+    const void *x;              /* [rows] rows of d: the head's input (normalised rows)  */
+    int64_t x_stride;
+    const void *w;              /* [vocab] rows of d; NULL: the context's lm_w and lm_b  */
+    int64_t w_stride;           /*   (then d = d_r, its vocab, ADN_T_F32, bias NULL)     */
+    const float *bias;          /* [vocab], NULL = 0                                     */
+    const int32_t *targets;     /* [rows]                                                */
+    const float *dloss;         /* [rows] dL/dloss_i, NULL = 1                           */
+    float *loss, *lse;          /* [rows] outputs, NULL where not wanted                 */
+    void *dx;                   /* [rows] rows of d                                      */
+    int64_t dx_stride;
+    void *dw;                   /* [vocab] rows of d                                     */
+    int64_t dw_stride;
+    float *db;                  /* [vocab]                                               */
+} adn_lm_loss_args;
+int adn_lm_loss_async(adn_ctx *ctx, const adn_lm_loss_args *args);
+
+/* y = x r gain, r = 1 / sqrt(mean(x^2) + eps), per row (gain [d] fp32, NULL = 1; d in [1, 8192],
+ * rows in [0, 2^24]).  Backward: a = dy gain, dx = r (a - x r^2 mean(a x)), dg = sum over the rows
+ * of dy x r (fp32); dx and dg may each be NULL where not wanted. */
+int adn_rms_norm_async(adn_ctx *ctx, int32_t rows, int32_t d, uint32_t dtype, const void *x, int64_t x_stride,
+                       const float *gain, float eps, void *y, int64_t y_stride);
+int adn_rms_norm_backward_async(adn_ctx *ctx, int32_t rows, int32_t d, uint32_t dtype, const void *x,
+                                int64_t x_stride, const float *gain, float eps, const void *dy, int64_t dy_stride,
+                                void *dx, int64_t dx_stride, float *dg);
+
+/* out_i = scale * table[tokens_i], i < n (n in [0, 2^24], vocab in [1, 2^24], d in [1, 8192]); rows
+ * without a token are 0.  table NULL: the context's embedding (then d = d_r, its vocab, ADN_T_F32).
+ * The gradient writes the whole table: dtable[v] = scale * sum of the dout_i with tokens_i = v, in
+ * the order of i, 0 where there is none. */
+int adn_embed_lookup_async(adn_ctx *ctx, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,
+                           const void *table, int64_t table_stride, float scale, void *out, int64_t out_stride);
+int adn_embed_grad_async(adn_ctx *ctx, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,
+                         const void *dout, int64_t dout_stride, float scale, void *dtable, int64_t dtable_stride);
+/* The ordinal of the GPU that a context was created on. */
+int adn_context_device(const adn_ctx *ctx, int32_t *device);
+
 /* --- input pipeline ------------------------------------------------------------------
  * Tokenizer::embed_context (tokenizer.rs:133-149) for the window ending at every position, as
  * the trainer builds the query of position i (trainer.rs:4690-4696: context =
