@@ -5,212 +5,869 @@
 //   dz_iv = g_i (exp(z_iv - lse_i) - [v = t(i)])
 //   dx = dz W,  dW = dz^T x,  db = sum_i dz_i
 //
-// The logits exist a piece of the vocabulary at a time: a first pass over the pieces merges each
-// row's running maximum and sum of exponentials, a second one forms the piece's logits again, turns
-// them into dz and multiplies it with both operands.  All sums in fp32.
+// Four products on the fp16 MFMA, 2 n V d operations each (n rows, V entries, width d): the logits
+// for lse (stored nowhere: their epilogue leaves each row's maximum and sum of exponentials per 256
+// entries), then a piece of the vocabulary at a time the logits again, whose epilogue stores the
+// piece's dz, and dz W and dz^T x from it.  The piece holds at most PIECE_BYTES, so the workspace
+// does not grow with n V.  Forming the logits twice costs a third more operations than keeping them,
+// n V values of 4 bytes.
+//
+// Operands are fp16 planes.  fp32 tensors: two planes, hi = f16(s x) and lo = f16(s x - hi), three
+// products hi hi + hi lo + lo hi (the split of the forward's products: 2^-22 of a product is lost).
+// bf16 tensors: one plane, exact (8 of 11 bits), one product.  dz is rounded to the same number of
+// planes: 22 bits or 11, where bf16 outputs keep 8.  The scales are powers of two.  W has one, by its
+// largest value (values below 2^-40 of it are lost, to the same absolute error as the rest).  Every row
+// of x has its own for the logits, 2^f_i, by the row's largest value, and dz_i is stored without the
+// power of two in g_i = m_i 2^e_i, so that neither a row's size nor its g_i matters to another row's
+// loss or dx.  dW sums over the rows: its planes of x hold x_i 2^(e_i + F), one F for all, by the
+// largest |x_i| 2^e_i.  All sums are fp32.
+//
+// Layout.  Every plane is stored as blocks of 32 rows x 16 columns, 1 KB each, the blocks of 32 rows
+// one after another along the columns; rows and columns are padded with zeros.  A block is what one
+// direct global->LDS load of a wave moves.  The one image serves a product over the columns (a lane
+// reads 8 consecutive columns of its row, ds_read_b128) and a product over the rows (the transposing
+// ds_read_b64_tr_b16: a group of 16 lanes reads 4 rows of 16 columns, 128 adjacent bytes, and each
+// lane gets one column), so x, W and dz are laid out once and no operand is ever transposed in memory.
 #include <algorithm>
+#include <cmath>
 
+#include "gemm_common.h"
 #include "train.h"
 
 namespace adn {
 
 namespace {
 
-constexpr int NT = 256;
-constexpr int BT = 64, BKS = 16;
-constexpr size_t PIECE_BYTES = 256u << 20;
+using gemm::lds_barrier;
 
-// C[i][j] = sum_k A(i,k) B(j,k) (+ bias[j], + C), A(i,k) = A[i ai + k ak], B(j,k) = B[j bj + k bk]:
-// 64 x 64 blocks, 4 x 4 values a thread.
-// Where `live` is set, terms k with live[k] < 0 are left out (rows without a target: their x is not read).
-template <typename TA, typename TB, typename TC>
-__global__ __launch_bounds__(NT) void k_tile_product(const TA *A, long ai, long ak, const TB *B, long bj, long bk, TC *C,
-                                                     long ci, int M, int N, int K, const float *bias, bool add,
-                                                     const int32_t *live) {
-    __shared__ float As[BKS][BT + 1], Bs[BKS][BT + 1];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const long i0 = (long)blockIdx.y * BT, j0 = (long)blockIdx.x * BT;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += BKS) {
-        for (int q = threadIdx.x; q < BT * BKS; q += NT) {
-            // neighbouring threads along the operand's unit stride
-            const int ka = ak == 1 ? q % BKS : q / BT, ia = ak == 1 ? q / BKS : q % BT;
-            const int kb = bk == 1 ? q % BKS : q / BT, jb = bk == 1 ? q / BKS : q % BT;
-            As[ka][ia] = i0 + ia < M && k0 + ka < K ? to_f32<TA>(A[(i0 + ia) * ai + (long)(k0 + ka) * ak]) : 0.0f;
-            Bs[kb][jb] = j0 + jb < N && k0 + kb < K && (!live || live[k0 + kb] >= 0) ? to_f32<TB>(B[(j0 + jb) * bj + (long)(k0 + kb) * bk]) : 0.0f;
+constexpr int NT = 256;             // threads a workgroup: 4 waves
+constexpr size_t PIECE_BYTES = 256u << 20;
+constexpr int TV = 256;             // entries a workgroup of the logits' product covers
+constexpr int STAGES = 3;           // k slices of the LDS ring
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int W_BLOCKS = 1024;      // blocks of the pass over |W|, one partial each
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) short4v lds_short4;
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {  // the other counters left alone
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// Chunk (8 halves) of a block's row r that holds columns [0, 8) in the LDS image of an operand read
+// along its columns: the b128 reads of 32 consecutive rows then use every bank alike.
+__device__ __forceinline__ int swz(int r) { return ((r >> 2) ^ (r >> 3)) & 1; }
+
+// A blocked matrix: planes `plane` halves apart, `ncb` column blocks in a row of blocks.
+struct Planes {
+    const _Float16 *p;
+    long plane;
+    int ncb;
+};
+
+// What the products share.  Rows (M) are the MFMA's rows, held in a lane's registers; columns (N)
+// its columns, one a lane.
+struct LossGemm {
+    Planes A, B;
+    int nM, nN, S;       // tiles of rows and columns, shares of K
+    int K;               // length of the product (a multiple of the slice), the same for every share but the last
+    int Ks;              // length of a share
+    int a_row0;          // first row of A (entries of the piece), a multiple of 32
+    // logits
+    const float *bias;
+    const int32_t *f;    // [rows padded] exponents of the rows' scales
+    const int32_t *tgt;  // [rows padded] targets, -1 = none
+    const int32_t *kw_dev;  // exponent of W's scale
+    int vocab, rows;
+    float *part_m, *part_s, *ztgt;      // [tile][rows padded]: maximum and sum of exponentials; the target's logit
+    long rows_pad;
+    const float *lse, *q, *g;           // per row: lse (in units of log 2), dz's factor (m_i 2^13), g_i
+    _Float16 *dz;                       // planes of the piece, blocks of rows x entries
+    long dz_plane;
+    int dz_ncb;
+    float *db_part;                     // [row tile][entries padded]
+    long db_ld;
+    // gradients
+    float *part;                        // [share][rows][ld] partial sums, or null: dst is written
+    long part_ld;
+    int add;                            // the partial sums are added to
+    void *dst;
+    long dst_stride;
+    int out_rows, out_cols;
+    const int32_t *e_row;               // exponent of a row's result (dx), or null: *e_all
+    const int32_t *e_all;
+};
+
+enum { LOGITS_STATS = 0, LOGITS_DZ = 1, GRAD = 2 };
+
+// One tile: WGM x WGN waves of WTM x WTN MFMA tiles of 32x32.  NP planes an operand; a k slice is
+// 16 KB values (24 KB of LDS for either NP at the largest tile: three slices and two workgroups a
+// CU, so that one's epilogue runs under the other's MFMAs).  TRA / TRB: the operand's rows are the
+// product's K.
+template <int MODE, typename T, int NP, int WTM, int WTN, int WGM, int WGN, bool TRA, bool TRB>
+__global__ __launch_bounds__(NT, 2) void k_loss_gemm(LossGemm p) {
+    static_assert(WGM * WGN == 4, "four waves");
+    constexpr int KB = NP == 2 ? 1 : 2;
+    constexpr int TM = WGM * WTM * 32, TN = WGN * WTN * 32;
+    constexpr int A_BLK = TM / 32 * KB, B_BLK = TN / 32 * KB;  // 1 KB loads a plane and slice
+    constexpr int A_PW = (A_BLK + 3) / 4, B_PW = (B_BLK + 3) / 4;
+    constexpr int LOADS = NP * (A_PW + B_PW);
+    constexpr int A_SZ = A_BLK * 512, B_SZ = B_BLK * 512;      // halves a plane and slice
+    constexpr int SLICE = NP * (A_SZ + B_SZ);
+    __shared__ __attribute__((aligned(1024))) _Float16 ring[STAGES * SLICE];
+    static_assert(STAGES * SLICE * 2 <= 80 * 1024, "two workgroups a CU");
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    const int r = lane & 31, hh = lane >> 5;
+    int s, mt, nt;
+    gemm::map_block(blockIdx.x, p.nM * p.nN * p.S, p.nM, p.nN, s, mt, nt);
+    const int k0 = s * p.Ks;
+    const int nk = (min(p.Ks, p.K - k0)) / (16 * KB);
+
+    // this wave's loads of a slice: per-lane source offsets (halves) at slice 0
+    long asrc[A_PW], bsrc[B_PW];
+    auto src_of = [&](bool tr, int idx, int tile0, const Planes &P) -> long {
+        if (!tr) {  // block (row block, k block)
+            const int rb = idx / KB, kb = idx % KB, row = lane >> 1;
+            return ((long)(tile0 / 32 + rb) * P.ncb + k0 / 16 + kb) * 512 + row * 16 + (((lane & 1) ^ swz(row)) * 8);
         }
-        __syncthreads();
+        if constexpr (KB == 2) {  // whole blocks of 32 k x 16 columns
+            const int cb = min(tile0 / 16 + idx, P.ncb - 1);
+            return ((long)(k0 / 32) * P.ncb + cb) * 512 + lane * 8;
+        } else {  // halves (16 k) of two neighbouring blocks
+            const int cb = min(tile0 / 16 + 2 * idx + (lane >> 5), P.ncb - 1);
+            return (long)cb * 512 + (lane & 31) * 8;  // the k block and half: step_of
+        }
+    };
+    // slice kt's offset from slice 0
+    auto step_of = [&](bool tr, int kt, const Planes &P) -> long {
+        if (!tr) return (long)kt * KB * 512;
+        if constexpr (KB == 2) return (long)kt * P.ncb * 512;
+        const int k = k0 / 16 + kt;
+        return (long)(k >> 1) * P.ncb * 512 + (k & 1) * 256;
+    };
+    // tr operands of whole blocks: TM / 16 loads; of half blocks: two blocks a load -- A_BLK in both
 #pragma unroll
-        for (int k = 0; k < BKS; ++k)
+    for (int j = 0; j < A_PW; ++j) asrc[j] = src_of(TRA, (wave + 4 * j) % A_BLK, p.a_row0 + mt * TM, p.A);
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+    for (int j = 0; j < B_PW; ++j) bsrc[j] = src_of(TRB, (wave + 4 * j) % B_BLK, nt * TN, p.B);
+    const _Float16 *Ap = p.A.p, *Bp = p.B.p;
+    auto issue = [&](int kt) {
+        _Float16 *base = ring + (kt % STAGES) * SLICE;
+        const long sa = step_of(TRA, kt, p.A), sb = step_of(TRB, kt, p.B);
 #pragma unroll
-                for (int b = 0; b < 4; ++b) acc[a][b] += As[k][ty + 16 * a] * Bs[k][tx + 16 * b];
-        __syncthreads();
-    }
+        for (int q = 0; q < NP; ++q) {
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+            for (int j = 0; j < A_PW; ++j)
+                __builtin_amdgcn_global_load_lds((const void *)(Ap + q * p.A.plane + asrc[j] + sa),
+                                                 (lds_void *)(base + q * A_SZ + ((wave + 4 * j) % A_BLK) * 512), 16, 0, 0);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const long i = i0 + ty + 16 * a, j = j0 + tx + 16 * b;
-            if (i < M && j < N) {
-                float v = acc[a][b] + (bias ? bias[j] : 0.0f);
-                if (add) v += to_f32<TC>(C[i * ci + j]);
-                C[i * ci + j] = from_f32<TC>(v);
+            for (int j = 0; j < B_PW; ++j)
+                __builtin_amdgcn_global_load_lds((const void *)(Bp + q * p.B.plane + bsrc[j] + sb),
+                                                 (lds_void *)(base + NP * A_SZ + q * B_SZ + ((wave + 4 * j) % B_BLK) * 512),
+                                                 16, 0, 0);
+        }
+    };
+    // MFMA operand of 32 rows (columns) `t` of the tile, k block kb of the slice
+    auto frag = [&](const _Float16 *img, bool tr, int t, int kb) -> half8 {
+        if (!tr) return *reinterpret_cast<const half8 *>(img + (t * KB + kb) * 512 + r * 16 + ((hh ^ swz(r)) * 8));
+        const _Float16 *a = img + (2 * t + ((lane >> 4) & 1)) * (KB * 256) + (kb * 16 + 8 * hh + ((lane >> 2) & 3)) * 16 +
+                            (lane & 3) * 4;
+        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)a);
+        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(a + 64));
+        return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    floatx16 acc[WTM][WTN];
+#pragma unroll
+    for (int i = 0; i < WTM; ++i)
+#pragma unroll
+        for (int j = 0; j < WTN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t)
+        if (t < nk) issue(t);
+    for (int kt = 0; kt < nk; ++kt) {
+        // slice kt is in LDS once this wave's later loads are all that is in flight; the barrier
+        // covers the other waves' loads, and their reads of the slot that is loaded next
+        if (kt + STAGES - 2 < nk)
+            wait_vmcnt<(STAGES - 2) * LOADS>();
+        else
+            wait_vmcnt<0>();
+        lds_barrier();
+        if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1);
+        const _Float16 *base = ring + (kt % STAGES) * SLICE;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            half8 a[NP][WTM];
+#pragma unroll
+            for (int q = 0; q < NP; ++q)
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) a[q][i] = frag(base + q * A_SZ, TRA, wm * WTM + i, kb);
+#pragma unroll
+            for (int j = 0; j < WTN; ++j) {
+                half8 b[NP];
+#pragma unroll
+                for (int q = 0; q < NP; ++q) b[q] = frag(base + NP * A_SZ + q * B_SZ, TRB, wn * WTN + j, kb);
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) {
+                    if constexpr (NP == 2) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1], acc[i][j], 0, 0, 0);
+                    }
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0], acc[i][j], 0, 0, 0);
+                }
             }
         }
+    }
+    lds_barrier();  // every wave is done with the ring
+
+    // Output layout of a 32x32 tile: lane holds column r; register e row 8 (e / 4) + 4 hh + e % 4.
+    if constexpr (MODE == GRAD) {
+        const int ec = p.e_all ? *p.e_all : 0;
+#pragma unroll
+        for (int i = 0; i < WTM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const long row = (long)mt * TM + (wm * WTM + i) * 32 + 8 * (e / 4) + 4 * hh + e % 4;
+                if (row >= p.out_rows) continue;
+                const int ex = p.part ? 0 : ec + (p.e_row ? p.e_row[row] : 0);
+#pragma unroll
+                for (int j = 0; j < WTN; ++j) {
+                    const int col = nt * TN + (wn * WTN + j) * 32 + r;
+                    if (col >= p.out_cols) continue;
+                    if (p.part) {
+                        float *o = p.part + ((long)s * p.out_rows + row) * p.part_ld + col;
+                        *o = p.add ? *o + acc[i][j][e] : acc[i][j][e];
+                    } else {
+                        ((T *)p.dst)[row * p.dst_stride + col] = from_f32<T>(ldexpf(acc[i][j][e], ex));
+                    }
+                }
+            }
+    } else {
+        static_assert(MODE == GRAD || (TM == TV && WGN == 1), "a wave's columns are the tile's");
+        // the tile's biases; entries beyond the vocabulary get -inf: no part of any sum.  From here on
+        // logits are in units of log 2 (z log2(e)), what exp2 takes.
+        float *bias_l = reinterpret_cast<float *>(ring);                   // [TM]
+        const int v0 = p.a_row0 + mt * TM;
+        for (int c = tid; c < TM; c += NT) {
+            float b = v0 + c < p.vocab ? (p.bias ? p.bias[v0 + c] : 0.0f) : -INFINITY;
+            if (b < -1e38f && b > -INFINITY) b = -1e38f;  // the type's lowest value stays finite
+            bias_l[c] = b * LOG2E;
+        }
+        lds_barrier();
+        const int kw = *p.kw_dev;
+        const int w0 = v0 + wm * WTM * 32;  // the wave's first entry
+        float unscale[WTN];
+#pragma unroll
+        for (int j = 0; j < WTN; ++j) unscale[j] = ldexpf(LOG2E, -(p.f[nt * TN + j * 32 + r] + kw));
+#pragma unroll
+        for (int i = 0; i < WTM; ++i)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4) {
+                const floatx4 b = *reinterpret_cast<const floatx4 *>(bias_l + (wm * WTM + i) * 32 + 8 * e4 + 4 * hh);
+#pragma unroll
+                for (int j = 0; j < WTN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i][j][4 * e4 + e] = __builtin_fmaf(acc[i][j][4 * e4 + e], unscale[j], b[e]);
+            }
+        if constexpr (MODE == LOGITS_STATS) {
+            float *red_m = bias_l + TM, *red_s = red_m + 4 * TN;           // [wave][TN]
+#pragma unroll
+            for (int j = 0; j < WTN; ++j) {
+                const long m = (long)nt * TN + j * 32 + r;
+                float mx = acc[0][j][0];
+#pragma unroll
+                for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float ref = mx == -INFINITY ? 0.0f : mx;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        sum += __builtin_amdgcn_exp2f(acc[i][j][e] - ref);
+                sum += __shfl_xor(sum, 32, 64);
+                if (hh == 0) {
+                    red_m[wave * TN + j * 32 + r] = mx;
+                    red_s[wave * TN + j * 32 + r] = sum;
+                }
+                // the target's logit, by the one lane that holds it
+                const int t = p.tgt[m] - w0;
+                if (__any(t >= 0 && t < WTM * 32))
+#pragma unroll
+                    for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) p.ztgt[m] = acc[i][j][e];
+            }
+            lds_barrier();
+            for (int c = tid; c < TN; c += NT) {
+                float mx = red_m[c];
+#pragma unroll
+                for (int w = 1; w < 4; ++w) mx = fmaxf(mx, red_m[w * TN + c]);
+                const float ref = mx == -INFINITY ? 0.0f : mx;
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    sum += red_s[w * TN + c] * __builtin_amdgcn_exp2f(red_m[w * TN + c] - ref);
+                const long o = (long)mt * p.rows_pad + nt * TN + c;
+                p.part_m[o] = mx;
+                p.part_s[o] = sum;
+            }
+        } else {
+            float *colsum = bias_l + TM + wave * (32 * WTM * 33);          // db: [WTM * 32 entries][32 + 1]
+            float bsum[WTM][16];
+#pragma unroll
+            for (int j = 0; j < WTN; ++j) {
+                const long m = (long)nt * TN + j * 32 + r;
+                const float lse = p.lse[m], qm = p.q[m], gm = p.g[m];
+                const int t = p.tgt[m] - w0;
+                const bool off = qm == 0.0f;  // no target, or nothing from upstream: exactly zero
+#pragma unroll
+                for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - lse);
+                if (__any(t >= 0 && t < WTM * 32))
+#pragma unroll
+                    for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) acc[i][j][e] -= 1.0f;
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) {
+                    // a register pair of 8 values becomes the two 16-byte chunks of a block's row
+                    // (columns 0-7 in the lower half of the wave, 8-15 in the upper one)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        unsigned pk[NP][4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            unsigned w[NP] = {};
+#pragma unroll
+                            for (int v = 0; v < 2; ++v) {
+                                const int e = 8 * h + 2 * u + v;
+                                float x = off ? 0.0f : acc[i][j][e] * qm;
+                                if (p.db_part) bsum[i][e] = (j ? bsum[i][e] : 0.0f) + (off ? 0.0f : acc[i][j][e] * gm);
+                                const _Float16 hi = (_Float16)x;
+                                w[0] |= (unsigned)__builtin_bit_cast(unsigned short, hi) << (16 * v);
+                                if constexpr (NP == 2)
+                                    w[1] |= (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(x - (float)hi)) << (16 * v);
+                            }
+#pragma unroll
+                            for (int q = 0; q < NP; ++q) pk[q][u] = w[q];
+                        }
+                        const long blk = (long)(nt * (TN / 32) + j) * p.dz_ncb + (long)mt * (TM / 16) + (wm * WTM + i) * 2 + h;
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) {
+                            const auto x0 = __builtin_amdgcn_permlane32_swap(pk[q][0], pk[q][2], false, false);
+                            const auto x1 = __builtin_amdgcn_permlane32_swap(pk[q][1], pk[q][3], false, false);
+                            const uint4v o = {x0[0], x1[0], x0[1], x1[1]};
+                            *reinterpret_cast<uint4v *>(p.dz + q * p.dz_plane + blk * 512 + r * 16 + hh * 8) = o;
+                        }
+                    }
+                }
+            }
+            if (p.db_part) {  // each entry's sum over the tile's rows, lanes in order
+#pragma unroll
+                for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) colsum[(i * 32 + 8 * (e / 4) + 4 * hh + e % 4) * 33 + r] = bsum[i][e];
+                lds_barrier();
+                if (lane < WTM * 32) {
+                    float t = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) t += colsum[lane * 33 + c];
+                    p.db_part[(long)nt * p.db_ld + v0 + wm * WTM * 32 + lane] = t;
+                }
+            }
+        }
+    }
 }
 
-template <typename TA, typename TB, typename TC>
-void tile_product(const TA *A, long ai, long ak, const TB *B, long bj, long bk, TC *C, long ci, int M, int N, int K,
-                  const float *bias, bool add, hipStream_t st, const int32_t *live = nullptr) {
-    const dim3 grid((unsigned)((N + BT - 1) / BT), (unsigned)((M + BT - 1) / BT));
-    k_tile_product<TA, TB, TC><<<grid, NT, 0, st>>>(A, ai, ak, B, bj, bk, C, ci, M, N, K, bias, add, live);
+// ---- operands ------------------------------------------------------------------------------
+// Exponent that takes a magnitude to [2^14, 2^15); 0 for zero and what is not finite.
+__device__ __forceinline__ int scale_exp(float mx) {
+    if (!(mx > 0.0f) || mx == INFINITY) return 0;
+    return 15 - (ilogbf(mx) + 1);
 }
 
-__device__ __forceinline__ float block_max(float v, float *red) {
+// e of |g| = m 2^e, m in [1, 2); 0 for zero and what is not finite
+__device__ __forceinline__ int exp_of(float g) {
+    const float a = fabsf(g);
+    return a > 0.0f && a < INFINITY ? ilogbf(a) : 0;
+}
+
+__device__ __forceinline__ float finite_abs(float v) {
+    const float a = fabsf(v);
+    return a < INFINITY ? a : 0.0f;  // NaN and inf stay in their own rows
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *row, int c, int d, float (&v)[8]) {
+    if constexpr (VEC) {
+        if (c + 8 <= d) {
+            typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(T) / 2; ++q) {
+                const V x = *reinterpret_cast<const V *>(row + c + q * (16 / (int)sizeof(T)));
+#pragma unroll
+                for (int j = 0; j < 16 / (int)sizeof(T); ++j) v[q * (16 / (int)sizeof(T)) + j] = to_f32<T>(x[j]);
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < d ? to_f32<T>(row[c + j]) : 0.0f;
+}
+
+template <int NP>
+__device__ __forceinline__ void store_planes(_Float16 *dst, long plane, const float (&v)[8], int ex) {
+    half8 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float x = ldexpf(v[j], ex);
+        hi[j] = (_Float16)x;
+        if constexpr (NP == 2) lo[j] = (_Float16)(x - (float)hi[j]);
+    }
+    *reinterpret_cast<half8 *>(dst) = hi;
+    if constexpr (NP == 2) *reinterpret_cast<half8 *>(dst + plane) = lo;
+}
+
+struct Prep {
+    const void *x;
+    long x_stride;
+    const void *w;
+    long w_stride;
+    int rows, d, vocab, dcb, w_blocks;  // dcb: column blocks of a row of width d
+    const int32_t *targets;
+    const float *dloss;
+    unsigned *err;
+    _Float16 *xp, *x2p, *wp;  // x for the logits, x for dW (null: not wanted), W
+    long x_plane, w_plane;
+    float *w_part;    // [w_blocks] largest |w| of each block's share
+    int32_t *f, *tgt; // [rows padded]
+    float *g, *gmax;  // [rows padded], [row blocks]: largest |x_i| 2^e_i
+    int32_t *kw;      // exponent of W's scale
+};
+
+__device__ __forceinline__ float block_max256(float v, float *red) {
     v = wave_max(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = red[0];
-    for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
-    return v;
+    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
-__device__ __forceinline__ float block_sum(float v, float *red) {
-    v = wave_sum(v);
+
+// The planes of 32 rows of x, row r times 2^ex[r] (zeros where live[r] < 0): chunk (column block, row,
+// half) by chunk, neighbouring threads side by side.
+template <typename T, int NP, bool VECX>
+__device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb, const int *live, const int *ex) {
+    for (int ch = threadIdx.x; ch < p.dcb * 64; ch += NT) {
+        const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (live[rl] >= 0) load8<T, VECX>((const T *)p.x + (rb * 32 + rl) * p.x_stride, c, p.d, x);
+        store_planes<NP>(dst + rb * p.dcb * 512 + (long)ch * 8, p.x_plane, x, ex[rl]);
+    }
+}
+
+// Blocks below w_blocks: the largest |w| of a share of the rows.  The others: 32 rows of x each, split
+// into planes with a scale of their own; rows without a target are zeros and are not read.
+template <typename T, int NP, bool VECX, bool VECW>
+__global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
+    __shared__ float red[4];
+    __shared__ float rmax[32][8];
+    __shared__ int fx[32], tg[32];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < p.w_blocks) {
+        float m = 0.0f;
+        const int nch = (p.d + 7) / 8;
+        const long total = (long)p.vocab * nch;
+        for (long i = (long)blockIdx.x * NT + tid; i < total; i += (long)p.w_blocks * NT) {
+            const long v = i / nch;
+            float x[8];
+            load8<T, VECW>((const T *)p.w + v * p.w_stride, (int)(i - v * nch) * 8, p.d, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
+        }
+        m = block_max256(m, red);
+        if (tid == 0) p.w_part[blockIdx.x] = m;
+        return;
+    }
+    const int rb = blockIdx.x - p.w_blocks;
+    {
+        const int rl = tid >> 3, part = tid & 7;  // 8 threads a row
+        const long i = (long)rb * 32 + rl;
+        int t = i < p.rows ? p.targets[i] : -1;
+        if (t >= p.vocab) {
+            if (part == 0) atomicOr(p.err, ADN_DEVERR_TOKEN);
+            t = -1;
+        }
+        if (t < 0) t = -1;
+        float m = 0.0f;
+        if (t >= 0)
+            for (int c = part * 8; c < p.d; c += 64) {
+                float x[8];
+                load8<T, VECX>((const T *)p.x + i * p.x_stride, c, p.d, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
+            }
+        rmax[rl][part] = m;
+        if (part == 0) tg[rl] = t;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    float gm = 0.0f;
+    if (tid < 32) {
+        float m = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) m = fmaxf(m, rmax[tid][c]);
+        const long i = (long)rb * 32 + tid;
+        const int t = tg[tid];
+        const float g = t < 0 ? 0.0f : p.dloss ? p.dloss[i] : 1.0f;
+        fx[tid] = scale_exp(m);
+        p.f[i] = fx[tid];
+        p.tgt[i] = t;
+        p.g[i] = g;
+        gm = g == 0.0f ? 0.0f : fminf(ldexpf(m, exp_of(g)), 0x1p127f);
+    }
+    if (tid < 64) {
+        gm = wave_max(gm);
+        if (tid == 0) p.gmax[rb] = gm;
+    }
     __syncthreads();
-    v = red[0];
-    for (int w = 1; w < NT / 64; ++w) v += red[w];
-    return v;
+    split_rows<T, NP, VECX>(p, p.xp, rb, tg, fx);
 }
 
-// Row i's target: its column, or -1 where it has none (negative, or beyond the vocabulary: an error
-// that the next synchronisation reports).
-__device__ __forceinline__ int target_of(const LossParams &p, int i) {
-    const int t = p.targets[i];
-    if (t >= p.vocab) {
-        if (threadIdx.x == 0) atomicOr(p.err, ADN_DEVERR_TOKEN);
-        return -1;
+// W's planes, and the exponent of its scale from the shares' maxima.
+template <typename T, int NP, bool VECW>
+__global__ __launch_bounds__(NT) void k_loss_split_w(Prep p) {
+    __shared__ float red[4];
+    const int tid = threadIdx.x;
+    float m = 0.0f;
+    for (int i = tid; i < p.w_blocks; i += NT) m = fmaxf(m, p.w_part[i]);
+    m = block_max256(m, red);
+    const int kw = scale_exp(m);
+    const long rb = blockIdx.x;
+    if (rb == 0 && tid == 0) *p.kw = kw;
+    for (int ch = tid; ch < p.dcb * 64; ch += NT) {
+        const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
+        const long v = rb * 32 + rl;
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (v < p.vocab) load8<T, VECW>((const T *)p.w + v * p.w_stride, c, p.d, x);
+        store_planes<NP>(p.wp + (rb * p.dcb) * 512 + (long)ch * 8, p.w_plane, x, kw);
     }
-    return t < 0 ? -1 : t;
 }
 
-// Merge a piece's logits [rows][n] into each row's maximum, sum and target logit; after the last
-// piece the row's lse and loss.  A block a row.
-__global__ __launch_bounds__(NT) void k_merge(LossParams p, const float *z, int v0, int n, float *stat, int last) {
-    __shared__ float red[NT / 64];
-    const int i = blockIdx.x, t = target_of(p, i);
-    const float *row = z + (long)i * n;
-    float m = -INFINITY;
-    bool bad = false;  // fmaxf passes NaN over
-    for (int c = threadIdx.x; c < n; c += NT) {
-        m = fmaxf(m, row[c]);
-        bad |= row[c] != row[c];
-    }
-    m = block_max(m, red);
-    bad = __syncthreads_or(bad);
-    const float om = v0 ? stat[i * 3L] : -INFINITY, os = v0 ? stat[i * 3L + 1] : 0.0f;
-    const float ot = v0 ? stat[i * 3L + 2] : 0.0f;
-    const float nm = fmaxf(m, om), ref = nm == -INFINITY ? 0.0f : nm;
+// ---- rows: lse, loss, dz's factors, the planes of x for dW ---------------------------------
+struct Rows {
+    int tiles, row_blocks;
+    long rows_pad;
+    const float *part_m, *part_s, *ztgt;
+    float *lse, *q;           // [rows padded]
+    int32_t *e_dx, *e_dw;     // exponents of the gradients' results: [rows padded] and one
+    float *out_loss, *out_lse;
+};
+
+// 32 rows a block, 8 threads share a row's tiles.
+template <typename T, int NP, bool VECX>
+__global__ __launch_bounds__(NT) void k_loss_rows(Rows p, Prep r) {
+    __shared__ float red[4];
+    __shared__ float sm[8][32], ss[8][32];
+    __shared__ int ex[32], tg[32];
+    const int tid = threadIdx.x, rl = tid & 31, part = tid >> 5;
+    float gm = 0.0f;
+    for (int i = tid; i < p.row_blocks; i += NT) gm = fmaxf(gm, r.gmax[i]);
+    const int F = scale_exp(block_max256(gm, red));
+    const long i = (long)blockIdx.x * 32 + rl;
+    float mx = -INFINITY;
+    for (int t = part; t < p.tiles; t += 8) mx = fmaxf(mx, p.part_m[(long)t * p.rows_pad + i]);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
     float s = 0.0f;
-    for (int c = threadIdx.x; c < n; c += NT) s += expf(row[c] - ref);
-    s = block_sum(s, red) + (v0 ? os * expf(om - ref) : 0.0f);
-    if (bad) s = NAN;
-    if (threadIdx.x) return;
-    const float tz = t >= v0 && t < v0 + n ? row[t - v0] : ot;
-    stat[i * 3L] = nm;
-    stat[i * 3L + 1] = s;
-    stat[i * 3L + 2] = tz;
-    if (last) {
-        const float lse = ref + logf(s);
-        p.lse[i] = t < 0 ? 0.0f : lse;
-        if (p.loss) p.loss[i] = t < 0 ? 0.0f : lse - tz;
+    for (int t = part; t < p.tiles; t += 8)
+        s += p.part_s[(long)t * p.rows_pad + i] * __builtin_amdgcn_exp2f(p.part_m[(long)t * p.rows_pad + i] - ref);
+    sm[part][rl] = mx;
+    ss[part][rl] = s;
+    __syncthreads();
+    if (tid == 0 && blockIdx.x == 0) *p.e_dw = -13 - F;
+    if (tid < 32) {
+        mx = sm[0][rl];
+#pragma unroll
+        for (int q = 1; q < 8; ++q) mx = fmaxf(mx, sm[q][rl]);
+        const float ref2 = mx == -INFINITY ? 0.0f : mx;
+        s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s += ss[q][rl] * __builtin_amdgcn_exp2f(sm[q][rl] - ref2);
+        const float lse = ref2 + log2f(s);  // in units of log 2, as the partials and the target's logit
+        const int t = r.tgt[i];
+        const float g = r.g[i];
+        const int e = exp_of(g);
+        p.lse[i] = lse;
+        p.q[i] = ldexpf(g, 13 - e);
+        p.e_dx[i] = e - 13 - *r.kw;
+        ex[rl] = e + F;
+        tg[rl] = g == 0.0f ? -1 : t;  // a row that gives nothing is not in F's range either
+        if (i < r.rows) {
+            if (p.out_lse) p.out_lse[i] = t < 0 ? 0.0f : lse * LN2;
+            if (p.out_loss) p.out_loss[i] = t < 0 ? 0.0f : (lse - p.ztgt[i]) * LN2;
+        }
+    }
+    if (!r.x2p) return;
+    __syncthreads();
+    split_rows<T, NP, VECX>(r, r.x2p, blockIdx.x, tg, ex);
+}
+
+// dst[row][col] = sum over the shares, in order, times 2^exponent
+template <typename T>
+__global__ __launch_bounds__(NT) void k_loss_join(const float *part, int S, int rows, int d, T *dst, long stride,
+                                                  const int32_t *e_row, const int32_t *e_all) {
+    const long n = (long)rows * d;
+    for (long i = (long)blockIdx.x * NT + threadIdx.x; i < n; i += (long)gridDim.x * NT) {
+        float s = 0.0f;
+        for (int q = 0; q < S; ++q) s += part[q * n + i];
+        const long row = i / d;
+        dst[row * stride + (i - row * d)] = from_f32<T>(ldexpf(s, (e_row ? e_row[row] : 0) + (e_all ? *e_all : 0)));
     }
 }
 
-// z -> dz in place, and the block's columns' share of db is left to k_col_sums.
-__global__ __launch_bounds__(NT) void k_dz(LossParams p, float *z, int v0, int n) {
-    const int i = blockIdx.x, t = target_of(p, i);
-    const float g = t < 0 ? 0.0f : p.dloss ? p.dloss[i] : 1.0f, lse = p.lse[i];
-    float *row = z + (long)i * n;
-    for (int c = threadIdx.x; c < n; c += NT)
-        row[c] = t < 0 ? 0.0f : g * (expf(row[c] - lse) - (v0 + c == t ? 1.0f : 0.0f));
-}
-
-__global__ __launch_bounds__(NT) void k_col_sums(const float *z, int rows, int n, float *db) {
-    const int c = blockIdx.x * NT + threadIdx.x;
-    if (c >= n) return;
+__global__ __launch_bounds__(NT) void k_loss_db(const float *part, int tiles, long ld, int n, float *db) {
+    const int v = blockIdx.x * NT + threadIdx.x;
+    if (v >= n) return;
     float s = 0.0f;
-    for (long i = 0; i < rows; ++i) s += z[i * n + c];
-    db[c] = s;
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) s += part[t * ld + v];
+    db[v] = s;
 }
 
 template <typename T>
-__global__ __launch_bounds__(NT) void k_round_rows(const float *src, int rows, int d, T *dst, long stride) {
-    const long i = blockIdx.x;
-    for (int c = threadIdx.x; c < d; c += NT) dst[i * stride + c] = from_f32<T>(src[i * d + c]);
+__global__ __launch_bounds__(NT) void k_loss_zero(T *dst, long rows, int d, long stride) {
+    for (long i = (long)blockIdx.x * NT + threadIdx.x; i < rows * d; i += (long)gridDim.x * NT)
+        dst[i / d * stride + i % d] = from_f32<T>(0.0f);
 }
 
-struct LossLayout {
-    int piece;
-    size_t z, stat, lse, dx, bytes;
+// ---- plan ----------------------------------------------------------------------------------
+constexpr int SLOTS = 512;  // workgroups that run at once: two a CU
+long round_up(long n, long to) { return (n + to - 1) / to * to; }
+
+struct LossPlan {
+    int np, tn;              // planes; rows a workgroup of the logits' product covers
+    int dcb;                 // column blocks of width d
+    long rows_pad, v_pad;    // rows of the planes of x (and dz), of W
+    int v_tiles;             // tiles of TV entries
+    int piece;               // entries a piece, a multiple of TV
+    int w_blocks;
+    int bn;                  // columns of a gradient tile
+    int dx_tiles, dx_split, dx_ks, dw_split, dw_ks;
+    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, q, e_dx, e_dw, dz, dx_part, dw_part, db_part, bytes;
 };
-LossLayout loss_layout(const LossParams &p) {
-    LossLayout L{};
-    const long rows = std::max(1, p.rows);
-    L.piece = (int)std::min<long>(p.vocab, std::max<long>(64, (long)(PIECE_BYTES / 4) / rows));
+
+// K of `len` (a multiple of 32) in at most `want` shares of whole 32s, each of 256 values at least
+void split_k(long len, long want, int *split, int *share) {
+    long s = std::max<long>(1, std::min(want, len / 256));
+    *share = (int)round_up((len + s - 1) / s, 32);
+    *split = (int)((len + *share - 1) / *share);
+}
+
+LossPlan loss_plan(const LossParams &p) {
+    LossPlan L{};
+    const bool grads = p.dx || p.dw || p.db;
+    L.np = p.dtype == ADN_T_F32 ? 2 : 1;
+    L.tn = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
+    L.dcb = (int)(round_up(p.d, 32) / 16);
+    L.rows_pad = round_up(p.rows, 128);
+    L.v_pad = round_up(p.vocab, TV);
+    L.v_tiles = (int)(L.v_pad / TV);
+    const long fit = (long)(PIECE_BYTES / (L.np * 2)) / L.rows_pad / TV * TV;
+    const long npieces = (L.v_pad + std::max<long>(TV, fit) - 1) / std::max<long>(TV, fit);
+    L.piece = (int)round_up((L.v_pad + npieces - 1) / npieces, TV);
+    L.w_blocks = (int)std::min<long>(W_BLOCKS, ((long)p.vocab * ((p.d + 7) / 8) + NT * 4 - 1) / (NT * 4));
+    L.bn = p.d > 128 ? 256 : p.d > 64 ? 128 : 64;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t r = at;
-        at += (bytes + 255) / 256 * 256;
+        at += (bytes + 1023) / 1024 * 1024;
         return r;
     };
-    L.z = take((size_t)rows * L.piece * 4);
-    L.stat = take((size_t)rows * 12);
-    L.lse = take((size_t)rows * 4);
-    L.dx = take(p.dx ? (size_t)rows * p.d * 4 : 0);
+    L.xp = take((size_t)L.rows_pad * L.dcb * 32 * L.np);
+    L.x2p = take(p.dw ? (size_t)L.rows_pad * L.dcb * 32 * L.np : 0);
+    L.wp = take((size_t)L.v_pad * L.dcb * 32 * L.np);
+    L.w_part = take(W_BLOCKS * 4);
+    L.f = take(L.rows_pad * 4);
+    L.tgt = take(L.rows_pad * 4);
+    L.g = take(L.rows_pad * 4);
+    L.gmax = take(L.rows_pad / 32 * 4);
+    L.kw = take(4);
+    L.part_m = take((size_t)L.v_tiles * L.rows_pad * 4);
+    L.part_s = take((size_t)L.v_tiles * L.rows_pad * 4);
+    L.ztgt = take(L.rows_pad * 4);
+    L.lse = take(L.rows_pad * 4);
+    L.q = take(L.rows_pad * 4);
+    L.e_dx = take(L.rows_pad * 4);
+    L.e_dw = take(4);
+    if (grads) {
+        const long nbn = (p.d + L.bn - 1) / L.bn;
+        L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
+        if (p.dx) {
+            const long tiles = L.rows_pad / 128 * nbn;
+            split_k(L.piece, (SLOTS + tiles - 1) / tiles, &L.dx_split, &L.dx_ks);
+            L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
+        }
+        if (p.dw) {
+            const long tiles = L.piece / 128 * nbn;
+            split_k(round_up(p.rows, 32), tiles >= SLOTS / 2 ? 1 : SLOTS / tiles, &L.dw_split, &L.dw_ks);
+            if (L.dw_split > 1) L.dw_part = take((size_t)L.dw_split * L.piece * p.d * 4);
+        }
+        if (p.db) L.db_part = take((size_t)(L.rows_pad / L.tn) * L.v_pad * 4);
+    }
     L.bytes = at;
     return L;
 }
 
+template <int MODE, typename T, int NP>
+void launch_logits(const LossGemm &g, int tn, hipStream_t st) {
+    const unsigned grid = (unsigned)(g.nM * g.nN);
+    if (tn == 128)
+        k_loss_gemm<MODE, T, NP, 2, 4, 4, 1, false, false><<<grid, NT, 0, st>>>(g);
+    else if (tn == 64)
+        k_loss_gemm<MODE, T, NP, 2, 2, 4, 1, false, false><<<grid, NT, 0, st>>>(g);
+    else
+        k_loss_gemm<MODE, T, NP, 2, 1, 4, 1, false, false><<<grid, NT, 0, st>>>(g);
+}
+
+template <typename T, int NP, bool TRA>
+void launch_grad(const LossGemm &g, int bn, hipStream_t st) {
+    const unsigned grid = (unsigned)(g.nM * g.nN * g.S);
+    if (bn == 256)
+        k_loss_gemm<GRAD, T, NP, 2, 4, 2, 2, TRA, true><<<grid, NT, 0, st>>>(g);
+    else if (bn == 128)
+        k_loss_gemm<GRAD, T, NP, 2, 2, 2, 2, TRA, true><<<grid, NT, 0, st>>>(g);
+    else
+        k_loss_gemm<GRAD, T, NP, 1, 2, 4, 1, TRA, true><<<grid, NT, 0, st>>>(g);
+}
+
+template <typename T, int NP>
+void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) {
+    const int eb = elem_bytes(p.dtype);
+    // rows of whole 16-byte pieces are loaded 8 values at a time (the tail of a row by itself)
+    const bool vx = (uintptr_t)p.x % 16 == 0 && p.x_stride * eb % 16 == 0;
+    const bool vw = (uintptr_t)p.w % 16 == 0 && p.w_stride * eb % 16 == 0;
+    Prep r{};
+    r.x = p.x, r.x_stride = p.x_stride, r.w = p.w, r.w_stride = p.w_stride;
+    r.rows = p.rows, r.d = p.d, r.vocab = p.vocab, r.dcb = L.dcb, r.w_blocks = L.w_blocks;
+    r.targets = p.targets, r.dloss = p.dloss, r.err = p.err;
+    r.xp = (_Float16 *)(ws + L.xp), r.x2p = p.dw ? (_Float16 *)(ws + L.x2p) : nullptr, r.wp = (_Float16 *)(ws + L.wp);
+    r.x_plane = L.rows_pad * L.dcb * 16, r.w_plane = L.v_pad * L.dcb * 16;
+    r.w_part = (float *)(ws + L.w_part);
+    r.f = (int32_t *)(ws + L.f), r.tgt = (int32_t *)(ws + L.tgt);
+    r.g = (float *)(ws + L.g), r.gmax = (float *)(ws + L.gmax);
+    r.kw = (int32_t *)(ws + L.kw);
+    const int row_blocks = (int)(L.rows_pad / 32);
+    const unsigned prep_grid = (unsigned)(L.w_blocks + row_blocks), split_grid = (unsigned)(L.v_pad / 32);
+    if (vx && vw)
+        k_loss_prep<T, NP, true, true><<<prep_grid, NT, 0, st>>>(r);
+    else if (vx)
+        k_loss_prep<T, NP, true, false><<<prep_grid, NT, 0, st>>>(r);
+    else if (vw)
+        k_loss_prep<T, NP, false, true><<<prep_grid, NT, 0, st>>>(r);
+    else
+        k_loss_prep<T, NP, false, false><<<prep_grid, NT, 0, st>>>(r);
+    if (vw)
+        k_loss_split_w<T, NP, true><<<split_grid, NT, 0, st>>>(r);
+    else
+        k_loss_split_w<T, NP, false><<<split_grid, NT, 0, st>>>(r);
+
+    const Planes X{r.xp, r.x_plane, L.dcb}, X2{r.x2p, r.x_plane, L.dcb}, W{r.wp, r.w_plane, L.dcb};
+    LossGemm z{};
+    z.A = W, z.B = X;
+    z.nM = L.v_tiles, z.nN = (int)(round_up(p.rows, L.tn) / L.tn), z.S = 1;
+    z.K = z.Ks = L.dcb * 16;
+    z.bias = p.bias, z.f = r.f, z.tgt = r.tgt, z.kw_dev = r.kw;
+    z.vocab = p.vocab, z.rows = p.rows, z.rows_pad = L.rows_pad;
+    z.part_m = (float *)(ws + L.part_m), z.part_s = (float *)(ws + L.part_s), z.ztgt = (float *)(ws + L.ztgt);
+    launch_logits<LOGITS_STATS, T, NP>(z, L.tn, st);
+
+    Rows q{};
+    q.tiles = L.v_tiles, q.row_blocks = row_blocks, q.rows_pad = L.rows_pad;
+    q.part_m = z.part_m, q.part_s = z.part_s, q.ztgt = z.ztgt;
+    q.lse = (float *)(ws + L.lse), q.q = (float *)(ws + L.q);
+    q.e_dx = (int32_t *)(ws + L.e_dx), q.e_dw = (int32_t *)(ws + L.e_dw);
+    q.out_loss = p.loss, q.out_lse = p.lse;
+    const unsigned rows_grid = (unsigned)(round_up(p.rows, L.tn) / 32);
+    if (vx)
+        k_loss_rows<T, NP, true><<<rows_grid, NT, 0, st>>>(q, r);
+    else
+        k_loss_rows<T, NP, false><<<rows_grid, NT, 0, st>>>(q, r);
+    if (!p.dx && !p.dw && !p.db) return;
+
+    z.lse = q.lse, z.q = q.q, z.g = r.g;
+    z.dz = (_Float16 *)(ws + L.dz), z.dz_plane = L.rows_pad * L.piece, z.dz_ncb = L.piece / 16;
+    z.db_part = p.db ? (float *)(ws + L.db_part) : nullptr, z.db_ld = L.v_pad;
+    const int nbn = (p.d + L.bn - 1) / L.bn;
+    for (long v0 = 0; v0 < L.v_pad; v0 += L.piece) {
+        const int n = (int)std::min<long>(L.piece, L.v_pad - v0);  // entries of the piece, padded
+        const Planes DZ{z.dz, z.dz_plane, z.dz_ncb};
+        z.a_row0 = (int)v0;
+        z.nM = n / TV;
+        launch_logits<LOGITS_DZ, T, NP>(z, L.tn, st);
+        if (p.dx) {
+            LossGemm g{};
+            g.A = DZ, g.B = W;
+            g.B.p += v0 / 32 * (long)W.ncb * 512;
+            g.nM = (int)(L.rows_pad / 128), g.nN = nbn, g.S = (n + L.dx_ks - 1) / L.dx_ks;
+            g.K = n, g.Ks = L.dx_ks;
+            g.part = (float *)(ws + L.dx_part), g.part_ld = p.d, g.add = v0 > 0;
+            g.out_rows = p.rows, g.out_cols = p.d;
+            launch_grad<T, NP, false>(g, L.bn, st);
+        }
+        if (p.dw) {
+            const int live = (int)std::min<long>(n, p.vocab - v0);
+            LossGemm g{};
+            g.A = DZ, g.B = X2;
+            g.nM = n / 128, g.nN = nbn, g.S = L.dw_split;
+            g.K = (int)round_up(p.rows, 32), g.Ks = L.dw_ks;
+            g.out_rows = live, g.out_cols = p.d;
+            T *dst = (T *)p.dw + v0 * p.dw_stride;
+            if (L.dw_split > 1)
+                g.part = (float *)(ws + L.dw_part), g.part_ld = p.d;
+            else
+                g.dst = dst, g.dst_stride = p.dw_stride, g.e_all = q.e_dw;
+            launch_grad<T, NP, true>(g, L.bn, st);
+            if (L.dw_split > 1)
+                k_loss_join<T><<<(unsigned)std::min<long>(2048, ((long)live * p.d + NT - 1) / NT), NT, 0, st>>>(
+                    g.part, L.dw_split, live, p.d, dst, p.dw_stride, nullptr, q.e_dw);
+        }
+    }
+    if (p.dx)
+        k_loss_join<T><<<(unsigned)std::min<long>(2048, ((long)p.rows * p.d + NT - 1) / NT), NT, 0, st>>>(
+            (float *)(ws + L.dx_part), L.dx_split, p.rows, p.d, (T *)p.dx, p.dx_stride, q.e_dx, nullptr);
+    if (p.db) k_loss_db<<<(p.vocab + NT - 1) / NT, NT, 0, st>>>(z.db_part, z.nN, z.db_ld, p.vocab, p.db);
+}
+
 }  // namespace
 
-size_t loss_workspace_bytes(const LossParams &p) { return loss_layout(p).bytes; }
+size_t loss_workspace_bytes(const LossParams &p) { return p.rows ? loss_plan(p).bytes : 0; }
 
-void launch_loss(const LossParams &q, void *ws, hipStream_t st) {
-    LossParams p = q;
-    const LossLayout L = loss_layout(p);
-    char *w8 = (char *)ws;
-    float *z = (float *)(w8 + L.z), *stat = (float *)(w8 + L.stat), *dxa = (float *)(w8 + L.dx);
-    if (!p.lse) p.lse = (float *)(w8 + L.lse);
+void launch_loss(const LossParams &p, void *ws, hipStream_t st) {
     dispatch_type(p.dtype, [&](auto ty) {
         typedef decltype(ty) T;
-        const T *x = (const T *)p.x, *w = (const T *)p.w;
-        for (int pass = 0; pass < (p.dx || p.dw || p.db ? 2 : 1); ++pass)
-            for (int v0 = 0; v0 < p.vocab; v0 += L.piece) {
-                const int n = std::min(L.piece, p.vocab - v0);
-                if (p.rows) {
-                    tile_product<T, T, float>(x, p.x_stride, 1, w + (long)v0 * p.w_stride, p.w_stride, 1, z, n, p.rows, n,
-                                              p.d, p.bias ? p.bias + v0 : nullptr, false, st);
-                    if (pass == 0) {
-                        k_merge<<<p.rows, NT, 0, st>>>(p, z, v0, n, stat, v0 + n == p.vocab);
-                        continue;
-                    }
-                    k_dz<<<p.rows, NT, 0, st>>>(p, z, v0, n);
-                }
-                if (pass == 0) continue;
-                if (p.dx && p.rows)
-                    tile_product<float, T, float>(z, n, 1, w + (long)v0 * p.w_stride, 1, p.w_stride, dxa, p.d, p.rows,
-                                                  p.d, n, nullptr, v0 > 0, st);
-                if (p.dw)
-                    tile_product<float, T, T>(z, 1, n, x, 1, p.x_stride, (T *)p.dw + (long)v0 * p.dw_stride, p.dw_stride,
-                                              n, p.d, p.rows, nullptr, false, st, p.targets);
-                if (p.db) k_col_sums<<<(n + NT - 1) / NT, NT, 0, st>>>(z, p.rows, n, p.db + v0);
-            }
-        if (p.dx && p.rows) k_round_rows<T><<<p.rows, NT, 0, st>>>(dxa, p.rows, p.d, (T *)p.dx, p.dx_stride);
+        if (p.rows == 0) {  // no row: the sums over the rows are zero
+            if (p.dw) k_loss_zero<T><<<2048, NT, 0, st>>>((T *)p.dw, p.vocab, p.d, p.dw_stride);
+            if (p.db) k_loss_zero<float><<<256, NT, 0, st>>>(p.db, 1, p.vocab, p.vocab);
+            return;
+        }
+        run_loss<T, std::is_same<T, float>::value ? 2 : 1>(p, loss_plan(p), (char *)ws, st);
     });
 }
 

@@ -2000,6 +2000,7 @@ int train_launch(adn_ctx *c, size_t bytes, F &&f) {
         f(ws);
         ADN_HIP(hipGetLastError());
     } catch (const HipError &e) {
+        (void)hipGetLastError();  // a refused allocation is not the next call's error
         return hip_fail(e);
     } catch (const std::exception &e) {
         return fail(ADN_E_HIP, e.what());
