@@ -43,7 +43,6 @@ using gemm::lds_barrier;
 constexpr int NT = 256;             // threads a workgroup: 4 waves
 constexpr size_t PIECE_BYTES = 256u << 20;
 constexpr int TV = 256;             // entries a workgroup of the logits' product covers
-constexpr int STAGES = 3;           // k slices of the LDS ring
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int W_BLOCKS = 1024;      // blocks of the pass over |W|, one partial each
 
@@ -57,6 +56,17 @@ template <int N>
 __device__ __forceinline__ void wait_vmcnt() {  // the other counters left alone
     static_assert(N >= 0 && N < 64, "vmcnt range");
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// 16 bytes a lane from base + off (base wave-uniform, off in bytes) to the LDS address `lds` + 16 lane.
+// In assembly so that the compiler does not take the transposing LDS reads for uses of it and wait for
+// every load in flight before each: the waits are wait_vmcnt's.  It has no register output; one wait
+// state lies between the write of m0 and its use.
+__device__ __forceinline__ void load_lds(const void *base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base)
+                 : "memory", "m0");
 }
 
 // Chunk (8 halves) of a block's row r that holds columns [0, 8) in the LDS image of an operand read
@@ -96,55 +106,69 @@ struct LossGemm {
     float *part;                        // [share][rows][ld] partial sums, or null: dst is written
     long part_ld;
     int add;                            // the partial sums are added to
-    void *dst;
+    void *dst;                          // [rows] of the result
     long dst_stride;
     int out_rows, out_cols;
-    const int32_t *e_row;               // exponent of a row's result (dx), or null: *e_all
-    const int32_t *e_all;
+    const int32_t *e_all;               // exponent of dst's values
 };
 
 enum { LOGITS_STATS = 0, LOGITS_DZ = 1, GRAD = 2 };
+
+// The two gradients of a piece in one launch: tiles of the one with the longer shares first.
+struct LossGrads {
+    LossGemm dw, dx;
+    int first;     // workgroups of the first gradient
+    int dx_first;
+};
 
 // One tile: WGM x WGN waves of WTM x WTN MFMA tiles of 32x32.  NP planes an operand; a k slice is
 // 16 KB values (24 KB of LDS for either NP at the largest tile: three slices and two workgroups a
 // CU, so that one's epilogue runs under the other's MFMAs).  TRA / TRB: the operand's rows are the
 // product's K.
+template <int NP, int WTM, int WTN, int WGM, int WGN>
+struct Tile {
+    static constexpr int KB = NP == 2 ? 1 : 2;
+    static constexpr int TM = WGM * WTM * 32, TN = WGN * WTN * 32;
+    static constexpr int A_BLK = TM / 32 * KB, B_BLK = TN / 32 * KB;  // 1 KB loads a plane and slice
+    static constexpr int NW = WGM * WGN;                              // waves
+    static constexpr int STAGES = NW == 8 ? 4 : 3;                    // slices of the LDS ring
+    static constexpr int RING = STAGES * NP * (A_BLK + B_BLK) * 512;  // halves
+    static_assert(RING * 2 <= (NW == 8 ? 160 : 80) * 1024, "one workgroup of 8 waves a CU, or two of 4");
+};
+
 template <int MODE, typename T, int NP, int WTM, int WTN, int WGM, int WGN, bool TRA, bool TRB>
-__global__ __launch_bounds__(NT, 2) void k_loss_gemm(LossGemm p) {
-    static_assert(WGM * WGN == 4, "four waves");
-    constexpr int KB = NP == 2 ? 1 : 2;
-    constexpr int TM = WGM * WTM * 32, TN = WGN * WTN * 32;
-    constexpr int A_BLK = TM / 32 * KB, B_BLK = TN / 32 * KB;  // 1 KB loads a plane and slice
-    constexpr int A_PW = (A_BLK + 3) / 4, B_PW = (B_BLK + 3) / 4;
+__device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *ring) {
+    typedef Tile<NP, WTM, WTN, WGM, WGN> G;
+    constexpr int KB = G::KB, TM = G::TM, TN = G::TN, A_BLK = G::A_BLK, B_BLK = G::B_BLK, NW = G::NW,
+                  STAGES = G::STAGES;
+    constexpr int A_PW = (A_BLK + NW - 1) / NW, B_PW = (B_BLK + NW - 1) / NW;
     constexpr int LOADS = NP * (A_PW + B_PW);
     constexpr int A_SZ = A_BLK * 512, B_SZ = B_BLK * 512;      // halves a plane and slice
     constexpr int SLICE = NP * (A_SZ + B_SZ);
-    __shared__ __attribute__((aligned(1024))) _Float16 ring[STAGES * SLICE];
-    static_assert(STAGES * SLICE * 2 <= 80 * 1024, "two workgroups a CU");
-
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
     const int r = lane & 31, hh = lane >> 5;
     int s, mt, nt;
-    gemm::map_block(blockIdx.x, p.nM * p.nN * p.S, p.nM, p.nN, s, mt, nt);
+    gemm::map_block(bid, p.nM * p.nN * p.S, p.nM, p.nN, s, mt, nt);
     const int k0 = s * p.Ks;
     const int nk = (min(p.Ks, p.K - k0)) / (16 * KB);
 
-    // this wave's loads of a slice: per-lane source offsets (halves) at slice 0
-    long asrc[A_PW], bsrc[B_PW];
+    // Direct global->LDS loads of a slice.  A load's address is a wave-uniform base plus a byte offset of
+    // the lane that is the same for every load of an operand.
+    auto lane_off = [&](bool tr) -> unsigned {
+        if (!tr) return (lane >> 1) * 32 + (((lane & 1) ^ swz(lane >> 1)) * 16);  // a block, its rows' chunks swizzled
+        // rows k of odd column blocks stand at k ^ 4, so that the two 128-byte pieces that 32 lanes
+        // read at once (4 rows of neighbouring column blocks) are in different halves of the banks
+        if constexpr (KB == 2) return (lane ^ ((wave & 1) * 8)) * 16;             // a block of 32 k x 16 columns
+        return (lane >> 5) * 1024 + ((lane & 31) ^ ((lane >> 5) * 8)) * 16;       // 16 k of two neighbouring blocks
+    };
+    // base of load idx at slice 0, in halves
     auto src_of = [&](bool tr, int idx, int tile0, const Planes &P) -> long {
-        if (!tr) {  // block (row block, k block)
-            const int rb = idx / KB, kb = idx % KB, row = lane >> 1;
-            return ((long)(tile0 / 32 + rb) * P.ncb + k0 / 16 + kb) * 512 + row * 16 + (((lane & 1) ^ swz(row)) * 8);
-        }
-        if constexpr (KB == 2) {  // whole blocks of 32 k x 16 columns
-            const int cb = min(tile0 / 16 + idx, P.ncb - 1);
-            return ((long)(k0 / 32) * P.ncb + cb) * 512 + lane * 8;
-        } else {  // halves (16 k) of two neighbouring blocks
-            const int cb = min(tile0 / 16 + 2 * idx + (lane >> 5), P.ncb - 1);
-            return (long)cb * 512 + (lane & 31) * 8;  // the k block and half: step_of
-        }
+        if (!tr) return ((long)(tile0 / 32 + idx / KB) * P.ncb + k0 / 16 + idx % KB) * 512;  // (row block, k block)
+        // columns past the matrix (a multiple of 32 wide) read its last blocks: outputs that are not stored
+        if constexpr (KB == 2) return ((long)(k0 / 32) * P.ncb + min(tile0 / 16 + idx, P.ncb - 2 + (idx & 1))) * 512;
+        return (long)min(tile0 / 16 + 2 * idx, P.ncb - 2) * 512;  // the k block and half: step_of
     };
     // slice kt's offset from slice 0
     auto step_of = [&](bool tr, int kt, const Planes &P) -> long {
@@ -153,35 +177,36 @@ __global__ __launch_bounds__(NT, 2) void k_loss_gemm(LossGemm p) {
         const int k = k0 / 16 + kt;
         return (long)(k >> 1) * P.ncb * 512 + (k & 1) * 256;
     };
-    // tr operands of whole blocks: TM / 16 loads; of half blocks: two blocks a load -- A_BLK in both
+    // a plane's slice of the tile is A_BLK (B_BLK) KB in either order; where the waves outnumber its
+    // loads some are issued twice, to the same place
+    long asrc[A_PW], bsrc[B_PW];
 #pragma unroll
-    for (int j = 0; j < A_PW; ++j) asrc[j] = src_of(TRA, (wave + 4 * j) % A_BLK, p.a_row0 + mt * TM, p.A);
+    for (int j = 0; j < A_PW; ++j) asrc[j] = src_of(TRA, (wave + NW * j) % A_BLK, p.a_row0 + mt * TM, p.A);
 #pragma unroll
-    for (int j = 0; j < B_PW; ++j) bsrc[j] = src_of(TRB, (wave + 4 * j) % B_BLK, nt * TN, p.B);
-    const _Float16 *Ap = p.A.p, *Bp = p.B.p;
+    for (int j = 0; j < B_PW; ++j) bsrc[j] = src_of(TRB, (wave + NW * j) % B_BLK, nt * TN, p.B);
+    const unsigned aoff = lane_off(TRA), boff = lane_off(TRB);
+    const unsigned ring0 = (unsigned)(uintptr_t)(lds_void *)ring;
     auto issue = [&](int kt) {
-        _Float16 *base = ring + (kt % STAGES) * SLICE;
-        const long sa = step_of(TRA, kt, p.A), sb = step_of(TRB, kt, p.B);
+        const unsigned base = ring0 + (kt % STAGES) * (SLICE * 2);
+        const _Float16 *Ap = p.A.p + step_of(TRA, kt, p.A), *Bp = p.B.p + step_of(TRB, kt, p.B);
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
 #pragma unroll
             for (int j = 0; j < A_PW; ++j)
-                __builtin_amdgcn_global_load_lds((const void *)(Ap + q * p.A.plane + asrc[j] + sa),
-                                                 (lds_void *)(base + q * A_SZ + ((wave + 4 * j) % A_BLK) * 512), 16, 0, 0);
+                load_lds(Ap + q * p.A.plane + asrc[j], aoff, base + (q * A_SZ + ((wave + NW * j) % A_BLK) * 512) * 2);
 #pragma unroll
             for (int j = 0; j < B_PW; ++j)
-                __builtin_amdgcn_global_load_lds((const void *)(Bp + q * p.B.plane + bsrc[j] + sb),
-                                                 (lds_void *)(base + NP * A_SZ + q * B_SZ + ((wave + 4 * j) % B_BLK) * 512),
-                                                 16, 0, 0);
+                load_lds(Bp + q * p.B.plane + bsrc[j], boff,
+                         base + (NP * A_SZ + q * B_SZ + ((wave + NW * j) % B_BLK) * 512) * 2);
         }
     };
     // MFMA operand of 32 rows (columns) `t` of the tile, k block kb of the slice
     auto frag = [&](const _Float16 *img, bool tr, int t, int kb) -> half8 {
         if (!tr) return *reinterpret_cast<const half8 *>(img + (t * KB + kb) * 512 + r * 16 + ((hh ^ swz(r)) * 8));
-        const _Float16 *a = img + (2 * t + ((lane >> 4) & 1)) * (KB * 256) + (kb * 16 + 8 * hh + ((lane >> 2) & 3)) * 16 +
-                            (lane & 3) * 4;
-        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)a);
-        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(a + 64));
+        const int odd = (lane >> 4) & 1;
+        const int at = (2 * t + odd) * (KB * 256) + (kb * 16 + 8 * hh + ((lane >> 2) & 3) + 4 * odd) * 16 + (lane & 3) * 4;
+        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(img + at));
+        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(img + (at ^ 64)));
         return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
@@ -234,25 +259,47 @@ __global__ __launch_bounds__(NT, 2) void k_loss_gemm(LossGemm p) {
     // Output layout of a 32x32 tile: lane holds column r; register e row 8 (e / 4) + 4 hh + e % 4.
     if constexpr (MODE == GRAD) {
         const int ec = p.e_all ? *p.e_all : 0;
+        const long r0 = (long)mt * TM + wm * WTM * 32 + 4 * hh;
+        const int c0 = nt * TN + wn * WTN * 32 + r;
+        auto store = [&](auto whole) {
+            constexpr bool W = decltype(whole)::value;  // an interior tile: nothing to check
 #pragma unroll
-        for (int i = 0; i < WTM; ++i)
+            for (int i = 0; i < WTM; ++i) {
+                auto in = [&](int rr, int j) { return W || (r0 + i * 32 + rr < p.out_rows && c0 + 32 * j < p.out_cols); };
+                if (p.part) {
+                    float *o = p.part + ((long)s * p.out_rows + r0 + i * 32) * p.part_ld + c0;
+                    if (p.add) {  // the earlier sums of 32 rows are loaded before the first store
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const long row = (long)mt * TM + (wm * WTM + i) * 32 + 8 * (e / 4) + 4 * hh + e % 4;
-                if (row >= p.out_rows) continue;
-                const int ex = p.part ? 0 : ec + (p.e_row ? p.e_row[row] : 0);
+                        for (int e = 0; e < 16; ++e)
 #pragma unroll
-                for (int j = 0; j < WTN; ++j) {
-                    const int col = nt * TN + (wn * WTN + j) * 32 + r;
-                    if (col >= p.out_cols) continue;
-                    if (p.part) {
-                        float *o = p.part + ((long)s * p.out_rows + row) * p.part_ld + col;
-                        *o = p.add ? *o + acc[i][j][e] : acc[i][j][e];
-                    } else {
-                        ((T *)p.dst)[row * p.dst_stride + col] = from_f32<T>(ldexpf(acc[i][j][e], ex));
+                            for (int j = 0; j < WTN; ++j) {
+                                const int rr = 8 * (e / 4) + e % 4;
+                                if (in(rr, j)) acc[i][j][e] += o[rr * p.part_ld + 32 * j];
+                            }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+#pragma unroll
+                        for (int j = 0; j < WTN; ++j) {
+                            const int rr = 8 * (e / 4) + e % 4;
+                            if (in(rr, j)) o[rr * p.part_ld + 32 * j] = acc[i][j][e];
+                        }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int rr = 8 * (e / 4) + e % 4;
+                        T *o = (T *)p.dst + (r0 + i * 32 + rr) * p.dst_stride + c0;
+#pragma unroll
+                        for (int j = 0; j < WTN; ++j)
+                            if (in(rr, j)) o[32 * j] = from_f32<T>(ldexpf(acc[i][j][e], ec));
                     }
                 }
             }
+        };
+        if ((long)mt * TM + TM <= p.out_rows && nt * TN + TN <= p.out_cols)
+            store(std::integral_constant<bool, true>{});
+        else
+            store(std::integral_constant<bool, false>{});
     } else {
         static_assert(MODE == GRAD || (TM == TV && WGN == 1), "a wave's columns are the tile's");
         // the tile's biases; entries beyond the vocabulary get -inf: no part of any sum.  From here on
@@ -396,6 +443,22 @@ __global__ __launch_bounds__(NT, 2) void k_loss_gemm(LossGemm p) {
             }
         }
     }
+}
+
+template <int MODE, typename T, int NP, int WTN>
+__global__ __launch_bounds__(NT, 2) void k_loss_logits(LossGemm p) {
+    __shared__ __attribute__((aligned(1024))) _Float16 ring[Tile<NP, 2, WTN, 4, 1>::RING];
+    loss_tile<MODE, T, NP, 2, WTN, 4, 1, false, false>(p, blockIdx.x, ring);
+}
+
+template <typename T, int NP, int WTM, int WTN, int WGM, int WGN>
+__global__ __launch_bounds__(64 * WGM * WGN, WGM * WGN == 8 ? 1 : 2) void k_loss_grads(LossGrads p) {
+    __shared__ __attribute__((aligned(1024))) _Float16 ring[Tile<NP, WTM, WTN, WGM, WGN>::RING];
+    const int b = blockIdx.x;
+    if ((b < p.first) == (p.dx_first != 0))
+        loss_tile<GRAD, T, NP, WTM, WTN, WGM, WGN, false, true>(p.dx, p.dx_first ? b : b - p.first, ring);
+    else
+        loss_tile<GRAD, T, NP, WTM, WTN, WGM, WGN, true, true>(p.dw, p.dx_first ? b - p.first : b, ring);
 }
 
 // ---- operands ------------------------------------------------------------------------------
@@ -668,16 +731,50 @@ struct LossPlan {
     int v_tiles;             // tiles of TV entries
     int piece;               // entries a piece, a multiple of TV
     int w_blocks;
-    int bn;                  // columns of a gradient tile
-    int dx_tiles, dx_split, dx_ks, dw_split, dw_ks;
+    int bm, bn;              // rows and columns of a gradient tile
+    int dx_split, dx_ks, dw_split, dw_ks;
     size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, q, e_dx, e_dw, dz, dx_part, dw_part, db_part, bytes;
 };
 
-// K of `len` (a multiple of 32) in at most `want` shares of whole 32s, each of 256 values at least
+// K of `len` (a multiple of 32) in at most `want` shares of whole 32s
 void split_k(long len, long want, int *split, int *share) {
-    long s = std::max<long>(1, std::min(want, len / 256));
-    *share = (int)round_up((len + s - 1) / s, 32);
+    *share = (int)round_up((len + want - 1) / want, 32);
     *split = (int)((len + *share - 1) / *share);
+}
+
+// Time of n1 units of length a and then n2 of length b (a >= b) on SLOTS slots, in order.
+double makespan(long n1, double a, long n2, double b, long SLOTS) {
+    const long full = n1 / SLOTS, m1 = n1 % SLOTS, free = SLOTS - m1;
+    const long fit = m1 ? free * (long)(a / b) : 0;  // units of b done beside the last a's
+    double t = full * a;
+    if (n2 <= fit) return t + std::max(m1 ? a : 0.0, (double)((n2 + free - 1) / free) * b);
+    return t + (m1 ? a : 0.0) + (double)((n2 - fit + SLOTS - 1) / SLOTS) * b;
+}
+
+// Shares of the two gradients' K: the pair with the shortest estimated time of their common launch.  A
+// unit is its K plus EPI for its prologue and epilogue (stores of a tile: as long as about 200 values of
+// K), and each share's partial sums pass through memory twice more (JOIN a tile, all slots at once).
+void pick_splits(long slots, long dx_tiles, long dx_k, long dw_tiles, long dw_k, int *dx_split, int *dx_ks,
+                 int *dw_split, int *dw_ks) {
+    constexpr double EPI = 200, JOIN = 250;
+    double best = INFINITY;
+    const long most_dx = dx_tiles ? std::max<long>(1, std::min<long>(64, dx_k / 256)) : 1;
+    const long most_dw = dw_tiles ? std::max<long>(1, std::min<long>(16, dw_k / 256)) : 1;
+    for (long sx = 1; sx <= most_dx; ++sx)
+        for (long sw = 1; sw <= most_dw; ++sw) {
+            int nx = 0, kx = 32, nw = 0, kw = 32;
+            if (dx_tiles) split_k(dx_k, sx, &nx, &kx);
+            if (dw_tiles) split_k(dw_k, sw, &nw, &kw);
+            const double a = kx + EPI, b = kw + EPI;
+            double t = a >= b ? makespan(dx_tiles * nx, a, dw_tiles * nw, b, slots)
+                              : makespan(dw_tiles * nw, b, dx_tiles * nx, a, slots);
+            t += JOIN * (dx_tiles * nx + (nw > 1 ? dw_tiles * nw : 0)) / slots;
+            if (t < best) {
+                best = t;
+                if (dx_tiles) *dx_split = nx, *dx_ks = kx;
+                if (dw_tiles) *dw_split = nw, *dw_ks = kw;
+            }
+        }
 }
 
 LossPlan loss_plan(const LossParams &p) {
@@ -686,7 +783,7 @@ LossPlan loss_plan(const LossParams &p) {
     L.np = p.dtype == ADN_T_F32 ? 2 : 1;
     L.tn = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
     L.dcb = (int)(round_up(p.d, 32) / 16);
-    L.rows_pad = round_up(p.rows, 128);
+    L.rows_pad = round_up(p.rows, 256);
     L.v_pad = round_up(p.vocab, TV);
     L.v_tiles = (int)(L.v_pad / TV);
     const long fit = (long)(PIECE_BYTES / (L.np * 2)) / L.rows_pad / TV * TV;
@@ -694,6 +791,7 @@ LossPlan loss_plan(const LossParams &p) {
     L.piece = (int)round_up((L.v_pad + npieces - 1) / npieces, TV);
     L.w_blocks = (int)std::min<long>(W_BLOCKS, ((long)p.vocab * ((p.d + 7) / 8) + NT * 4 - 1) / (NT * 4));
     L.bn = p.d > 128 ? 256 : p.d > 64 ? 128 : 64;
+    L.bm = L.bn == 256 && getenv("BM") ? atoi(getenv("BM")) : 128;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -719,16 +817,11 @@ LossPlan loss_plan(const LossParams &p) {
     if (grads) {
         const long nbn = (p.d + L.bn - 1) / L.bn;
         L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
-        if (p.dx) {
-            const long tiles = L.rows_pad / 128 * nbn;
-            split_k(L.piece, (SLOTS + tiles - 1) / tiles, &L.dx_split, &L.dx_ks);
-            L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
-        }
-        if (p.dw) {
-            const long tiles = L.piece / 128 * nbn;
-            split_k(round_up(p.rows, 32), tiles >= SLOTS / 2 ? 1 : SLOTS / tiles, &L.dw_split, &L.dw_ks);
-            if (L.dw_split > 1) L.dw_part = take((size_t)L.dw_split * L.piece * p.d * 4);
-        }
+        pick_splits(L.bm == 256 ? SLOTS / 2 : SLOTS, p.dx ? round_up(p.rows, L.bm) / L.bm * nbn : 0, L.piece,
+                    p.dw ? round_up(std::min<long>(L.piece, p.vocab), L.bm) / L.bm * nbn : 0,
+                    round_up(p.rows, 32), &L.dx_split, &L.dx_ks, &L.dw_split, &L.dw_ks);
+        if (p.dx) L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
+        if (p.dw && L.dw_split > 1) L.dw_part = take((size_t)L.dw_split * L.piece * p.d * 4);
         if (p.db) L.db_part = take((size_t)(L.rows_pad / L.tn) * L.v_pad * 4);
     }
     L.bytes = at;
@@ -739,22 +832,27 @@ template <int MODE, typename T, int NP>
 void launch_logits(const LossGemm &g, int tn, hipStream_t st) {
     const unsigned grid = (unsigned)(g.nM * g.nN);
     if (tn == 128)
-        k_loss_gemm<MODE, T, NP, 2, 4, 4, 1, false, false><<<grid, NT, 0, st>>>(g);
+        k_loss_logits<MODE, T, NP, 4><<<grid, NT, 0, st>>>(g);
     else if (tn == 64)
-        k_loss_gemm<MODE, T, NP, 2, 2, 4, 1, false, false><<<grid, NT, 0, st>>>(g);
+        k_loss_logits<MODE, T, NP, 2><<<grid, NT, 0, st>>>(g);
     else
-        k_loss_gemm<MODE, T, NP, 2, 1, 4, 1, false, false><<<grid, NT, 0, st>>>(g);
+        k_loss_logits<MODE, T, NP, 1><<<grid, NT, 0, st>>>(g);
 }
 
-template <typename T, int NP, bool TRA>
-void launch_grad(const LossGemm &g, int bn, hipStream_t st) {
-    const unsigned grid = (unsigned)(g.nM * g.nN * g.S);
-    if (bn == 256)
-        k_loss_gemm<GRAD, T, NP, 2, 4, 2, 2, TRA, true><<<grid, NT, 0, st>>>(g);
+template <typename T, int NP>
+void launch_grads(LossGrads &g, int bm, int bn, hipStream_t st) {
+    const int ndx = g.dx.nM * g.dx.nN * g.dx.S, ndw = g.dw.nM * g.dw.nN * g.dw.S;  // 0: not wanted
+    g.dx_first = ndx && (!ndw || g.dx.Ks >= g.dw.Ks);
+    g.first = g.dx_first ? ndx : ndw;
+    const unsigned grid = (unsigned)(ndx + ndw);
+    if (bm == 256)
+        k_loss_grads<T, NP, 2, 4, 4, 2><<<grid, 2 * NT, 0, st>>>(g);
+    else if (bn == 256)
+        k_loss_grads<T, NP, 2, 4, 2, 2><<<grid, NT, 0, st>>>(g);
     else if (bn == 128)
-        k_loss_gemm<GRAD, T, NP, 2, 2, 2, 2, TRA, true><<<grid, NT, 0, st>>>(g);
+        k_loss_grads<T, NP, 2, 2, 2, 2><<<grid, NT, 0, st>>>(g);
     else
-        k_loss_gemm<GRAD, T, NP, 1, 2, 4, 1, TRA, true><<<grid, NT, 0, st>>>(g);
+        k_loss_grads<T, NP, 1, 2, 4, 1><<<grid, NT, 0, st>>>(g);
 }
 
 template <typename T, int NP>
@@ -821,33 +919,33 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         z.a_row0 = (int)v0;
         z.nM = n / TV;
         launch_logits<LOGITS_DZ, T, NP>(z, L.tn, st);
+        const int live = (int)std::min<long>(n, p.vocab - v0);
+        T *dst = p.dw ? (T *)p.dw + v0 * p.dw_stride : nullptr;
+        LossGrads g{};
         if (p.dx) {
-            LossGemm g{};
-            g.A = DZ, g.B = W;
-            g.B.p += v0 / 32 * (long)W.ncb * 512;
-            g.nM = (int)(L.rows_pad / 128), g.nN = nbn, g.S = (n + L.dx_ks - 1) / L.dx_ks;
-            g.K = n, g.Ks = L.dx_ks;
-            g.part = (float *)(ws + L.dx_part), g.part_ld = p.d, g.add = v0 > 0;
-            g.out_rows = p.rows, g.out_cols = p.d;
-            launch_grad<T, NP, false>(g, L.bn, st);
+            LossGemm &x = g.dx;
+            x.A = DZ, x.B = W;
+            x.B.p += v0 / 32 * (long)W.ncb * 512;
+            x.nM = (int)(round_up(p.rows, L.bm) / L.bm), x.nN = nbn, x.S = (n + L.dx_ks - 1) / L.dx_ks;
+            x.K = n, x.Ks = L.dx_ks;
+            x.part = (float *)(ws + L.dx_part), x.part_ld = p.d, x.add = v0 > 0;
+            x.out_rows = p.rows, x.out_cols = p.d;
         }
         if (p.dw) {
-            const int live = (int)std::min<long>(n, p.vocab - v0);
-            LossGemm g{};
-            g.A = DZ, g.B = X2;
-            g.nM = n / 128, g.nN = nbn, g.S = L.dw_split;
-            g.K = (int)round_up(p.rows, 32), g.Ks = L.dw_ks;
-            g.out_rows = live, g.out_cols = p.d;
-            T *dst = (T *)p.dw + v0 * p.dw_stride;
+            LossGemm &w = g.dw;
+            w.A = DZ, w.B = X2;
+            w.nM = (live + L.bm - 1) / L.bm, w.nN = nbn, w.S = L.dw_split;
+            w.K = (int)round_up(p.rows, 32), w.Ks = L.dw_ks;
+            w.out_rows = live, w.out_cols = p.d;
             if (L.dw_split > 1)
-                g.part = (float *)(ws + L.dw_part), g.part_ld = p.d;
+                w.part = (float *)(ws + L.dw_part), w.part_ld = p.d;
             else
-                g.dst = dst, g.dst_stride = p.dw_stride, g.e_all = q.e_dw;
-            launch_grad<T, NP, true>(g, L.bn, st);
-            if (L.dw_split > 1)
-                k_loss_join<T><<<(unsigned)std::min<long>(2048, ((long)live * p.d + NT - 1) / NT), NT, 0, st>>>(
-                    g.part, L.dw_split, live, p.d, dst, p.dw_stride, nullptr, q.e_dw);
+                w.dst = dst, w.dst_stride = p.dw_stride, w.e_all = q.e_dw;
         }
+        if (p.dx || p.dw) launch_grads<T, NP>(g, L.bm, L.bn, st);
+        if (p.dw && L.dw_split > 1)
+            k_loss_join<T><<<(unsigned)std::min<long>(2048, ((long)live * p.d + NT - 1) / NT), NT, 0, st>>>(
+                g.dw.part, L.dw_split, live, p.d, dst, p.dw_stride, nullptr, q.e_dw);
     }
     if (p.dx)
         k_loss_join<T><<<(unsigned)std::min<long>(2048, ((long)p.rows * p.d + NT - 1) / NT), NT, 0, st>>>(
