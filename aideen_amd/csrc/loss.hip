@@ -42,7 +42,10 @@ using gemm::lds_barrier;
 
 constexpr int NT = 256;             // threads a workgroup: 4 waves
 constexpr size_t PIECE_BYTES = 256u << 20;
+constexpr int BM = 128;             // rows of a gradient tile
 constexpr int TV = 256;             // entries a workgroup of the logits' product covers
+constexpr int STAGES = 3;           // k slices of the LDS ring
+constexpr int NW = 4;               // waves of a workgroup
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int W_BLOCKS = 1024;      // blocks of the pass over |W|, one partial each
 
@@ -67,6 +70,12 @@ __device__ __forceinline__ void load_lds(const void *base, unsigned off, unsigne
                  :
                  : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base)
                  : "memory", "m0");
+}
+
+// e of |g| = m 2^e, m in [1, 2); 0 for zero and what is not finite
+__device__ __forceinline__ int exp_of(float g) {
+    const float a = fabsf(g);
+    return a > 0.0f && a < INFINITY ? ilogbf(a) : 0;
 }
 
 // Chunk (8 halves) of a block's row r that holds columns [0, 8) in the LDS image of an operand read
@@ -96,7 +105,7 @@ struct LossGemm {
     int vocab, rows;
     float *part_m, *part_s, *ztgt;      // [tile][rows padded]: maximum and sum of exponentials; the target's logit
     long rows_pad;
-    const float *lse, *q, *g;           // per row: lse (in units of log 2), dz's factor (m_i 2^13), g_i
+    const float *lse, *g;               // per row: lse (in units of log 2), g_i = m_i 2^e_i (dz's factor: m_i 2^13)
     _Float16 *dz;                       // planes of the piece, blocks of rows x entries
     long dz_plane;
     int dz_ncb;
@@ -130,17 +139,15 @@ struct Tile {
     static constexpr int KB = NP == 2 ? 1 : 2;
     static constexpr int TM = WGM * WTM * 32, TN = WGN * WTN * 32;
     static constexpr int A_BLK = TM / 32 * KB, B_BLK = TN / 32 * KB;  // 1 KB loads a plane and slice
-    static constexpr int NW = WGM * WGN;                              // waves
-    static constexpr int STAGES = NW == 8 ? 4 : 3;                    // slices of the LDS ring
     static constexpr int RING = STAGES * NP * (A_BLK + B_BLK) * 512;  // halves
-    static_assert(RING * 2 <= (NW == 8 ? 160 : 80) * 1024, "one workgroup of 8 waves a CU, or two of 4");
+    static_assert(WGM * WGN == 4, "four waves");
+    static_assert(RING * 2 <= 80 * 1024, "two workgroups a CU");
 };
 
 template <int MODE, typename T, int NP, int WTM, int WTN, int WGM, int WGN, bool TRA, bool TRB>
 __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *ring) {
     typedef Tile<NP, WTM, WTN, WGM, WGN> G;
-    constexpr int KB = G::KB, TM = G::TM, TN = G::TN, A_BLK = G::A_BLK, B_BLK = G::B_BLK, NW = G::NW,
-                  STAGES = G::STAGES;
+    constexpr int KB = G::KB, TM = G::TM, TN = G::TN, A_BLK = G::A_BLK, B_BLK = G::B_BLK;
     constexpr int A_PW = (A_BLK + NW - 1) / NW, B_PW = (B_BLK + NW - 1) / NW;
     constexpr int LOADS = NP * (A_PW + B_PW);
     constexpr int A_SZ = A_BLK * 512, B_SZ = B_BLK * 512;      // halves a plane and slice
@@ -380,7 +387,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
                 const long m = (long)nt * TN + j * 32 + r;
-                const float lse = p.lse[m], qm = p.q[m], gm = p.g[m];
+                const float lse = p.lse[m], gm = p.g[m], qm = ldexpf(gm, 13 - exp_of(gm));
                 const int t = p.tgt[m] - w0;
                 const bool off = qm == 0.0f;  // no target, or nothing from upstream: exactly zero
 #pragma unroll
@@ -452,7 +459,7 @@ __global__ __launch_bounds__(NT, 2) void k_loss_logits(LossGemm p) {
 }
 
 template <typename T, int NP, int WTM, int WTN, int WGM, int WGN>
-__global__ __launch_bounds__(64 * WGM * WGN, WGM * WGN == 8 ? 1 : 2) void k_loss_grads(LossGrads p) {
+__global__ __launch_bounds__(NT, 2) void k_loss_grads(LossGrads p) {
     __shared__ __attribute__((aligned(1024))) _Float16 ring[Tile<NP, WTM, WTN, WGM, WGN>::RING];
     const int b = blockIdx.x;
     if ((b < p.first) == (p.dx_first != 0))
@@ -466,12 +473,6 @@ __global__ __launch_bounds__(64 * WGM * WGN, WGM * WGN == 8 ? 1 : 2) void k_loss
 __device__ __forceinline__ int scale_exp(float mx) {
     if (!(mx > 0.0f) || mx == INFINITY) return 0;
     return 15 - (ilogbf(mx) + 1);
-}
-
-// e of |g| = m 2^e, m in [1, 2); 0 for zero and what is not finite
-__device__ __forceinline__ int exp_of(float g) {
-    const float a = fabsf(g);
-    return a > 0.0f && a < INFINITY ? ilogbf(a) : 0;
 }
 
 __device__ __forceinline__ float finite_abs(float v) {
@@ -515,16 +516,18 @@ struct Prep {
     long x_stride;
     const void *w;
     long w_stride;
-    int rows, d, vocab, dcb, w_blocks;  // dcb: column blocks of a row of width d
+    int rows, d, vocab, dcb;     // dcb: column blocks of a row of width d
+    int w_blocks, row_blocks;    // blocks of the pass over |W|; blocks of 32 rows of x
+    int w_rows;                  // blocks of 32 rows of W
     const int32_t *targets;
     const float *dloss;
     unsigned *err;
-    _Float16 *xp, *x2p, *wp;  // x for the logits, x for dW (null: not wanted), W
+    _Float16 *xp, *x2p, *wp;     // x for the logits, x for dW (null: not wanted), W
     long x_plane, w_plane;
-    float *w_part;    // [w_blocks] largest |w| of each block's share
-    int32_t *f, *tgt; // [rows padded]
-    float *g, *gmax;  // [rows padded], [row blocks]: largest |x_i| 2^e_i
-    int32_t *kw;      // exponent of W's scale
+    float *w_part;               // [w_blocks] largest |w| of each block's share
+    int32_t *f, *tgt;            // [rows padded]
+    float *g, *gmax;             // [rows padded], [row blocks]: largest |x_i| 2^e_i
+    int32_t *kw, *e_dw;          // exponent of W's scale; of dW's results
 };
 
 __device__ __forceinline__ float block_max256(float v, float *red) {
@@ -547,30 +550,36 @@ __device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb
     }
 }
 
-// Blocks below w_blocks: the largest |w| of a share of the rows.  The others: 32 rows of x each, split
-// into planes with a scale of their own; rows without a target are zeros and are not read.
+// The first row_blocks blocks: 32 rows of x each, split into planes with a scale of their own; rows
+// without a target are zeros and are not read.  The others: the largest |w| of a share of W.
 template <typename T, int NP, bool VECX, bool VECW>
 __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
     __shared__ float red[4];
     __shared__ float rmax[32][8];
     __shared__ int fx[32], tg[32];
     const int tid = threadIdx.x;
-    if ((int)blockIdx.x < p.w_blocks) {
+    if ((int)blockIdx.x >= p.row_blocks) {
         float m = 0.0f;
-        const int nch = (p.d + 7) / 8;
-        const long total = (long)p.vocab * nch;
-        for (long i = (long)blockIdx.x * NT + tid; i < total; i += (long)p.w_blocks * NT) {
-            const long v = i / nch;
-            float x[8];
-            load8<T, VECW>((const T *)p.w + v * p.w_stride, (int)(i - v * nch) * 8, p.d, x);
+        const int nch = (p.d + 7) / 8, b = blockIdx.x - p.row_blocks;
+        const long total = (long)p.vocab * nch, step = (long)p.w_blocks * NT;
+        // four chunks in flight
+        for (long i = (long)b * NT + tid; i < total; i += 4 * step) {
+            float x[4][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
+            for (int u = 0; u < 4; ++u) {
+                const long k = min(i + u * step, total - 1), v = k / nch;
+                load8<T, VECW>((const T *)p.w + v * p.w_stride, (int)(k - v * nch) * 8, p.d, x[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[u][j]));
         }
         m = block_max256(m, red);
-        if (tid == 0) p.w_part[blockIdx.x] = m;
+        if (tid == 0) p.w_part[b] = m;
         return;
     }
-    const int rb = blockIdx.x - p.w_blocks;
+    const int rb = blockIdx.x;
     {
         const int rl = tid >> 3, part = tid & 7;  // 8 threads a row
         const long i = (long)rb * 32 + rl;
@@ -582,6 +591,7 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
         if (t < 0) t = -1;
         float m = 0.0f;
         if (t >= 0)
+#pragma unroll 4
             for (int c = part * 8; c < p.d; c += 64) {
                 float x[8];
                 load8<T, VECX>((const T *)p.x + i * p.x_stride, c, p.d, x);
@@ -614,104 +624,131 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
     split_rows<T, NP, VECX>(p, p.xp, rb, tg, fx);
 }
 
-// W's planes, and the exponent of its scale from the shares' maxima.
-template <typename T, int NP, bool VECW>
-__global__ __launch_bounds__(NT) void k_loss_split_w(Prep p) {
+// The blocks that follow k_loss_prep's maxima: the planes of x for dW (the first blocks, where they are
+// wanted), and W's planes.
+template <typename T, int NP, bool VECX, bool VECW>
+__global__ __launch_bounds__(NT) void k_loss_split(Prep p) {
     __shared__ float red[4];
-    const int tid = threadIdx.x;
+    __shared__ int ex[32], live[32];
+    const int tid = threadIdx.x, xb = p.x2p ? p.row_blocks : 0;
+    const bool of_x = (int)blockIdx.x < xb;
     float m = 0.0f;
-    for (int i = tid; i < p.w_blocks; i += NT) m = fmaxf(m, p.w_part[i]);
-    m = block_max256(m, red);
-    const int kw = scale_exp(m);
-    const long rb = blockIdx.x;
-    if (rb == 0 && tid == 0) *p.kw = kw;
+    const float *part = of_x ? p.gmax : p.w_part;
+    const int n = of_x ? p.row_blocks : p.w_blocks;
+    for (int i = tid; i < n; i += NT) m = fmaxf(m, part[i]);
+    const int e = scale_exp(block_max256(m, red));
+    if (of_x) {
+        const long rb = blockIdx.x;
+        if (rb == 0 && tid == 0) *p.e_dw = -13 - e;
+        if (tid < 32) {
+            const float g = p.g[rb * 32 + tid];
+            ex[tid] = exp_of(g) + e;
+            live[tid] = g == 0.0f ? -1 : 0;  // a row that gives nothing is not in the scale's range
+        }
+        __syncthreads();
+        split_rows<T, NP, VECX>(p, p.x2p, rb, live, ex);
+        return;
+    }
+    const long rb = (int)blockIdx.x - xb;
+    if (rb == 0 && tid == 0) *p.kw = e;
     for (int ch = tid; ch < p.dcb * 64; ch += NT) {
         const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
         const long v = rb * 32 + rl;
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (v < p.vocab) load8<T, VECW>((const T *)p.w + v * p.w_stride, c, p.d, x);
-        store_planes<NP>(p.wp + (rb * p.dcb) * 512 + (long)ch * 8, p.w_plane, x, kw);
+        store_planes<NP>(p.wp + (rb * p.dcb) * 512 + (long)ch * 8, p.w_plane, x, e);
     }
 }
 
-// ---- rows: lse, loss, dz's factors, the planes of x for dW ---------------------------------
+// ---- rows: lse and loss from the tiles' partials -------------------------------------------
 struct Rows {
-    int tiles, row_blocks;
+    int rows, tiles;
     long rows_pad;
     const float *part_m, *part_s, *ztgt;
-    float *lse, *q;           // [rows padded]
-    int32_t *e_dx, *e_dw;     // exponents of the gradients' results: [rows padded] and one
+    const int32_t *tgt;
+    float *lse;               // [rows padded], in units of log 2
     float *out_loss, *out_lse;
 };
 
-// 32 rows a block, 8 threads share a row's tiles.
-template <typename T, int NP, bool VECX>
-__global__ __launch_bounds__(NT) void k_loss_rows(Rows p, Prep r) {
-    __shared__ float red[4];
-    __shared__ float sm[8][32], ss[8][32];
-    __shared__ int ex[32], tg[32];
-    const int tid = threadIdx.x, rl = tid & 31, part = tid >> 5;
-    float gm = 0.0f;
-    for (int i = tid; i < p.row_blocks; i += NT) gm = fmaxf(gm, r.gmax[i]);
-    const int F = scale_exp(block_max256(gm, red));
-    const long i = (long)blockIdx.x * 32 + rl;
-    float mx = -INFINITY;
-    for (int t = part; t < p.tiles; t += 8) mx = fmaxf(mx, p.part_m[(long)t * p.rows_pad + i]);
-    const float ref = mx == -INFINITY ? 0.0f : mx;
-    float s = 0.0f;
-    for (int t = part; t < p.tiles; t += 8)
-        s += p.part_s[(long)t * p.rows_pad + i] * __builtin_amdgcn_exp2f(p.part_m[(long)t * p.rows_pad + i] - ref);
+// 16 rows a block; 16 threads share a row's tiles, eight loads in flight each.
+__global__ __launch_bounds__(NT) void k_loss_rows(Rows p) {
+    __shared__ float sm[16][17], ss[16][17];
+    const int rl = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const long i = (long)blockIdx.x * 16 + rl;
+    float mx = -INFINITY, s = 0.0f;
+    for (int t0 = part; t0 < p.tiles; t0 += 16 * 8) {
+        float m[8], v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int t = t0 + 16 * u;
+            const long o = (long)min(t, p.tiles - 1) * p.rows_pad + i;
+            m[u] = p.part_m[o];
+            v[u] = p.part_s[o];
+            if (t >= p.tiles) m[u] = -INFINITY, v[u] = 0.0f;
+        }
+        float nm = mx;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) nm = fmaxf(nm, m[u]);
+        const float ref = nm == -INFINITY ? 0.0f : nm;
+        s *= __builtin_amdgcn_exp2f(mx - ref);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += v[u] * __builtin_amdgcn_exp2f(m[u] - ref);
+        mx = nm;
+    }
     sm[part][rl] = mx;
     ss[part][rl] = s;
     __syncthreads();
-    if (tid == 0 && blockIdx.x == 0) *p.e_dw = -13 - F;
-    if (tid < 32) {
-        mx = sm[0][rl];
+    if (part) return;
 #pragma unroll
-        for (int q = 1; q < 8; ++q) mx = fmaxf(mx, sm[q][rl]);
-        const float ref2 = mx == -INFINITY ? 0.0f : mx;
-        s = 0.0f;
+    for (int q = 1; q < 16; ++q) mx = fmaxf(mx, sm[q][rl]);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    s = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) s += ss[q][rl] * __builtin_amdgcn_exp2f(sm[q][rl] - ref2);
-        const float lse = ref2 + log2f(s);  // in units of log 2, as the partials and the target's logit
-        const int t = r.tgt[i];
-        const float g = r.g[i];
-        const int e = exp_of(g);
-        p.lse[i] = lse;
-        p.q[i] = ldexpf(g, 13 - e);
-        p.e_dx[i] = e - 13 - *r.kw;
-        ex[rl] = e + F;
-        tg[rl] = g == 0.0f ? -1 : t;  // a row that gives nothing is not in F's range either
-        if (i < r.rows) {
-            if (p.out_lse) p.out_lse[i] = t < 0 ? 0.0f : lse * LN2;
-            if (p.out_loss) p.out_loss[i] = t < 0 ? 0.0f : (lse - p.ztgt[i]) * LN2;
-        }
-    }
-    if (!r.x2p) return;
-    __syncthreads();
-    split_rows<T, NP, VECX>(r, r.x2p, blockIdx.x, tg, ex);
+    for (int q = 0; q < 16; ++q) s += ss[q][rl] * __builtin_amdgcn_exp2f(sm[q][rl] - ref);
+    const float lse = ref + log2f(s);
+    p.lse[i] = lse;
+    if (i >= p.rows) return;
+    const bool there = p.tgt[i] >= 0;
+    if (p.out_lse) p.out_lse[i] = there ? lse * LN2 : 0.0f;
+    if (p.out_loss) p.out_loss[i] = there ? (lse - p.ztgt[i]) * LN2 : 0.0f;
 }
 
-// dst[row][col] = sum over the shares, in order, times 2^exponent
+// ---- shares of the gradients ---------------------------------------------------------------
+// dst[row][col] = sum over the shares, in order, times 2^exponent: of dW all alike (e_all), of dx a
+// row's own, e_i - 13 - kw (g).  Blocks from n_blocks on: db, the tiles' sums in order.
+struct Join {
+    const float *part;
+    int S, rows, d;
+    void *dst;
+    long stride;
+    const int32_t *e_all, *kw;
+    const float *g;
+    int n_blocks;
+    const float *db_part;
+    int db_tiles, vocab;
+    long db_ld;
+    float *db;
+};
 template <typename T>
-__global__ __launch_bounds__(NT) void k_loss_join(const float *part, int S, int rows, int d, T *dst, long stride,
-                                                  const int32_t *e_row, const int32_t *e_all) {
-    const long n = (long)rows * d;
-    for (long i = (long)blockIdx.x * NT + threadIdx.x; i < n; i += (long)gridDim.x * NT) {
+__global__ __launch_bounds__(NT) void k_loss_join(Join p) {
+    if ((int)blockIdx.x >= p.n_blocks) {
+        const int v = ((int)blockIdx.x - p.n_blocks) * NT + threadIdx.x;
+        if (v >= p.vocab) return;
         float s = 0.0f;
-        for (int q = 0; q < S; ++q) s += part[q * n + i];
-        const long row = i / d;
-        dst[row * stride + (i - row * d)] = from_f32<T>(ldexpf(s, (e_row ? e_row[row] : 0) + (e_all ? *e_all : 0)));
-    }
-}
-
-__global__ __launch_bounds__(NT) void k_loss_db(const float *part, int tiles, long ld, int n, float *db) {
-    const int v = blockIdx.x * NT + threadIdx.x;
-    if (v >= n) return;
-    float s = 0.0f;
 #pragma unroll 8
-    for (int t = 0; t < tiles; ++t) s += part[t * ld + v];
-    db[v] = s;
+        for (int t = 0; t < p.db_tiles; ++t) s += p.db_part[t * p.db_ld + v];
+        p.db[v] = s;
+        return;
+    }
+    const long n = (long)p.rows * p.d;
+    for (long i = (long)blockIdx.x * NT + threadIdx.x; i < n; i += (long)p.n_blocks * NT) {
+        float s = 0.0f;
+#pragma unroll 8
+        for (int q = 0; q < p.S; ++q) s += p.part[q * n + i];
+        const long row = i / p.d;
+        const int e = p.g ? exp_of(p.g[row]) - 13 - *p.kw : *p.e_all;
+        ((T *)p.dst)[row * p.stride + (i - row * p.d)] = from_f32<T>(ldexpf(s, e));
+    }
 }
 
 template <typename T>
@@ -731,9 +768,9 @@ struct LossPlan {
     int v_tiles;             // tiles of TV entries
     int piece;               // entries a piece, a multiple of TV
     int w_blocks;
-    int bm, bn;              // rows and columns of a gradient tile
+    int bn;                  // columns of a gradient tile
     int dx_split, dx_ks, dw_split, dw_ks;
-    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, q, e_dx, e_dw, dz, dx_part, dw_part, db_part, bytes;
+    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, e_dw, dz, dx_part, dw_part, db_part, bytes;
 };
 
 // K of `len` (a multiple of 32) in at most `want` shares of whole 32s
@@ -743,7 +780,7 @@ void split_k(long len, long want, int *split, int *share) {
 }
 
 // Time of n1 units of length a and then n2 of length b (a >= b) on SLOTS slots, in order.
-double makespan(long n1, double a, long n2, double b, long SLOTS) {
+double makespan(long n1, double a, long n2, double b) {
     const long full = n1 / SLOTS, m1 = n1 % SLOTS, free = SLOTS - m1;
     const long fit = m1 ? free * (long)(a / b) : 0;  // units of b done beside the last a's
     double t = full * a;
@@ -754,7 +791,7 @@ double makespan(long n1, double a, long n2, double b, long SLOTS) {
 // Shares of the two gradients' K: the pair with the shortest estimated time of their common launch.  A
 // unit is its K plus EPI for its prologue and epilogue (stores of a tile: as long as about 200 values of
 // K), and each share's partial sums pass through memory twice more (JOIN a tile, all slots at once).
-void pick_splits(long slots, long dx_tiles, long dx_k, long dw_tiles, long dw_k, int *dx_split, int *dx_ks,
+void pick_splits(long dx_tiles, long dx_k, long dw_tiles, long dw_k, int *dx_split, int *dx_ks,
                  int *dw_split, int *dw_ks) {
     constexpr double EPI = 200, JOIN = 250;
     double best = INFINITY;
@@ -766,9 +803,9 @@ void pick_splits(long slots, long dx_tiles, long dx_k, long dw_tiles, long dw_k,
             if (dx_tiles) split_k(dx_k, sx, &nx, &kx);
             if (dw_tiles) split_k(dw_k, sw, &nw, &kw);
             const double a = kx + EPI, b = kw + EPI;
-            double t = a >= b ? makespan(dx_tiles * nx, a, dw_tiles * nw, b, slots)
-                              : makespan(dw_tiles * nw, b, dx_tiles * nx, a, slots);
-            t += JOIN * (dx_tiles * nx + (nw > 1 ? dw_tiles * nw : 0)) / slots;
+            double t = a >= b ? makespan(dx_tiles * nx, a, dw_tiles * nw, b)
+                              : makespan(dw_tiles * nw, b, dx_tiles * nx, a);
+            t += JOIN * (dx_tiles * nx + (nw > 1 ? dw_tiles * nw : 0)) / SLOTS;
             if (t < best) {
                 best = t;
                 if (dx_tiles) *dx_split = nx, *dx_ks = kx;
@@ -783,7 +820,7 @@ LossPlan loss_plan(const LossParams &p) {
     L.np = p.dtype == ADN_T_F32 ? 2 : 1;
     L.tn = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
     L.dcb = (int)(round_up(p.d, 32) / 16);
-    L.rows_pad = round_up(p.rows, 256);
+    L.rows_pad = round_up(p.rows, BM);
     L.v_pad = round_up(p.vocab, TV);
     L.v_tiles = (int)(L.v_pad / TV);
     const long fit = (long)(PIECE_BYTES / (L.np * 2)) / L.rows_pad / TV * TV;
@@ -791,7 +828,6 @@ LossPlan loss_plan(const LossParams &p) {
     L.piece = (int)round_up((L.v_pad + npieces - 1) / npieces, TV);
     L.w_blocks = (int)std::min<long>(W_BLOCKS, ((long)p.vocab * ((p.d + 7) / 8) + NT * 4 - 1) / (NT * 4));
     L.bn = p.d > 128 ? 256 : p.d > 64 ? 128 : 64;
-    L.bm = L.bn == 256 && getenv("BM") ? atoi(getenv("BM")) : 128;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -811,14 +847,12 @@ LossPlan loss_plan(const LossParams &p) {
     L.part_s = take((size_t)L.v_tiles * L.rows_pad * 4);
     L.ztgt = take(L.rows_pad * 4);
     L.lse = take(L.rows_pad * 4);
-    L.q = take(L.rows_pad * 4);
-    L.e_dx = take(L.rows_pad * 4);
     L.e_dw = take(4);
     if (grads) {
         const long nbn = (p.d + L.bn - 1) / L.bn;
         L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
-        pick_splits(L.bm == 256 ? SLOTS / 2 : SLOTS, p.dx ? round_up(p.rows, L.bm) / L.bm * nbn : 0, L.piece,
-                    p.dw ? round_up(std::min<long>(L.piece, p.vocab), L.bm) / L.bm * nbn : 0,
+        pick_splits(p.dx ? round_up(p.rows, BM) / BM * nbn : 0, L.piece,
+                    p.dw ? round_up(std::min<long>(L.piece, p.vocab), BM) / BM * nbn : 0,
                     round_up(p.rows, 32), &L.dx_split, &L.dx_ks, &L.dw_split, &L.dw_ks);
         if (p.dx) L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
         if (p.dw && L.dw_split > 1) L.dw_part = take((size_t)L.dw_split * L.piece * p.d * 4);
@@ -840,20 +874,20 @@ void launch_logits(const LossGemm &g, int tn, hipStream_t st) {
 }
 
 template <typename T, int NP>
-void launch_grads(LossGrads &g, int bm, int bn, hipStream_t st) {
+void launch_grads(LossGrads &g, int bn, hipStream_t st) {
     const int ndx = g.dx.nM * g.dx.nN * g.dx.S, ndw = g.dw.nM * g.dw.nN * g.dw.S;  // 0: not wanted
     g.dx_first = ndx && (!ndw || g.dx.Ks >= g.dw.Ks);
     g.first = g.dx_first ? ndx : ndw;
     const unsigned grid = (unsigned)(ndx + ndw);
-    if (bm == 256)
-        k_loss_grads<T, NP, 2, 4, 4, 2><<<grid, 2 * NT, 0, st>>>(g);
-    else if (bn == 256)
+    if (bn == 256)
         k_loss_grads<T, NP, 2, 4, 2, 2><<<grid, NT, 0, st>>>(g);
     else if (bn == 128)
         k_loss_grads<T, NP, 2, 2, 2, 2><<<grid, NT, 0, st>>>(g);
     else
         k_loss_grads<T, NP, 1, 2, 4, 1><<<grid, NT, 0, st>>>(g);
 }
+
+int join_blocks(long n) { return (int)std::min<long>(2048, (n + NT - 1) / NT); }
 
 template <typename T, int NP>
 void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) {
@@ -863,28 +897,31 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     const bool vw = (uintptr_t)p.w % 16 == 0 && p.w_stride * eb % 16 == 0;
     Prep r{};
     r.x = p.x, r.x_stride = p.x_stride, r.w = p.w, r.w_stride = p.w_stride;
-    r.rows = p.rows, r.d = p.d, r.vocab = p.vocab, r.dcb = L.dcb, r.w_blocks = L.w_blocks;
+    r.rows = p.rows, r.d = p.d, r.vocab = p.vocab, r.dcb = L.dcb;
+    r.w_blocks = L.w_blocks, r.row_blocks = (int)(L.rows_pad / 32), r.w_rows = (int)(L.v_pad / 32);
     r.targets = p.targets, r.dloss = p.dloss, r.err = p.err;
     r.xp = (_Float16 *)(ws + L.xp), r.x2p = p.dw ? (_Float16 *)(ws + L.x2p) : nullptr, r.wp = (_Float16 *)(ws + L.wp);
     r.x_plane = L.rows_pad * L.dcb * 16, r.w_plane = L.v_pad * L.dcb * 16;
     r.w_part = (float *)(ws + L.w_part);
     r.f = (int32_t *)(ws + L.f), r.tgt = (int32_t *)(ws + L.tgt);
     r.g = (float *)(ws + L.g), r.gmax = (float *)(ws + L.gmax);
-    r.kw = (int32_t *)(ws + L.kw);
-    const int row_blocks = (int)(L.rows_pad / 32);
-    const unsigned prep_grid = (unsigned)(L.w_blocks + row_blocks), split_grid = (unsigned)(L.v_pad / 32);
+    r.kw = (int32_t *)(ws + L.kw), r.e_dw = (int32_t *)(ws + L.e_dw);
+    const unsigned prep_grid = (unsigned)(r.row_blocks + r.w_blocks);
+    const unsigned split_grid = (unsigned)((r.x2p ? r.row_blocks : 0) + r.w_rows);
+    auto prep = [&](auto vecx, auto vecw) {
+        constexpr bool VX = decltype(vecx)::value, VW = decltype(vecw)::value;
+        k_loss_prep<T, NP, VX, VW><<<prep_grid, NT, 0, st>>>(r);
+        k_loss_split<T, NP, VX, VW><<<split_grid, NT, 0, st>>>(r);
+    };
+    using std::bool_constant;
     if (vx && vw)
-        k_loss_prep<T, NP, true, true><<<prep_grid, NT, 0, st>>>(r);
+        prep(bool_constant<true>{}, bool_constant<true>{});
     else if (vx)
-        k_loss_prep<T, NP, true, false><<<prep_grid, NT, 0, st>>>(r);
+        prep(bool_constant<true>{}, bool_constant<false>{});
     else if (vw)
-        k_loss_prep<T, NP, false, true><<<prep_grid, NT, 0, st>>>(r);
+        prep(bool_constant<false>{}, bool_constant<true>{});
     else
-        k_loss_prep<T, NP, false, false><<<prep_grid, NT, 0, st>>>(r);
-    if (vw)
-        k_loss_split_w<T, NP, true><<<split_grid, NT, 0, st>>>(r);
-    else
-        k_loss_split_w<T, NP, false><<<split_grid, NT, 0, st>>>(r);
+        prep(bool_constant<false>{}, bool_constant<false>{});
 
     const Planes X{r.xp, r.x_plane, L.dcb}, X2{r.x2p, r.x_plane, L.dcb}, W{r.wp, r.w_plane, L.dcb};
     LossGemm z{};
@@ -897,19 +934,13 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     launch_logits<LOGITS_STATS, T, NP>(z, L.tn, st);
 
     Rows q{};
-    q.tiles = L.v_tiles, q.row_blocks = row_blocks, q.rows_pad = L.rows_pad;
-    q.part_m = z.part_m, q.part_s = z.part_s, q.ztgt = z.ztgt;
-    q.lse = (float *)(ws + L.lse), q.q = (float *)(ws + L.q);
-    q.e_dx = (int32_t *)(ws + L.e_dx), q.e_dw = (int32_t *)(ws + L.e_dw);
-    q.out_loss = p.loss, q.out_lse = p.lse;
-    const unsigned rows_grid = (unsigned)(round_up(p.rows, L.tn) / 32);
-    if (vx)
-        k_loss_rows<T, NP, true><<<rows_grid, NT, 0, st>>>(q, r);
-    else
-        k_loss_rows<T, NP, false><<<rows_grid, NT, 0, st>>>(q, r);
+    q.rows = p.rows, q.tiles = L.v_tiles, q.rows_pad = L.rows_pad;
+    q.part_m = z.part_m, q.part_s = z.part_s, q.ztgt = z.ztgt, q.tgt = r.tgt;
+    q.lse = (float *)(ws + L.lse), q.out_loss = p.loss, q.out_lse = p.lse;
+    k_loss_rows<<<(unsigned)(round_up(p.rows, L.tn) / 16), NT, 0, st>>>(q);
     if (!p.dx && !p.dw && !p.db) return;
 
-    z.lse = q.lse, z.q = q.q, z.g = r.g;
+    z.lse = q.lse, z.g = r.g;
     z.dz = (_Float16 *)(ws + L.dz), z.dz_plane = L.rows_pad * L.piece, z.dz_ncb = L.piece / 16;
     z.db_part = p.db ? (float *)(ws + L.db_part) : nullptr, z.db_ld = L.v_pad;
     const int nbn = (p.d + L.bn - 1) / L.bn;
@@ -926,7 +957,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
             LossGemm &x = g.dx;
             x.A = DZ, x.B = W;
             x.B.p += v0 / 32 * (long)W.ncb * 512;
-            x.nM = (int)(round_up(p.rows, L.bm) / L.bm), x.nN = nbn, x.S = (n + L.dx_ks - 1) / L.dx_ks;
+            x.nM = (int)(round_up(p.rows, BM) / BM), x.nN = nbn, x.S = (n + L.dx_ks - 1) / L.dx_ks;
             x.K = n, x.Ks = L.dx_ks;
             x.part = (float *)(ws + L.dx_part), x.part_ld = p.d, x.add = v0 > 0;
             x.out_rows = p.rows, x.out_cols = p.d;
@@ -934,23 +965,28 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         if (p.dw) {
             LossGemm &w = g.dw;
             w.A = DZ, w.B = X2;
-            w.nM = (live + L.bm - 1) / L.bm, w.nN = nbn, w.S = L.dw_split;
+            w.nM = (live + BM - 1) / BM, w.nN = nbn, w.S = L.dw_split;
             w.K = (int)round_up(p.rows, 32), w.Ks = L.dw_ks;
             w.out_rows = live, w.out_cols = p.d;
             if (L.dw_split > 1)
                 w.part = (float *)(ws + L.dw_part), w.part_ld = p.d;
             else
-                w.dst = dst, w.dst_stride = p.dw_stride, w.e_all = q.e_dw;
+                w.dst = dst, w.dst_stride = p.dw_stride, w.e_all = r.e_dw;
         }
-        if (p.dx || p.dw) launch_grads<T, NP>(g, L.bm, L.bn, st);
-        if (p.dw && L.dw_split > 1)
-            k_loss_join<T><<<(unsigned)std::min<long>(2048, ((long)live * p.d + NT - 1) / NT), NT, 0, st>>>(
-                g.dw.part, L.dw_split, live, p.d, dst, p.dw_stride, nullptr, q.e_dw);
+        if (p.dx || p.dw) launch_grads<T, NP>(g, L.bn, st);
+        if (p.dw && L.dw_split > 1) {
+            Join j{};
+            j.part = g.dw.part, j.S = L.dw_split, j.rows = live, j.d = p.d, j.dst = dst, j.stride = p.dw_stride;
+            j.e_all = r.e_dw, j.n_blocks = join_blocks((long)live * p.d);
+            k_loss_join<T><<<j.n_blocks, NT, 0, st>>>(j);
+        }
     }
-    if (p.dx)
-        k_loss_join<T><<<(unsigned)std::min<long>(2048, ((long)p.rows * p.d + NT - 1) / NT), NT, 0, st>>>(
-            (float *)(ws + L.dx_part), L.dx_split, p.rows, p.d, (T *)p.dx, p.dx_stride, q.e_dx, nullptr);
-    if (p.db) k_loss_db<<<(p.vocab + NT - 1) / NT, NT, 0, st>>>(z.db_part, z.nN, z.db_ld, p.vocab, p.db);
+    if (!p.dx && !p.db) return;
+    Join j{};
+    j.part = (float *)(ws + L.dx_part), j.S = L.dx_split, j.rows = p.rows, j.d = p.d, j.dst = p.dx, j.stride = p.dx_stride;
+    j.g = r.g, j.kw = r.kw, j.n_blocks = p.dx ? join_blocks((long)p.rows * p.d) : 0;
+    j.db_part = z.db_part, j.db_tiles = z.nN, j.db_ld = z.db_ld, j.vocab = p.vocab, j.db = p.db;
+    k_loss_join<T><<<j.n_blocks + (p.db ? (p.vocab + NT - 1) / NT : 0), NT, 0, st>>>(j);
 }
 
 }  // namespace
