@@ -47,6 +47,7 @@ constexpr int TV = 256;             // entries a workgroup of the logits' produc
 constexpr int STAGES = 3;           // k slices of the LDS ring
 constexpr int NW = 4;               // waves of a workgroup
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int XR = 8;               // rows of x a block splits
 constexpr int W_BLOCKS = 1024;      // blocks of the pass over |W|, one partial each
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -517,7 +518,7 @@ struct Prep {
     const void *w;
     long w_stride;
     int rows, d, vocab, dcb;     // dcb: column blocks of a row of width d
-    int w_blocks, row_blocks;    // blocks of the pass over |W|; blocks of 32 rows of x
+    int w_blocks, row_blocks;    // blocks of the pass over |W|; blocks of XR rows of x
     int w_rows;                  // blocks of 32 rows of W
     const int32_t *targets;
     const float *dloss;
@@ -538,25 +539,29 @@ __device__ __forceinline__ float block_max256(float v, float *red) {
     return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// The planes of 32 rows of x, row r times 2^ex[r] (zeros where live[r] < 0): chunk (column block, row,
-// half) by chunk, neighbouring threads side by side.
+// The planes of XR rows of x, row r times 2^ex[r] (zeros where live[r] < 0): chunk (column block, row,
+// half) by chunk, neighbouring threads side by side.  XR = 8: four blocks share a block row of 32, so
+// that 4096 rows fill the chip.
 template <typename T, int NP, bool VECX>
 __device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb, const int *live, const int *ex) {
-    for (int ch = threadIdx.x; ch < p.dcb * 64; ch += NT) {
-        const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
+    const long row0 = rb * XR;
+    dst += row0 / 32 * p.dcb * 512 + row0 % 32 * 16;
+#pragma unroll 4
+    for (int ch = threadIdx.x; ch < p.dcb * 2 * XR; ch += NT) {
+        const int cb = ch / (2 * XR), rl = (ch >> 1) % XR, c = cb * 16 + (ch & 1) * 8;
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (live[rl] >= 0) load8<T, VECX>((const T *)p.x + (rb * 32 + rl) * p.x_stride, c, p.d, x);
-        store_planes<NP>(dst + rb * p.dcb * 512 + (long)ch * 8, p.x_plane, x, ex[rl]);
+        if (live[rl] >= 0) load8<T, VECX>((const T *)p.x + (row0 + rl) * p.x_stride, c, p.d, x);
+        store_planes<NP>(dst + (long)cb * 512 + rl * 16 + (ch & 1) * 8, p.x_plane, x, ex[rl]);
     }
 }
 
-// The first row_blocks blocks: 32 rows of x each, split into planes with a scale of their own; rows
+// The first row_blocks blocks: XR rows of x each, split into planes with a scale of their own; rows
 // without a target are zeros and are not read.  The others: the largest |w| of a share of W.
 template <typename T, int NP, bool VECX, bool VECW>
 __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
     __shared__ float red[4];
-    __shared__ float rmax[32][8];
-    __shared__ int fx[32], tg[32];
+    __shared__ float rmax[XR];
+    __shared__ int fx[XR], tg[XR];
     const int tid = threadIdx.x;
     if ((int)blockIdx.x >= p.row_blocks) {
         float m = 0.0f;
@@ -581,8 +586,9 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
     }
     const int rb = blockIdx.x;
     {
-        const int rl = tid >> 3, part = tid & 7;  // 8 threads a row
-        const long i = (long)rb * 32 + rl;
+        constexpr int PER = NT / XR;  // threads a row: half a wave
+        const int rl = tid / PER, part = tid % PER;
+        const long i = (long)rb * XR + rl;
         int t = i < p.rows ? p.targets[i] : -1;
         if (t >= p.vocab) {
             if (part == 0) atomicOr(p.err, ADN_DEVERR_TOKEN);
@@ -592,35 +598,31 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
         float m = 0.0f;
         if (t >= 0)
 #pragma unroll 4
-            for (int c = part * 8; c < p.d; c += 64) {
+            for (int c = part * 8; c < p.d; c += 8 * PER) {
                 float x[8];
                 load8<T, VECX>((const T *)p.x + i * p.x_stride, c, p.d, x);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
             }
-        rmax[rl][part] = m;
-        if (part == 0) tg[rl] = t;
-    }
-    __syncthreads();
-    float gm = 0.0f;
-    if (tid < 32) {
-        float m = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) m = fmaxf(m, rmax[tid][c]);
-        const long i = (long)rb * 32 + tid;
-        const int t = tg[tid];
-        const float g = t < 0 ? 0.0f : p.dloss ? p.dloss[i] : 1.0f;
-        fx[tid] = scale_exp(m);
-        p.f[i] = fx[tid];
-        p.tgt[i] = t;
-        p.g[i] = g;
-        gm = g == 0.0f ? 0.0f : fminf(ldexpf(m, exp_of(g)), 0x1p127f);
-    }
-    if (tid < 64) {
-        gm = wave_max(gm);
-        if (tid == 0) p.gmax[rb] = gm;
+        for (int off = PER / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        if (part == 0) {
+            const float g = t < 0 ? 0.0f : p.dloss ? p.dloss[i] : 1.0f;
+            tg[rl] = t;
+            fx[rl] = scale_exp(m);
+            p.f[i] = fx[rl];
+            p.tgt[i] = t;
+            p.g[i] = g;
+            rmax[rl] = g == 0.0f ? 0.0f : fminf(ldexpf(m, exp_of(g)), 0x1p127f);
+        }
     }
     __syncthreads();
+    if (tid == 0) {
+        float m = rmax[0];
+#pragma unroll
+        for (int r = 1; r < XR; ++r) m = fmaxf(m, rmax[r]);
+        p.gmax[rb] = m;
+    }
     split_rows<T, NP, VECX>(p, p.xp, rb, tg, fx);
 }
 
@@ -629,7 +631,7 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
 template <typename T, int NP, bool VECX, bool VECW>
 __global__ __launch_bounds__(NT) void k_loss_split(Prep p) {
     __shared__ float red[4];
-    __shared__ int ex[32], live[32];
+    __shared__ int ex[XR], live[XR];
     const int tid = threadIdx.x, xb = p.x2p ? p.row_blocks : 0;
     const bool of_x = (int)blockIdx.x < xb;
     float m = 0.0f;
@@ -640,8 +642,8 @@ __global__ __launch_bounds__(NT) void k_loss_split(Prep p) {
     if (of_x) {
         const long rb = blockIdx.x;
         if (rb == 0 && tid == 0) *p.e_dw = -13 - e;
-        if (tid < 32) {
-            const float g = p.g[rb * 32 + tid];
+        if (tid < XR) {
+            const float g = p.g[rb * XR + tid];
             ex[tid] = exp_of(g) + e;
             live[tid] = g == 0.0f ? -1 : 0;  // a row that gives nothing is not in the scale's range
         }
@@ -788,30 +790,39 @@ double makespan(long n1, double a, long n2, double b) {
     return t + (m1 ? a : 0.0) + (double)((n2 - fit + SLOTS - 1) / SLOTS) * b;
 }
 
-// Shares of the two gradients' K: the pair with the shortest estimated time of their common launch.  A
-// unit is its K plus EPI for its prologue and epilogue (stores of a tile: as long as about 200 values of
-// K), and each share's partial sums pass through memory twice more (JOIN a tile, all slots at once).
-void pick_splits(long dx_tiles, long dx_k, long dw_tiles, long dw_k, int *dx_split, int *dx_ks,
-                 int *dw_split, int *dw_ks) {
-    constexpr double EPI = 200, JOIN = 250;
+// Shares of the two gradients' K: the pair with the shortest estimated time of their common launch, in
+// values of K of a unit.  A unit is its K plus EPI for its prologue and epilogue (stores of a tile: as
+// long as about 200 values of K).  Partial sums are written and read again: two passes of their bytes
+// at 5 TB/s, where a value of K takes a unit about 0.044 us (two planes) or 0.022 us (one).
+struct GradSizes {
+    int np;
+    long dx_tiles, dx_k, dx_elems;  // elements of dx, of a piece of dW
+    long dw_tiles, dw_k, dw_elems;
+};
+void pick_splits(const GradSizes &g, int *dx_split, int *dx_ks, int *dw_split, int *dw_ks) {
+    constexpr double EPI = 200;
+    constexpr int SHARES[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
+    const double join = 8.0 / (g.np == 2 ? 2.2e5 : 1.1e5);  // K values an element of a share
     double best = INFINITY;
-    const long most_dx = dx_tiles ? std::max<long>(1, std::min<long>(64, dx_k / 256)) : 1;
-    const long most_dw = dw_tiles ? std::max<long>(1, std::min<long>(16, dw_k / 256)) : 1;
-    for (long sx = 1; sx <= most_dx; ++sx)
-        for (long sw = 1; sw <= most_dw; ++sw) {
-            int nx = 0, kx = 32, nw = 0, kw = 32;
-            if (dx_tiles) split_k(dx_k, sx, &nx, &kx);
-            if (dw_tiles) split_k(dw_k, sw, &nw, &kw);
+    for (int sx : SHARES) {
+        if (sx > 1 && g.dx_k / sx < 256) break;  // (none wanted: K = 0)
+        int nx = 0, kx = 32;
+        if (g.dx_tiles) split_k(g.dx_k, sx, &nx, &kx);
+        for (int sw : SHARES) {
+            if (sw > 1 && g.dw_k / sw < 256) break;
+            int nw = 0, kw = 32;
+            if (g.dw_tiles) split_k(g.dw_k, sw, &nw, &kw);
             const double a = kx + EPI, b = kw + EPI;
-            double t = a >= b ? makespan(dx_tiles * nx, a, dw_tiles * nw, b)
-                              : makespan(dw_tiles * nw, b, dx_tiles * nx, a);
-            t += JOIN * (dx_tiles * nx + (nw > 1 ? dw_tiles * nw : 0)) / SLOTS;
+            double t = a >= b ? makespan(g.dx_tiles * nx, a, g.dw_tiles * nw, b)
+                              : makespan(g.dw_tiles * nw, b, g.dx_tiles * nx, a);
+            t += join * ((double)g.dx_elems * nx + (nw > 1 ? (double)g.dw_elems * nw : 0.0));
             if (t < best) {
                 best = t;
-                if (dx_tiles) *dx_split = nx, *dx_ks = kx;
-                if (dw_tiles) *dw_split = nw, *dw_ks = kw;
+                if (g.dx_tiles) *dx_split = nx, *dx_ks = kx;
+                if (g.dw_tiles) *dw_split = nw, *dw_ks = kw;
             }
         }
+    }
 }
 
 LossPlan loss_plan(const LossParams &p) {
@@ -841,7 +852,7 @@ LossPlan loss_plan(const LossParams &p) {
     L.f = take(L.rows_pad * 4);
     L.tgt = take(L.rows_pad * 4);
     L.g = take(L.rows_pad * 4);
-    L.gmax = take(L.rows_pad / 32 * 4);
+    L.gmax = take(L.rows_pad / XR * 4);
     L.kw = take(4);
     L.part_m = take((size_t)L.v_tiles * L.rows_pad * 4);
     L.part_s = take((size_t)L.v_tiles * L.rows_pad * 4);
@@ -851,9 +862,13 @@ LossPlan loss_plan(const LossParams &p) {
     if (grads) {
         const long nbn = (p.d + L.bn - 1) / L.bn;
         L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
-        pick_splits(p.dx ? round_up(p.rows, BM) / BM * nbn : 0, L.piece,
-                    p.dw ? round_up(std::min<long>(L.piece, p.vocab), BM) / BM * nbn : 0,
-                    round_up(p.rows, 32), &L.dx_split, &L.dx_ks, &L.dw_split, &L.dw_ks);
+        GradSizes g{L.np};
+        if (p.dx) g.dx_tiles = round_up(p.rows, BM) / BM * nbn, g.dx_k = L.piece, g.dx_elems = (long)p.rows * p.d;
+        if (p.dw) {
+            const long n = std::min<long>(L.piece, p.vocab);
+            g.dw_tiles = round_up(n, BM) / BM * nbn, g.dw_k = round_up(p.rows, 32), g.dw_elems = n * p.d;
+        }
+        pick_splits(g, &L.dx_split, &L.dx_ks, &L.dw_split, &L.dw_ks);
         if (p.dx) L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
         if (p.dw && L.dw_split > 1) L.dw_part = take((size_t)L.dw_split * L.piece * p.d * 4);
         if (p.db) L.db_part = take((size_t)(L.rows_pad / L.tn) * L.v_pad * 4);
@@ -898,7 +913,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     Prep r{};
     r.x = p.x, r.x_stride = p.x_stride, r.w = p.w, r.w_stride = p.w_stride;
     r.rows = p.rows, r.d = p.d, r.vocab = p.vocab, r.dcb = L.dcb;
-    r.w_blocks = L.w_blocks, r.row_blocks = (int)(L.rows_pad / 32), r.w_rows = (int)(L.v_pad / 32);
+    r.w_blocks = L.w_blocks, r.row_blocks = (int)(L.rows_pad / XR), r.w_rows = (int)(L.v_pad / 32);
     r.targets = p.targets, r.dloss = p.dloss, r.err = p.err;
     r.xp = (_Float16 *)(ws + L.xp), r.x2p = p.dw ? (_Float16 *)(ws + L.x2p) : nullptr, r.wp = (_Float16 *)(ws + L.wp);
     r.x_plane = L.rows_pad * L.dcb * 16, r.w_plane = L.v_pad * L.dcb * 16;
@@ -991,9 +1006,12 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
 
 }  // namespace
 
-size_t loss_workspace_bytes(const LossParams &p) { return p.rows ? loss_plan(p).bytes : 0; }
+size_t loss_workspace_bytes(const LossParams &p) {
+    return p.rows == 0 ? 0 : loss_few_ok(p) ? loss_few_workspace_bytes(p) : loss_plan(p).bytes;
+}
 
 void launch_loss(const LossParams &p, void *ws, hipStream_t st) {
+    if (p.rows && loss_few_ok(p)) return launch_loss_few(p, ws, st);
     dispatch_type(p.dtype, [&](auto ty) {
         typedef decltype(ty) T;
         if (p.rows == 0) {  // no row: the sums over the rows are zero

@@ -55,6 +55,10 @@ struct LossParams {
 // Workspace of a call, in bytes, and the launches, which lay it out the same way.
 size_t loss_workspace_bytes(const LossParams &p);
 void launch_loss(const LossParams &p, void *ws, hipStream_t st);
+// A few rows and small problems (loss_few.hip); the others go through the products of loss.hip.
+bool loss_few_ok(const LossParams &p);
+size_t loss_few_workspace_bytes(const LossParams &p);
+void launch_loss_few(const LossParams &p, void *ws, hipStream_t st);
 
 // ---- RMS norm of rows (norm.hip) -----------------------------------------------------------
 struct NormParams {
