@@ -3,11 +3,17 @@
 //
 //   out[i] = scale E[tok_i]            dE[v] = scale sum over i with tok_i = v of dout[i]
 //
-// The gradient adds each table row's positions in ascending order, so it is the same bits on every
-// run: the positions are sorted by token (a stable radix sort of 8 bits a pass), the sorted list is
-// cut into chunks, a wave adds one chunk's rows in order and stores the table rows that begin and
-// end in it; of a row that crosses chunks every chunk stores a partial sum, and a second kernel
-// adds those in chunk order.  Rows without a token are zeros, written by a fill of the whole table.
+// The gradient adds each table row's positions in a fixed order, so it is the same bits on every run.
+//
+// Up to FEW positions: one launch.  A block a position compares its token with all the others; the
+// first block of a token adds the token's rows, its waves a quarter of them each.  Other blocks write
+// zeros where no token is.
+//
+// More: the positions are sorted by token (a stable radix sort of 8 bits a pass), the sorted list is
+// cut into chunks, a wave adds one chunk's rows in order and stores the table rows that begin and end
+// in it; of a row that crosses chunks every chunk stores a partial sum, and a last kernel adds those in
+// chunk order (a frequent token has thousands of positions).  The sort's launches are short and leave
+// most of the chip idle: their other blocks write the table's zeros, the larger part of all bytes.
 #include <algorithm>
 
 #include "train.h"
@@ -18,8 +24,11 @@ namespace {
 
 constexpr int NT = 256;
 constexpr int RADIX = 256;
-constexpr int TILE = 2048;            // keys a block of a radix pass
+constexpr int TILE = 1024;                // keys a block of a radix pass
 constexpr int W_KEYS = TILE / (NT / 64);  // consecutive keys a wave of it
+constexpr int OWN_PREFIX = 128;           // blocks up to which each forms its own offsets
+constexpr int FEW = 1024;
+constexpr int C0 = 32;                    // sorted entries a wave adds at a time
 
 // The key of position i: its token, or `vocab` (sorted behind every token) where it has none.
 __device__ __forceinline__ unsigned key_of(const int32_t *tokens, long i, int vocab, unsigned *err) {
@@ -56,25 +65,154 @@ __global__ __launch_bounds__(NT) void k_lookup(TableParams p) {
     }
 }
 
+// Zeros in rows v0 + first, + step, ... below v1 of the table, a wave a row.
+template <typename T, bool VEC>
+__device__ __forceinline__ void zero_rows(T *dst, long stride, int d, long v0, long v1, long first, long step) {
+    constexpr int W = VEC ? 16 / (int)sizeof(T) : 1;
+    typedef typename VecT<T, W>::type V;
+    V z;
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] = from_f32<T>(0.0f);
+    const int lane = threadIdx.x & 63;
+    for (long v = v0 + first; v < v1; v += step)
+        for (int c = lane * W; c < d; c += 64 * W) *reinterpret_cast<V *>(dst + v * stride + c) = z;
+}
+
+// ---- few positions -------------------------------------------------------------------------
+// Blocks below n: position blockIdx.x.  The others: FEW_ROWS rows of the table each.
+constexpr int FEW_ROWS = 64;
+template <typename T, bool VEC>
+__global__ __launch_bounds__(NT) void k_grad_few(TableParams p) {
+    constexpr int W = VEC ? 16 / (int)sizeof(T) : 1;
+    typedef typename VecT<T, W>::type V;
+    __shared__ int list[FEW];
+    __shared__ int here[FEW_ROWS];
+    __shared__ float part[3][64 * W];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if ((int)blockIdx.x >= p.n) {
+        const long v0 = (long)((int)blockIdx.x - p.n) * FEW_ROWS, v1 = min(v0 + FEW_ROWS, (long)p.vocab);
+        if (tid < FEW_ROWS) here[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < p.n; i += NT) {
+            const int t = p.tokens[i];
+            if (t >= v0 && t < v1) here[t - v0] = 1;
+        }
+        __syncthreads();
+        for (long v = v0 + wave; v < v1; v += NT / 64)
+            if (!here[v - v0]) zero_rows<T, VEC>((T *)p.dst, p.dst_stride, p.d, v, v + 1, 0, 1);
+        return;
+    }
+    const int me = p.tokens[blockIdx.x];
+    if (me >= p.vocab && tid == 0) atomicOr(p.err, ADN_DEVERR_TOKEN);
+    if (me < 0 || me >= p.vocab) return;
+    // the positions of this token in order: every wave finds them all
+    int m = 0;
+    bool first = true;
+    for (int i0 = 0; i0 < p.n; i0 += 64 * 8) {
+        int t[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) t[u] = i0 + u * 64 + lane < p.n ? p.tokens[i0 + u * 64 + lane] : -1;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const unsigned long long hit = __ballot(t[u] == me);
+            const int i = i0 + u * 64 + lane;
+            if (hit && m == 0) first = i0 + u * 64 + __ffsll(hit) - 1 == (int)blockIdx.x;
+            if (wave == 0 && t[u] == me) list[m + __popcll(hit & ((1ull << lane) - 1))] = i;
+            m += __popcll(hit);
+        }
+        if (!first) return;  // an earlier block adds this token (all waves agree)
+    }
+    __syncthreads();
+    const int per = (m + 3) / 4, a = min(m, wave * per), b = min(m, a + per);
+    for (int c0 = 0; c0 < p.d; c0 += 64 * W) {
+        const int c = c0 + lane * W;
+        float acc[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) acc[j] = 0.0f;
+        if (c < p.d)
+            for (int e0 = a; e0 < b; e0 += 8) {
+                V v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    v[u] = *reinterpret_cast<const V *>((const T *)p.src + (long)list[min(e0 + u, b - 1)] * p.src_stride + c);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (e0 + u < b)
+#pragma unroll
+                        for (int j = 0; j < W; ++j) acc[j] += to_f32<T>(v[u][j]);
+            }
+        if (m > 1) {  // the waves' sums in order
+            __syncthreads();
+            if (wave)
+#pragma unroll
+                for (int j = 0; j < W; ++j) part[wave - 1][lane * W + j] = acc[j];
+            __syncthreads();
+            if (wave == 0)
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+#pragma unroll
+                    for (int j = 0; j < W; ++j) acc[j] += part[q][lane * W + j];
+        }
+        if (wave == 0 && c < p.d) {
+            V o;
+#pragma unroll
+            for (int j = 0; j < W; ++j) o[j] = from_f32<T>(acc[j] * p.scale);
+            *reinterpret_cast<V *>((T *)p.dst + (long)me * p.dst_stride + c) = o;
+        }
+    }
+}
+
 // ---- radix sort of (token, position) -------------------------------------------------------
-// cnt[digit][block] = keys of the block's tile with that digit.  First pass: the keys are formed
-// from the tokens (and the positions are their indexes).
-template <bool FIRST>
-__global__ __launch_bounds__(NT) void k_radix_count(const unsigned *keys, const int32_t *tokens, int n, int vocab,
-                                                    int shift, unsigned *cnt, int nblocks, unsigned *err) {
+struct Sort {
+    const int32_t *tokens;
+    int n, vocab, nblocks;      // blocks of TILE keys
+    int passes;
+    unsigned *keys[2];          // keys and positions, alternating
+    int32_t *pos[2];
+    unsigned *cnt;              // [digit][block]: counts of a pass
+    bool own_prefix;            // offsets formed by the moving blocks, else in place by k_scan
+    unsigned *err;
+    // zeros of the table, written by the launches' other blocks: a share of the rows each
+    void *dst;
+    long dst_stride;
+    int d;
+    bool vec;
+    int launch, launches;
+};
+
+template <typename T>
+__device__ __forceinline__ void sort_zero(const Sort &s) {
+    const long v0 = (long)s.vocab * s.launch / s.launches, v1 = (long)s.vocab * (s.launch + 1) / s.launches;
+    const long first = ((long)blockIdx.x - s.nblocks) * (NT / 64) + (threadIdx.x >> 6);
+    const long step = ((long)gridDim.x - s.nblocks) * (NT / 64);
+    if (s.vec)
+        zero_rows<T, true>((T *)s.dst, s.dst_stride, s.d, v0, v1, first, step);
+    else
+        zero_rows<T, false>((T *)s.dst, s.dst_stride, s.d, v0, v1, first, step);
+}
+
+// cnt[digit][block] = keys of the block's tile with the pass's digit (the first pass forms the keys from
+// the tokens).  Counting a pass's digits while the pass before it moves the keys was 60 us slower at
+// 32768 positions: a few digits are most of the keys, and their counters take one atomic at a time.
+template <typename T>
+__global__ __launch_bounds__(NT) void k_radix_count(Sort s, int pass) {
+    if ((int)blockIdx.x >= s.nblocks) return sort_zero<T>(s);
     __shared__ unsigned h[RADIX];
     h[threadIdx.x] = 0;
     __syncthreads();
+    const unsigned *keys = s.keys[(pass & 1) ^ 1];
     const long base = (long)blockIdx.x * TILE;
-    for (int j = threadIdx.x; j < TILE; j += NT) {
-        const long i = base + j;
-        if (i < n) {
-            const unsigned k = FIRST ? key_of(tokens, i, vocab, err) : keys[i];
-            atomicAdd(&h[(k >> shift) & (RADIX - 1)], 1u);
-        }
+    unsigned k[TILE / NT];
+#pragma unroll
+    for (int j = 0; j < TILE / NT; ++j) {
+        const long i = base + j * NT + threadIdx.x;
+        k[j] = i >= s.n ? 0 : pass ? keys[i] : key_of(s.tokens, i, s.vocab, s.err);
     }
+#pragma unroll
+    for (int j = 0; j < TILE / NT; ++j)
+        if (base + j * NT + threadIdx.x < s.n) atomicAdd(&h[(k[j] >> (8 * pass)) & (RADIX - 1)], 1u);
     __syncthreads();
-    cnt[(long)threadIdx.x * nblocks + blockIdx.x] = h[threadIdx.x];
+    s.cnt[(long)threadIdx.x * s.nblocks + blockIdx.x] = h[threadIdx.x];
 }
 
 // Exclusive prefix sum in place over `m` counts, one block.
@@ -104,42 +242,73 @@ __global__ __launch_bounds__(1024) void k_scan(unsigned *cnt, long m) {
     }
 }
 
-// Moves each key and its position to its place: offset[digit][block] plus its rank among the
-// tile's keys of that digit, in order (stable).
-template <bool FIRST>
-__global__ __launch_bounds__(NT) void k_radix_move(const unsigned *keys, const int32_t *pos, const int32_t *tokens,
-                                                   int n, int vocab, int shift, const unsigned *offset, int nblocks,
-                                                   unsigned *keys_out, int32_t *pos_out) {
+// Moves each key and its position to its place: the number of smaller digits, of its digit in earlier
+// blocks, and its rank among the tile's keys of that digit (stable).
+template <typename T>
+__global__ __launch_bounds__(NT) void k_radix_move(Sort s, int pass) {
+    if ((int)blockIdx.x >= s.nblocks) return sort_zero<T>(s);
     __shared__ unsigned at[NT / 64][RADIX];  // next place of each wave's keys of a digit
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __shared__ unsigned wsum[NT / 64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, shift = 8 * pass;
+    const unsigned *cnt = s.cnt, *keys = s.keys[(pass & 1) ^ 1];
+    const int32_t *pos = s.pos[(pass & 1) ^ 1];
+    unsigned *keys_out = s.keys[pass & 1];
+    int32_t *pos_out = s.pos[pass & 1];
+#pragma unroll
     for (int q = 0; q < NT / 64; ++q) at[q][threadIdx.x] = 0;
-    __syncthreads();
+    // keys of the digit threadIdx.x: in earlier blocks, and in all
+    unsigned before = 0, all = 0;
+    if (s.own_prefix) {
+#pragma unroll 16
+        for (int b = 0; b < s.nblocks; ++b) {
+            const unsigned c = cnt[(long)threadIdx.x * s.nblocks + b];
+            before += b < (int)blockIdx.x ? c : 0;
+            all += c;
+        }
+    } else {
+        before = cnt[(long)threadIdx.x * s.nblocks + blockIdx.x];
+    }
     const long base = (long)blockIdx.x * TILE + (long)w * W_KEYS;
     unsigned key[W_KEYS / 64];
+    int32_t from[W_KEYS / 64];
 #pragma unroll
     for (int j = 0; j < W_KEYS / 64; ++j) {
         const long i = base + j * 64 + lane;
         key[j] = 0;
-        if (i < n) {
-            key[j] = FIRST ? key_of(tokens, i, vocab, nullptr) : keys[i];
-            atomicAdd(&at[w][(key[j] >> shift) & (RADIX - 1)], 1u);
+        from[j] = (int32_t)i;
+        if (i < s.n) {
+            key[j] = pass ? keys[i] : key_of(s.tokens, i, s.vocab, nullptr);
+            if (pass) from[j] = pos[i];
         }
     }
-    __syncthreads();
-    {
-        unsigned o = offset[(long)threadIdx.x * nblocks + blockIdx.x];
+    if (s.own_prefix) {  // plus the keys of smaller digits
+        unsigned sum = all;
 #pragma unroll
-        for (int q = 0; q < NT / 64; ++q) {
-            const unsigned c = at[q][threadIdx.x];
-            at[q][threadIdx.x] = o;
-            o += c;
+        for (int off = 1; off < 64; off <<= 1) {
+            const unsigned o = __shfl_up(sum, off, 64);
+            if (lane >= off) sum += o;
         }
+        if (lane == 63) wsum[w] = sum;
+        __syncthreads();
+        before += sum - all;
+        for (int q = 0; q < w; ++q) before += wsum[q];
+    } else {
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < W_KEYS / 64; ++j)
+        if (base + j * 64 + lane < s.n) atomicAdd(&at[w][(key[j] >> shift) & (RADIX - 1)], 1u);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NT / 64; ++q) {
+        const unsigned c = at[q][threadIdx.x];
+        at[q][threadIdx.x] = before;
+        before += c;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < W_KEYS / 64; ++j) {
-        const long i = base + j * 64 + lane;
-        const bool in = i < n;
+        const bool in = base + j * 64 + lane < s.n;
         const unsigned dig = (key[j] >> shift) & (RADIX - 1);
         unsigned long long same = __ballot(in);
 #pragma unroll
@@ -155,24 +324,12 @@ __global__ __launch_bounds__(NT) void k_radix_move(const unsigned *keys, const i
         __builtin_amdgcn_wave_barrier();
         if (in) {
             keys_out[o + rank] = key[j];
-            pos_out[o + rank] = FIRST ? (int32_t)i : pos[i];
+            pos_out[o + rank] = from[j];
         }
     }
 }
 
 // ---- sums of the sorted rows ----------------------------------------------------------------
-template <typename T, bool VEC>
-__global__ __launch_bounds__(NT) void k_zero_table(T *dst, int vocab, int d, long stride) {
-    constexpr int W = VEC ? 16 / (int)sizeof(T) : 1;
-    typedef typename VecT<T, W>::type V;
-    V z;
-#pragma unroll
-    for (int j = 0; j < W; ++j) z[j] = from_f32<T>(0.0f);
-    const int lane = threadIdx.x & 63;
-    for (long v = (long)blockIdx.x * (NT / 64) + (threadIdx.x >> 6); v < vocab; v += (long)gridDim.x * (NT / 64))
-        for (int c = lane * W; c < d; c += 64 * W) *reinterpret_cast<V *>(dst + v * stride + c) = z;
-}
-
 // A wave adds the rows of sorted entries [chunk C, + C) in order, 64 W columns from strip * 64 W.
 // part[chunk][0]: the sum of a table row that began in an earlier chunk; part[chunk][1]: of one
 // that begins here and goes on in the next.
@@ -186,68 +343,93 @@ __global__ __launch_bounds__(64) void k_chunk_sums(TableParams p, const unsigned
     const long b = a + C < p.n ? a + C : (long)p.n;
     const int c = (int)(blockIdx.y * 64 + lane) * W;
     const bool in = c < p.d;
-    const unsigned none = (unsigned)p.vocab;
+    const int cc = in ? c : 0;  // lanes beyond the row load what they do not use
     float acc[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-    bool began = a == 0 || keys[a - 1] != keys[a];  // the current table row begins in this chunk
-    for (long e = a; e < b; ++e) {
-        const unsigned k = keys[e];
-        if (k >= none) break;  // positions without a token are the last ones
-        if (in) {
-            const V v = *reinterpret_cast<const V *>((const T *)p.src + (long)pos[e] * p.src_stride + c);
+    bool began = a == 0;  // the current table row begins in this chunk
+    // C0 entries: keys of entries e0 - 1 .. e0 + C0 in the lanes 0 .. C0 + 1, positions in 0 .. C0 - 1
+    for (long e0 = a; e0 < b; e0 += C0) {
+        const long ke = e0 - 1 + lane;
+        const int kl = lane < C0 + 2 && ke >= 0 && ke < p.n ? (int)keys[ke] : -1;
+        const int pl = lane < C0 && e0 + lane < b ? pos[e0 + lane] : 0;
+        if (e0 == a && a > 0) began = __builtin_amdgcn_readlane(kl, 0) != __builtin_amdgcn_readlane(kl, 1);
+        if (__builtin_amdgcn_readlane(kl, 1) >= p.vocab) break;  // positions without a token are the last ones
 #pragma unroll
-            for (int j = 0; j < W; ++j) acc[j] += to_f32<T>(v[j]);
-        }
-        const bool last = e + 1 == p.n || keys[e + 1] != k;  // the table row's last position
-        if (!last && e + 1 < b) continue;
-        if (in) {
-            if (last && began) {
-                V o;
+        for (int g = 0; g < C0; g += 8) {
+            if (e0 + g >= b) break;
+            V v[8];
 #pragma unroll
-                for (int j = 0; j < W; ++j) o[j] = from_f32<T>(acc[j] * p.scale);
-                *reinterpret_cast<V *>((T *)p.dst + (long)k * p.dst_stride + c) = o;
-            } else {
-                float *q = part + (chunk * 2 + (began ? 1 : 0)) * p.d + c;
+            for (int u = 0; u < 8; ++u) {
+                const long at = __builtin_amdgcn_readlane(pl, g + u);  // 0 behind the end: not used
+                v[u] = *reinterpret_cast<const V *>((const T *)p.src + at * p.src_stride + cc);
+            }
 #pragma unroll
-                for (int j = 0; j < W; ++j) q[j] = acc[j];
+            for (int u = 0; u < 8; ++u) {
+                const int k = __builtin_amdgcn_readlane(kl, g + u + 1), kn = __builtin_amdgcn_readlane(kl, g + u + 2);
+                if (e0 + g + u >= b || k >= p.vocab) break;
+#pragma unroll
+                for (int j = 0; j < W; ++j) acc[j] += to_f32<T>(v[u][j]);
+                const bool last = kn != k;  // the table row's last position
+                if (!last && e0 + g + u + 1 < b) continue;
+                if (in) {
+                    if (last && began) {
+                        V o;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) o[j] = from_f32<T>(acc[j] * p.scale);
+                        *reinterpret_cast<V *>((T *)p.dst + (long)k * p.dst_stride + c) = o;
+                    } else {
+                        float *q = part + (chunk * 2 + (began ? 1 : 0)) * p.d + c;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) q[j] = acc[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < W; ++j) acc[j] = 0.0f;
+                began = true;
             }
         }
-#pragma unroll
-        for (int j = 0; j < W; ++j) acc[j] = 0.0f;
-        began = true;
     }
 }
 
-// Table rows that begin in a chunk and end in a later one: their partial sums in chunk order.
+// Table rows that begin in a chunk and end in a later one: their partial sums in chunk order, the
+// waves a quarter of the chunks each.
 template <typename T>
-__global__ __launch_bounds__(64) void k_join_sums(TableParams p, const unsigned *keys, int C, const float *part) {
+__global__ __launch_bounds__(NT) void k_join_sums(TableParams p, const unsigned *keys, int C, const float *part) {
+    __shared__ float sum[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long chunk = blockIdx.x, a = chunk * C, b = a + C;
     if (b >= p.n) return;
-    const unsigned k = keys[b - 1];
-    if (k >= (unsigned)p.vocab || keys[b] != k) return;       // nothing goes on
-    if (keys[a] == k && a > 0 && keys[a - 1] == k) return;    // it began in an earlier chunk
-    // the chunks that hold the rest: from the next one to the one with its last position
-    long lo = b, hi = p.n;  // first sorted entry behind it
-    while (lo < hi) {
-        const long mid = (lo + hi) / 2;
-        if (keys[mid] <= k)
-            lo = mid + 1;
-        else
-            hi = mid;
+    const unsigned k = keys[b - 1], kb = keys[b], ka = keys[a], kz = keys[a > 0 ? a - 1 : 0];
+    if (k >= (unsigned)p.vocab || kb != k) return;  // nothing goes on
+    if (a > 0 && ka == k && kz == k) return;        // it began in an earlier chunk
+    // the chunks that begin with the row: chunk + 1 .. chunk + m
+    const long chunks = (p.n + C - 1) / C;
+    long m = 0;
+    for (;;) {
+        const long q = chunk + 1 + m + lane;
+        const unsigned long long on = __ballot(q < chunks && keys[min(q * C, (long)p.n - 1)] == k);
+        m += on == ~0ull ? 64 : __ffsll(~on) - 1;
+        if (on != ~0ull) break;
     }
-    const long end = (lo - 1) / C;
-    const int c = (int)(blockIdx.y * 64 + threadIdx.x);
-    if (c >= p.d) return;
-    float acc = part[(chunk * 2 + 1) * p.d + c];
-#pragma unroll 8
-    for (long q = chunk + 1; q <= end; ++q) acc += part[q * 2 * p.d + c];
+    const int c = (int)(blockIdx.y * 64 + lane);
+    const long per = (m + 3) / 4, q0 = chunk + 1 + min(m, wave * per), q1 = chunk + 1 + min(m, (wave + 1) * per);
+    float acc = 0.0f;
+    if (c < p.d) {
+        if (wave == 0) acc = part[(chunk * 2 + 1) * p.d + c];
+#pragma unroll 16
+        for (long q = q0; q < q1; ++q) acc += part[q * 2 * p.d + c];
+    }
+    if (wave) sum[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave || c >= p.d) return;
+    acc = ((acc + sum[0][lane]) + sum[1][lane]) + sum[2][lane];
     ((T *)p.dst)[(long)k * p.dst_stride + c] = from_f32<T>(acc * p.scale);
 }
 
-// Sorted entries a chunk: 32, more where there would be over 2048 chunks (a frequent token's
-// partial sums are added one after another).
-int chunk_len(long n) { return (int)std::max<long>(32, (n + 2047) / 2048); }
+// Sorted entries a chunk: C0, more where there would be over 2048 chunks (a frequent token's partial
+// sums are added one after another).
+int chunk_len(long n) { return (int)((std::max<long>(C0, (n + 2047) / 2048) + C0 - 1) / C0 * C0); }
 
 struct GradLayout {
     size_t keys[2], pos[2], cnt, part, bytes;
@@ -289,55 +471,62 @@ void launch_embed_lookup(const TableParams &p, hipStream_t st) {
     });
 }
 
-size_t embed_grad_workspace_bytes(const TableParams &p) { return grad_layout(p).bytes; }
+size_t embed_grad_workspace_bytes(const TableParams &p) { return p.n <= FEW ? 0 : grad_layout(p).bytes; }
 
 void launch_embed_grad(const TableParams &p, void *ws, hipStream_t st) {
     const int eb = elem_bytes(p.dtype);
     const bool vdst = rows_vec16(p.dst, p.dst_stride, p.d, eb);
-    dispatch_type(p.dtype, [&](auto t) {
-        typedef decltype(t) T;
-        const unsigned grid = (unsigned)std::min<long>(2048, ((long)p.vocab + NT / 64 - 1) / (NT / 64));
-        if (vdst)
-            k_zero_table<T, true><<<grid, NT, 0, st>>>((T *)p.dst, p.vocab, p.d, p.dst_stride);
-        else
-            k_zero_table<T, false><<<grid, NT, 0, st>>>((T *)p.dst, p.vocab, p.d, p.dst_stride);
-    });
-    if (p.n == 0) return;
+    const bool vec = vdst && rows_vec16(p.src, p.src_stride, p.d, eb);
+    if (p.n <= FEW) {
+        dispatch_type(p.dtype, [&](auto t) {
+            typedef decltype(t) T;
+            const unsigned grid = (unsigned)(p.n + (p.vocab + FEW_ROWS - 1) / FEW_ROWS);
+            if (vec)
+                k_grad_few<T, true><<<grid, NT, 0, st>>>(p);
+            else
+                k_grad_few<T, false><<<grid, NT, 0, st>>>(p);
+        });
+        return;
+    }
     const GradLayout L = grad_layout(p);
     char *w = (char *)ws;
-    unsigned *keys[2] = {(unsigned *)(w + L.keys[0]), (unsigned *)(w + L.keys[1])};
-    int32_t *pos[2] = {(int32_t *)(w + L.pos[0]), (int32_t *)(w + L.pos[1])};
-    unsigned *cnt = (unsigned *)(w + L.cnt);
-    float *part = (float *)(w + L.part);
-    int cur = 0;
-    for (int shift = 0; shift < 32 && (shift == 0 || (p.vocab >> shift) > 0); shift += 8) {  // keys are 0 .. vocab
-        const int nxt = shift ? cur ^ 1 : 0;
-        if (shift == 0) {
-            k_radix_count<true><<<L.nblocks, NT, 0, st>>>(nullptr, p.tokens, p.n, p.vocab, 0, cnt, L.nblocks, p.err);
-            k_scan<<<1, 1024, 0, st>>>(cnt, (long)RADIX * L.nblocks);
-            k_radix_move<true><<<L.nblocks, NT, 0, st>>>(nullptr, nullptr, p.tokens, p.n, p.vocab, 0, cnt, L.nblocks,
-                                                         keys[nxt], pos[nxt]);
-        } else {
-            k_radix_count<false><<<L.nblocks, NT, 0, st>>>(keys[cur], nullptr, p.n, p.vocab, shift, cnt, L.nblocks,
-                                                           nullptr);
-            k_scan<<<1, 1024, 0, st>>>(cnt, (long)RADIX * L.nblocks);
-            k_radix_move<false><<<L.nblocks, NT, 0, st>>>(keys[cur], pos[cur], nullptr, p.n, p.vocab, shift, cnt,
-                                                          L.nblocks, keys[nxt], pos[nxt]);
-        }
-        cur = nxt;
+    Sort s{};
+    s.tokens = p.tokens, s.n = p.n, s.vocab = p.vocab, s.nblocks = L.nblocks;
+    for (int i = 0; i < 2; ++i) {
+        s.keys[i] = (unsigned *)(w + L.keys[i]);
+        s.pos[i] = (int32_t *)(w + L.pos[i]);
     }
+    s.cnt = (unsigned *)(w + L.cnt);
+    s.passes = 1;
+    while (s.passes < 4 && (p.vocab >> (8 * s.passes)) > 0) ++s.passes;  // keys are 0 .. vocab
+    s.own_prefix = L.nblocks <= OWN_PREFIX;
+    s.err = p.err;
+    s.dst = p.dst, s.dst_stride = p.dst_stride, s.d = p.d, s.vec = vdst;
+    s.launches = 2 * s.passes;
+    float *part = (float *)(w + L.part);
     const int C = chunk_len(p.n);
     const unsigned chunks = (unsigned)(((long)p.n + C - 1) / C);
-    const bool vec = vdst && rows_vec16(p.src, p.src_stride, p.d, eb);
+    const long counts = (long)RADIX * L.nblocks;
     dispatch_type(p.dtype, [&](auto t) {
         typedef decltype(t) T;
+        // zero-writing blocks: a wave has about eight rows of a launch's share
+        const unsigned zb = (unsigned)std::max<long>(1, std::min<long>(1024, p.vocab / (s.launches * 32L)));
+        for (int pass = 0; pass < s.passes; ++pass) {
+            s.launch = 2 * pass;
+            k_radix_count<T><<<L.nblocks + zb, NT, 0, st>>>(s, pass);
+            if (!s.own_prefix) k_scan<<<1, 1024, 0, st>>>(s.cnt, counts);
+            s.launch = 2 * pass + 1;
+            k_radix_move<T><<<L.nblocks + zb, NT, 0, st>>>(s, pass);
+        }
+        const unsigned *keys = s.keys[(s.passes & 1) ^ 1];
+        const int32_t *pos = s.pos[(s.passes & 1) ^ 1];
         const int W = vec ? 16 / (int)sizeof(T) : 1;
         const dim3 grid(chunks, (unsigned)((p.d + 64 * W - 1) / (64 * W)));
         if (vec)
-            k_chunk_sums<T, true><<<grid, 64, 0, st>>>(p, keys[cur], pos[cur], C, part);
+            k_chunk_sums<T, true><<<grid, 64, 0, st>>>(p, keys, pos, C, part);
         else
-            k_chunk_sums<T, false><<<grid, 64, 0, st>>>(p, keys[cur], pos[cur], C, part);
-        k_join_sums<T><<<dim3(chunks, (unsigned)((p.d + 63) / 64)), 64, 0, st>>>(p, keys[cur], C, part);
+            k_chunk_sums<T, false><<<grid, 64, 0, st>>>(p, keys, pos, C, part);
+        k_join_sums<T><<<dim3(chunks, (unsigned)((p.d + 63) / 64)), NT, 0, st>>>(p, keys, C, part);
     });
 }
 

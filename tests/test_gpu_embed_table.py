@@ -224,7 +224,7 @@ def test_capture_before_the_workspace_is_there():
     b = GpuDeqBackend(synth.ModelConfig(d=64, H=2, V=300, N=1, flags=0), 1, 1)
     stream = torch.cuda.Stream()
     b.set_stream(stream.cuda_stream)
-    table, dout, toks = make(300, 64, 90, F32)
+    table, dout, toks = make(3000, 64, 90, F32)  # sorted: up to 1024 positions need no workspace
     out = torch.zeros_like(table)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
