@@ -51,7 +51,15 @@ def _dev_i(t) -> Optional[C.POINTER(C.c_int32)]:
     return None if t is None else C.cast(C.c_void_p(t.data_ptr()), _I32P)
 
 
-_DTYPES = {"torch.float32": _lib.ADN_T_F32, "torch.bfloat16": _lib.ADN_T_BF16}
+_DTYPE_NAMES = {"torch.float32": _lib.ADN_T_F32, "torch.bfloat16": _lib.ADN_T_BF16, "torch.int32": "i32"}
+_DTYPES: Dict[object, object] = {}  # torch dtype -> ADN_T_* or "i32", None for any other; filled as they are met
+
+
+def _dtype_code(dtype):
+    try:
+        return _DTYPES[dtype]
+    except KeyError:
+        return _DTYPES.setdefault(dtype, _DTYPE_NAMES.get(str(dtype)))
 
 
 def _invalid(msg: str) -> "_lib.AdnError":
@@ -266,27 +274,27 @@ class GpuDeqBackend:
     # call alike) with adjacent elements in a row and any row stride, vectors float32, ids int32.
     def _matrix(self, t, name: str, rows: int, d: int, dtype=None):
         """(pointer, row stride) of a [rows][d] tensor."""
-        if tuple(t.shape) != (rows, d):
+        if t.shape != (rows, d):
             raise _invalid(f"{name} must have the shape ({rows}, {d}), got {tuple(t.shape)}")
         if dtype is not None and t.dtype != dtype:
             raise _invalid(f"{name} must be {dtype} as the call's other matrices, got {t.dtype}")
-        self._on_device(t, name)
-        if d > 1 and t.stride(1) != 1:
+        if t.get_device() != self.device:
+            raise _invalid(f"{name} must be on the context's GPU (cuda:{self.device}), got {t.device}")
+        stride, unit = t.stride()
+        if unit != 1 and d > 1:
             raise _invalid(f"{name}: the elements of a row must be adjacent")
-        return t.data_ptr(), (t.stride(0) if rows > 1 else d)
+        return t.data_ptr(), (stride if rows > 1 else d)
 
-    def _vector(self, t, name: str, n: int, dtype: str = "torch.float32"):
+    def _vector(self, t, name: str, n: int, code=_lib.ADN_T_F32):
         """Pointer of a contiguous [n] tensor; None for None."""
         if t is None:
             return None
-        if t.dim() != 1 or t.shape[0] != n or str(t.dtype) != dtype or (n > 1 and t.stride(0) != 1):
-            raise _invalid(f"{name} must be a contiguous {dtype} tensor of {n} elements")
-        self._on_device(t, name)
-        return t.data_ptr()
-
-    def _on_device(self, t, name: str) -> None:
-        if not t.is_cuda or t.device.index != self.device:
+        if t.dim() != 1 or t.shape[0] != n or _dtype_code(t.dtype) != code or (n > 1 and t.stride(0) != 1):
+            kind = "torch.int32" if code == "i32" else "torch.float32"
+            raise _invalid(f"{name} must be a contiguous {kind} tensor of {n} elements")
+        if t.get_device() != self.device:
             raise _invalid(f"{name} must be on the context's GPU (cuda:{self.device}), got {t.device}")
+        return t.data_ptr()
 
     @property
     def device(self) -> int:
@@ -299,8 +307,8 @@ class GpuDeqBackend:
 
     @staticmethod
     def _dtype(t) -> int:
-        code = _DTYPES.get(str(t.dtype))
-        if code is None:
+        code = _dtype_code(t.dtype)
+        if code is None or code == "i32":
             raise _invalid(f"float32 or bfloat16 expected, got {t.dtype}")
         return code
 
@@ -321,7 +329,7 @@ class GpuDeqBackend:
         if w is not None:
             a.w, a.w_stride = self._matrix(w, "w", V, d, x.dtype)
         a.bias = self._vector(bias, "bias", V)
-        a.targets = self._vector(targets, "targets", rows, "torch.int32")
+        a.targets = self._vector(targets, "targets", rows, "i32")
         a.dloss = self._vector(dloss, "dloss", rows)
         a.loss = self._vector(outputs.get("loss"), "loss", rows)
         a.lse = self._vector(outputs.get("lse"), "lse", rows)
@@ -374,7 +382,7 @@ class GpuDeqBackend:
         tp, ts = (None, d) if table is None else self._matrix(table, "table", V, d, out.dtype)
         op, os_ = self._matrix(out, "out", n, d)
         check(lib().adn_embed_lookup_async(self._ctx, n, d, V, self._dtype(out),
-                                           self._vector(tokens, "tokens", n, "torch.int32"), tp, ts, scale, op, os_))
+                                           self._vector(tokens, "tokens", n, "i32"), tp, ts, scale, op, os_))
 
     def embed_grad_async(self, dout, tokens, dtable, *, scale: float = 1.0) -> None:
         """The table's gradient: dtable[v] = scale * sum of the rows dout[i] with tokens[i] = v, in the
@@ -386,7 +394,7 @@ class GpuDeqBackend:
         sp, ss = self._matrix(dout, "dout", n, d)
         dp, ds = self._matrix(dtable, "dtable", V, d, dout.dtype)
         check(lib().adn_embed_grad_async(self._ctx, n, d, V, self._dtype(dout),
-                                         self._vector(tokens, "tokens", n, "torch.int32"), sp, ss, scale, dp, ds))
+                                         self._vector(tokens, "tokens", n, "i32"), sp, ss, scale, dp, ds))
 
     # reference-named conveniences ---------------------------------------------------------
     def run_forward_deq(self, batch, seq, max_iters, eps, damping, s_in):

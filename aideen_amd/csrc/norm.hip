@@ -31,31 +31,22 @@ struct Cols {
     __device__ __forceinline__ static int col(int lane, int e) { return ((e / W) * TEAM + lane) * W + e % W; }
 };
 
+// A lane's share of a row as it is loaded: E elements in pieces of W.
 template <typename T, int TEAM, int E, bool VEC>
-__device__ __forceinline__ void load_row(const T *row, int d, int lane, float (&v)[E]) {
+struct Row {
     typedef Cols<T, TEAM, VEC> C;
-    if constexpr (VEC) {
-        typedef typename VecOf<T, C::W>::type V;
+    typedef typename VecOf<T, C::W>::type V;
+    V v[E / C::W];
+    __device__ __forceinline__ void load(const T *row, int d, int lane) {
 #pragma unroll
-        for (int e = 0; e < E; e += C::W) {
-            const int c = C::col(lane, e);
-            if (c < d) {
-                const V x = *reinterpret_cast<const V *>(row + c);
-#pragma unroll
-                for (int j = 0; j < C::W; ++j) v[e + j] = to_f32<T>(x[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < C::W; ++j) v[e + j] = 0.0f;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int c = C::col(lane, e);
-            v[e] = c < d ? to_f32<T>(row[c]) : 0.0f;
+        for (int q = 0; q < E / C::W; ++q) {
+            const int c = C::col(lane, q * C::W);
+            v[q] = V{};
+            if (c < d) v[q] = *reinterpret_cast<const V *>(row + c);
         }
     }
-}
+    __device__ __forceinline__ float operator[](int e) const { return to_f32<T>(v[e / C::W][e % C::W]); }
+};
 
 template <typename T, int TEAM, int E, bool VEC>
 __device__ __forceinline__ void store_row(T *row, int d, int lane, const float (&v)[E]) {
@@ -118,12 +109,16 @@ __global__ __launch_bounds__(NB) void k_rms_norm(NormParams p) {
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
     const long row = (long)blockIdx.x * (NB / TEAM) + team;
     if (row >= p.rows) return;  // a whole wave (TEAM 64) or never (a block a row)
+    Row<T, TEAM, E, VEC> x;
     float v[E], g[E];
-    load_row<T, TEAM, E, VEC>((const T *)p.x + row * p.x_stride, p.d, lane, v);
+    x.load((const T *)p.x + row * p.x_stride, p.d, lane);
     load_gain<T, TEAM, E, VEC>(p.gain, p.d, lane, g);
     float s[1] = {0.0f};
 #pragma unroll
-    for (int e = 0; e < E; ++e) s[0] += v[e] * v[e];
+    for (int e = 0; e < E; ++e) {
+        v[e] = x[e];
+        s[0] += v[e] * v[e];
+    }
     team_sum<TEAM, 1>(s, red);
     const float r = 1.0f / sqrtf(s[0] / (float)p.d + p.eps);
 #pragma unroll
@@ -140,10 +135,20 @@ __global__ __launch_bounds__(NB) void k_rms_norm_back(NormParams p, float *part)
     load_gain<T, TEAM, E, VEC>(p.gain, p.d, lane, g);
 #pragma unroll
     for (int e = 0; e < E; ++e) dg[e] = 0.0f;
-    for (long row = (long)blockIdx.x * TEAMS + team; row < p.rows; row += (long)gridDim.x * TEAMS) {
-        float x[E], dy[E];
-        load_row<T, TEAM, E, VEC>((const T *)p.x + row * p.x_stride, p.d, lane, x);
-        load_row<T, TEAM, E, VEC>((const T *)p.dy + row * p.dy_stride, p.d, lane, dy);
+    // the next row is loaded while this one is used
+    const long step = (long)gridDim.x * TEAMS;
+    long row = (long)blockIdx.x * TEAMS + team;
+    Row<T, TEAM, E, VEC> xn, dyn;
+    if (row < p.rows) {
+        xn.load((const T *)p.x + row * p.x_stride, p.d, lane);
+        dyn.load((const T *)p.dy + row * p.dy_stride, p.d, lane);
+    }
+    for (; row < p.rows; row += step) {
+        const Row<T, TEAM, E, VEC> x = xn, dy = dyn;
+        if (row + step < p.rows) {
+            xn.load((const T *)p.x + (row + step) * p.x_stride, p.d, lane);
+            dyn.load((const T *)p.dy + (row + step) * p.dy_stride, p.d, lane);
+        }
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -153,12 +158,13 @@ __global__ __launch_bounds__(NB) void k_rms_norm_back(NormParams p, float *part)
         team_sum<TEAM, 2>(s, red);
         const float r = 1.0f / sqrtf(s[0] / (float)p.d + p.eps);
         const float k = r * r * (s[1] / (float)p.d);
+        float dx[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             dg[e] += dy[e] * (x[e] * r);
-            x[e] = r * (dy[e] * g[e] - x[e] * k);
+            dx[e] = r * (dy[e] * g[e] - x[e] * k);
         }
-        if (p.dx) store_row<T, TEAM, E, VEC>((T *)p.dx + row * p.dx_stride, p.d, lane, x);
+        if (p.dx) store_row<T, TEAM, E, VEC>((T *)p.dx + row * p.dx_stride, p.d, lane, dx);
     }
     if (!part) return;
     // the block's teams in order, then one partial row a block
@@ -182,24 +188,25 @@ __global__ __launch_bounds__(NB) void k_rms_norm_back(NormParams p, float *part)
     }
 }
 
-// dst[c] = sum over the n partial rows: four waves of a block each take a quarter of the rows of 64
-// columns in order, then the quarters in order.
-__global__ __launch_bounds__(NB) void k_sum_rows(const float *part, int n, int d, float *dst) {
-    __shared__ float red[NB / 64][64];
+// dst[c] = sum over the n partial rows: 16 waves of a block each take a share of the rows of 64 columns
+// in order, then the shares in order.
+__global__ __launch_bounds__(1024) void k_sum_rows(const float *part, int n, int d, float *dst) {
+    constexpr int WAVES = 16;
+    __shared__ float red[WAVES][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int c = blockIdx.x * 64 + lane;
-    const int per = (n + NB / 64 - 1) / (NB / 64);
+    const int per = (n + WAVES - 1) / WAVES;
     const int a = w * per, b = min(n, a + per);
     float s = 0.0f;
     if (c < d) {
-#pragma unroll 8
+#pragma unroll 16
         for (int i = a; i < b; ++i) s += part[(long)i * d + c];
     }
     red[w][lane] = s;
     __syncthreads();
     if (w == 0 && c < d) {
 #pragma unroll
-        for (int q = 1; q < NB / 64; ++q) s += red[q][lane];
+        for (int q = 1; q < WAVES; ++q) s += red[q][lane];
         dst[c] = s;
     }
 }
@@ -262,7 +269,7 @@ void launch_norm_backward(const NormParams &p, void *ws, hipStream_t st) {
                     k_rms_norm_back<T, TEAM, E, false><<<blocks, NB, 0, st>>>(p, part);
             });
         });
-    if (p.dg) k_sum_rows<<<(p.d + 63) / 64, NB, 0, st>>>(part, blocks, p.d, p.dg);
+    if (p.dg) k_sum_rows<<<(p.d + 63) / 64, 1024, 0, st>>>(part, blocks, p.d, p.dg);
 }
 
 }  // namespace adn
