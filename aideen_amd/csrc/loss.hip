@@ -44,7 +44,6 @@ constexpr int NT = 256;             // threads a workgroup: 4 waves
 constexpr size_t PIECE_BYTES = 256u << 20;
 constexpr int BM = 128;             // rows of a gradient tile
 constexpr int TV = 256;             // entries a workgroup of the logits' product covers
-constexpr int STAGES = 3;           // k slices of the LDS ring
 constexpr int NW = 4;               // waves of a workgroup
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int XR = 8;               // rows of x a block splits
@@ -140,7 +139,10 @@ struct Tile {
     static constexpr int KB = NP == 2 ? 1 : 2;
     static constexpr int TM = WGM * WTM * 32, TN = WGN * WTN * 32;
     static constexpr int A_BLK = TM / 32 * KB, B_BLK = TN / 32 * KB;  // 1 KB loads a plane and slice
-    static constexpr int RING = STAGES * NP * (A_BLK + B_BLK) * 512;  // halves
+    static constexpr int SLICE = NP * (A_BLK + B_BLK) * 512;           // halves of a k slice
+    // slices of the LDS ring: what half of a CU's LDS holds, three to six
+    static constexpr int FIT = 80 * 512 / SLICE, STAGES = FIT < 3 ? 3 : FIT > 6 ? 6 : FIT;
+    static constexpr int RING = STAGES * SLICE;
     static_assert(WGM * WGN == 4, "four waves");
     static_assert(RING * 2 <= 80 * 1024, "two workgroups a CU");
 };
@@ -148,11 +150,11 @@ struct Tile {
 template <int MODE, typename T, int NP, int WTM, int WTN, int WGM, int WGN, bool TRA, bool TRB>
 __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *ring) {
     typedef Tile<NP, WTM, WTN, WGM, WGN> G;
-    constexpr int KB = G::KB, TM = G::TM, TN = G::TN, A_BLK = G::A_BLK, B_BLK = G::B_BLK;
+    constexpr int KB = G::KB, TM = G::TM, TN = G::TN, A_BLK = G::A_BLK, B_BLK = G::B_BLK, STAGES = G::STAGES;
     constexpr int A_PW = (A_BLK + NW - 1) / NW, B_PW = (B_BLK + NW - 1) / NW;
     constexpr int LOADS = NP * (A_PW + B_PW);
     constexpr int A_SZ = A_BLK * 512, B_SZ = B_BLK * 512;      // halves a plane and slice
-    constexpr int SLICE = NP * (A_SZ + B_SZ);
+    constexpr int SLICE = G::SLICE;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
@@ -775,10 +777,24 @@ struct LossPlan {
     size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, e_dw, dz, dx_part, dw_part, db_part, bytes;
 };
 
-// K of `len` (a multiple of 32) in at most `want` shares of whole 32s
+// K of `len` (a multiple of 32) in at most `want` shares of whole 32s, each not empty
 void split_k(long len, long want, int *split, int *share) {
     *share = (int)round_up((len + want - 1) / want, 32);
     *split = (int)((len + *share - 1) / *share);
+}
+
+// Rows a workgroup of the logits' product covers.  A k slice takes a tile of 128, 64 or 32 rows about 0.8,
+// 0.5 or 0.38 us, whether the chip is full (then its products) or not (then a round trip): 2000 rows
+// against 512 entries run 26 us on 128 rows a tile and 13 on 32, 8192 against 50257 best on 128.
+int pick_tn(long rows, long v_tiles) {
+    int best = 128;
+    double least = INFINITY;
+    for (int tn : {128, 64, 32}) {
+        const double n = (double)((rows + tn - 1) / tn * v_tiles) / SLOTS;
+        const double t = (n <= 1 ? 1.0 : n + 0.3) * (tn == 128 ? 0.8 : tn == 64 ? 0.5 : 0.38);
+        if (t < least) least = t, best = tn;
+    }
+    return best;
 }
 
 // Time of n1 units of length a and then n2 of length b (a >= b) on SLOTS slots, in order.
@@ -790,46 +806,56 @@ double makespan(long n1, double a, long n2, double b) {
     return t + (m1 ? a : 0.0) + (double)((n2 - fit + SLOTS - 1) / SLOTS) * b;
 }
 
-// Shares of the two gradients' K: the pair with the shortest estimated time of their common launch, in
-// values of K of a unit.  A unit is its K plus EPI for its prologue and epilogue (stores of a tile: as
-// long as about 200 values of K).  Partial sums are written and read again: two passes of their bytes
-// at 5 TB/s, where a value of K takes a unit about 0.044 us (two planes) or 0.022 us (one).
+// Columns of the gradients' tiles and the shares of their K: the choice with the shortest estimated time of
+// the common launch, in values of K of a unit of 128 x 256.  A narrower tile takes 0.62 (128 columns) or
+// 0.45 (64) of it a value of K (2000 rows against 512 entries of 512: 103, 99 and 96 us a call), a
+// prologue and epilogue as long as 60 values and 140 more for the stores of 256 columns.  Partial sums
+// are written and read again: two passes of their bytes at 5 TB/s, where a value of K takes a unit about
+// 0.044 us (two planes) or 0.022 us (one).
 struct GradSizes {
-    int np;
-    long dx_tiles, dx_k, dx_elems;  // elements of dx, of a piece of dW
-    long dw_tiles, dw_k, dw_elems;
+    int np, d;
+    long dx_rows, dx_k, dx_elems;  // 128-row tiles, length of the sum, elements of dx; 0: not wanted
+    long dw_rows, dw_k, dw_elems;  // of a piece of dW
 };
-void pick_splits(const GradSizes &g, int *dx_split, int *dx_ks, int *dw_split, int *dw_ks) {
-    constexpr double EPI = 200;
-    constexpr int SHARES[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
+struct GradPick {
+    int bn, dx_split, dx_ks, dw_split, dw_ks;
+};
+GradPick pick_grads(const GradSizes &g) {
+    constexpr int SHARES[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
     const double join = 8.0 / (g.np == 2 ? 2.2e5 : 1.1e5);  // K values an element of a share
     double best = INFINITY;
-    for (int sx : SHARES) {
-        if (sx > 1 && g.dx_k / sx < 256) break;  // (none wanted: K = 0)
-        int nx = 0, kx = 32;
-        if (g.dx_tiles) split_k(g.dx_k, sx, &nx, &kx);
-        for (int sw : SHARES) {
-            if (sw > 1 && g.dw_k / sw < 256) break;
-            int nw = 0, kw = 32;
-            if (g.dw_tiles) split_k(g.dw_k, sw, &nw, &kw);
-            const double a = kx + EPI, b = kw + EPI;
-            double t = a >= b ? makespan(g.dx_tiles * nx, a, g.dw_tiles * nw, b)
-                              : makespan(g.dw_tiles * nw, b, g.dx_tiles * nx, a);
-            t += join * ((double)g.dx_elems * nx + (nw > 1 ? (double)g.dw_elems * nw : 0.0));
-            if (t < best) {
-                best = t;
-                if (g.dx_tiles) *dx_split = nx, *dx_ks = kx;
-                if (g.dw_tiles) *dw_split = nw, *dw_ks = kw;
+    GradPick pick{};
+    for (int bn : {256, 128, 64}) {
+        if (bn > 64 && g.d <= bn / 2) continue;
+        const double unit = bn == 256 ? 1.0 : bn == 128 ? 0.62 : 0.45, epi = 60 + 140.0 * bn / 256;
+        const long nbn = (g.d + bn - 1) / bn;
+        for (int sx : SHARES) {
+            if (sx > 1 && g.dx_k / sx < 256) break;
+            int nx = 0, kx = 32;
+            if (g.dx_rows) split_k(g.dx_k, sx, &nx, &kx);
+            for (int sw : SHARES) {
+                if (sw > 1 && g.dw_k / sw < 256) break;
+                int nw = 0, kw = 32;
+                if (g.dw_rows) split_k(g.dw_k, sw, &nw, &kw);
+                const double a = kx * unit + epi, b = kw * unit + epi;
+                const long ux = g.dx_rows * nbn * nx, uw = g.dw_rows * nbn * nw;
+                double t = a >= b ? makespan(ux, a, uw, b) : makespan(uw, b, ux, a);
+                t += join * ((double)g.dx_elems * nx + (nw > 1 ? (double)g.dw_elems * nw : 0.0));
+                if (t < best) {
+                    best = t;
+                    pick = {bn, nx, kx, nw, kw};
+                }
             }
         }
     }
+    return pick;
 }
 
 LossPlan loss_plan(const LossParams &p) {
     LossPlan L{};
     const bool grads = p.dx || p.dw || p.db;
     L.np = p.dtype == ADN_T_F32 ? 2 : 1;
-    L.tn = p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
+    L.tn = pick_tn(p.rows, round_up(p.vocab, TV) / TV);
     L.dcb = (int)(round_up(p.d, 32) / 16);
     L.rows_pad = round_up(p.rows, BM);
     L.v_pad = round_up(p.vocab, TV);
@@ -838,7 +864,6 @@ LossPlan loss_plan(const LossParams &p) {
     const long npieces = (L.v_pad + std::max<long>(TV, fit) - 1) / std::max<long>(TV, fit);
     L.piece = (int)round_up((L.v_pad + npieces - 1) / npieces, TV);
     L.w_blocks = (int)std::min<long>(W_BLOCKS, ((long)p.vocab * ((p.d + 7) / 8) + NT * 4 - 1) / (NT * 4));
-    L.bn = p.d > 128 ? 256 : p.d > 64 ? 128 : 64;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -860,15 +885,15 @@ LossPlan loss_plan(const LossParams &p) {
     L.lse = take(L.rows_pad * 4);
     L.e_dw = take(4);
     if (grads) {
-        const long nbn = (p.d + L.bn - 1) / L.bn;
         L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
-        GradSizes g{L.np};
-        if (p.dx) g.dx_tiles = round_up(p.rows, BM) / BM * nbn, g.dx_k = L.piece, g.dx_elems = (long)p.rows * p.d;
+        GradSizes g{L.np, p.d};
+        if (p.dx) g.dx_rows = round_up(p.rows, BM) / BM, g.dx_k = L.piece, g.dx_elems = (long)p.rows * p.d;
         if (p.dw) {
             const long n = std::min<long>(L.piece, p.vocab);
-            g.dw_tiles = round_up(n, BM) / BM * nbn, g.dw_k = round_up(p.rows, 32), g.dw_elems = n * p.d;
+            g.dw_rows = round_up(n, BM) / BM, g.dw_k = round_up(p.rows, 32), g.dw_elems = n * p.d;
         }
-        pick_splits(g, &L.dx_split, &L.dx_ks, &L.dw_split, &L.dw_ks);
+        const GradPick k = pick_grads(g);
+        L.bn = k.bn, L.dx_split = k.dx_split, L.dx_ks = k.dx_ks, L.dw_split = k.dw_split, L.dw_ks = k.dw_ks;
         if (p.dx) L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
         if (p.dw && L.dw_split > 1) L.dw_part = take((size_t)L.dw_split * L.piece * p.d * 4);
         if (p.db) L.db_part = take((size_t)(L.rows_pad / L.tn) * L.v_pad * 4);
