@@ -63,10 +63,11 @@ __device__ __forceinline__ void wait_vmcnt() {  // the other counters left alone
 
 // 16 bytes a lane from base + off (base wave-uniform, off in bytes) to the LDS address `lds` + 16 lane.
 // In assembly so that the compiler does not take the transposing LDS reads for uses of it and wait for
-// every load in flight before each: the waits are wait_vmcnt's.  It has no register output; one wait
-// state lies between the write of m0 and its use.
+// every load in flight before each: the waits are wait_vmcnt's.  It has no register output.  The compiler
+// does not see into it, so it keeps the wait states itself: one between the write of m0 and its use, five
+// before a scalar base that a vector instruction may just have written.
 __device__ __forceinline__ void load_lds(const void *base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base)
                  : "memory", "m0");

@@ -1987,24 +1987,30 @@ std::string first_of(std::initializer_list<std::string> msgs) {
 
 constexpr int TRAIN_MAX_ROWS = 1 << 24, LOSS_MAX_ROWS = 1 << 20;
 
-// Runs f() (the launches) on the context's device with `bytes` of workspace.
+// Runs f() with nothing thrown past the C entry.
 template <typename F>
-int train_launch(adn_ctx *c, size_t bytes, F &&f) {
+int train_entry(F &&f) {
     try {
-        DeviceScope scope(c->device);
-        void *ws = nullptr;
-        if (bytes) {
-            ws = train_workspace(c, bytes);
-            if (!ws) return ADN_E_CAPACITY;
-        }
-        f(ws);
-        ADN_HIP(hipGetLastError());
+        return f();
     } catch (const HipError &e) {
         (void)hipGetLastError();  // a refused allocation is not the next call's error
         return hip_fail(e);
     } catch (const std::exception &e) {
         return fail(ADN_E_HIP, e.what());
     }
+}
+
+// Runs f() (the launches) on the context's device with `bytes` of workspace.
+template <typename F>
+int train_launch(adn_ctx *c, size_t bytes, F &&f) {
+    DeviceScope scope(c->device);
+    void *ws = nullptr;
+    if (bytes) {
+        ws = train_workspace(c, bytes);
+        if (!ws) return ADN_E_CAPACITY;
+    }
+    f(ws);
+    ADN_HIP(hipGetLastError());
     return ADN_OK;
 }
 
@@ -2019,100 +2025,110 @@ int adn_context_device(const adn_ctx *c, int32_t *device) {
 }
 
 int adn_lm_loss_async(adn_ctx *c, const adn_lm_loss_args *a) {
-    if (!c || !a) return fail(ADN_E_INVALID, "null argument");
-    std::string msg = check_sizes(a->rows, LOSS_MAX_ROWS, a->d, a->vocab, a->dtype);
-    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
-    if (!a->loss && !a->lse && !a->dx && !a->dw && !a->db) return fail(ADN_E_INVALID, "no output is wanted");
-    LossParams p{};
-    p.rows = a->rows, p.d = a->d, p.vocab = a->vocab, p.dtype = a->dtype;
-    p.w = a->w, p.w_stride = a->w_stride, p.bias = a->bias;
-    if (!a->w) {
-        if (!c->has_weights) return fail(ADN_E_NO_WEIGHTS, "adn_lm_loss_async without w before adn_upload_weights");
-        if (a->dtype != ADN_T_F32 || a->d != c->D.d || a->vocab != c->D.V || a->bias)
-            return fail(ADN_E_INVALID, "w NULL is the context's head: ADN_T_F32, its d_r and vocab, bias NULL");
-        p.w = c->lm_w, p.w_stride = c->D.d, p.bias = c->lm_b;
-    }
-    msg = first_of({check_rows("x", a->x, a->x_stride, a->rows, a->d, a->dtype),
-                    check_rows("w", p.w, p.w_stride, a->vocab, a->d, a->dtype),
-                    a->dx ? check_rows("dx", a->dx, a->dx_stride, a->rows, a->d, a->dtype) : "",
-                    a->dw ? check_rows("dw", a->dw, a->dw_stride, a->vocab, a->d, a->dtype) : "",
-                    a->rows > 0 && !a->targets ? "null targets" : "", check_words("bias", p.bias),
-                    check_words("targets", a->targets), check_words("dloss", a->dloss), check_words("loss", a->loss),
-                    check_words("lse", a->lse), check_words("db", a->db)});
-    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
-    p.x = a->x, p.x_stride = a->x_stride;
-    p.targets = a->targets, p.dloss = a->dloss;
-    p.loss = a->loss, p.lse = a->lse;
-    p.dx = a->dx, p.dx_stride = a->dx_stride;
-    p.dw = a->dw, p.dw_stride = a->dw_stride;
-    p.db = a->db;
-    p.err = c->d_err;
-    return train_launch(c, loss_workspace_bytes(p), [&](void *ws) { launch_loss(p, ws, c->stream); });
+    return train_entry([&]() -> int {
+        if (!c || !a) return fail(ADN_E_INVALID, "null argument");
+        std::string msg = check_sizes(a->rows, LOSS_MAX_ROWS, a->d, a->vocab, a->dtype);
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        if (!a->loss && !a->lse && !a->dx && !a->dw && !a->db) return fail(ADN_E_INVALID, "no output is wanted");
+        LossParams p{};
+        p.rows = a->rows, p.d = a->d, p.vocab = a->vocab, p.dtype = a->dtype;
+        p.w = a->w, p.w_stride = a->w_stride, p.bias = a->bias;
+        if (!a->w) {
+            if (!c->has_weights) return fail(ADN_E_NO_WEIGHTS, "adn_lm_loss_async without w before adn_upload_weights");
+            if (a->dtype != ADN_T_F32 || a->d != c->D.d || a->vocab != c->D.V || a->bias)
+                return fail(ADN_E_INVALID, "w NULL is the context's head: ADN_T_F32, its d_r and vocab, bias NULL");
+            p.w = c->lm_w, p.w_stride = c->D.d, p.bias = c->lm_b;
+        }
+        msg = first_of({check_rows("x", a->x, a->x_stride, a->rows, a->d, a->dtype),
+                        check_rows("w", p.w, p.w_stride, a->vocab, a->d, a->dtype),
+                        a->dx ? check_rows("dx", a->dx, a->dx_stride, a->rows, a->d, a->dtype) : "",
+                        a->dw ? check_rows("dw", a->dw, a->dw_stride, a->vocab, a->d, a->dtype) : "",
+                        a->rows > 0 && !a->targets ? "null targets" : "", check_words("bias", p.bias),
+                        check_words("targets", a->targets), check_words("dloss", a->dloss), check_words("loss", a->loss),
+                        check_words("lse", a->lse), check_words("db", a->db)});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        p.x = a->x, p.x_stride = a->x_stride;
+        p.targets = a->targets, p.dloss = a->dloss;
+        p.loss = a->loss, p.lse = a->lse;
+        p.dx = a->dx, p.dx_stride = a->dx_stride;
+        p.dw = a->dw, p.dw_stride = a->dw_stride;
+        p.db = a->db;
+        p.err = c->d_err;
+        return train_launch(c, loss_workspace_bytes(p), [&](void *ws) { launch_loss(p, ws, c->stream); });
+    });
 }
 
 int adn_rms_norm_async(adn_ctx *c, int32_t rows, int32_t d, uint32_t dtype, const void *x, int64_t x_stride,
                        const float *gain, float eps, void *y, int64_t y_stride) {
-    if (!c) return fail(ADN_E_INVALID, "null context");
-    std::string msg = check_sizes(rows, TRAIN_MAX_ROWS, d, 1, dtype);
-    if (msg.empty())
-        msg = first_of({check_rows("x", x, x_stride, rows, d, dtype), check_rows("y", y, y_stride, rows, d, dtype),
-                        check_words("gain", gain), eps >= 0.0f ? "" : "eps must be >= 0"});
-    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
-    NormParams p{};
-    p.rows = rows, p.d = d, p.dtype = dtype;
-    p.x = x, p.x_stride = x_stride, p.gain = gain, p.eps = eps;
-    p.y = y, p.y_stride = y_stride;
-    return train_launch(c, 0, [&](void *) { launch_norm(p, c->stream); });
+    return train_entry([&]() -> int {
+        if (!c) return fail(ADN_E_INVALID, "null context");
+        std::string msg = check_sizes(rows, TRAIN_MAX_ROWS, d, 1, dtype);
+        if (msg.empty())
+            msg = first_of({check_rows("x", x, x_stride, rows, d, dtype), check_rows("y", y, y_stride, rows, d, dtype),
+                            check_words("gain", gain), eps >= 0.0f ? "" : "eps must be >= 0"});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        NormParams p{};
+        p.rows = rows, p.d = d, p.dtype = dtype;
+        p.x = x, p.x_stride = x_stride, p.gain = gain, p.eps = eps;
+        p.y = y, p.y_stride = y_stride;
+        return train_launch(c, 0, [&](void *) { launch_norm(p, c->stream); });
+    });
 }
 
 int adn_rms_norm_backward_async(adn_ctx *c, int32_t rows, int32_t d, uint32_t dtype, const void *x,
                                 int64_t x_stride, const float *gain, float eps, const void *dy, int64_t dy_stride,
                                 void *dx, int64_t dx_stride, float *dg) {
-    if (!c) return fail(ADN_E_INVALID, "null context");
-    std::string msg = check_sizes(rows, TRAIN_MAX_ROWS, d, 1, dtype);
-    if (msg.empty() && !dx && !dg) msg = "no output is wanted";
-    if (msg.empty())
-        msg = first_of({check_rows("x", x, x_stride, rows, d, dtype), check_rows("dy", dy, dy_stride, rows, d, dtype),
-                        dx ? check_rows("dx", dx, dx_stride, rows, d, dtype) : "", check_words("gain", gain),
-                        check_words("dg", dg), eps >= 0.0f ? "" : "eps must be >= 0"});
-    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
-    NormParams p{};
-    p.rows = rows, p.d = d, p.dtype = dtype;
-    p.x = x, p.x_stride = x_stride, p.gain = gain, p.eps = eps;
-    p.dy = dy, p.dy_stride = dy_stride, p.dx = dx, p.dx_stride = dx_stride, p.dg = dg;
-    return train_launch(c, norm_backward_workspace_bytes(p), [&](void *ws) { launch_norm_backward(p, ws, c->stream); });
+    return train_entry([&]() -> int {
+        if (!c) return fail(ADN_E_INVALID, "null context");
+        std::string msg = check_sizes(rows, TRAIN_MAX_ROWS, d, 1, dtype);
+        if (msg.empty() && !dx && !dg) msg = "no output is wanted";
+        if (msg.empty())
+            msg = first_of({check_rows("x", x, x_stride, rows, d, dtype), check_rows("dy", dy, dy_stride, rows, d, dtype),
+                            dx ? check_rows("dx", dx, dx_stride, rows, d, dtype) : "", check_words("gain", gain),
+                            check_words("dg", dg), eps >= 0.0f ? "" : "eps must be >= 0"});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        NormParams p{};
+        p.rows = rows, p.d = d, p.dtype = dtype;
+        p.x = x, p.x_stride = x_stride, p.gain = gain, p.eps = eps;
+        p.dy = dy, p.dy_stride = dy_stride, p.dx = dx, p.dx_stride = dx_stride, p.dg = dg;
+        return train_launch(c, norm_backward_workspace_bytes(p), [&](void *ws) { launch_norm_backward(p, ws, c->stream); });
+    });
 }
 
 int adn_embed_lookup_async(adn_ctx *c, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,
                            const void *table, int64_t table_stride, float scale, void *out, int64_t out_stride) {
-    if (!c) return fail(ADN_E_INVALID, "null context");
-    std::string msg = check_sizes(n, TRAIN_MAX_ROWS, d, vocab, dtype);
-    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
-    if (!table) {
-        if (!c->has_weights) return fail(ADN_E_NO_WEIGHTS, "adn_embed_lookup_async without a table before adn_upload_weights");
-        if (dtype != ADN_T_F32 || d != c->D.d || vocab != c->D.V)
-            return fail(ADN_E_INVALID, "table NULL is the context's embedding: ADN_T_F32, its d_r and vocab");
-        table = c->embed, table_stride = c->D.d;
-    }
-    msg = first_of({check_rows("table", table, table_stride, vocab, d, dtype),
-                    check_rows("out", out, out_stride, n, d, dtype), n > 0 && !tokens ? "null tokens" : "",
-                    check_words("tokens", tokens)});
-    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
-    TableParams p{n, d, vocab, dtype, tokens, scale, table, table_stride, out, out_stride, c->d_err};
-    return train_launch(c, 0, [&](void *) { launch_embed_lookup(p, c->stream); });
+    return train_entry([&]() -> int {
+        if (!c) return fail(ADN_E_INVALID, "null context");
+        std::string msg = check_sizes(n, TRAIN_MAX_ROWS, d, vocab, dtype);
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        if (!table) {
+            if (!c->has_weights) return fail(ADN_E_NO_WEIGHTS, "adn_embed_lookup_async without a table before adn_upload_weights");
+            if (dtype != ADN_T_F32 || d != c->D.d || vocab != c->D.V)
+                return fail(ADN_E_INVALID, "table NULL is the context's embedding: ADN_T_F32, its d_r and vocab");
+            table = c->embed, table_stride = c->D.d;
+        }
+        msg = first_of({check_rows("table", table, table_stride, vocab, d, dtype),
+                        check_rows("out", out, out_stride, n, d, dtype), n > 0 && !tokens ? "null tokens" : "",
+                        check_words("tokens", tokens)});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        TableParams p{n, d, vocab, dtype, tokens, scale, table, table_stride, out, out_stride, c->d_err};
+        return train_launch(c, 0, [&](void *) { launch_embed_lookup(p, c->stream); });
+    });
 }
 
 int adn_embed_grad_async(adn_ctx *c, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,
                          const void *dout, int64_t dout_stride, float scale, void *dtable, int64_t dtable_stride) {
-    if (!c) return fail(ADN_E_INVALID, "null context");
-    std::string msg = check_sizes(n, TRAIN_MAX_ROWS, d, vocab, dtype);
-    if (msg.empty())
-        msg = first_of({check_rows("dout", dout, dout_stride, n, d, dtype),
-                        check_rows("dtable", dtable, dtable_stride, vocab, d, dtype),
-                        n > 0 && !tokens ? "null tokens" : "", check_words("tokens", tokens)});
-    if (!msg.empty()) return fail(ADN_E_INVALID, msg);
-    TableParams p{n, d, vocab, dtype, tokens, scale, dout, dout_stride, dtable, dtable_stride, c->d_err};
-    return train_launch(c, embed_grad_workspace_bytes(p), [&](void *ws) { launch_embed_grad(p, ws, c->stream); });
+    return train_entry([&]() -> int {
+        if (!c) return fail(ADN_E_INVALID, "null context");
+        std::string msg = check_sizes(n, TRAIN_MAX_ROWS, d, vocab, dtype);
+        if (msg.empty())
+            msg = first_of({check_rows("dout", dout, dout_stride, n, d, dtype),
+                            check_rows("dtable", dtable, dtable_stride, vocab, d, dtype),
+                            n > 0 && !tokens ? "null tokens" : "", check_words("tokens", tokens)});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        TableParams p{n, d, vocab, dtype, tokens, scale, dout, dout_stride, dtable, dtable_stride, c->d_err};
+        return train_launch(c, embed_grad_workspace_bytes(p), [&](void *ws) { launch_embed_grad(p, ws, c->stream); });
+    });
 }
 
 }  // extern "C"

@@ -85,7 +85,9 @@ CASES = [(1, 1, 1, "uniform"), (1, 64, 50257, "uniform"), (2, 7, 3, "uniform"), 
          (64, 192, 65, "uniform"), (65, 33, 1000, "padded"), (255, 512, 300, "zipf"), (257, 100, 256, "uniform"), (2047, 64, 255, "zipf"),
          (2049, 64, 257, "zipf"), (4097, 96, 70000, "uniform"), (5000, 64, 100, "runs"), (8192, 72, 50257, "zipf"), (9001, 48, 65, "uniform"),
          (20000, 32, 7, "one"), (33000, 16, 65535, "zipf"), (33000, 16, 65536, "padded"), (70001, 8, 300, "zipf"), (300, 2048, 500, "zipf"),
-         (100, 8192, 20, "zipf"), (3000, 4, 1 << 24, "uniform"), (2048, 64, 50257, "one"), (16384, 64, 1024, "padded")]
+         (100, 8192, 20, "zipf"), (3000, 4, 1 << 24, "uniform"), (2048, 64, 50257, "one"), (16384, 64, 1024, "padded"), (1023, 64, 40, "zipf"),
+         (1024, 130, 50257, "padded"), (1025, 64, 40, "zipf"), (1000, 64, 3, "one"), (140001, 8, 300, "zipf"), (131072, 8, 2000, "ends"),
+         (131073, 8, 70001, "padded")]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])

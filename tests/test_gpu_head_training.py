@@ -89,3 +89,47 @@ def test_training_step(B, T, d, H, V):
     mag = torch.zeros((V, d), device="cuda", dtype=torch.float64).index_add_(0, toks.long(), src.double().abs())
     near(dE, ref, (n + 2) * 2.0 ** -24 * mag, "dE")
     be.close()
+
+
+def test_training_step_in_a_graph():
+    """The head's part of a step captured as one graph and replayed with other work in between: the eager step's bits."""
+    n, d, V = 600, 256, 5000
+    be = GpuDeqBackend(synth.ModelConfig(d=64, H=2, V=300, N=1, flags=0), 1, 1)
+    stream = torch.cuda.Stream()
+    be.set_stream(stream.cuda_stream)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    toks = torch.randint(-1, V, (n,), device="cuda", generator=g, dtype=torch.int32)
+    tgt = torch.randint(-1, V, (n,), device="cuda", generator=g, dtype=torch.int32)
+    table, w, gain, up = rnd(V, d), rnd(V, d) * 0.1, rnd(d) * 0.1 + 1, torch.full((n,), 1.0 / n, device="cuda")
+    o = {k: torch.empty(s, device="cuda") for k, s in dict(x=(n, d), y=(n, d), loss=(n,), dy=(n, d), dw=(V, d), dx=(n, d), dg=(d,),
+                                                           dE=(V, d)).items()}
+
+    def step():
+        be.embed_lookup_async(toks, o["x"], table=table, scale=d ** 0.5)
+        be.rms_norm_async(o["x"], o["y"], gain=gain)
+        be.lm_loss_async(o["y"], tgt, w=w, dloss=up, outputs=dict(loss=o["loss"], dx=o["dy"], dw=o["dw"]))
+        be.rms_norm_backward_async(o["x"], o["dy"], gain=gain, outputs=dict(dx=o["dx"], dg=o["dg"]))
+        be.embed_grad_async(o["dx"], toks, o["dE"], scale=d ** 0.5)
+    torch.cuda.synchronize()
+    step()
+    be.synchronize()
+    ref = {k: v.clone() for k, v in o.items()}
+    assert all(torch.isfinite(v).all() for v in ref.values())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for rep in range(4):
+        for v in o.values():
+            v.fill_(7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o[k], ref[k]) for k in ref), rep
+        assert float((torch.ones(1 << 20, device="cuda") * 2).sum()) == 2.0 ** 21
+        if rep == 1:
+            step()
+            be.synchronize()
+            assert all(torch.equal(o[k], ref[k]) for k in ref)
+    be.close()

@@ -153,6 +153,51 @@ def test_large_vocabulary(be, rows, dtype):
     check(out, *reference(s), rows)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,d,V", [(300, 64, 50257), (5000, 64, 50257), (257, 512, 20011), (700, 192, 30011), (3001, 256, 9973),
+                                      (1300, 1536, 4001)])
+def test_large_tiles_and_many_pieces(be, rows, d, V, dtype):
+    """Grids of more than a round of the chip, whose tiles are the large ones; 5000 rows take several pieces of the vocabulary, of
+    which the last is the smaller, and add dx up over them."""
+    log(f"loss {rows} x {d} x {V} {dtype}")
+    s = make(rows, d, V, dtype, bias=True, pad=0.1)
+    out = call(be, s, buffers(s))
+    check(out, *reference(s), rows)
+
+
+@pytest.mark.parametrize("rows", [3, 20, 200])
+def test_row_without_any_entry(be, rows):
+    """A bias of -inf everywhere leaves no entry: nothing is a number, and the next call is as ever."""
+    s = make(rows, 64, 700, bias=True)
+    keep = s["bias"].clone()
+    s["bias"][:] = float("-inf")
+    out = call(be, s, buffers(s))
+    assert torch.isnan(out["loss"]).all() and torch.isnan(out["dx"]).all() and torch.isnan(out["dw"]).all()
+    assert (out["lse"] == float("-inf")).all()
+    s["bias"] = keep
+    check(call(be, s, buffers(s)), *reference(s), rows)
+
+
+def test_two_contexts_side_by_side():
+    """Two contexts on two streams, their calls enqueued without a wait in between."""
+    both = []
+    for seed in (1, 2):
+        b = GpuDeqBackend(synth.ModelConfig(d=64, H=2, V=300, N=1, flags=0), 1, 1)
+        st = torch.cuda.Stream()
+        b.set_stream(st.cuda_stream)
+        s = make(400, 256, 6000, bias=True, seed=seed)
+        both.append((b, s, buffers(s), st))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for b, s, out, _st in both:
+            b.lm_loss_async(s["x"], s["targets"], w=s["w"], bias=s["bias"], dloss=s["dloss"], outputs=out)
+    for b, s, out, _st in both:
+        b.synchronize()
+        check(out, *reference(s), "two contexts")
+    for b, *_ in both:
+        b.close()
+
+
 @pytest.mark.parametrize("what", [("loss",), ("lse",), ("dx",), ("dw",), ("db",), ("loss", "dx"), ("dw", "lse")])
 @pytest.mark.parametrize("rows", [5, 150])
 def test_outputs_apart(be, what, rows):
