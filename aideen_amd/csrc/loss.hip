@@ -79,6 +79,20 @@ __device__ __forceinline__ int exp_of(float g) {
     return a > 0.0f && a < INFINITY ? ilogbf(a) : 0;
 }
 
+// Exponent that takes a magnitude to [2^14, 2^15); 0 for zero and what is not finite.
+__device__ __forceinline__ int scale_exp(float mx) {
+    if (!(mx > 0.0f) || mx == INFINITY) return 0;
+    return 15 - (ilogbf(mx) + 1);
+}
+
+__device__ __forceinline__ float block_max256(float v, float *red) {
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
 // Chunk (8 halves) of a block's row r that holds columns [0, 8) in the LDS image of an operand read
 // along its columns: the b128 reads of 32 consecutive rows then use every bank alike.
 __device__ __forceinline__ int swz(int r) { return ((r >> 2) ^ (r >> 3)) & 1; }
@@ -106,6 +120,11 @@ struct LossGemm {
     int vocab, rows;
     float *part_m, *part_s, *ztgt;      // [tile][rows padded]: maximum and sum of exponentials; the target's logit
     long rows_pad;
+    const void *w_raw;                  // LOGITS_RAW: W's rows as they are, their stride in bytes, the
+    unsigned w_stride;                  //   partial maxima of |W|
+    const float *w_part;
+    int w_blocks;
+    float *out_loss, *out_lse;          // LOGITS_ALL: [rows] or null
     const float *lse, *g;               // per row: lse (in units of log 2), g_i = m_i 2^e_i (dz's factor: m_i 2^13)
     _Float16 *dz;                       // planes of the piece, blocks of rows x entries
     long dz_plane;
@@ -122,7 +141,10 @@ struct LossGemm {
     const int32_t *e_all;               // exponent of dst's values
 };
 
-enum { LOGITS_STATS = 0, LOGITS_DZ = 1, GRAD = 2 };
+// The logits' epilogues: each row's maximum and sum of a tile of entries (RAW: W's rows read as they are
+// and split on the way to the MFMA, for losses alone, where planes of W would be read once); dz of a
+// piece; both in one where a tile holds the whole vocabulary.
+enum { LOGITS_STATS = 0, LOGITS_DZ = 1, GRAD = 2, LOGITS_RAW = 3, LOGITS_ALL = 4 };
 
 // The two gradients of a piece in one launch: tiles of the one with the longer shares first.
 struct LossGrads {
@@ -190,7 +212,28 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
     };
     // a plane's slice of the tile is A_BLK (B_BLK) KB in either order; where the waves outnumber its
     // loads some are issued twice, to the same place
+    constexpr bool RAW = MODE == LOGITS_RAW;
     long asrc[A_PW], bsrc[B_PW];
+    // RAW: load idx is 16 rows of 64 bytes (4 chunks, swizzled by the row), a lane a chunk
+    constexpr int R_PW = NP * A_PW;
+    unsigned roff[RAW ? R_PW : 1];
+    const char *rbase = nullptr;
+    int kw_raw = 0;
+    auto swz4 = [](int row) { return ((row >> 1) ^ (row >> 2)) & 3; };
+    if constexpr (RAW) {
+        static_assert(A_BLK * NP % NW == 0, "whole loads a wave");
+        const int row0 = p.a_row0 + mt * TM;
+        rbase = (const char *)p.w_raw + (long)row0 * p.w_stride;
+#pragma unroll
+        for (int j = 0; j < R_PW; ++j) {
+            const int row = (wave + NW * j) * 16 + (lane >> 2);
+            roff[j] = (unsigned)min(row, p.vocab - 1 - row0) * p.w_stride + (((lane & 3) ^ swz4(row)) * 16);
+        }
+        float m = 0.0f;  // W's scale
+        for (int i = tid; i < p.w_blocks; i += NT) m = fmaxf(m, p.w_part[i]);
+        kw_raw = scale_exp(block_max256(m, reinterpret_cast<float *>(ring)));
+        __syncthreads();
+    }
 #pragma unroll
     for (int j = 0; j < A_PW; ++j) asrc[j] = src_of(TRA, (wave + NW * j) % A_BLK, p.a_row0 + mt * TM, p.A);
 #pragma unroll
@@ -200,10 +243,14 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
     auto issue = [&](int kt) {
         const unsigned base = ring0 + (kt % STAGES) * (SLICE * 2);
         const _Float16 *Ap = p.A.p + step_of(TRA, kt, p.A), *Bp = p.B.p + step_of(TRB, kt, p.B);
+        if constexpr (RAW) {
+#pragma unroll
+            for (int j = 0; j < R_PW; ++j) load_lds(rbase + kt * 64, roff[j], base + (wave + NW * j) * 1024);
+        }
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
 #pragma unroll
-            for (int j = 0; j < A_PW; ++j)
+            for (int j = 0; !RAW && j < A_PW; ++j)
                 load_lds(Ap + q * p.A.plane + asrc[j], aoff, base + (q * A_SZ + ((wave + NW * j) % A_BLK) * 512) * 2);
 #pragma unroll
             for (int j = 0; j < B_PW; ++j)
@@ -219,6 +266,32 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
         const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(img + at));
         const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(img + (at ^ 64)));
         return __builtin_bit_cast(half8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    // RAW: the planes of 32 rows' 8 values a lane, split here
+    auto raw_frag = [&](const _Float16 *img, int t, int kb, half8 &hi, half8 &lo) {
+        const int row = t * 32 + r;
+        const char *at = (const char *)img + row * 64;
+        float v[8];
+        if constexpr (NP == 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const floatx4 x = *reinterpret_cast<const floatx4 *>(at + (((2 * hh + h) ^ swz4(row)) * 16));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[4 * h + u] = x[u];
+            }
+        } else {
+            typedef T V8 __attribute__((ext_vector_type(16 / sizeof(T))));
+            const V8 x = *reinterpret_cast<const V8 *>(at + (((2 * kb + hh) ^ swz4(row)) * 16));
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = to_f32<T>(x[u % (16 / (int)sizeof(T))]);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float x = ldexpf(v[u], kw_raw);
+            hi[u] = (_Float16)x;
+            if constexpr (NP == 2) lo[u] = (_Float16)(x - (float)hi[u]);  // (one plane: lo is hi)
+        }
     };
 
     floatx16 acc[WTM][WTN];
@@ -245,10 +318,15 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             half8 a[NP][WTM];
+            if constexpr (RAW) {
 #pragma unroll
-            for (int q = 0; q < NP; ++q)
+                for (int i = 0; i < WTM; ++i) raw_frag(base, wm * WTM + i, kb, a[0][i], a[NP - 1][i]);
+            } else {
 #pragma unroll
-                for (int i = 0; i < WTM; ++i) a[q][i] = frag(base + q * A_SZ, TRA, wm * WTM + i, kb);
+                for (int q = 0; q < NP; ++q)
+#pragma unroll
+                    for (int i = 0; i < WTM; ++i) a[q][i] = frag(base + q * A_SZ, TRA, wm * WTM + i, kb);
+            }
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
                 half8 b[NP];
@@ -312,7 +390,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
         else
             store(std::integral_constant<bool, false>{});
     } else {
-        static_assert(MODE == GRAD || (TM == TV && WGN == 1), "a wave's columns are the tile's");
+        static_assert(TM == TV && WGN == 1, "a wave's columns are the tile's");
         // the tile's biases; entries beyond the vocabulary get -inf: no part of any sum.  From here on
         // logits are in units of log 2 (z log2(e)), what exp2 takes.
         float *bias_l = reinterpret_cast<float *>(ring);                   // [TM]
@@ -323,7 +401,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             bias_l[c] = b * LOG2E;
         }
         lds_barrier();
-        const int kw = *p.kw_dev;
+        const int kw = RAW ? kw_raw : *p.kw_dev;
         const int w0 = v0 + wm * WTM * 32;  // the wave's first entry
         float unscale[WTN];
 #pragma unroll
@@ -339,8 +417,8 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                     for (int e = 0; e < 4; ++e)
                         acc[i][j][4 * e4 + e] = __builtin_fmaf(acc[i][j][4 * e4 + e], unscale[j], b[e]);
             }
-        if constexpr (MODE == LOGITS_STATS) {
-            float *red_m = bias_l + TM, *red_s = red_m + 4 * TN;           // [wave][TN]
+        float *red_m = bias_l + TM, *red_s = red_m + 4 * TN;               // [wave][TN]
+        if constexpr (MODE != LOGITS_DZ) {
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
                 const long m = (long)nt * TN + j * 32 + r;
@@ -364,7 +442,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 }
                 // the target's logit, by the one lane that holds it
                 const int t = p.tgt[m] - w0;
-                if (__any(t >= 0 && t < WTM * 32))
+                if (MODE != LOGITS_ALL && __any(t >= 0 && t < WTM * 32))
 #pragma unroll
                     for (int i = 0; i < WTM; ++i)
 #pragma unroll
@@ -372,7 +450,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                             if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) p.ztgt[m] = acc[i][j][e];
             }
             lds_barrier();
-            for (int c = tid; c < TN; c += NT) {
+            for (int c = tid; MODE != LOGITS_ALL && c < TN; c += NT) {
                 float mx = red_m[c];
 #pragma unroll
                 for (int w = 1; w < 4; ++w) mx = fmaxf(mx, red_m[w * TN + c]);
@@ -385,14 +463,40 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 p.part_m[o] = mx;
                 p.part_s[o] = sum;
             }
-        } else {
-            float *colsum = bias_l + TM + wave * (32 * WTM * 33);          // db: [WTM * 32 entries][32 + 1]
+        }
+        if constexpr (MODE == LOGITS_DZ || MODE == LOGITS_ALL) {
+            float *colsum = red_s + 4 * TN + wave * (32 * WTM * 33);       // db: [WTM * 32 entries][32 + 1]
             float bsum[WTM][16];
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
                 const long m = (long)nt * TN + j * 32 + r;
-                const float lse = p.lse[m], gm = p.g[m], qm = ldexpf(gm, 13 - exp_of(gm));
-                const int t = p.tgt[m] - w0;
+                const float gm = p.g[m], qm = ldexpf(gm, 13 - exp_of(gm));
+                const int tm = p.tgt[m], t = tm - w0;
+                float lse;
+                if constexpr (MODE == LOGITS_ALL) {
+                    float mx = red_m[j * 32 + r];
+#pragma unroll
+                    for (int w = 1; w < 4; ++w) mx = fmaxf(mx, red_m[w * TN + j * 32 + r]);
+                    const float ref = mx == -INFINITY ? 0.0f : mx;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        sum += red_s[w * TN + j * 32 + r] * __builtin_amdgcn_exp2f(red_m[w * TN + j * 32 + r] - ref);
+                    lse = ref + log2f(sum);
+                    if (wave == 0 && hh == 0 && m < p.rows) {
+                        if (p.out_lse) p.out_lse[m] = tm >= 0 ? lse * LN2 : 0.0f;
+                        if (p.out_loss && tm < 0) p.out_loss[m] = 0.0f;
+                    }
+                    if (p.out_loss && __any(t >= 0 && t < WTM * 32))
+#pragma unroll
+                        for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) p.out_loss[m] = (lse - acc[i][j][e]) * LN2;
+                    if (!p.dz) continue;
+                } else {
+                    lse = p.lse[m];
+                }
                 const bool off = qm == 0.0f;  // no target, or nothing from upstream: exactly zero
 #pragma unroll
                 for (int i = 0; i < WTM; ++i)
@@ -439,7 +543,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                     }
                 }
             }
-            if (p.db_part) {  // each entry's sum over the tile's rows, lanes in order
+            if (p.dz && p.db_part) {  // each entry's sum over the tile's rows, lanes in order
 #pragma unroll
                 for (int i = 0; i < WTM; ++i)
 #pragma unroll
@@ -473,12 +577,6 @@ __global__ __launch_bounds__(NT, 2) void k_loss_grads(LossGrads p) {
 }
 
 // ---- operands ------------------------------------------------------------------------------
-// Exponent that takes a magnitude to [2^14, 2^15); 0 for zero and what is not finite.
-__device__ __forceinline__ int scale_exp(float mx) {
-    if (!(mx > 0.0f) || mx == INFINITY) return 0;
-    return 15 - (ilogbf(mx) + 1);
-}
-
 __device__ __forceinline__ float finite_abs(float v) {
     const float a = fabsf(v);
     return a < INFINITY ? a : 0.0f;  // NaN and inf stay in their own rows
@@ -533,14 +631,6 @@ struct Prep {
     float *g, *gmax;             // [rows padded], [row blocks]: largest |x_i| 2^e_i
     int32_t *kw, *e_dw;          // exponent of W's scale; of dW's results
 };
-
-__device__ __forceinline__ float block_max256(float v, float *red) {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
 
 // The planes of XR rows of x, row r times 2^ex[r] (zeros where live[r] < 0): chunk (column block, row,
 // half) by chunk, neighbouring threads side by side.  XR = 8: four blocks share a block row of 32, so
@@ -767,6 +857,7 @@ constexpr int SLOTS = 512;  // workgroups that run at once: two a CU
 long round_up(long n, long to) { return (n + to - 1) / to * to; }
 
 struct LossPlan {
+    bool raw;                // losses alone: W goes to the product as it is
     int np, tn;              // planes; rows a workgroup of the logits' product covers
     int dcb;                 // column blocks of width d
     long rows_pad, v_pad;    // rows of the planes of x (and dz), of W
@@ -859,6 +950,12 @@ LossPlan loss_plan(const LossParams &p) {
     L.tn = pick_tn(p.rows, round_up(p.vocab, TV) / TV);
     L.dcb = (int)(round_up(p.d, 32) / 16);
     L.rows_pad = round_up(p.rows, BM);
+    {   // rows of W in whole slices of 16-byte pieces, a tile's offsets in 32 bits (256 rows of 512 against
+        // 50257: 107 us with planes of W, 71 without)
+        const long bytes = p.w_stride * elem_bytes(p.dtype);
+        L.raw = !grads && p.vocab > TV && p.d % (L.np == 2 ? 16 : 32) == 0 && (uintptr_t)p.w % 16 == 0 && bytes % 16 == 0 &&
+                bytes < (1L << 31) / TV;
+    }
     L.v_pad = round_up(p.vocab, TV);
     L.v_tiles = (int)(L.v_pad / TV);
     const long fit = (long)(PIECE_BYTES / (L.np * 2)) / L.rows_pad / TV * TV;
@@ -873,7 +970,7 @@ LossPlan loss_plan(const LossParams &p) {
     };
     L.xp = take((size_t)L.rows_pad * L.dcb * 32 * L.np);
     L.x2p = take(p.dw ? (size_t)L.rows_pad * L.dcb * 32 * L.np : 0);
-    L.wp = take((size_t)L.v_pad * L.dcb * 32 * L.np);
+    L.wp = take(L.raw ? 0 : (size_t)L.v_pad * L.dcb * 32 * L.np);
     L.w_part = take(W_BLOCKS * 4);
     L.f = take(L.rows_pad * 4);
     L.tgt = take(L.rows_pad * 4);
@@ -947,12 +1044,13 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     r.f = (int32_t *)(ws + L.f), r.tgt = (int32_t *)(ws + L.tgt);
     r.g = (float *)(ws + L.g), r.gmax = (float *)(ws + L.gmax);
     r.kw = (int32_t *)(ws + L.kw), r.e_dw = (int32_t *)(ws + L.e_dw);
+    const bool grads = p.dx || p.dw || p.db;
     const unsigned prep_grid = (unsigned)(r.row_blocks + r.w_blocks);
     const unsigned split_grid = (unsigned)((r.x2p ? r.row_blocks : 0) + r.w_rows);
     auto prep = [&](auto vecx, auto vecw) {
         constexpr bool VX = decltype(vecx)::value, VW = decltype(vecw)::value;
         k_loss_prep<T, NP, VX, VW><<<prep_grid, NT, 0, st>>>(r);
-        k_loss_split<T, NP, VX, VW><<<split_grid, NT, 0, st>>>(r);
+        if (!L.raw) k_loss_split<T, NP, VX, VW><<<split_grid, NT, 0, st>>>(r);
     };
     using std::bool_constant;
     if (vx && vw)
@@ -972,25 +1070,39 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     z.bias = p.bias, z.f = r.f, z.tgt = r.tgt, z.kw_dev = r.kw;
     z.vocab = p.vocab, z.rows = p.rows, z.rows_pad = L.rows_pad;
     z.part_m = (float *)(ws + L.part_m), z.part_s = (float *)(ws + L.part_s), z.ztgt = (float *)(ws + L.ztgt);
-    launch_logits<LOGITS_STATS, T, NP>(z, L.tn, st);
+    z.g = r.g;
+    if (grads) {
+        z.dz = (_Float16 *)(ws + L.dz), z.dz_plane = L.rows_pad * L.piece, z.dz_ncb = L.piece / 16;
+        z.db_part = p.db ? (float *)(ws + L.db_part) : nullptr, z.db_ld = L.v_pad;
+    }
+    const bool all = L.v_tiles == 1;  // one tile holds the vocabulary: one pass
+    if (all) {
+        z.out_loss = p.loss, z.out_lse = p.lse;
+        launch_logits<LOGITS_ALL, T, NP>(z, L.tn, st);
+    } else {
+        if (L.raw) {
+            z.K = z.Ks = p.d;
+            z.w_raw = p.w, z.w_stride = (unsigned)(p.w_stride * eb), z.w_part = r.w_part, z.w_blocks = r.w_blocks;
+            launch_logits<LOGITS_RAW, T, NP>(z, L.tn, st);
+        } else {
+            launch_logits<LOGITS_STATS, T, NP>(z, L.tn, st);
+        }
+        Rows q{};
+        q.rows = p.rows, q.tiles = L.v_tiles, q.rows_pad = L.rows_pad;
+        q.part_m = z.part_m, q.part_s = z.part_s, q.ztgt = z.ztgt, q.tgt = r.tgt;
+        q.lse = (float *)(ws + L.lse), q.out_loss = p.loss, q.out_lse = p.lse;
+        k_loss_rows<<<(unsigned)(round_up(p.rows, L.tn) / 16), NT, 0, st>>>(q);
+        z.lse = q.lse;
+    }
+    if (!grads) return;
 
-    Rows q{};
-    q.rows = p.rows, q.tiles = L.v_tiles, q.rows_pad = L.rows_pad;
-    q.part_m = z.part_m, q.part_s = z.part_s, q.ztgt = z.ztgt, q.tgt = r.tgt;
-    q.lse = (float *)(ws + L.lse), q.out_loss = p.loss, q.out_lse = p.lse;
-    k_loss_rows<<<(unsigned)(round_up(p.rows, L.tn) / 16), NT, 0, st>>>(q);
-    if (!p.dx && !p.dw && !p.db) return;
-
-    z.lse = q.lse, z.g = r.g;
-    z.dz = (_Float16 *)(ws + L.dz), z.dz_plane = L.rows_pad * L.piece, z.dz_ncb = L.piece / 16;
-    z.db_part = p.db ? (float *)(ws + L.db_part) : nullptr, z.db_ld = L.v_pad;
     const int nbn = (p.d + L.bn - 1) / L.bn;
     for (long v0 = 0; v0 < L.v_pad; v0 += L.piece) {
         const int n = (int)std::min<long>(L.piece, L.v_pad - v0);  // entries of the piece, padded
         const Planes DZ{z.dz, z.dz_plane, z.dz_ncb};
         z.a_row0 = (int)v0;
         z.nM = n / TV;
-        launch_logits<LOGITS_DZ, T, NP>(z, L.tn, st);
+        if (!all) launch_logits<LOGITS_DZ, T, NP>(z, L.tn, st);
         const int live = (int)std::min<long>(n, p.vocab - v0);
         T *dst = p.dw ? (T *)p.dw + v0 * p.dw_stride : nullptr;
         LossGrads g{};
