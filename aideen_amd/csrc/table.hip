@@ -5,9 +5,10 @@
 //
 // The gradient adds each table row's positions in a fixed order, so it is the same bits on every run.
 //
-// Up to FEW positions: one launch.  A block a position compares its token with all the others; the
-// first block of a token adds the token's rows, its waves a quarter of them each.  Other blocks write
-// zeros where no token is.
+// Up to FEW positions: one launch.  A block a position compares its token with all the others (eight
+// 64-bit masks a wave); the first block of a token adds the token's rows, its waves an eighth of them
+// each.  Other blocks write zeros where no token is, which is most of the time: 256 positions of 512
+// columns of 50257 entries 16 us (6.3 TB/s), 4096 30 us (sorted 46).
 //
 // More: the positions are sorted by token (a stable radix sort of 8 bits a pass), the sorted list is
 // cut into chunks, a wave adds one chunk's rows in order and stores the table rows that begin and end
@@ -27,7 +28,8 @@ constexpr int RADIX = 256;
 constexpr int TILE = 1024;                // keys a block of a radix pass
 constexpr int W_KEYS = TILE / (NT / 64);  // consecutive keys a wave of it
 constexpr int OWN_PREFIX = 128;           // blocks up to which each forms its own offsets
-constexpr int FEW = 1024;
+constexpr int FW = 8;                     // waves of a block of the few
+constexpr int FEW = FW * 8 * 64;
 constexpr int C0 = 32;                    // sorted entries a wave adds at a time
 
 // The key of position i: its token, or `vocab` (sorted behind every token) where it has none.
@@ -82,61 +84,81 @@ __device__ __forceinline__ void zero_rows(T *dst, long stride, int d, long v0, l
 // Blocks below n: position blockIdx.x.  The others: FEW_ROWS rows of the table each.
 constexpr int FEW_ROWS = 64;
 template <typename T, bool VEC>
-__global__ __launch_bounds__(NT) void k_grad_few(TableParams p) {
-    constexpr int W = VEC ? 16 / (int)sizeof(T) : 1;
+__global__ __launch_bounds__(64 * FW) void k_grad_few(TableParams p) {
+    constexpr int W = VEC ? 16 / (int)sizeof(T) : 1, LOADS = 16;
     typedef typename VecT<T, W>::type V;
     __shared__ int list[FEW];
+    __shared__ int cnt[FW], lead[FW];
     __shared__ int here[FEW_ROWS];
-    __shared__ float part[3][64 * W];
+    __shared__ float part[FW - 1][64 * W];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if ((int)blockIdx.x >= p.n) {
         const long v0 = (long)((int)blockIdx.x - p.n) * FEW_ROWS, v1 = min(v0 + FEW_ROWS, (long)p.vocab);
         if (tid < FEW_ROWS) here[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < p.n; i += NT) {
+#pragma unroll 8
+        for (int i = tid; i < p.n; i += 64 * FW) {
             const int t = p.tokens[i];
             if (t >= v0 && t < v1) here[t - v0] = 1;
         }
         __syncthreads();
-        for (long v = v0 + wave; v < v1; v += NT / 64)
+        for (long v = v0 + wave; v < v1; v += FW)
             if (!here[v - v0]) zero_rows<T, VEC>((T *)p.dst, p.dst_stride, p.d, v, v + 1, 0, 1);
         return;
+    }
+    // the positions of this token in order: wave w looks at [w S, (w + 1) S)
+    const int S = ((p.n + FW - 1) / FW + 63) / 64 * 64;  // at most 8 x 64
+    int t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int i = wave * S + u * 64 + lane;
+        t[u] = u * 64 < S && i < p.n ? p.tokens[i] : -1;
     }
     const int me = p.tokens[blockIdx.x];
     if (me >= p.vocab && tid == 0) atomicOr(p.err, ADN_DEVERR_TOKEN);
     if (me < 0 || me >= p.vocab) return;
-    // the positions of this token in order: every wave finds them all
-    int m = 0;
-    bool first = true;
-    for (int i0 = 0; i0 < p.n; i0 += 64 * 8) {
-        int t[8];
+    int mine = 0, first = FEW;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) t[u] = i0 + u * 64 + lane < p.n ? p.tokens[i0 + u * 64 + lane] : -1;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const unsigned long long hit = __ballot(t[u] == me);
-            const int i = i0 + u * 64 + lane;
-            if (hit && m == 0) first = i0 + u * 64 + __ffsll(hit) - 1 == (int)blockIdx.x;
-            if (wave == 0 && t[u] == me) list[m + __popcll(hit & ((1ull << lane) - 1))] = i;
-            m += __popcll(hit);
-        }
-        if (!first) return;  // an earlier block adds this token (all waves agree)
+    for (int u = 7; u >= 0; --u) {
+        const unsigned long long hit = __ballot(t[u] == me);
+        mine += __popcll(hit);
+        if (hit) first = wave * S + u * 64 + __ffsll(hit) - 1;
+    }
+    if (lane == 0) {
+        cnt[wave] = mine;
+        lead[wave] = first;
     }
     __syncthreads();
-    const int per = (m + 3) / 4, a = min(m, wave * per), b = min(m, a + per);
+    int m = 0, at = 0;
+    first = FEW;
+#pragma unroll
+    for (int w = 0; w < FW; ++w) {
+        if (w == wave) at = m;
+        m += cnt[w];
+        first = min(first, lead[w]);
+    }
+    if (first != (int)blockIdx.x) return;  // an earlier block adds this token (all waves agree)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const unsigned long long hit = __ballot(t[u] == me);
+        if (t[u] == me) list[at + __popcll(hit & ((1ull << lane) - 1))] = wave * S + u * 64 + lane;
+        at += __popcll(hit);
+    }
+    __syncthreads();
+    const int per = (m + FW - 1) / FW, a = min(m, wave * per), b = min(m, a + per);
     for (int c0 = 0; c0 < p.d; c0 += 64 * W) {
         const int c = c0 + lane * W;
         float acc[W];
 #pragma unroll
         for (int j = 0; j < W; ++j) acc[j] = 0.0f;
         if (c < p.d)
-            for (int e0 = a; e0 < b; e0 += 8) {
-                V v[8];
+            for (int e0 = a; e0 < b; e0 += LOADS) {
+                V v[LOADS];
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    v[u] = *reinterpret_cast<const V *>((const T *)p.src + (long)list[min(e0 + u, b - 1)] * p.src_stride + c);
+                for (int u = 0; u < LOADS; ++u)
+                    if (e0 + u < b) v[u] = *reinterpret_cast<const V *>((const T *)p.src + (long)list[e0 + u] * p.src_stride + c);
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                for (int u = 0; u < LOADS; ++u)
                     if (e0 + u < b)
 #pragma unroll
                         for (int j = 0; j < W; ++j) acc[j] += to_f32<T>(v[u][j]);
@@ -149,7 +171,7 @@ __global__ __launch_bounds__(NT) void k_grad_few(TableParams p) {
             __syncthreads();
             if (wave == 0)
 #pragma unroll
-                for (int q = 0; q < 3; ++q)
+                for (int q = 0; q < FW - 1; ++q)
 #pragma unroll
                     for (int j = 0; j < W; ++j) acc[j] += part[q][lane * W + j];
         }
@@ -400,17 +422,18 @@ __global__ __launch_bounds__(NT) void k_join_sums(TableParams p, const unsigned 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long chunk = blockIdx.x, a = chunk * C, b = a + C;
     if (b >= p.n) return;
+    // the chunks that begin with the row: chunk + 1 .. chunk + m (64 of them looked at beside the rest)
+    const long chunks = (p.n + C - 1) / C;
     const unsigned k = keys[b - 1], kb = keys[b], ka = keys[a], kz = keys[a > 0 ? a - 1 : 0];
+    unsigned ahead = keys[min((chunk + 1 + lane) * C, (long)p.n - 1)];
     if (k >= (unsigned)p.vocab || kb != k) return;  // nothing goes on
     if (a > 0 && ka == k && kz == k) return;        // it began in an earlier chunk
-    // the chunks that begin with the row: chunk + 1 .. chunk + m
-    const long chunks = (p.n + C - 1) / C;
     long m = 0;
     for (;;) {
-        const long q = chunk + 1 + m + lane;
-        const unsigned long long on = __ballot(q < chunks && keys[min(q * C, (long)p.n - 1)] == k);
+        const unsigned long long on = __ballot(chunk + 1 + m + lane < chunks && ahead == k);
         m += on == ~0ull ? 64 : __ffsll(~on) - 1;
         if (on != ~0ull) break;
+        ahead = keys[min((chunk + 1 + m + lane) * C, (long)p.n - 1)];
     }
     const int c = (int)(blockIdx.y * 64 + lane);
     const long per = (m + 3) / 4, q0 = chunk + 1 + min(m, wave * per), q1 = chunk + 1 + min(m, (wave + 1) * per);
@@ -482,9 +505,9 @@ void launch_embed_grad(const TableParams &p, void *ws, hipStream_t st) {
             typedef decltype(t) T;
             const unsigned grid = (unsigned)(p.n + (p.vocab + FEW_ROWS - 1) / FEW_ROWS);
             if (vec)
-                k_grad_few<T, true><<<grid, NT, 0, st>>>(p);
+                k_grad_few<T, true><<<grid, 64 * FW, 0, st>>>(p);
             else
-                k_grad_few<T, false><<<grid, NT, 0, st>>>(p);
+                k_grad_few<T, false><<<grid, 64 * FW, 0, st>>>(p);
         });
         return;
     }

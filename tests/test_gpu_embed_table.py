@@ -86,7 +86,8 @@ CASES = [(1, 1, 1, "uniform"), (1, 64, 50257, "uniform"), (2, 7, 3, "uniform"), 
          (2049, 64, 257, "zipf"), (4097, 96, 70000, "uniform"), (5000, 64, 100, "runs"), (8192, 72, 50257, "zipf"), (9001, 48, 65, "uniform"),
          (20000, 32, 7, "one"), (33000, 16, 65535, "zipf"), (33000, 16, 65536, "padded"), (70001, 8, 300, "zipf"), (300, 2048, 500, "zipf"),
          (100, 8192, 20, "zipf"), (3000, 4, 1 << 24, "uniform"), (2048, 64, 50257, "one"), (16384, 64, 1024, "padded"), (1023, 64, 40, "zipf"),
-         (1024, 130, 50257, "padded"), (1025, 64, 40, "zipf"), (1000, 64, 3, "one"), (140001, 8, 300, "zipf"), (131072, 8, 2000, "ends"),
+         (1024, 130, 50257, "padded"), (1025, 64, 40, "zipf"), (1000, 64, 3, "one"), (4095, 64, 700, "zipf"), (4096, 48, 50257, "padded"), (4096, 2048, 9, "one"), (513, 64, 20, "zipf"),
+         (140001, 8, 300, "zipf"), (131072, 8, 2000, "ends"),
          (131073, 8, 70001, "padded")]
 
 
@@ -226,7 +227,7 @@ def test_capture_before_the_workspace_is_there():
     b = GpuDeqBackend(synth.ModelConfig(d=64, H=2, V=300, N=1, flags=0), 1, 1)
     stream = torch.cuda.Stream()
     b.set_stream(stream.cuda_stream)
-    table, dout, toks = make(3000, 64, 90, F32)  # sorted: up to 1024 positions need no workspace
+    table, dout, toks = make(5000, 64, 90, F32)  # sorted: up to 4096 positions need no workspace
     out = torch.zeros_like(table)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
