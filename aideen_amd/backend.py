@@ -385,8 +385,8 @@ class GpuDeqBackend:
                                            self._vector(tokens, "tokens", n, "i32"), tp, ts, scale, op, os_))
 
     def embed_grad_async(self, dout, tokens, dtable, *, scale: float = 1.0) -> None:
-        """The table's gradient: dtable[v] = scale * sum of the rows dout[i] with tokens[i] = v, in the
-        order of i; every row of dtable is written."""
+        """The table's gradient: dtable[v] = scale * sum of the rows dout[i] with tokens[i] = v, always added
+        in the same order; every row of dtable is written."""
         if dout.dim() != 2 or dtable.dim() != 2:
             raise _invalid("dout and dtable must be matrices")
         n, d = dout.shape

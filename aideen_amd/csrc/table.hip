@@ -237,17 +237,33 @@ __global__ __launch_bounds__(NT) void k_radix_count(Sort s, int pass) {
     s.cnt[(long)threadIdx.x * s.nblocks + blockIdx.x] = h[threadIdx.x];
 }
 
-// Exclusive prefix sum in place over `m` counts, one block.
+// Exclusive prefix sum in place over `m` counts (a multiple of 8), one block, 8 counts a thread.
 __global__ __launch_bounds__(1024) void k_scan(unsigned *cnt, long m) {
+    typedef unsigned uint4v __attribute__((ext_vector_type(4)));
     __shared__ unsigned wsum[16];
-    __shared__ unsigned carry;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    if (threadIdx.x == 0) carry = 0;
-    __syncthreads();
-    for (long base = 0; base < m; base += 1024) {
-        const long i = base + threadIdx.x;
-        const unsigned v = i < m ? cnt[i] : 0;
-        unsigned s = v;
+    unsigned carry = 0;
+    uint4v next[2] = {};
+    auto fetch = [&](long i) {
+        if (i < m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) next[h] = *reinterpret_cast<const uint4v *>(cnt + i + 4 * h);
+        else
+            next[0] = next[1] = uint4v{};
+    };
+    fetch((long)threadIdx.x * 8);
+    for (long base = 0; base < m; base += 1024 * 8) {
+        const long i = base + (long)threadIdx.x * 8;
+        uint4v v[2] = {next[0], next[1]};
+        fetch(i + 1024 * 8);
+        unsigned sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const unsigned c = v[j / 4][j % 4];
+            v[j / 4][j % 4] = sum;
+            sum += c;
+        }
+        unsigned s = sum;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const unsigned o = __shfl_up(s, off, 64);
@@ -255,11 +271,20 @@ __global__ __launch_bounds__(1024) void k_scan(unsigned *cnt, long m) {
         }
         if (lane == 63) wsum[w] = s;
         __syncthreads();
-        unsigned before = carry;
-        for (int q = 0; q < w; ++q) before += wsum[q];
-        if (i < m) cnt[i] = before + s - v;
-        __syncthreads();
-        if (threadIdx.x == 1023) carry = before + s;
+        unsigned before = carry, all = 0;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            before += q < w ? wsum[q] : 0;
+            all += wsum[q];
+        }
+        carry += all;
+        before += s - sum;
+        if (i < m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                v[h] += before;
+                *reinterpret_cast<uint4v *>(cnt + i + 4 * h) = v[h];
+            }
         __syncthreads();
     }
 }
@@ -341,8 +366,12 @@ __global__ __launch_bounds__(NT) void k_radix_move(Sort s, int pass) {
         const int rank = __popcll(same & ((1ull << lane) - 1));
         unsigned o = 0;
         if (in) o = at[w][dig];
-        __builtin_amdgcn_wave_barrier();  // every lane has read the place before the first of a digit moves it on
+        // every lane has read the place before the first of a digit moves it on (the wave's LDS operations
+        // run in order; the fences keep the compiler to it)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
         if (in && rank == 0) at[w][dig] = o + (unsigned)__popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (in) {
             keys_out[o + rank] = key[j];

@@ -314,8 +314,8 @@ int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const flo
  * must not overlap.  Sizes are the call's own (the context's configuration bounds them only where
  * its weights are used).  Matrices are rows of d elements at a stride in elements (>= d) of the type
  * dtype; any alignment of whole elements is served (16-byte aligned rows at the full rate).  Sums
- * are taken in fp32 in an order that the sizes alone decide, so equal calls give equal bits; each
- * output is rounded once to its type.  A token or target id < 0 marks a position without one (a
+ * are taken in fp32 in an order that the call's sizes, ids and alignment decide, never the schedule,
+ * so equal calls give equal bits; each output is rounded once to its type.  A token or target id < 0 marks a position without one (a
  * padded batch); ids >= vocab are treated so too and reported by the next adn_synchronize().
  * Workspaces belong to the context, grow to the largest request and are kept until it is destroyed:
  * a call that would have to grow one is refused under stream capture (ADN_E_CAPACITY), so run a
@@ -326,9 +326,11 @@ int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const flo
 /* loss_i = lse_i - z_i,t(i), z = x w^T + bias, lse_i = log sum_v exp(z_iv); with dz_iv = dloss_i
  * (exp(z_iv - lse_i) - [v = t(i)]): dx = dz w, dw = dz^T x, db = sum_i dz_i.  The logits are formed
  * a piece of the vocabulary at a time and never kept.  Rows without a target are left out: their x
- * is not read, their loss, lse and dx are 0.  A bias of -inf or of the type's lowest value takes an
- * entry out of the vocabulary; a row whose logits are all -inf, or not a number, has a loss, a dx
- * and a share of dw that are not numbers. */
+ * does not matter, their loss, lse and dx are 0.  A bias of -inf or of the type's lowest value takes
+ * an entry out of the vocabulary (finite ones below -1e38 count as -1e38); a row whose logits are all
+ * -inf, or not a number, has a loss, a dx and a share of dw that are not numbers.  Precision: fp32
+ * operands keep 22 bits in the products and bf16 ones all of theirs, dz 22 and 11; w's entries are
+ * resolved to 2^-39 of its largest, dz to 2^-38 of its dloss (db from the unrounded dz). */
 typedef struct adn_lm_loss_args {
     int32_t rows, d, vocab;     /* rows in [0, 2^20], d in [1, 8192], vocab in [1, 2^24] */
     uint32_t dtype;             /* ADN_T_*: x, w, dx and dw                               */
@@ -359,8 +361,8 @@ int adn_rms_norm_backward_async(adn_ctx *ctx, int32_t rows, int32_t d, uint32_t 
 
 /* out_i = scale * table[tokens_i], i < n (n in [0, 2^24], vocab in [1, 2^24], d in [1, 8192]); rows
  * without a token are 0.  table NULL: the context's embedding (then d = d_r, its vocab, ADN_T_F32).
- * The gradient writes the whole table: dtable[v] = scale * sum of the dout_i with tokens_i = v, in
- * the order of i, 0 where there is none. */
+ * The gradient writes the whole table: dtable[v] = scale * the sum of the dout_i with tokens_i = v
+ * (shares of them in the order of i, then the shares), 0 where there is none. */
 int adn_embed_lookup_async(adn_ctx *ctx, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,
                            const void *table, int64_t table_stride, float scale, void *out, int64_t out_stride);
 int adn_embed_grad_async(adn_ctx *ctx, int32_t n, int32_t d, int32_t vocab, uint32_t dtype, const int32_t *tokens,

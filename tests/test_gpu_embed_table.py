@@ -148,7 +148,7 @@ def test_bad_values_stay_in_their_rows(be):
     assert torch.equal(bad, toks == toks[9])
 
 
-@pytest.mark.parametrize("n", [40, 4000])
+@pytest.mark.parametrize("n", [40, 4000, 4500])
 def test_token_beyond_the_table_is_reported(be, n):
     table, dout, toks = make(n, 64, 50, F32)
     toks[5] = 50
