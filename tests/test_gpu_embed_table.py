@@ -102,9 +102,10 @@ def test_against_definition(be, n, d, V, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n", [137, 4300])
 @pytest.mark.parametrize("offset,extra", [(1, 3), (8, 8), (0, 1)])
-def test_strides_and_alignment(be, offset, extra, dtype):
-    n, d, V = 137, 200, 90
+def test_strides_and_alignment(be, offset, extra, n, dtype):
+    d, V = 200, 90
     table, dout, toks = make(n, d, V, dtype, "zipf")
     tight = run(be, table, dout, toks, 0.5)
 

@@ -210,7 +210,7 @@ def test_outputs_apart(be, what, rows):
     check(full, *reference(s), rows)
 
 
-@pytest.mark.parametrize("rows", [1, 6, 200])
+@pytest.mark.parametrize("rows", [1, 6, 200, 600])
 def test_no_row_has_a_target(be, rows):
     s = make(rows, 64, 500)
     s["targets"][:] = -1
@@ -292,7 +292,7 @@ def test_sharp_rows(be, rows, dtype):
 
 
 @pytest.mark.parametrize("scale", [1e-20, 1e15])
-@pytest.mark.parametrize("rows", [4, 150])
+@pytest.mark.parametrize("rows", [4, 150, 600])
 def test_weights_of_any_size(be, rows, scale):
     """Operands far from 1: a head of 1e-20 (or 1e15) with rows of the inverse size."""
     s = make(rows, 64, 400, dloss=None)
@@ -304,7 +304,7 @@ def test_weights_of_any_size(be, rows, scale):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("rows", [5, 133])
+@pytest.mark.parametrize("rows", [5, 133, 600])
 @pytest.mark.parametrize("offset,extra", [(0, 8), (1, 3), (8, 0)])
 def test_strides_and_alignment(be, rows, offset, extra, dtype):
     """Rows at a stride, bases off 16 bytes: same bits as tight rows, nothing written between them."""
@@ -330,8 +330,9 @@ def test_strides_and_alignment(be, rows, offset, extra, dtype):
         assert torch.equal(gaps, torch.full_like(gaps, 5.0)) and (store[:offset] == 5.0).all()
 
 
-def test_target_beyond_the_vocabulary_is_reported(be):
-    s = make(70, 64, 200)
+@pytest.mark.parametrize("rows", [4, 70, 600])
+def test_target_beyond_the_vocabulary_is_reported(be, rows):
+    s = make(rows, 64, 200)
     clean = dict(s, targets=s["targets"].clone())
     clean["targets"][3] = -1
     ref = call(be, clean, buffers(s))
@@ -345,6 +346,20 @@ def test_target_beyond_the_vocabulary_is_reported(be):
     be.synchronize()  # reported once
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,d,V,offset,extra", [(70, 96, 700, 0, 0), (70, 96, 700, 8, 16), (70, 96, 700, 1, 3), (530, 100, 1500, 0, 4),
+                                                   (33, 64, 257, 4, 1), (260, 512, 5003, 0, 0)])
+def test_losses_alone(be, rows, d, V, offset, extra, dtype):
+    """Without gradients W is read as it stands where its rows allow it: any stride and base."""
+    s = make(rows, d, V, dtype, bias=True, pad=0.1)
+    store = torch.full((offset + V * (d + extra),), float("nan"), device="cuda", dtype=dtype)
+    w = store[offset:].view(V, d + extra)[:, :d]
+    w.copy_(s["w"])
+    out = call(be, dict(s, w=w), buffers(s, ("loss", "lse")))
+    ref, tol = reference(s)
+    check(out, ref, tol, (rows, d, V, offset, extra))
+
+
 def test_empty_batch(be):
     s = make(1, 64, 300)
     out = buffers(s)
@@ -355,7 +370,7 @@ def test_empty_batch(be):
     assert (out["dw"] == 0).all() and (out["db"] == 0).all()
 
 
-@pytest.mark.parametrize("rows", [3, 90])
+@pytest.mark.parametrize("rows", [3, 90, 600])
 def test_uploaded_head(rows):
     """w None: the context's lm_w and lm_b."""
     mc = synth.ModelConfig(d=128, H=2, V=515, N=1, flags=0)
@@ -378,7 +393,7 @@ def test_uploaded_head(rows):
     b.close()
 
 
-@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("rows", [4, 200, 600])
 def test_gradients_against_differences(be, rows):
     """Central differences of the losses' sum along random directions.  A step h of a direction of unit size changes each
     logit by about h; the difference's own error is the loss's (2 tol / 2h a row) and the third derivative's, at most h^2 a
