@@ -155,7 +155,7 @@ def test_large_vocabulary(be, rows, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows,d,V", [(300, 64, 50257), (5000, 64, 50257), (257, 512, 20011), (700, 192, 30011), (3001, 256, 9973),
-                                      (1300, 1536, 4001)])
+                                      (1300, 1536, 4001), (1 << 20, 16, 65), (200001, 40, 600)])
 def test_large_tiles_and_many_pieces(be, rows, d, V, dtype):
     """Grids of more than a round of the chip, whose tiles are the large ones; 5000 rows take several pieces of the vocabulary, of
     which the last is the smaller, and add dx up over them."""
