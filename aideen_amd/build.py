@@ -17,7 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libaideen_hip.so")
 SOURCES = ["gemm.hip", "gemm_split.hip", "deq.hip", "memory.hip", "embed.hip", "adjoint.hip", "head.hip", "scan.hip", "misc.hip",
-           "loss.hip", "loss_few.hip", "norm.hip", "table.hip", "runtime.hip", "aidn.cpp", "bpe.cpp"]
+           "loss.hip", "loss_few.hip", "loss_mid.hip", "norm.hip", "table.hip", "runtime.hip", "aidn.cpp", "bpe.cpp"]
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")

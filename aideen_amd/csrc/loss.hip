@@ -1150,11 +1150,15 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
 }  // namespace
 
 size_t loss_workspace_bytes(const LossParams &p) {
-    return p.rows == 0 ? 0 : loss_few_ok(p) ? loss_few_workspace_bytes(p) : loss_plan(p).bytes;
+    return p.rows == 0 ? 0
+           : loss_few_ok(p) ? loss_few_workspace_bytes(p)
+           : loss_mid_ok(p) ? loss_mid_workspace_bytes(p)
+                            : loss_plan(p).bytes;
 }
 
 void launch_loss(const LossParams &p, void *ws, hipStream_t st) {
     if (p.rows && loss_few_ok(p)) return launch_loss_few(p, ws, st);
+    if (p.rows && loss_mid_ok(p)) return launch_loss_mid(p, ws, st);
     dispatch_type(p.dtype, [&](auto ty) {
         typedef decltype(ty) T;
         if (p.rows == 0) {  // no row: the sums over the rows are zero

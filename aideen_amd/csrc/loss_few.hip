@@ -1,7 +1,7 @@
 // The vocabulary cross entropy (loss.hip has the mathematics) of a few rows, and of small problems: fp32
 // arithmetic on the operands as they are, two launches each.
 //
-// A few rows (at most 8 of 512, 4 of 1024, 2 of 2048) read W at the rate of HBM whatever is done with it,
+// A few rows (at most 8 of 512, 4 of 1024, 2 of 2048; 4 where loss_mid.hip can take more) read W at the rate of HBM whatever is done with it,
 // so W is read once: the first kernel has R rows of x in registers, a wave takes one row of W at a time
 // (its elements in the lanes), forms its R logits, and adds it, weighted by exp(z - m) with the running
 // maximum m, to the wave's share of sum_v exp(z_v) w_v -- dx but for the target and the normalisation.
@@ -533,9 +533,16 @@ void dispatch_few(const LossParams &p, F &&f) {
     });
 }
 
-bool few(const LossParams &p) { return p.d <= 2048 && p.rows <= 64 / lane_elems(p.d); }
+// Five to eight rows need as many sums over the wave again: 512 columns of 50257 entries 113 to 119 us, of 8192
+// 46, where loss_mid.hip takes 80 and 34.
+bool few(const LossParams &p) {
+    return p.d <= 2048 && p.rows <= std::min(64 / lane_elems(p.d), loss_mid_ok(p) ? 4 : MAX_ROWS);
+}
+// Up to 64 rows go to loss_mid.hip unless W is small: 128 entries of 128 columns 18 us here and 23 to 26 there
+// (fp32), of 512 columns 23 and 25 to 31, 512 of 512 columns 48 and 26 to 31.
 bool small(const LossParams &p) {
-    return !few(p) && p.rows <= SMALL_ROWS && p.vocab <= SMALL_VOCAB && (long)p.rows * p.vocab * p.d <= SMALL;
+    return !few(p) && p.rows <= SMALL_ROWS && p.vocab <= SMALL_VOCAB && (long)p.rows * p.vocab * p.d <= SMALL &&
+           !(loss_mid_ok(p) && (long)p.vocab * p.d > 1 << 16);
 }
 
 struct FewLayout {

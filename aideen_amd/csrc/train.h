@@ -60,6 +60,11 @@ bool loss_few_ok(const LossParams &p);
 size_t loss_few_workspace_bytes(const LossParams &p);
 void launch_loss_few(const LossParams &p, void *ws, hipStream_t st);
 
+// Up to 64 rows that W's bytes bound (loss_mid.hip).
+bool loss_mid_ok(const LossParams &p);
+size_t loss_mid_workspace_bytes(const LossParams &p);
+void launch_loss_mid(const LossParams &p, void *ws, hipStream_t st);
+
 // ---- RMS norm of rows (norm.hip) -----------------------------------------------------------
 struct NormParams {
     int rows, d;

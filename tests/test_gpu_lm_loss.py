@@ -131,6 +131,9 @@ SHAPES = [
     (31, 100, 2100), (32, 256, 512), (33, 192, 65), (63, 16, 129), (64, 64, 64), (65, 31, 1023), (100, 320, 700),
     (127, 512, 256), (128, 192, 65), (129, 48, 3001), (255, 512, 1025), (257, 130, 777), (300, 1024, 513),
     (531, 96, 2049), (40, 2048, 900), (1025, 64, 97), (70, 4100, 50),
+    # up to 64 rows: as many as fit a wave's lanes, in 128-byte pieces of W, and of other widths
+    (7, 100, 300), (6, 33, 4000), (8, 500, 1001), (5, 64, 100), (64, 2048, 600), (33, 160, 3001), (9, 8192, 130), (64, 32, 2066),
+    (48, 4096, 1000), (50, 1056, 700), (64, 64, 64 * 1030 + 1), (5, 128, 20000), (63, 8192, 2000),
 ]
 
 
@@ -240,7 +243,7 @@ def test_padded_rows_are_not_read(be, rows, dtype):
 
 
 @pytest.mark.parametrize("low", [float("-inf"), torch.finfo(F32).min])
-@pytest.mark.parametrize("rows", [4, 130])
+@pytest.mark.parametrize("rows", [4, 20, 130])
 def test_entries_out_of_the_vocabulary(be, rows, low):
     """A bias of -inf or the lowest value takes entries out, whole tiles of them too."""
     s = make(rows, 64, 1500, bias=True)
@@ -253,7 +256,7 @@ def test_entries_out_of_the_vocabulary(be, rows, low):
     assert torch.equal(out["db"][10:40], torch.zeros_like(out["db"][10:40]))
 
 
-@pytest.mark.parametrize("rows", [3, 140])
+@pytest.mark.parametrize("rows", [3, 20, 140])
 def test_bad_rows_stay_their_own(be, rows):
     """A row of NaN or inf has a loss and a dx that are no numbers; the other rows' are as without it."""
     s = make(rows, 128, 600)
@@ -281,7 +284,7 @@ def test_rows_of_unlike_size(be, rows):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("rows", [4, 20, 200])
 def test_sharp_rows(be, rows, dtype):
     """Logits up to thousands: softmax weights of one and of zero, losses of zero and of thousands."""
     s = make(rows, 64, 900, dtype, spread=300.0)
@@ -292,10 +295,10 @@ def test_sharp_rows(be, rows, dtype):
 
 
 @pytest.mark.parametrize("scale", [1e-20, 1e15])
-@pytest.mark.parametrize("rows", [4, 150, 600])
-def test_weights_of_any_size(be, rows, scale):
+@pytest.mark.parametrize("rows,V", [(4, 400), (150, 400), (600, 400), (40, 1500)])
+def test_weights_of_any_size(be, rows, V, scale):
     """Operands far from 1: a head of 1e-20 (or 1e15) with rows of the inverse size."""
-    s = make(rows, 64, 400, dloss=None)
+    s = make(rows, 64, V, dloss=None)
     s["w"] *= scale
     s["w"][5] = 0
     s["x"] /= scale
@@ -304,7 +307,7 @@ def test_weights_of_any_size(be, rows, scale):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("rows", [5, 133, 600])
+@pytest.mark.parametrize("rows", [5, 21, 133, 600])
 @pytest.mark.parametrize("offset,extra", [(0, 8), (1, 3), (8, 0)])
 def test_strides_and_alignment(be, rows, offset, extra, dtype):
     """Rows at a stride, bases off 16 bytes: same bits as tight rows, nothing written between them."""
@@ -330,13 +333,40 @@ def test_strides_and_alignment(be, rows, offset, extra, dtype):
         assert torch.equal(gaps, torch.full_like(gaps, 5.0)) and (store[:offset] == 5.0).all()
 
 
-@pytest.mark.parametrize("rows", [4, 70, 600])
-def test_target_beyond_the_vocabulary_is_reported(be, rows):
-    s = make(rows, 64, 200)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [11, 64])
+def test_strides_of_up_to_64_rows(be, rows, dtype):
+    """As above where W's rows stand on 16 bytes and the other matrices anywhere."""
+    d, V = 192, 1333
+    s = make(rows, d, V, dtype, bias=True, pad=0.2)
+    tight = call(be, s, buffers(s))
+
+    def spaced(t, offset, extra):
+        n, m = t.shape
+        store = torch.full((offset + n * (m + extra),), 5.0, device="cuda", dtype=t.dtype)
+        v = store[offset:].view(n, m + extra)[:, :m]
+        v.copy_(t)
+        return v, store
+    for o, e in ((1, 3), (8, 8), (0, 2)):
+        loose = dict(s, x=spaced(s["x"], o, e)[0], w=spaced(s["w"], 8, 24)[0])
+        out = buffers(s)
+        out["dx"], dxs = spaced(out["dx"], o, e)
+        out["dw"], dws = spaced(out["dw"], o, e)
+        call(be, loose, out)
+        for k in tight:
+            assert torch.equal(out[k], tight[k]), (k, o, e)
+        for store, n in ((dxs, rows), (dws, V)):
+            gaps = store[o:].view(n, d + e)[:, d:]
+            assert torch.equal(gaps, torch.full_like(gaps, 5.0)) and (store[:o] == 5.0).all()
+
+
+@pytest.mark.parametrize("rows,V", [(4, 200), (70, 200), (600, 200), (30, 2000)])
+def test_target_beyond_the_vocabulary_is_reported(be, rows, V):
+    s = make(rows, 64, V)
     clean = dict(s, targets=s["targets"].clone())
     clean["targets"][3] = -1
     ref = call(be, clean, buffers(s))
-    s["targets"][3] = 200
+    s["targets"][3] = V
     out = buffers(s)
     be.lm_loss_async(s["x"], s["targets"], w=s["w"], dloss=s["dloss"], outputs=out)
     with pytest.raises(AdnError, match="outside"):
@@ -348,7 +378,8 @@ def test_target_beyond_the_vocabulary_is_reported(be, rows):
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows,d,V,offset,extra", [(70, 96, 700, 0, 0), (70, 96, 700, 8, 16), (70, 96, 700, 1, 3), (530, 100, 1500, 0, 4),
-                                                   (33, 64, 257, 4, 1), (260, 512, 5003, 0, 0)])
+                                                   (33, 64, 257, 4, 1), (260, 512, 5003, 0, 0), (20, 64, 3000, 8, 8),
+                                                   (64, 256, 1111, 0, 0)])
 def test_losses_alone(be, rows, d, V, offset, extra, dtype):
     """Without gradients W is read as it stands where its rows allow it: any stride and base."""
     s = make(rows, d, V, dtype, bias=True, pad=0.1)
@@ -370,7 +401,7 @@ def test_empty_batch(be):
     assert (out["dw"] == 0).all() and (out["db"] == 0).all()
 
 
-@pytest.mark.parametrize("rows", [3, 90, 600])
+@pytest.mark.parametrize("rows", [3, 20, 90, 600])
 def test_uploaded_head(rows):
     """w None: the context's lm_w and lm_b."""
     mc = synth.ModelConfig(d=128, H=2, V=515, N=1, flags=0)
