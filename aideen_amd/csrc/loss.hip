@@ -10,7 +10,7 @@
 // entries), then a piece of the vocabulary at a time the logits again, whose epilogue stores the
 // piece's dz, and dz W and dz^T x from it.  The piece holds at most PIECE_BYTES, so the workspace
 // does not grow with n V.  Forming the logits twice costs a third more operations than keeping them,
-// n V values of 4 bytes.
+// n V values of 4 bytes, which is done where they are few (loss_plan).
 //
 // Operands are fp16 planes.  fp32 tensors: two planes, hi = f16(s x) and lo = f16(s x - hi), three
 // products hi hi + hi lo + lo hi (the split of the forward's products: 2^-22 of a product is lost).
@@ -125,6 +125,7 @@ struct LossGemm {
     const float *w_part;
     int w_blocks;
     float *out_loss, *out_lse;          // LOGITS_ALL: [rows] or null
+    float *z;                           // kept logits, a workgroup's registers as they are, or null
     const float *lse, *g;               // per row: lse (in units of log 2), g_i = m_i 2^e_i (dz's factor: m_i 2^13)
     _Float16 *dz;                       // planes of the piece, blocks of rows x entries
     long dz_plane;
@@ -143,8 +144,9 @@ struct LossGemm {
 
 // The logits' epilogues: each row's maximum and sum of a tile of entries (RAW: W's rows read as they are
 // and split on the way to the MFMA, for losses alone, where planes of W would be read once); dz of a
-// piece; both in one where a tile holds the whole vocabulary.
-enum { LOGITS_STATS = 0, LOGITS_DZ = 1, GRAD = 2, LOGITS_RAW = 3, LOGITS_ALL = 4 };
+// piece, from the product again or (KEPT) from the logits that the first pass kept; both in one where a
+// tile holds the whole vocabulary.
+enum { LOGITS_STATS = 0, LOGITS_DZ = 1, GRAD = 2, LOGITS_RAW = 3, LOGITS_ALL = 4, LOGITS_KEPT = 5 };
 
 // The two gradients of a piece in one launch: tiles of the one with the longer shares first.
 struct LossGrads {
@@ -302,6 +304,23 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
+    // KEPT: this tile's logits, 16 bytes a lane side by side
+    const auto kept = [&](int i, int j, int e4) -> floatx4 * {
+        const long tile = (long)(p.a_row0 / TV + mt) * p.nN + nt;
+        return reinterpret_cast<floatx4 *>(p.z) + (((tile * NW + wave) * WTM + i) * WTN + j) * 256 + e4 * 64 + lane;
+    };
+    if constexpr (MODE == LOGITS_KEPT) {
+#pragma unroll
+        for (int i = 0; i < WTM; ++i)
+#pragma unroll
+            for (int j = 0; j < WTN; ++j)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4) {
+                    const floatx4 t = *kept(i, j, e4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * e4 + e] = t[e];
+                }
+    } else {
 #pragma unroll
     for (int t = 0; t < STAGES - 1; ++t)
         if (t < nk) issue(t);
@@ -347,6 +366,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 }
             }
         }
+    }
     }
     lds_barrier();  // every wave is done with the ring
 
@@ -396,11 +416,12 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             store(std::integral_constant<bool, false>{});
     } else {
         static_assert(TM == TV && WGN == 1, "a wave's columns are the tile's");
+        constexpr bool KEPT = MODE == LOGITS_KEPT;
         // the tile's biases; entries beyond the vocabulary get -inf: no part of any sum.  From here on
         // logits are in units of log 2 (z log2(e)), what exp2 takes.
         float *bias_l = reinterpret_cast<float *>(ring);                   // [TM]
         const int v0 = p.a_row0 + mt * TM;
-        for (int c = tid; c < TM; c += NT) {
+        for (int c = tid; !KEPT && c < TM; c += NT) {
             float b = v0 + c < p.vocab ? (p.bias ? p.bias[v0 + c] : 0.0f) : -INFINITY;
             if (b < -1e38f && b > -INFINITY) b = -1e38f;  // the type's lowest value stays finite
             bias_l[c] = b * LOG2E;
@@ -410,9 +431,9 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
         const int w0 = v0 + wm * WTM * 32;  // the wave's first entry
         float unscale[WTN];
 #pragma unroll
-        for (int j = 0; j < WTN; ++j) unscale[j] = ldexpf(LOG2E, -(p.f[nt * TN + j * 32 + r] + kw));
+        for (int j = 0; !KEPT && j < WTN; ++j) unscale[j] = ldexpf(LOG2E, -(p.f[nt * TN + j * 32 + r] + kw));
 #pragma unroll
-        for (int i = 0; i < WTM; ++i)
+        for (int i = 0; !KEPT && i < WTM; ++i)
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const floatx4 b = *reinterpret_cast<const floatx4 *>(bias_l + (wm * WTM + i) * 32 + 8 * e4 + 4 * hh);
@@ -421,9 +442,14 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         acc[i][j][4 * e4 + e] = __builtin_fmaf(acc[i][j][4 * e4 + e], unscale[j], b[e]);
+                if constexpr (MODE == LOGITS_STATS)
+                    if (p.z)
+#pragma unroll
+                        for (int j = 0; j < WTN; ++j)
+                            *kept(i, j, e4) = floatx4{acc[i][j][4 * e4], acc[i][j][4 * e4 + 1], acc[i][j][4 * e4 + 2], acc[i][j][4 * e4 + 3]};
             }
         float *red_m = bias_l + TM, *red_s = red_m + 4 * TN;               // [wave][TN]
-        if constexpr (MODE != LOGITS_DZ) {
+        if constexpr (MODE != LOGITS_DZ && !KEPT) {
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
                 const long m = (long)nt * TN + j * 32 + r;
@@ -469,7 +495,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 p.part_s[o] = sum;
             }
         }
-        if constexpr (MODE == LOGITS_DZ || MODE == LOGITS_ALL) {
+        if constexpr (MODE == LOGITS_DZ || MODE == LOGITS_ALL || KEPT) {
             float *colsum = red_s + 4 * TN + wave * (32 * WTM * 33);       // db: [WTM * 32 entries][32 + 1]
             float bsum[WTM][16];
 #pragma unroll
@@ -863,6 +889,7 @@ long round_up(long n, long to) { return (n + to - 1) / to * to; }
 
 struct LossPlan {
     bool raw;                // losses alone: W goes to the product as it is
+    bool keep;               // the logits are kept for dz
     int np, tn;              // planes; rows a workgroup of the logits' product covers
     int dcb;                 // column blocks of width d
     long rows_pad, v_pad;    // rows of the planes of x (and dz), of W
@@ -871,7 +898,7 @@ struct LossPlan {
     int w_blocks;
     int bn;                  // columns of a gradient tile
     int dx_split, dx_ks, dw_split, dw_ks;
-    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, e_dw, dz, dx_part, dw_part, db_part, bytes;
+    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, e_dw, z, dz, dx_part, dw_part, db_part, bytes;
 };
 
 // K of `len` (a multiple of 32) in at most `want` shares of whole 32s, each not empty
@@ -987,6 +1014,14 @@ LossPlan loss_plan(const LossParams &p) {
     L.ztgt = take(L.rows_pad * 4);
     L.lse = take(L.rows_pad * 4);
     L.e_dw = take(4);
+    {   // Logits of no more bytes than a piece of dz are kept where their product takes longer than writing and
+        // reading them: 512 rows against 50257 entries 1389 -> 1122 us (fp32, d = 2048), 391 -> 353 (512), 152 ->
+        // 163 (128); 592 -> 530 (bf16, 2048), 185 -> 188 (512).  A few of them stay in the caches: 512 rows
+        // against 2000 entries 158 -> 121 (fp32, 2048), 47 -> 45 (128), 50 -> 46 (bf16, 512).
+        const long bytes = L.rows_pad * L.v_pad * 4;
+        L.keep = grads && L.v_tiles > 1 && bytes <= ((long)p.d * (L.np == 2 ? 3 : 1) >= 1024 ? (long)PIECE_BYTES : 16L << 20);
+    }
+    L.z = take(L.keep ? (size_t)round_up(p.rows, L.tn) * L.v_pad * 4 : 0);
     if (grads) {
         L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
         GradSizes g{L.np, p.d};
@@ -1090,6 +1125,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
             z.w_raw = p.w, z.w_stride = (unsigned)(p.w_stride * eb), z.w_part = r.w_part, z.w_blocks = r.w_blocks;
             launch_logits<LOGITS_RAW, T, NP>(z, L.tn, st);
         } else {
+            z.z = L.keep ? (float *)(ws + L.z) : nullptr;
             launch_logits<LOGITS_STATS, T, NP>(z, L.tn, st);
         }
         Rows q{};
@@ -1107,7 +1143,10 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         const Planes DZ{z.dz, z.dz_plane, z.dz_ncb};
         z.a_row0 = (int)v0;
         z.nM = n / TV;
-        if (!all) launch_logits<LOGITS_DZ, T, NP>(z, L.tn, st);
+        if (L.keep)
+            launch_logits<LOGITS_KEPT, T, NP>(z, L.tn, st);
+        else if (!all)
+            launch_logits<LOGITS_DZ, T, NP>(z, L.tn, st);
         const int live = (int)std::min<long>(n, p.vocab - v0);
         T *dst = p.dw ? (T *)p.dw + v0 * p.dw_stride : nullptr;
         LossGrads g{};

@@ -315,8 +315,9 @@ int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const flo
  * its weights are used).  Matrices are rows of d elements at a stride in elements (>= d) of the type
  * dtype; any alignment of whole elements is served (16-byte aligned rows at the full rate).  Sums
  * are taken in fp32 in an order that the call's sizes, ids and alignment decide, never the schedule,
- * so equal calls give equal bits; each output is rounded once to its type.  A token or target id < 0 marks a position without one (a
- * padded batch); ids >= vocab are treated so too and reported by the next adn_synchronize().
+ * so equal calls give equal bits; each output is rounded once to its type.  A token or target id < 0
+ * marks a position without one (a padded batch); ids >= vocab are treated so too and reported by the
+ * next adn_synchronize().
  * Workspaces belong to the context, grow to the largest request and are kept until it is destroyed:
  * a call that would have to grow one is refused under stream capture (ADN_E_CAPACITY), so run a
  * call once before capturing it, and do not replay graphs of one context side by side. */
@@ -325,10 +326,12 @@ int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const flo
 
 /* loss_i = lse_i - z_i,t(i), z = x w^T + bias, lse_i = log sum_v exp(z_iv); with dz_iv = dloss_i
  * (exp(z_iv - lse_i) - [v = t(i)]): dx = dz w, dw = dz^T x, db = sum_i dz_i.  The logits are formed
- * a piece of the vocabulary at a time and never kept.  Rows without a target are left out: their x
- * does not matter, their loss, lse and dx are 0.  A bias of -inf or of the type's lowest value takes
- * an entry out of the vocabulary (finite ones below -1e38 count as -1e38); a row whose logits are all
- * -inf, or not a number, has a loss, a dx and a share of dw that are not numbers.  Precision: fp32
+ * a piece of the vocabulary at a time and kept (in the workspace) only where they are few: of up to
+ * 64 rows, or 256 MB of them.  Rows without a target are left out: their x does not matter, their
+ * loss, lse and dx are 0.  A bias of -inf or of the type's lowest value takes an entry out of the
+ * vocabulary (finite ones below -1e38 count as -1e38; its row of w is read and has to be finite); a
+ * row whose logits are all -inf, or not a number, has a loss, a dx and a share of dw that are not
+ * numbers.  Precision: fp32
  * operands keep at least 21 bits in the products and bf16 ones all of theirs, dz 21 and 11; w's
  * entries are resolved to 2^-39 of its largest, dz to 2^-38 of its dloss (db from the unrounded dz). */
 typedef struct adn_lm_loss_args {
