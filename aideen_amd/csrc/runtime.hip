@@ -1952,8 +1952,15 @@ void *train_workspace(adn_ctx *c, size_t bytes) {
         set_error("the workspace would have to grow under stream capture: run the call once before capturing it");
         return nullptr;
     }
-    bytes = std::max(bytes, c->train_ws.bytes + c->train_ws.bytes / 2);
-    c->train_ws.p = dmalloc(c, bytes);
+    const size_t more = std::max(bytes, c->train_ws.bytes + c->train_ws.bytes / 2);
+    try {
+        c->train_ws.p = dmalloc(c, more);
+        bytes = more;
+    } catch (const HipError &) {
+        if (more == bytes) throw;
+        (void)hipGetLastError();
+        c->train_ws.p = dmalloc(c, bytes);  // no room to grow by half: the request alone
+    }
     c->train_ws.bytes = bytes;
     return c->train_ws.p;
 }

@@ -524,5 +524,9 @@ def test_refusals(be):
     refused("other matrices", outputs=dict(dx=ok["dx"].bfloat16()))
     refused("d must be", x=torch.zeros((2, 8193), device="cuda"), targets=s["targets"][:2], dloss=s["dloss"][:2],
             w=torch.zeros((300, 8193), device="cuda"), outputs=dict(loss=ok["loss"][:2]))
+    many = (1 << 20) + 1
+    refused("number of rows", x=torch.zeros((many, 1), device="cuda"), targets=torch.zeros(many, device="cuda", dtype=torch.int32),
+            w=torch.zeros((300, 1), device="cuda"), dloss=None, outputs=dict(loss=torch.zeros(many, device="cuda")))
+    refused("vocab", w=torch.zeros(((1 << 24) + 1, 1), device="cuda"), bias=None, x=s["x"][:, :1].contiguous(), outputs=dict(loss=ok["loss"]))
     refused("vocab", w=s["w"][:0], bias=None, outputs=dict(loss=ok["loss"]))
     be.synchronize()

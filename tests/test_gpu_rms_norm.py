@@ -232,6 +232,8 @@ def test_refusals(be):
     refused("eps", lambda: be.rms_norm_async(x, y, eps=float("nan")))
     refused("stride", lambda: be.rms_norm_async(x[:1].expand(8, 64), y))
     refused("d must be", lambda: be.rms_norm_async(torch.zeros((1, 8193), device="cuda"), torch.zeros((1, 8193), device="cuda")))
+    many = torch.zeros(((1 << 24) + 1, 1), device="cuda")
+    refused("number of rows", lambda: be.rms_norm_async(many, torch.empty_like(many)))
     refused("no output", lambda: be.rms_norm_backward_async(x, dy, outputs={}))
     refused("unknown", lambda: be.rms_norm_backward_async(x, dy, outputs=dict(dgain=gain)))
     refused("shape", lambda: be.rms_norm_backward_async(x, dy[:4], outputs=dict(dx=y)))
