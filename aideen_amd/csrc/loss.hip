@@ -16,7 +16,7 @@
 // products hi hi + hi lo + lo hi (the split of the forward's products: 2^-22 of a product is lost).
 // bf16 tensors: one plane, exact (8 of 11 bits), one product.  dz is rounded to the same number of
 // planes: 22 bits or 11, where bf16 outputs keep 8.  The scales are powers of two.  W has one, by its
-// largest value (values below 2^-40 of it are lost, to the same absolute error as the rest).  Every row
+// largest value (values below 2^-37 of it are lost, to the same absolute error as the rest).  Every row
 // of x has its own for the logits, 2^f_i, by the row's largest value, and dz_i is stored without the
 // power of two in g_i = m_i 2^e_i, so that neither a row's size nor its g_i matters to another row's
 // loss or dx.  dW sums over the rows: its planes of x hold x_i 2^(e_i + F), one F for all, by the
@@ -47,6 +47,7 @@ constexpr int TV = 256;             // entries a workgroup of the logits' produc
 constexpr int NW = 4;               // waves of a workgroup
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int XR = 8;               // rows of x a block splits
+constexpr long SAMPLE_FROM = 32L << 20;  // bytes of W from which its scale is taken from a sample
 constexpr int W_BLOCKS = 1024;      // blocks of the pass over |W|, one partial each
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -79,6 +80,11 @@ __device__ __forceinline__ int exp_of(float g) {
     return a > 0.0f && a < INFINITY ? ilogbf(a) : 0;
 }
 
+__device__ __forceinline__ float finite_abs(float v) {
+    const float a = fabsf(v);
+    return a < INFINITY ? a : 0.0f;  // NaN and inf stay in their own rows
+}
+
 // Exponent that takes a magnitude to [2^14, 2^15); 0 for zero and what is not finite.
 __device__ __forceinline__ int scale_exp(float mx) {
     if (!(mx > 0.0f) || mx == INFINITY) return 0;
@@ -91,6 +97,31 @@ __device__ __forceinline__ float block_max256(float v, float *red) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// W's scale is taken from a sample of its rows, HEAD powers of two below what their largest value allows,
+// so that W is not read once for its scale alone; the kernels that split W find its largest value on the
+// way, and are launched once more for a W that the sample's scale does not fit (they end at once for
+// one that it does): 256 rows of 512 against 50257 entries, losses alone, 69 us for 60.
+constexpr int HEAD = 3;
+// The exponent from the sample's partial maxima (0 where they are: W's own are needed); `redo`: from what
+// the first launch reported, false where that is nothing.
+__device__ __forceinline__ bool scale_of_w(const float *part, int n, int head, const unsigned *w_max, bool redo, float *red,
+                                           int &kw, bool &blank) {
+    if (redo) {
+        kw = scale_exp(__builtin_bit_cast(float, *w_max));
+        return *w_max != 0;
+    }
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < n; i += NT) m = fmaxf(m, part[i]);
+    m = block_max256(m, red);
+    kw = m > 0.0f ? scale_exp(m) - head : 0;
+    blank = m == 0.0f;
+    return true;
+}
+// Reports the largest value of a share of W that the sample's scale does not fit (blank: any).
+__device__ __forceinline__ void report_w(float top, int kw, bool blank, unsigned *w_max) {
+    if (blank ? top > 0.0f : ldexpf(top, kw) > 65000.0f) atomicMax(w_max, __builtin_bit_cast(unsigned, top));
 }
 
 // Chunk (8 halves) of a block's row r that holds columns [0, 8) in the LDS image of an operand read
@@ -123,7 +154,8 @@ struct LossGemm {
     const void *w_raw;                  // LOGITS_RAW: W's rows as they are, their stride in bytes, the
     unsigned w_stride;                  //   partial maxima of |W|
     const float *w_part;
-    int w_blocks;
+    int w_blocks, w_head, w_redo;       //   of the sampled rows (scale_of_w)
+    unsigned *w_max;
     float *out_loss, *out_lse;          // LOGITS_ALL: [rows] or null
     float *z;                           // kept logits, a workgroup's registers as they are, or null
     const float *lse, *g;               // per row: lse (in units of log 2), g_i = m_i 2^e_i (dz's factor: m_i 2^13)
@@ -221,6 +253,8 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
     unsigned roff[RAW ? R_PW : 1];
     const char *rbase = nullptr;
     int kw_raw = 0;
+    float top_raw = 0.0f;
+    bool blank_raw = false;
     auto swz4 = [](int row) { return ((row >> 1) ^ (row >> 2)) & 3; };
     if constexpr (RAW) {
         static_assert(A_BLK * NP % NW == 0, "whole loads a wave");
@@ -231,9 +265,8 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             const int row = (wave + NW * j) * 16 + (lane >> 2);
             roff[j] = (unsigned)min(row, p.vocab - 1 - row0) * p.w_stride + (((lane & 3) ^ swz4(row)) * 16);
         }
-        float m = 0.0f;  // W's scale
-        for (int i = tid; i < p.w_blocks; i += NT) m = fmaxf(m, p.w_part[i]);
-        kw_raw = scale_exp(block_max256(m, reinterpret_cast<float *>(ring)));
+        if (!scale_of_w(p.w_part, p.w_blocks, p.w_head, p.w_max, p.w_redo, reinterpret_cast<float *>(ring), kw_raw, blank_raw))
+            return;
         __syncthreads();
     }
 #pragma unroll
@@ -290,6 +323,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
+            top_raw = fmaxf(top_raw, finite_abs(v[u]));
             const float x = ldexpf(v[u], kw_raw);
             hi[u] = (_Float16)x;
             if constexpr (NP == 2) lo[u] = (_Float16)(x - (float)hi[u]);  // (one plane: lo is hi)
@@ -367,6 +401,12 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             }
         }
     }
+    }
+    if constexpr (RAW) {
+        if (p.w_head && !p.w_redo && nt == 0) {
+            const float top = wave_max(top_raw);
+            if (lane == 0) report_w(top, kw_raw, blank_raw, p.w_max);
+        }
     }
     lds_barrier();  // every wave is done with the ring
 
@@ -608,11 +648,6 @@ __global__ __launch_bounds__(NT, 2) void k_loss_grads(LossGrads p) {
 }
 
 // ---- operands ------------------------------------------------------------------------------
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a < INFINITY ? a : 0.0f;  // NaN and inf stay in their own rows
-}
-
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T *row, int c, int d, float (&v)[8]) {
     if constexpr (VEC) {
@@ -651,6 +686,8 @@ struct Prep {
     long w_stride;
     int rows, d, vocab, dcb;     // dcb: column blocks of a row of width d
     int w_blocks, row_blocks;    // blocks of the pass over |W|; blocks of XR rows of x
+    int w_sample, w_step, w_head;  // rows of that pass, one of every w_step; HEAD, or 0: all of them
+    unsigned *w_max;             // W's largest value, found by the split (w_head)
     int w_rows;                  // blocks of 32 rows of W
     const int32_t *targets;
     const float *dloss;
@@ -690,14 +727,14 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
     if ((int)blockIdx.x >= p.row_blocks) {
         float m = 0.0f;
         const int nch = (p.d + 7) / 8, b = blockIdx.x - p.row_blocks;
-        const long total = (long)p.vocab * nch, step = (long)p.w_blocks * NT;
+        const long total = (long)p.w_sample * nch, step = (long)p.w_blocks * NT;
         // four chunks in flight
         for (long i = (long)b * NT + tid; i < total; i += 4 * step) {
             float x[4][8];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const long k = min(i + u * step, total - 1), v = k / nch;
-                load8<T, VECW>((const T *)p.w + v * p.w_stride, (int)(k - v * nch) * 8, p.d, x[u]);
+                load8<T, VECW>((const T *)p.w + v * p.w_step * p.w_stride, (int)(k - v * nch) * 8, p.d, x[u]);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
@@ -706,6 +743,7 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
         }
         m = block_max256(m, red);
         if (tid == 0) p.w_part[b] = m;
+        if (tid == 0 && b == 0) *p.w_max = 0;
         return;
     }
     const int rb = blockIdx.x;
@@ -751,19 +789,16 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
 }
 
 // The blocks that follow k_loss_prep's maxima: the planes of x for dW (the first blocks, where they are
-// wanted), and W's planes.
+// wanted), and W's planes, each block those of every gridDim-th block of 32 rows.
 template <typename T, int NP, bool VECX, bool VECW>
-__global__ __launch_bounds__(NT) void k_loss_split(Prep p) {
+__global__ __launch_bounds__(NT) void k_loss_split(Prep p, int redo) {
     __shared__ float red[4];
     __shared__ int ex[XR], live[XR];
-    const int tid = threadIdx.x, xb = p.x2p ? p.row_blocks : 0;
-    const bool of_x = (int)blockIdx.x < xb;
-    float m = 0.0f;
-    const float *part = of_x ? p.gmax : p.w_part;
-    const int n = of_x ? p.row_blocks : p.w_blocks;
-    for (int i = tid; i < n; i += NT) m = fmaxf(m, part[i]);
-    const int e = scale_exp(block_max256(m, red));
-    if (of_x) {
+    const int tid = threadIdx.x, xb = p.x2p && !redo ? p.row_blocks : 0;
+    if ((int)blockIdx.x < xb) {
+        float m = 0.0f;
+        for (int i = tid; i < p.row_blocks; i += NT) m = fmaxf(m, p.gmax[i]);
+        const int e = scale_exp(block_max256(m, red));
         const long rb = blockIdx.x;
         if (rb == 0 && tid == 0) *p.e_dw = -13 - e;
         if (tid < XR) {
@@ -775,14 +810,24 @@ __global__ __launch_bounds__(NT) void k_loss_split(Prep p) {
         split_rows<T, NP, VECX>(p, p.x2p, rb, live, ex);
         return;
     }
-    const long rb = (int)blockIdx.x - xb;
-    if (rb == 0 && tid == 0) *p.kw = e;
-    for (int ch = tid; ch < p.dcb * 64; ch += NT) {
-        const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
-        const long v = rb * 32 + rl;
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (v < p.vocab) load8<T, VECW>((const T *)p.w + v * p.w_stride, c, p.d, x);
-        store_planes<NP>(p.wp + (rb * p.dcb) * 512 + (long)ch * 8, p.w_plane, x, e);
+    int e;
+    bool blank = false;
+    if (!scale_of_w(p.w_part, p.w_blocks, p.w_head, p.w_max, redo, red, e, blank)) return;
+    if ((int)blockIdx.x == xb && tid == 0) *p.kw = e;
+    float top = 0.0f;
+    for (long rb = (int)blockIdx.x - xb; rb < p.w_rows; rb += (int)gridDim.x - xb)
+        for (int ch = tid; ch < p.dcb * 64; ch += NT) {
+            const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
+            const long v = rb * 32 + rl;
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (v < p.vocab) load8<T, VECW>((const T *)p.w + v * p.w_stride, c, p.d, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(x[j]));
+            store_planes<NP>(p.wp + (rb * p.dcb) * 512 + (long)ch * 8, p.w_plane, x, e);
+        }
+    if (p.w_head && !redo) {
+        top = block_max256(top, red);
+        if (tid == 0) report_w(top, e, blank, p.w_max);
     }
 }
 
@@ -895,10 +940,10 @@ struct LossPlan {
     long rows_pad, v_pad;    // rows of the planes of x (and dz), of W
     int v_tiles;             // tiles of TV entries
     int piece;               // entries a piece, a multiple of TV
-    int w_blocks;
+    int w_blocks, w_sample, w_step, w_head;
     int bn;                  // columns of a gradient tile
     int dx_split, dx_ks, dw_split, dw_ks;
-    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, part_m, part_s, ztgt, lse, e_dw, z, dz, dx_part, dw_part, db_part, bytes;
+    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, w_max, part_m, part_s, ztgt, lse, e_dw, z, dz, dx_part, dw_part, db_part, bytes;
 };
 
 // K of `len` (a multiple of 32) in at most `want` shares of whole 32s, each not empty
@@ -983,7 +1028,7 @@ LossPlan loss_plan(const LossParams &p) {
     L.dcb = (int)(round_up(p.d, 32) / 16);
     L.rows_pad = round_up(p.rows, BM);
     {   // rows of W in whole slices of 16-byte pieces, a tile's offsets in 32 bits (256 rows of 512 against
-        // 50257: 107 us with planes of W, 71 without)
+        // 50257: 107 us with planes of W, 71 without, before the scale was sampled)
         const long bytes = p.w_stride * elem_bytes(p.dtype);
         L.raw = !grads && p.vocab > TV && p.d % (L.np == 2 ? 16 : 32) == 0 && (uintptr_t)p.w % 16 == 0 && bytes % 16 == 0 &&
                 bytes < (1L << 31) / TV;
@@ -993,7 +1038,14 @@ LossPlan loss_plan(const LossParams &p) {
     const long fit = (long)(PIECE_BYTES / (L.np * 2)) / L.rows_pad / TV * TV;
     const long npieces = (L.v_pad + std::max<long>(TV, fit) - 1) / std::max<long>(TV, fit);
     L.piece = (int)round_up((L.v_pad + npieces - 1) / npieces, TV);
-    L.w_blocks = (int)std::min<long>(W_BLOCKS, ((long)p.vocab * ((p.d + 7) / 8) + NT * 4 - 1) / (NT * 4));
+    {   // W's scale from one row in 32 where W is large: 128 rows against 50257 entries 328 -> 294 us (fp32, d =
+        // 1024), 98 -> 94 (bf16, 512); below, the launch costs what it saves (8192 entries: 60 and 62, 46 and 48)
+        const bool all = (long)p.vocab * p.d * elem_bytes(p.dtype) < SAMPLE_FROM;
+        L.w_step = all ? 1 : 32;
+        L.w_sample = (p.vocab + L.w_step - 1) / L.w_step;
+        L.w_head = all ? 0 : HEAD;
+        L.w_blocks = (int)std::min<long>(W_BLOCKS, ((long)L.w_sample * ((p.d + 7) / 8) + NT * 4 - 1) / (NT * 4));
+    }
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t r = at;
@@ -1009,6 +1061,7 @@ LossPlan loss_plan(const LossParams &p) {
     L.g = take(L.rows_pad * 4);
     L.gmax = take(L.rows_pad / XR * 4);
     L.kw = take(4);
+    L.w_max = take(4);
     L.part_m = take((size_t)L.v_tiles * L.rows_pad * 4);
     L.part_s = take((size_t)L.v_tiles * L.rows_pad * 4);
     L.ztgt = take(L.rows_pad * 4);
@@ -1081,6 +1134,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     r.xp = (_Float16 *)(ws + L.xp), r.x2p = p.dw ? (_Float16 *)(ws + L.x2p) : nullptr, r.wp = (_Float16 *)(ws + L.wp);
     r.x_plane = L.rows_pad * L.dcb * 16, r.w_plane = L.v_pad * L.dcb * 16;
     r.w_part = (float *)(ws + L.w_part);
+    r.w_sample = L.w_sample, r.w_step = L.w_step, r.w_head = L.w_head, r.w_max = (unsigned *)(ws + L.w_max);
     r.f = (int32_t *)(ws + L.f), r.tgt = (int32_t *)(ws + L.tgt);
     r.g = (float *)(ws + L.g), r.gmax = (float *)(ws + L.gmax);
     r.kw = (int32_t *)(ws + L.kw), r.e_dw = (int32_t *)(ws + L.e_dw);
@@ -1090,7 +1144,9 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     auto prep = [&](auto vecx, auto vecw) {
         constexpr bool VX = decltype(vecx)::value, VW = decltype(vecw)::value;
         k_loss_prep<T, NP, VX, VW><<<prep_grid, NT, 0, st>>>(r);
-        if (!L.raw) k_loss_split<T, NP, VX, VW><<<split_grid, NT, 0, st>>>(r);
+        if (L.raw) return;
+        k_loss_split<T, NP, VX, VW><<<split_grid, NT, 0, st>>>(r, 0);
+        if (L.w_head) k_loss_split<T, NP, VX, VW><<<std::min(r.w_rows, 1024), NT, 0, st>>>(r, 1);
     };
     using std::bool_constant;
     if (vx && vw)
@@ -1123,7 +1179,12 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         if (L.raw) {
             z.K = z.Ks = p.d;
             z.w_raw = p.w, z.w_stride = (unsigned)(p.w_stride * eb), z.w_part = r.w_part, z.w_blocks = r.w_blocks;
+            z.w_head = L.w_head, z.w_max = r.w_max;
             launch_logits<LOGITS_RAW, T, NP>(z, L.tn, st);
+            if (L.w_head) {
+                z.w_redo = 1;
+                launch_logits<LOGITS_RAW, T, NP>(z, L.tn, st);
+            }
         } else {
             z.z = L.keep ? (float *)(ws + L.z) : nullptr;
             launch_logits<LOGITS_STATS, T, NP>(z, L.tn, st);

@@ -332,7 +332,7 @@ int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const flo
  * vocabulary (finite ones below -1e38 count as -1e38; its row of w is read and has to be finite); a
  * row whose logits are all -inf, or not a number, has a loss, a dx and a share of dw that are not
  * numbers.  Precision: fp32 operands keep at least 21 bits in the products and bf16 ones all of
- * theirs, dz 21 and 11; w's entries are resolved to 2^-39 of its largest, dz to 2^-38 of its dloss
+ * theirs, dz 21 and 11; w's entries are resolved to 2^-36 of its largest, dz to 2^-38 of its dloss
  * (db from the unrounded dz). */
 typedef struct adn_lm_loss_args {
     int32_t rows, d, vocab;     /* rows in [0, 2^20], d in [1, 8192], vocab in [1, 2^24] */

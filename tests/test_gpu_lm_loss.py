@@ -309,6 +309,33 @@ def test_weights_of_any_size(be, rows, V, scale):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["large row", "zeros in the sample", "small sample", "small weights", "as the sample"])
+@pytest.mark.parametrize("grads", [True, False])
+def test_weights_unlike_their_sample(be, grads, kind, dtype):
+    """A large W's scale comes from one row in 32: rows that it does not fit, and samples that say nothing."""
+    s = make(100, 256, 70000, dtype, bias=True, pad=0.1)
+    w = s["w"]
+    if kind == "large row":
+        w[17] *= 1000
+        w[19999] *= 100
+    elif kind == "zeros in the sample":
+        w[::32] = 0
+        w *= 2.0 ** -60
+        s["x"] *= 2.0 ** 60
+    elif kind == "small sample":
+        w[::32] *= 2.0 ** -20
+    elif kind == "small weights":
+        w *= 2.0 ** -70
+        w[5] *= 2.0 ** -20
+        s["x"] *= 2.0 ** 70
+    else:
+        w[1::32] *= 7
+    out = call(be, s, buffers(s) if grads else buffers(s, ("loss", "lse")))
+    ref, tol = reference(s)
+    check(out, ref, tol, kind)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows", [5, 21, 133, 600])
 @pytest.mark.parametrize("offset,extra", [(0, 8), (1, 3), (8, 0)])
 def test_strides_and_alignment(be, rows, offset, extra, dtype):
