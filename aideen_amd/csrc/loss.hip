@@ -16,7 +16,7 @@
 // products hi hi + hi lo + lo hi (the split of the forward's products: 2^-22 of a product is lost).
 // bf16 tensors: one plane, exact (8 of 11 bits), one product.  dz is rounded to the same number of
 // planes: 22 bits or 11, where bf16 outputs keep 8.  The scales are powers of two.  W has one, by its
-// largest value (values below 2^-37 of it are lost, to the same absolute error as the rest).  Every row
+// largest value (values below 2^-36 of it are lost, to the same absolute error as the rest).  Every row
 // of x has its own for the logits, 2^f_i, by the row's largest value, and dz_i is stored without the
 // power of two in g_i = m_i 2^e_i, so that neither a row's size nor its g_i matters to another row's
 // loss or dx.  dW sums over the rows: its planes of x hold x_i 2^(e_i + F), one F for all, by the
