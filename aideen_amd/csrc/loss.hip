@@ -356,51 +356,51 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 }
     } else {
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t)
-        if (t < nk) issue(t);
-    for (int kt = 0; kt < nk; ++kt) {
-        // slice kt is in LDS once this wave's later loads are all that is in flight; the barrier
-        // covers the other waves' loads, and their reads of the slot that is loaded next
-        if (kt + STAGES - 2 < nk)
-            wait_vmcnt<(STAGES - 2) * LOADS>();
-        else
-            wait_vmcnt<0>();
-        lds_barrier();
-        if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1);
-        const _Float16 *base = ring + (kt % STAGES) * SLICE;
+        for (int t = 0; t < STAGES - 1; ++t)
+            if (t < nk) issue(t);
+        for (int kt = 0; kt < nk; ++kt) {
+            // slice kt is in LDS once this wave's later loads are all that is in flight; the barrier
+            // covers the other waves' loads, and their reads of the slot that is loaded next
+            if (kt + STAGES - 2 < nk)
+                wait_vmcnt<(STAGES - 2) * LOADS>();
+            else
+                wait_vmcnt<0>();
+            lds_barrier();
+            if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1);
+            const _Float16 *base = ring + (kt % STAGES) * SLICE;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            half8 a[NP][WTM];
-            if constexpr (RAW) {
+            for (int kb = 0; kb < KB; ++kb) {
+                half8 a[NP][WTM];
+                if constexpr (RAW) {
 #pragma unroll
-                for (int i = 0; i < WTM; ++i) raw_frag(base, wm * WTM + i, kb, a[0][i], a[NP - 1][i]);
-            } else {
+                    for (int i = 0; i < WTM; ++i) raw_frag(base, wm * WTM + i, kb, a[0][i], a[NP - 1][i]);
+                } else {
 #pragma unroll
-                for (int q = 0; q < NP; ++q)
+                    for (int q = 0; q < NP; ++q)
 #pragma unroll
-                    for (int i = 0; i < WTM; ++i) a[q][i] = frag(base + q * A_SZ, TRA, wm * WTM + i, kb);
-            }
-            half8 b[NP][WTN];
+                        for (int i = 0; i < WTM; ++i) a[q][i] = frag(base + q * A_SZ, TRA, wm * WTM + i, kb);
+                }
+                half8 b[NP][WTN];
 #pragma unroll
-            for (int j = 0; j < WTN; ++j)
+                for (int j = 0; j < WTN; ++j)
 #pragma unroll
-                for (int q = 0; q < NP; ++q) b[q][j] = frag(base + NP * A_SZ + q * B_SZ, TRB, wn * WTN + j, kb);
-            // all of a k block's reads before its first MFMA: left to itself the compiler reads the last
-            // columns halfway and waits there (8192 x 512 fp32 4600 us for 4505, 4096 x 2048 bf16 3285 for 3218)
-            __builtin_amdgcn_sched_barrier(0);
+                    for (int q = 0; q < NP; ++q) b[q][j] = frag(base + NP * A_SZ + q * B_SZ, TRB, wn * WTN + j, kb);
+                // all of a k block's reads before its first MFMA: left to itself the compiler reads the last
+                // columns halfway and waits there (8192 x 512 fp32 4600 us for 4505, 4096 x 2048 bf16 3285 for 3218)
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < WTN; ++j) {
+                for (int j = 0; j < WTN; ++j) {
 #pragma unroll
-                for (int i = 0; i < WTM; ++i) {
-                    if constexpr (NP == 2) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
+                    for (int i = 0; i < WTM; ++i) {
+                        if constexpr (NP == 2) {
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
+                        }
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
                     }
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
                 }
             }
         }
-    }
     }
     if constexpr (RAW) {
         if (p.w_head && !p.w_redo && nt == 0) {
