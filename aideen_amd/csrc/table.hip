@@ -6,9 +6,11 @@
 // The gradient adds each table row's positions in a fixed order, so it is the same bits on every run.
 //
 // Up to FEW positions: one launch.  A block a position compares its token with all the others (eight
-// 64-bit masks a wave); the first block of a token adds the token's rows, its waves an eighth of them
-// each.  Other blocks write zeros where no token is, which is most of the time: 256 positions of 512
-// columns of 50257 entries 16 us (6.3 TB/s), 4096 30 us (sorted 46).
+// 64-bit masks a wave).  The blocks of a token share its columns, 64 lanes' at a time: a wave adds all the
+// rows of its columns where they are few, an eighth of them where they are many (4096 positions of 2048
+// columns on 65 tokens, the most frequent a fifth: 79 us with one block a token, 17 shared).  Other blocks
+// write zeros where no token is, which is most of the time: 256 positions of 512 columns of 50257 entries
+// 16 us (6.3 TB/s), 4096 30 us (sorted 46).
 //
 // More: the positions are sorted by token (a stable radix sort of 8 bits a pass), the sorted list is
 // cut into chunks, a wave adds one chunk's rows in order and stores the table rows that begin and end
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(64 * FW) void k_grad_few(TableParams p) {
     constexpr int W = VEC ? 16 / (int)sizeof(T) : 1, LOADS = 16;
     typedef typename VecT<T, W>::type V;
     __shared__ int list[FEW];
-    __shared__ int cnt[FW], lead[FW];
+    __shared__ int cnt[FW], ahead[FW];
     __shared__ int here[FEW_ROWS];
     __shared__ float part[FW - 1][64 * W];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -117,27 +119,30 @@ __global__ __launch_bounds__(64 * FW) void k_grad_few(TableParams p) {
     const int me = p.tokens[blockIdx.x];
     if (me >= p.vocab && tid == 0) atomicOr(p.err, ADN_DEVERR_TOKEN);
     if (me < 0 || me >= p.vocab) return;
-    int mine = 0, first = FEW;
+    int mine = 0, before = 0;
 #pragma unroll
-    for (int u = 7; u >= 0; --u) {
-        const unsigned long long hit = __ballot(t[u] == me);
-        mine += __popcll(hit);
-        if (hit) first = wave * S + u * 64 + __ffsll(hit) - 1;
+    for (int u = 0; u < 8; ++u) {
+        mine += __popcll(__ballot(t[u] == me));
+        before += __popcll(__ballot(t[u] == me && wave * S + u * 64 + lane < (int)blockIdx.x));
     }
     if (lane == 0) {
         cnt[wave] = mine;
-        lead[wave] = first;
+        ahead[wave] = before;
     }
     __syncthreads();
-    int m = 0, at = 0;
-    first = FEW;
+    int m = 0, at = 0, rank = 0;
 #pragma unroll
     for (int w = 0; w < FW; ++w) {
         if (w == wave) at = m;
         m += cnt[w];
-        first = min(first, lead[w]);
+        rank += ahead[w];
     }
-    if (first != (int)blockIdx.x) return;  // an earlier block adds this token (all waves agree)
+    // the token's blocks, one a position, share its columns: a wave a strip of 64 lanes' where the rows are
+    // few, else a block a strip, its waves an eighth of the rows each
+    const int strips = (p.d + 64 * W - 1) / (64 * W);
+    const bool light = m <= LOADS;
+    const int sharers = min(m, light ? (strips + FW - 1) / FW : strips);
+    if (rank >= sharers) return;  // (all waves agree)
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
         const unsigned long long hit = __ballot(t[u] == me);
@@ -145,9 +150,9 @@ __global__ __launch_bounds__(64 * FW) void k_grad_few(TableParams p) {
         at += __popcll(hit);
     }
     __syncthreads();
-    const int per = (m + FW - 1) / FW, a = min(m, wave * per), b = min(m, a + per);
-    for (int c0 = 0; c0 < p.d; c0 += 64 * W) {
-        const int c = c0 + lane * W;
+    const int per = light ? m : (m + FW - 1) / FW, a = light ? 0 : min(m, wave * per), b = min(m, a + per);
+    for (int s = light ? rank * FW + wave : rank; s < strips; s += light ? sharers * FW : sharers) {
+        const int c = (s * 64 + lane) * W;
         float acc[W];
 #pragma unroll
         for (int j = 0; j < W; ++j) acc[j] = 0.0f;
@@ -163,19 +168,19 @@ __global__ __launch_bounds__(64 * FW) void k_grad_few(TableParams p) {
 #pragma unroll
                         for (int j = 0; j < W; ++j) acc[j] += to_f32<T>(v[u][j]);
             }
-        if (m > 1) {  // the waves' sums in order
+        if (!light) {  // the waves' sums in order
             __syncthreads();
             if (wave)
 #pragma unroll
                 for (int j = 0; j < W; ++j) part[wave - 1][lane * W + j] = acc[j];
             __syncthreads();
-            if (wave == 0)
+            if (wave) continue;
 #pragma unroll
-                for (int q = 0; q < FW - 1; ++q)
+            for (int q = 0; q < FW - 1; ++q)
 #pragma unroll
-                    for (int j = 0; j < W; ++j) acc[j] += part[q][lane * W + j];
+                for (int j = 0; j < W; ++j) acc[j] += part[q][lane * W + j];
         }
-        if (wave == 0 && c < p.d) {
+        if (c < p.d) {
             V o;
 #pragma unroll
             for (int j = 0; j < W; ++j) o[j] = from_f32<T>(acc[j] * p.scale);

@@ -88,7 +88,7 @@ CASES = [(1, 1, 1, "uniform"), (1, 64, 50257, "uniform"), (2, 7, 3, "uniform"), 
          (100, 8192, 20, "zipf"), (3000, 4, 1 << 24, "uniform"), (2048, 64, 50257, "one"), (16384, 64, 1024, "padded"), (1023, 64, 40, "zipf"),
          (1024, 130, 50257, "padded"), (1025, 64, 40, "zipf"), (1000, 64, 3, "one"), (4095, 64, 700, "zipf"), (4096, 48, 50257, "padded"), (4096, 2048, 9, "one"), (513, 64, 20, "zipf"),
          (140001, 8, 300, "zipf"), (131072, 8, 2000, "ends"),
-         (131073, 8, 70001, "padded")]
+         (131073, 8, 70001, "padded"), (2952, 2048, 512, "zipf"), (2000, 520, 9, "zipf"), (100, 1000, 6, "uniform"), (500, 8192, 31, "zipf")]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
