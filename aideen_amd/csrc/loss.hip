@@ -171,7 +171,7 @@ struct LossGemm {
     void *dst;                          // [rows] of the result
     long dst_stride;
     int out_rows, out_cols;
-    const int32_t *e_all;               // exponent of dst's values
+    const int32_t *e_all;               // exponent of dst's values (dx: of g and kw_dev)
 };
 
 // The logits' epilogues: each row's maximum and sum of a tile of entries (RAW: W's rows read as they are
@@ -412,7 +412,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 
     // Output layout of a 32x32 tile: lane holds column r; register e row 8 (e / 4) + 4 hh + e % 4.
     if constexpr (MODE == GRAD) {
-        const int ec = p.e_all ? *p.e_all : 0;
+        const int ec = p.e_all ? *p.e_all : p.g ? *p.kw_dev : 0;  // g: dx, a row's own exponent
         const long r0 = (long)mt * TM + wm * WTM * 32 + 4 * hh;
         const int c0 = nt * TN + wn * WTN * 32 + r;
         auto store = [&](auto whole) {
@@ -443,9 +443,10 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                     for (int e = 0; e < 16; ++e) {
                         const int rr = 8 * (e / 4) + e % 4;
                         T *o = (T *)p.dst + (r0 + i * 32 + rr) * p.dst_stride + c0;
+                        const int er = p.g ? exp_of(p.g[r0 + i * 32 + rr]) - 13 - ec : ec;
 #pragma unroll
                         for (int j = 0; j < WTN; ++j)
-                            if (in(rr, j)) o[32 * j] = from_f32<T>(ldexpf(acc[i][j][e], ec));
+                            if (in(rr, j)) o[32 * j] = from_f32<T>(ldexpf(acc[i][j][e], er));
                     }
                 }
             }
@@ -688,7 +689,7 @@ struct Prep {
     int w_blocks, row_blocks;    // blocks of the pass over |W|; blocks of XR rows of x
     int w_sample, w_step, w_head;  // rows of that pass, one of every w_step; HEAD, or 0: all of them
     unsigned *w_max;             // W's largest value, found by the split (w_head)
-    int w_rows;                  // blocks of 32 rows of W
+    int w_rows, w_cols;          // blocks of 32 rows of W, and blocks that share the columns of each
     const int32_t *targets;
     const float *dloss;
     unsigned *err;
@@ -789,7 +790,8 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
 }
 
 // The blocks that follow k_loss_prep's maxima: the planes of x for dW (the first blocks, where they are
-// wanted), and W's planes, each block those of every gridDim-th block of 32 rows.
+// wanted), and W's planes, each block those of every so many-th block of 32 rows, of a share of the columns
+// where W has few rows.
 template <typename T, int NP, bool VECX, bool VECW>
 __global__ __launch_bounds__(NT) void k_loss_split(Prep p, int redo) {
     __shared__ float red[4];
@@ -815,8 +817,10 @@ __global__ __launch_bounds__(NT) void k_loss_split(Prep p, int redo) {
     if (!scale_of_w(p.w_part, p.w_blocks, p.w_head, p.w_max, redo, red, e, blank)) return;
     if ((int)blockIdx.x == xb && tid == 0) *p.kw = e;
     float top = 0.0f;
-    for (long rb = (int)blockIdx.x - xb; rb < p.w_rows; rb += (int)gridDim.x - xb)
-        for (int ch = tid; ch < p.dcb * 64; ch += NT) {
+    const int b = (int)blockIdx.x - xb, part = b % p.w_cols, per = (p.dcb + p.w_cols - 1) / p.w_cols;
+    const int ch1 = min((part + 1) * per, p.dcb) * 64;
+    for (long rb = b / p.w_cols; rb < p.w_rows; rb += ((int)gridDim.x - xb) / p.w_cols)
+        for (int ch = part * per * 64 + tid; ch < ch1; ch += NT) {
             const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
             const long v = rb * 32 + rl;
             float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -892,6 +896,7 @@ struct Join {
     int S, rows, d;
     void *dst;
     long stride;
+    bool vec;            // rows of whole fours, aligned as such
     const int32_t *e_all, *kw;
     const float *g;
     int n_blocks;
@@ -912,6 +917,21 @@ __global__ __launch_bounds__(NT) void k_loss_join(Join p) {
         return;
     }
     const long n = (long)p.rows * p.d;
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    if (p.vec) {  // four columns a thread
+        for (long i = (long)blockIdx.x * NT + threadIdx.x; i < n / 4; i += (long)p.n_blocks * NT) {
+            floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+            for (int q = 0; q < p.S; ++q) s += *reinterpret_cast<const floatx4 *>(p.part + q * n + i * 4);
+            const long row = n / 4 <= 0xffffffffl ? (unsigned)i / (unsigned)(p.d / 4) : i / (p.d / 4);
+            const int e = p.g ? exp_of(p.g[row]) - 13 - *p.kw : *p.e_all;
+            V4 o;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[u] = from_f32<T>(ldexpf(s[u], e));
+            *reinterpret_cast<V4 *>((T *)p.dst + row * p.stride + (i * 4 - row * p.d)) = o;
+        }
+        return;
+    }
     for (long i = (long)blockIdx.x * NT + threadIdx.x; i < n; i += (long)p.n_blocks * NT) {
         float s = 0.0f;
 #pragma unroll 8
@@ -935,6 +955,7 @@ long round_up(long n, long to) { return (n + to - 1) / to * to; }
 struct LossPlan {
     bool raw;                // losses alone: W goes to the product as it is
     bool keep;               // the logits are kept for dz
+    bool dx_whole;           // dx is written by its product
     int np, tn;              // planes; rows a workgroup of the logits' product covers
     int dcb;                 // column blocks of width d
     long rows_pad, v_pad;    // rows of the planes of x (and dz), of W
@@ -984,6 +1005,7 @@ double makespan(long n1, double a, long n2, double b) {
 struct GradSizes {
     int np, d;
     long dx_rows, dx_k, dx_elems;  // 128-row tiles, length of the sum, elements of dx; 0: not wanted
+    bool whole;                    // one piece: dx of one share is written as it is
     long dw_rows, dw_k, dw_elems;  // of a piece of dW
 };
 struct GradPick {
@@ -1009,7 +1031,7 @@ GradPick pick_grads(const GradSizes &g) {
                 const double a = kx * unit + epi, b = kw * unit + epi;
                 const long ux = g.dx_rows * nbn * nx, uw = g.dw_rows * nbn * nw;
                 double t = a >= b ? makespan(ux, a, uw, b) : makespan(uw, b, ux, a);
-                t += join * ((double)g.dx_elems * nx + (nw > 1 ? (double)g.dw_elems * nw : 0.0));
+                t += join * ((double)g.dx_elems * (g.whole && nx == 1 ? 0 : nx) + (nw > 1 ? (double)g.dw_elems * nw : 0.0));
                 if (t < best) {
                     best = t;
                     pick = {bn, nx, kx, nw, kw};
@@ -1083,9 +1105,11 @@ LossPlan loss_plan(const LossParams &p) {
             const long n = std::min<long>(L.piece, p.vocab);
             g.dw_rows = round_up(n, BM) / BM, g.dw_k = round_up(p.rows, 32), g.dw_elems = n * p.d;
         }
+        g.whole = L.piece == L.v_pad;
         const GradPick k = pick_grads(g);
         L.bn = k.bn, L.dx_split = k.dx_split, L.dx_ks = k.dx_ks, L.dw_split = k.dw_split, L.dw_ks = k.dw_ks;
-        if (p.dx) L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
+        L.dx_whole = p.dx && g.whole && L.dx_split == 1;
+        if (p.dx && !L.dx_whole) L.dx_part = take((size_t)L.dx_split * p.rows * p.d * 4);
         if (p.dw && L.dw_split > 1) L.dw_part = take((size_t)L.dw_split * L.piece * p.d * 4);
         if (p.db) L.db_part = take((size_t)(L.rows_pad / L.tn) * L.v_pad * 4);
     }
@@ -1119,6 +1143,9 @@ void launch_grads(LossGrads &g, int bn, hipStream_t st) {
 }
 
 int join_blocks(long n) { return (int)std::min<long>(2048, (n + NT - 1) / NT); }
+bool join_vec(const Join &j, int eb) {
+    return j.d % 4 == 0 && (uintptr_t)j.dst % (4 * eb) == 0 && j.stride % 4 == 0;
+}
 
 template <typename T, int NP>
 void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) {
@@ -1130,6 +1157,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     r.x = p.x, r.x_stride = p.x_stride, r.w = p.w, r.w_stride = p.w_stride;
     r.rows = p.rows, r.d = p.d, r.vocab = p.vocab, r.dcb = L.dcb;
     r.w_blocks = L.w_blocks, r.row_blocks = (int)(L.rows_pad / XR), r.w_rows = (int)(L.v_pad / 32);
+    r.w_cols = std::max(1, std::min(1024 / r.w_rows, L.dcb / 4));  // 1142 rows of 2048: 20 us for 8
     r.targets = p.targets, r.dloss = p.dloss, r.err = p.err;
     r.xp = (_Float16 *)(ws + L.xp), r.x2p = p.dw ? (_Float16 *)(ws + L.x2p) : nullptr, r.wp = (_Float16 *)(ws + L.wp);
     r.x_plane = L.rows_pad * L.dcb * 16, r.w_plane = L.v_pad * L.dcb * 16;
@@ -1140,13 +1168,13 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     r.kw = (int32_t *)(ws + L.kw), r.e_dw = (int32_t *)(ws + L.e_dw);
     const bool grads = p.dx || p.dw || p.db;
     const unsigned prep_grid = (unsigned)(r.row_blocks + r.w_blocks);
-    const unsigned split_grid = (unsigned)((r.x2p ? r.row_blocks : 0) + r.w_rows);
+    const unsigned split_grid = (unsigned)((r.x2p ? r.row_blocks : 0) + r.w_rows * r.w_cols);
     auto prep = [&](auto vecx, auto vecw) {
         constexpr bool VX = decltype(vecx)::value, VW = decltype(vecw)::value;
         k_loss_prep<T, NP, VX, VW><<<prep_grid, NT, 0, st>>>(r);
         if (L.raw) return;
         k_loss_split<T, NP, VX, VW><<<split_grid, NT, 0, st>>>(r, 0);
-        if (L.w_head) k_loss_split<T, NP, VX, VW><<<std::min(r.w_rows, 1024), NT, 0, st>>>(r, 1);
+        if (L.w_head) k_loss_split<T, NP, VX, VW><<<std::min(r.w_rows, 1024) * r.w_cols, NT, 0, st>>>(r, 1);
     };
     using std::bool_constant;
     if (vx && vw)
@@ -1217,7 +1245,10 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
             x.B.p += v0 / 32 * (long)W.ncb * 512;
             x.nM = (int)(round_up(p.rows, BM) / BM), x.nN = nbn, x.S = (n + L.dx_ks - 1) / L.dx_ks;
             x.K = n, x.Ks = L.dx_ks;
-            x.part = (float *)(ws + L.dx_part), x.part_ld = p.d, x.add = v0 > 0;
+            if (L.dx_whole)
+                x.dst = p.dx, x.dst_stride = p.dx_stride, x.g = r.g, x.kw_dev = r.kw;
+            else
+                x.part = (float *)(ws + L.dx_part), x.part_ld = p.d, x.add = v0 > 0;
             x.out_rows = p.rows, x.out_cols = p.d;
         }
         if (p.dw) {
@@ -1235,14 +1266,17 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         if (p.dw && L.dw_split > 1) {
             Join j{};
             j.part = g.dw.part, j.S = L.dw_split, j.rows = live, j.d = p.d, j.dst = dst, j.stride = p.dw_stride;
-            j.e_all = r.e_dw, j.n_blocks = join_blocks((long)live * p.d);
+            j.vec = join_vec(j, eb);
+            j.e_all = r.e_dw, j.n_blocks = join_blocks((long)live * p.d / (j.vec ? 4 : 1));
             k_loss_join<T><<<j.n_blocks, NT, 0, st>>>(j);
         }
     }
-    if (!p.dx && !p.db) return;
+    const bool join_dx = p.dx && !L.dx_whole;
+    if (!join_dx && !p.db) return;
     Join j{};
     j.part = (float *)(ws + L.dx_part), j.S = L.dx_split, j.rows = p.rows, j.d = p.d, j.dst = p.dx, j.stride = p.dx_stride;
-    j.g = r.g, j.kw = r.kw, j.n_blocks = p.dx ? join_blocks((long)p.rows * p.d) : 0;
+    j.vec = join_vec(j, eb);
+    j.g = r.g, j.kw = r.kw, j.n_blocks = join_dx ? join_blocks((long)p.rows * p.d / (j.vec ? 4 : 1)) : 0;
     j.db_part = z.db_part, j.db_tiles = z.nN, j.db_ld = z.db_ld, j.vocab = p.vocab, j.db = p.db;
     k_loss_join<T><<<j.n_blocks + (p.db ? (p.vocab + NT - 1) / NT : 0), NT, 0, st>>>(j);
 }
