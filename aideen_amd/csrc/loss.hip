@@ -907,13 +907,19 @@ struct Join {
 };
 template <typename T>
 __global__ __launch_bounds__(NT) void k_loss_join(Join p) {
-    if ((int)blockIdx.x >= p.n_blocks) {
-        const int v = ((int)blockIdx.x - p.n_blocks) * NT + threadIdx.x;
-        if (v >= p.vocab) return;
+    if ((int)blockIdx.x >= p.n_blocks) {  // 64 entries, the waves a quarter of the tiles each
+        __shared__ float red[4][64];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int v = ((int)blockIdx.x - p.n_blocks) * 64 + lane;
+        const int per = (p.db_tiles + 3) / 4, t1 = min(p.db_tiles, (wave + 1) * per);
         float s = 0.0f;
-#pragma unroll 8
-        for (int t = 0; t < p.db_tiles; ++t) s += p.db_part[t * p.db_ld + v];
-        p.db[v] = s;
+        if (v < p.vocab) {
+#pragma unroll 16
+            for (int t = wave * per; t < t1; ++t) s += p.db_part[t * p.db_ld + v];
+        }
+        red[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && v < p.vocab) p.db[v] = ((s + red[1][lane]) + red[2][lane]) + red[3][lane];
         return;
     }
     const long n = (long)p.rows * p.d;
@@ -1278,7 +1284,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     j.vec = join_vec(j, eb);
     j.g = r.g, j.kw = r.kw, j.n_blocks = join_dx ? join_blocks((long)p.rows * p.d / (j.vec ? 4 : 1)) : 0;
     j.db_part = z.db_part, j.db_tiles = z.nN, j.db_ld = z.db_ld, j.vocab = p.vocab, j.db = p.db;
-    k_loss_join<T><<<j.n_blocks + (p.db ? (p.vocab + NT - 1) / NT : 0), NT, 0, st>>>(j);
+    k_loss_join<T><<<j.n_blocks + (p.db ? (p.vocab + 63) / 64 : 0), NT, 0, st>>>(j);
 }
 
 }  // namespace

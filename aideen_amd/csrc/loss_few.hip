@@ -27,7 +27,7 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int MAX_SHARES = 512;     // blocks that share the vocabulary
 constexpr int MAX_ROWS = 8;         // of the few
 constexpr long SMALL = 1L << 23;
-constexpr int SMALL_ROWS = 512, SMALL_VOCAB = 512;  // a block walks all of one of them
+constexpr int SMALL_ROWS = 256, SMALL_VOCAB = 256;  // a block walks all of one of them
 
 struct Few {
     LossParams p;
@@ -539,7 +539,8 @@ bool few(const LossParams &p) {
     return p.d <= 2048 && p.rows <= std::min(64 / lane_elems(p.d), loss_mid_ok(p) ? 4 : MAX_ROWS);
 }
 // Up to 64 rows go to loss_mid.hip unless W is small: 128 entries of 128 columns 18 us here and 23 to 26 there
-// (fp32), of 512 columns 23 and 25 to 31, 512 of 512 columns 48 and 26 to 31.
+// (fp32), of 512 columns 23 and 25 to 31, 512 of 512 columns 48 and 26 to 31.  A block walks all rows or
+// all entries 64 at a time: 512 rows of 64 against 65 entries 43 us here and 29 on loss.hip's products.
 bool small(const LossParams &p) {
     return !few(p) && p.rows <= SMALL_ROWS && p.vocab <= SMALL_VOCAB && (long)p.rows * p.vocab * p.d <= SMALL &&
            !(loss_mid_ok(p) && (long)p.vocab * p.d > 1 << 16);

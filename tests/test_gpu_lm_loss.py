@@ -133,6 +133,7 @@ SHAPES = [
     (531, 96, 2049), (40, 2048, 900), (1025, 64, 97), (70, 4100, 50),
     # up to 64 rows: as many as fit a wave's lanes, in 128-byte pieces of W, and of other widths
     (7, 100, 300), (6, 33, 4000), (8, 500, 1001), (5, 64, 100), (64, 2048, 600), (33, 160, 3001), (9, 8192, 130), (64, 32, 2066),
+    (256, 100, 256), (199, 64, 250), (257, 64, 250), (2100, 96, 130), (11001, 256, 128),
     # logits kept or formed again, on tiles of every size
     (65, 512, 300), (1000, 352, 5000), (2000, 640, 2100), (130, 1024, 900), (600, 2048, 3000), (400, 64, 4000), (5000, 64, 1500),
     (48, 4096, 1000), (50, 1056, 700), (64, 64, 64 * 1030 + 1), (5, 128, 20000), (63, 8192, 2000),
