@@ -478,7 +478,7 @@ def test_gradients_against_differences(be, rows):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("rows,d,V", [(1, 512, 5000), (30, 128, 2000), (300, 192, 3000)])
+@pytest.mark.parametrize("rows,d,V", [(1, 512, 5000), (30, 128, 2000), (300, 192, 3000), (100, 512, 40000)])
 def test_same_bits_again_and_in_a_graph(be, rows, d, V, dtype):
     """Equal calls give equal bits; a captured call replayed with other work and a larger call (which grows the workspace)
     in between does too."""
