@@ -203,11 +203,17 @@ _KEPT = []
 
 
 def _backend():
-    """The one context that a program keeps; its stream is the one that the tensors are used on."""
+    """The one context that a program keeps.  A context has a stream of its own unless it is handed another, and torch's
+    default stream cannot be handed over: torch's work moves to a stream that both use, behind what the default one holds,
+    so that every tensor is made, used and read in one order."""
     if not _KEPT:
         from aideen_amd import synth
         from aideen_amd.backend import GpuDeqBackend
-        _KEPT.append(GpuDeqBackend(synth.ModelConfig(d=512, H=8, V=50257, flags=0), 1, 1))
+        be, stream = GpuDeqBackend(synth.ModelConfig(d=512, H=8, V=50257, flags=0), 1, 1), torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
+        be.set_stream(stream.cuda_stream)
+        _KEPT.append(be)
     return _KEPT[0]
 
 
