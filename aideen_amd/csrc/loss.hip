@@ -17,10 +17,13 @@
 // bf16 tensors: one plane, exact (8 of 11 bits), one product.  dz is rounded to the same number of
 // planes: 22 bits or 11, where bf16 outputs keep 8.  The scales are powers of two.  W has one, by its
 // largest value (values below 2^-36 of it are lost, to the same absolute error as the rest).  Every row
-// of x has its own for the logits, 2^f_i, by the row's largest value, and dz_i is stored without the
-// power of two in g_i = m_i 2^e_i, so that neither a row's size nor its g_i matters to another row's
-// loss or dx.  dW sums over the rows: its planes of x hold x_i 2^(e_i + F), one F for all, by the
-// largest |x_i| 2^e_i.  All sums are fp32.
+// of x has its own for the logits, 2^f_i, by the row's largest value, so that a row's size does not
+// matter to another row's loss.  dz_i is stored as (softmax - onehot) / c_i, c_i in [1, 2) the mantissa of
+// 1 - softmax_i,t(i): the target's value is then a power of two, rounded by nothing.  With g_i = m_i 2^e_i
+// in it (a mean's 1 / n is alike for all rows) or without c_i (the softmax of an untrained head is too), one
+// plane would round all targets the same way, up to 3e-4 of the whole gradient.  dx takes c_i g_i in fp32
+// behind its product, so that g_i does not matter to another row's dx either; dW sums over the rows, its
+// planes of x hold x_i c_i m_i 2^(e_i + F), one F for all, by the largest |x_i| 2^e_i.  All sums are fp32.
 //
 // Layout.  Every plane is stored as blocks of 32 rows x 16 columns, 1 KB each, the blocks of 32 rows
 // one after another along the columns; rows and columns are padded with zeros.  A block is what one
@@ -84,6 +87,23 @@ __device__ __forceinline__ float finite_abs(float v) {
     const float a = fabsf(v);
     return a < INFINITY ? a : 0.0f;  // NaN and inf stay in their own rows
 }
+
+// A product rounded to fp32 before it is split: left to itself the compiler rounds the product of the one use
+// straight to fp16 and of the other by way of fp32, and the two halves no longer belong together.
+__device__ __forceinline__ float rounded(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
+// The mantissa of v, in [1, 2); 1 for zero.
+__device__ __forceinline__ float mantissa(float v) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & 0x007fffffu) | 0x3f800000u);
+}
+// c_i of a row: of its softmax at the target, less one
+__device__ __forceinline__ float row_unit(float z_target, float lse) { return mantissa(__builtin_amdgcn_exp2f(z_target - lse) - 1.0f); }
+// c_i m_i
+__device__ __forceinline__ float row_factor(float g, float c) { return ldexpf(g, -exp_of(g)) * c; }
+constexpr int DZ_EXP = 14;  // (softmax - onehot) / c is stored times 2^14, at most 2^14
 
 // Exponent that takes a magnitude to [2^14, 2^15); 0 for zero and what is not finite.
 __device__ __forceinline__ int scale_exp(float mx) {
@@ -158,7 +178,8 @@ struct LossGemm {
     unsigned *w_max;
     float *out_loss, *out_lse;          // LOGITS_ALL: [rows] or null
     float *z;                           // kept logits, a workgroup's registers as they are, or null
-    const float *lse, *g;               // per row: lse (in units of log 2), g_i = m_i 2^e_i (dz's factor: m_i 2^13)
+    const float *lse, *g, *c, *h;       // per row: lse (in units of log 2), g_i = m_i 2^e_i, c_i, c_i m_i
+    float *out_c, *out_h;               // LOGITS_ALL: the last two
     _Float16 *dz;                       // planes of the piece, blocks of rows x entries
     long dz_plane;
     int dz_ncb;
@@ -439,14 +460,30 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                             if (in(rr, j)) o[rr * p.part_ld + 32 * j] = acc[i][j][e];
                         }
                 } else {
+                    int er[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) er[e] = ec;
+                    if (p.g) {  // the rows' factors, loaded before the first store
+                        float g[16], h[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            g[e] = p.g[r0 + i * 32 + 8 * (e / 4) + e % 4];
+                            h[e] = p.h[r0 + i * 32 + 8 * (e / 4) + e % 4];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            er[e] = exp_of(g[e]) - DZ_EXP - ec;
+#pragma unroll
+                            for (int j = 0; j < WTN; ++j) acc[i][j][e] *= h[e];
+                        }
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int rr = 8 * (e / 4) + e % 4;
                         T *o = (T *)p.dst + (r0 + i * 32 + rr) * p.dst_stride + c0;
-                        const int er = p.g ? exp_of(p.g[r0 + i * 32 + rr]) - 13 - ec : ec;
 #pragma unroll
                         for (int j = 0; j < WTN; ++j)
-                            if (in(rr, j)) o[32 * j] = from_f32<T>(ldexpf(acc[i][j][e], er));
+                            if (in(rr, j)) o[32 * j] = from_f32<T>(ldexpf(acc[i][j][e], er[e]));
                     }
                 }
             }
@@ -489,7 +526,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                         for (int j = 0; j < WTN; ++j)
                             *kept(i, j, e4) = floatx4{acc[i][j][4 * e4], acc[i][j][4 * e4 + 1], acc[i][j][4 * e4 + 2], acc[i][j][4 * e4 + 3]};
             }
-        float *red_m = bias_l + TM, *red_s = red_m + 4 * TN;               // [wave][TN]
+        float *red_m = bias_l + TM, *red_s = red_m + 4 * TN, *zt = red_s + 4 * TN;  // [wave][TN] twice, [TN]
         if constexpr (MODE != LOGITS_DZ && !KEPT) {
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
@@ -514,12 +551,12 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 }
                 // the target's logit, by the one lane that holds it
                 const int t = p.tgt[m] - w0;
-                if (MODE != LOGITS_ALL && __any(t >= 0 && t < WTM * 32))
+                if (__any(t >= 0 && t < WTM * 32))
 #pragma unroll
                     for (int i = 0; i < WTM; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) p.ztgt[m] = acc[i][j][e];
+                            if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) *(MODE == LOGITS_ALL ? zt + j * 32 + r : p.ztgt + m) = acc[i][j][e];
             }
             lds_barrier();
             for (int c = tid; MODE != LOGITS_ALL && c < TN; c += NT) {
@@ -537,14 +574,14 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             }
         }
         if constexpr (MODE == LOGITS_DZ || MODE == LOGITS_ALL || KEPT) {
-            float *colsum = red_s + 4 * TN + wave * (32 * WTM * 33);       // db: [WTM * 32 entries][32 + 1]
+            float *colsum = zt + TN + wave * (32 * WTM * 33);              // db: [WTM * 32 entries][32 + 1]
             float bsum[WTM][16];
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
                 const long m = (long)nt * TN + j * 32 + r;
-                const float gm = p.g[m], qm = ldexpf(gm, 13 - exp_of(gm));
+                const float gm = p.g[m];
                 const int tm = p.tgt[m], t = tm - w0;
-                float lse;
+                float lse, cm;
                 if constexpr (MODE == LOGITS_ALL) {
                     float mx = red_m[j * 32 + r];
 #pragma unroll
@@ -555,21 +592,20 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                     for (int w = 0; w < 4; ++w)
                         sum += red_s[w * TN + j * 32 + r] * __builtin_amdgcn_exp2f(red_m[w * TN + j * 32 + r] - ref);
                     lse = ref + log2f(sum);
-                    if (wave == 0 && hh == 0 && m < p.rows) {
-                        if (p.out_lse) p.out_lse[m] = tm >= 0 ? lse * LN2 : 0.0f;
-                        if (p.out_loss && tm < 0) p.out_loss[m] = 0.0f;
+                    const float z = tm >= 0 ? zt[j * 32 + r] : lse;
+                    cm = row_unit(z, lse);
+                    if (wave == 0 && hh == 0) {
+                        if (p.out_lse && m < p.rows) p.out_lse[m] = tm >= 0 ? lse * LN2 : 0.0f;
+                        if (p.out_loss && m < p.rows) p.out_loss[m] = tm >= 0 ? (lse - z) * LN2 : 0.0f;
+                        if (p.dz) p.out_c[m] = cm, p.out_h[m] = row_factor(gm, cm);
                     }
-                    if (p.out_loss && __any(t >= 0 && t < WTM * 32))
-#pragma unroll
-                        for (int i = 0; i < WTM; ++i)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) p.out_loss[m] = (lse - acc[i][j][e]) * LN2;
                     if (!p.dz) continue;
                 } else {
                     lse = p.lse[m];
+                    cm = p.c[m];
                 }
-                const bool off = qm == 0.0f;  // no target, or nothing from upstream: exactly zero
+                const float qm = (1 << DZ_EXP) / cm;
+                const bool off = gm == 0.0f;  // no target, or nothing from upstream: exactly zero
 #pragma unroll
                 for (int i = 0; i < WTM; ++i)
 #pragma unroll
@@ -594,7 +630,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 #pragma unroll
                             for (int v = 0; v < 2; ++v) {
                                 const int e = 8 * h + 2 * u + v;
-                                float x = off ? 0.0f : acc[i][j][e] * qm;
+                                const float x = off ? 0.0f : rounded(acc[i][j][e] * qm);
                                 if (p.db_part) bsum[i][e] = (j ? bsum[i][e] : 0.0f) + (off ? 0.0f : acc[i][j][e] * gm);
                                 const _Float16 hi = (_Float16)x;
                                 w[0] |= (unsigned)__builtin_bit_cast(unsigned short, hi) << (16 * v);
@@ -667,12 +703,13 @@ __device__ __forceinline__ void load8(const T *row, int c, int d, float (&v)[8])
     for (int j = 0; j < 8; ++j) v[j] = c + j < d ? to_f32<T>(row[c + j]) : 0.0f;
 }
 
+// v 2^ex f
 template <int NP>
-__device__ __forceinline__ void store_planes(_Float16 *dst, long plane, const float (&v)[8], int ex) {
+__device__ __forceinline__ void store_planes(_Float16 *dst, long plane, const float (&v)[8], int ex, float f = 1.0f) {
     half8 hi, lo;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float x = ldexpf(v[j], ex);
+        const float x = rounded(ldexpf(v[j], ex) * f);
         hi[j] = (_Float16)x;
         if constexpr (NP == 2) lo[j] = (_Float16)(x - (float)hi[j]);
     }
@@ -698,14 +735,16 @@ struct Prep {
     float *w_part;               // [w_blocks] largest |w| of each block's share
     int32_t *f, *tgt;            // [rows padded]
     float *g, *gmax;             // [rows padded], [row blocks]: largest |x_i| 2^e_i
+    float *c, *h;                // [rows padded]: c_i, c_i m_i
     int32_t *kw, *e_dw;          // exponent of W's scale; of dW's results
 };
 
-// The planes of XR rows of x, row r times 2^ex[r] (zeros where live[r] < 0): chunk (column block, row,
+// The planes of XR rows of x, row r times 2^ex[r] f[r] (zeros where live[r] < 0): chunk (column block, row,
 // half) by chunk, neighbouring threads side by side.  XR = 8: four blocks share a block row of 32, so
 // that 4096 rows fill the chip.
 template <typename T, int NP, bool VECX>
-__device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb, const int *live, const int *ex) {
+__device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb, const int *live, const int *ex,
+                                           const float *f) {
     const long row0 = rb * XR;
     dst += row0 / 32 * p.dcb * 512 + row0 % 32 * 16;
 #pragma unroll 4
@@ -713,8 +752,27 @@ __device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb
         const int cb = ch / (2 * XR), rl = (ch >> 1) % XR, c = cb * 16 + (ch & 1) * 8;
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (live[rl] >= 0) load8<T, VECX>((const T *)p.x + (row0 + rl) * p.x_stride, c, p.d, x);
-        store_planes<NP>(dst + (long)cb * 512 + rl * 16 + (ch & 1) * 8, p.x_plane, x, ex[rl]);
+        store_planes<NP>(dst + (long)cb * 512 + rl * 16 + (ch & 1) * 8, p.x_plane, x, ex[rl], f ? f[rl] : 1.0f);
     }
+}
+
+// The planes of x for dW, rows [rb XR, + XR), whose c_i m_i are f: from k_loss_prep's maxima.
+template <typename T, int NP, bool VECX>
+__device__ __forceinline__ void split_x2(const Prep &p, long rb, const float *f) {
+    __shared__ float red[4];
+    __shared__ int ex[XR], live[XR];
+    const int tid = threadIdx.x;
+    float m = 0.0f;
+    for (int i = tid; i < p.row_blocks; i += NT) m = fmaxf(m, p.gmax[i]);
+    const int e = scale_exp(block_max256(m, red)) - 2;  // c_i m_i < 4
+    if (rb == 0 && tid == 0) *p.e_dw = -DZ_EXP - e;
+    if (tid < XR) {
+        const float g = p.g[rb * XR + tid];
+        ex[tid] = exp_of(g) + e;
+        live[tid] = g == 0.0f ? -1 : 0;  // a row that gives nothing is not in the scale's range
+    }
+    __syncthreads();
+    split_rows<T, NP, VECX>(p, p.x2p, rb, live, ex, f);
 }
 
 // The first row_blocks blocks: XR rows of x each, split into planes with a scale of their own; rows
@@ -786,40 +844,23 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
         for (int r = 1; r < XR; ++r) m = fmaxf(m, rmax[r]);
         p.gmax[rb] = m;
     }
-    split_rows<T, NP, VECX>(p, p.xp, rb, tg, fx);
+    split_rows<T, NP, VECX>(p, p.xp, rb, tg, fx, nullptr);
 }
 
-// The blocks that follow k_loss_prep's maxima: the planes of x for dW (the first blocks, where they are
-// wanted), and W's planes, each block those of every so many-th block of 32 rows, of a share of the columns
-// where W has few rows.
-template <typename T, int NP, bool VECX, bool VECW>
+// W's planes, from k_loss_prep's maxima: each block those of every so many-th block of 32 rows, of a share
+// of the columns where W has few rows.
+template <typename T, int NP, bool VECW>
 __global__ __launch_bounds__(NT) void k_loss_split(Prep p, int redo) {
     __shared__ float red[4];
-    __shared__ int ex[XR], live[XR];
-    const int tid = threadIdx.x, xb = p.x2p && !redo ? p.row_blocks : 0;
-    if ((int)blockIdx.x < xb) {
-        float m = 0.0f;
-        for (int i = tid; i < p.row_blocks; i += NT) m = fmaxf(m, p.gmax[i]);
-        const int e = scale_exp(block_max256(m, red));
-        const long rb = blockIdx.x;
-        if (rb == 0 && tid == 0) *p.e_dw = -13 - e;
-        if (tid < XR) {
-            const float g = p.g[rb * XR + tid];
-            ex[tid] = exp_of(g) + e;
-            live[tid] = g == 0.0f ? -1 : 0;  // a row that gives nothing is not in the scale's range
-        }
-        __syncthreads();
-        split_rows<T, NP, VECX>(p, p.x2p, rb, live, ex);
-        return;
-    }
+    const int tid = threadIdx.x;
     int e;
     bool blank = false;
     if (!scale_of_w(p.w_part, p.w_blocks, p.w_head, p.w_max, redo, red, e, blank)) return;
-    if ((int)blockIdx.x == xb && tid == 0) *p.kw = e;
+    if (blockIdx.x == 0 && tid == 0) *p.kw = e;
     float top = 0.0f;
-    const int b = (int)blockIdx.x - xb, part = b % p.w_cols, per = (p.dcb + p.w_cols - 1) / p.w_cols;
+    const int b = blockIdx.x, part = b % p.w_cols, per = (p.dcb + p.w_cols - 1) / p.w_cols;
     const int ch1 = min((part + 1) * per, p.dcb) * 64;
-    for (long rb = b / p.w_cols; rb < p.w_rows; rb += ((int)gridDim.x - xb) / p.w_cols)
+    for (long rb = b / p.w_cols; rb < p.w_rows; rb += (int)gridDim.x / p.w_cols)
         for (int ch = part * per * 64 + tid; ch < ch1; ch += NT) {
             const int cb = ch >> 6, rl = (ch >> 1) & 31, c = cb * 16 + (ch & 1) * 8;
             const long v = rb * 32 + rl;
@@ -845,17 +886,20 @@ struct Rows {
     float *out_loss, *out_lse;
 };
 
-// 16 rows a block; 16 threads share a row's tiles, eight loads in flight each.
-__global__ __launch_bounds__(NT) void k_loss_rows(Rows p) {
-    __shared__ float sm[16][17], ss[16][17];
-    const int rl = threadIdx.x & 15, part = threadIdx.x >> 4;
-    const long i = (long)blockIdx.x * 16 + rl;
+// XR rows a block; 32 threads share a row's tiles, eight loads in flight each.  Where dW is wanted, then
+// the rows' planes of x for it.
+template <typename T, int NP, bool VECX>
+__global__ __launch_bounds__(NT) void k_loss_rows(Rows p, Prep pr) {
+    constexpr int PARTS = NT / XR;
+    __shared__ float sm[PARTS][XR + 1], ss[PARTS][XR + 1], f[XR];
+    const int rl = threadIdx.x % XR, part = threadIdx.x / XR;
+    const long i = (long)blockIdx.x * XR + rl;
     float mx = -INFINITY, s = 0.0f;
-    for (int t0 = part; t0 < p.tiles; t0 += 16 * 8) {
+    for (int t0 = part; t0 < p.tiles; t0 += PARTS * 8) {
         float m[8], v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const int t = t0 + 16 * u;
+            const int t = t0 + PARTS * u;
             const long o = (long)min(t, p.tiles - 1) * p.rows_pad + i;
             m[u] = p.part_m[o];
             v[u] = p.part_s[o];
@@ -873,24 +917,41 @@ __global__ __launch_bounds__(NT) void k_loss_rows(Rows p) {
     sm[part][rl] = mx;
     ss[part][rl] = s;
     __syncthreads();
-    if (part) return;
+    if (part == 0) {
 #pragma unroll
-    for (int q = 1; q < 16; ++q) mx = fmaxf(mx, sm[q][rl]);
-    const float ref = mx == -INFINITY ? 0.0f : mx;
-    s = 0.0f;
+        for (int q = 1; q < PARTS; ++q) mx = fmaxf(mx, sm[q][rl]);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        s = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 16; ++q) s += ss[q][rl] * __builtin_amdgcn_exp2f(sm[q][rl] - ref);
-    const float lse = ref + log2f(s);
-    p.lse[i] = lse;
-    if (i >= p.rows) return;
-    const bool there = p.tgt[i] >= 0;
-    if (p.out_lse) p.out_lse[i] = there ? lse * LN2 : 0.0f;
-    if (p.out_loss) p.out_loss[i] = there ? (lse - p.ztgt[i]) * LN2 : 0.0f;
+        for (int q = 0; q < PARTS; ++q) s += ss[q][rl] * __builtin_amdgcn_exp2f(sm[q][rl] - ref);
+        const float lse = ref + log2f(s);
+        const bool there = p.tgt[i] >= 0;
+        const float z = there ? p.ztgt[i] : lse, c = row_unit(z, lse);
+        p.lse[i] = lse;
+        pr.c[i] = c;
+        pr.h[i] = f[rl] = row_factor(pr.g[i], c);
+        if (i < p.rows) {
+            if (p.out_lse) p.out_lse[i] = there ? lse * LN2 : 0.0f;
+            if (p.out_loss) p.out_loss[i] = there ? (lse - z) * LN2 : 0.0f;
+        }
+    }
+    if (!pr.x2p) return;
+    __syncthreads();
+    split_x2<T, NP, VECX>(pr, blockIdx.x, f);
+}
+
+// Those planes by themselves, where one tile of the logits' product was the whole vocabulary.
+template <typename T, int NP, bool VECX>
+__global__ __launch_bounds__(NT) void k_loss_x2(Prep p) {
+    __shared__ float f[XR];
+    if (threadIdx.x < XR) f[threadIdx.x] = p.h[(long)blockIdx.x * XR + threadIdx.x];
+    __syncthreads();
+    split_x2<T, NP, VECX>(p, blockIdx.x, f);
 }
 
 // ---- shares of the gradients ---------------------------------------------------------------
 // dst[row][col] = sum over the shares, in order, times 2^exponent: of dW all alike (e_all), of dx a
-// row's own, e_i - 13 - kw (g).  Blocks from n_blocks on: db, the tiles' sums in order.
+// row's own, e_i - 14 - kw (g), and c_i m_i (h).  Blocks from n_blocks on: db, the tiles' sums in order.
 struct Join {
     const float *part;
     int S, rows, d;
@@ -898,7 +959,7 @@ struct Join {
     long stride;
     bool vec;            // rows of whole fours, aligned as such
     const int32_t *e_all, *kw;
-    const float *g;
+    const float *g, *h;
     int n_blocks;
     const float *db_part;
     int db_tiles, vocab;
@@ -930,10 +991,11 @@ __global__ __launch_bounds__(NT) void k_loss_join(Join p) {
 #pragma unroll 8
             for (int q = 0; q < p.S; ++q) s += *reinterpret_cast<const floatx4 *>(p.part + q * n + i * 4);
             const long row = n / 4 <= 0xffffffffl ? (unsigned)i / (unsigned)(p.d / 4) : i / (p.d / 4);
-            const int e = p.g ? exp_of(p.g[row]) - 13 - *p.kw : *p.e_all;
+            const int e = p.g ? exp_of(p.g[row]) - DZ_EXP - *p.kw : *p.e_all;
+            const float h = p.g ? p.h[row] : 1.0f;
             V4 o;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) o[u] = from_f32<T>(ldexpf(s[u], e));
+            for (int u = 0; u < 4; ++u) o[u] = from_f32<T>(ldexpf(s[u] * h, e));
             *reinterpret_cast<V4 *>((T *)p.dst + row * p.stride + (i * 4 - row * p.d)) = o;
         }
         return;
@@ -943,8 +1005,8 @@ __global__ __launch_bounds__(NT) void k_loss_join(Join p) {
 #pragma unroll 8
         for (int q = 0; q < p.S; ++q) s += p.part[q * n + i];
         const long row = i / p.d;
-        const int e = p.g ? exp_of(p.g[row]) - 13 - *p.kw : *p.e_all;
-        ((T *)p.dst)[row * p.stride + (i - row * p.d)] = from_f32<T>(ldexpf(s, e));
+        const int e = p.g ? exp_of(p.g[row]) - DZ_EXP - *p.kw : *p.e_all;
+        ((T *)p.dst)[row * p.stride + (i - row * p.d)] = from_f32<T>(ldexpf(s * (p.g ? p.h[row] : 1.0f), e));
     }
 }
 
@@ -970,7 +1032,7 @@ struct LossPlan {
     int w_blocks, w_sample, w_step, w_head;
     int bn;                  // columns of a gradient tile
     int dx_split, dx_ks, dw_split, dw_ks;
-    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, w_max, part_m, part_s, ztgt, lse, e_dw, z, dz, dx_part, dw_part, db_part, bytes;
+    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, w_max, part_m, part_s, ztgt, lse, c, h, e_dw, z, dz, dx_part, dw_part, db_part, bytes;
 };
 
 // K of `len` (a multiple of 32) in at most `want` shares of whole 32s, each not empty
@@ -1094,6 +1156,8 @@ LossPlan loss_plan(const LossParams &p) {
     L.part_s = take((size_t)L.v_tiles * L.rows_pad * 4);
     L.ztgt = take(L.rows_pad * 4);
     L.lse = take(L.rows_pad * 4);
+    L.c = take(L.rows_pad * 4);
+    L.h = take(L.rows_pad * 4);
     L.e_dw = take(4);
     {   // Logits of no more bytes than a piece of dz are kept where their product takes longer than writing and
         // reading them: 512 rows against 50257 entries 1389 -> 1122 us (fp32, d = 2048), 391 -> 353 (512), 152 ->
@@ -1171,16 +1235,16 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     r.w_sample = L.w_sample, r.w_step = L.w_step, r.w_head = L.w_head, r.w_max = (unsigned *)(ws + L.w_max);
     r.f = (int32_t *)(ws + L.f), r.tgt = (int32_t *)(ws + L.tgt);
     r.g = (float *)(ws + L.g), r.gmax = (float *)(ws + L.gmax);
+    r.c = (float *)(ws + L.c), r.h = (float *)(ws + L.h);
     r.kw = (int32_t *)(ws + L.kw), r.e_dw = (int32_t *)(ws + L.e_dw);
     const bool grads = p.dx || p.dw || p.db;
     const unsigned prep_grid = (unsigned)(r.row_blocks + r.w_blocks);
-    const unsigned split_grid = (unsigned)((r.x2p ? r.row_blocks : 0) + r.w_rows * r.w_cols);
     auto prep = [&](auto vecx, auto vecw) {
         constexpr bool VX = decltype(vecx)::value, VW = decltype(vecw)::value;
         k_loss_prep<T, NP, VX, VW><<<prep_grid, NT, 0, st>>>(r);
         if (L.raw) return;
-        k_loss_split<T, NP, VX, VW><<<split_grid, NT, 0, st>>>(r, 0);
-        if (L.w_head) k_loss_split<T, NP, VX, VW><<<std::min(r.w_rows, 1024) * r.w_cols, NT, 0, st>>>(r, 1);
+        k_loss_split<T, NP, VW><<<(unsigned)(r.w_rows * r.w_cols), NT, 0, st>>>(r, 0);
+        if (L.w_head) k_loss_split<T, NP, VW><<<std::min(r.w_rows, 1024) * r.w_cols, NT, 0, st>>>(r, 1);
     };
     using std::bool_constant;
     if (vx && vw)
@@ -1200,7 +1264,8 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     z.bias = p.bias, z.f = r.f, z.tgt = r.tgt, z.kw_dev = r.kw;
     z.vocab = p.vocab, z.rows = p.rows, z.rows_pad = L.rows_pad;
     z.part_m = (float *)(ws + L.part_m), z.part_s = (float *)(ws + L.part_s), z.ztgt = (float *)(ws + L.ztgt);
-    z.g = r.g;
+    z.g = r.g, z.c = z.out_c = r.c, z.h = z.out_h = r.h;
+    const unsigned row_grid = (unsigned)(round_up(p.rows, L.tn) / XR);
     if (grads) {
         z.dz = (_Float16 *)(ws + L.dz), z.dz_plane = L.rows_pad * L.piece, z.dz_ncb = L.piece / 16;
         z.db_part = p.db ? (float *)(ws + L.db_part) : nullptr, z.db_ld = L.v_pad;
@@ -1209,6 +1274,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     if (all) {
         z.out_loss = p.loss, z.out_lse = p.lse;
         launch_logits<LOGITS_ALL, T, NP>(z, L.tn, st);
+        if (r.x2p) vx ? k_loss_x2<T, NP, true><<<row_grid, NT, 0, st>>>(r) : k_loss_x2<T, NP, false><<<row_grid, NT, 0, st>>>(r);
     } else {
         if (L.raw) {
             z.K = z.Ks = p.d;
@@ -1227,7 +1293,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         q.rows = p.rows, q.tiles = L.v_tiles, q.rows_pad = L.rows_pad;
         q.part_m = z.part_m, q.part_s = z.part_s, q.ztgt = z.ztgt, q.tgt = r.tgt;
         q.lse = (float *)(ws + L.lse), q.out_loss = p.loss, q.out_lse = p.lse;
-        k_loss_rows<<<(unsigned)(round_up(p.rows, L.tn) / 16), NT, 0, st>>>(q);
+        vx ? k_loss_rows<T, NP, true><<<row_grid, NT, 0, st>>>(q, r) : k_loss_rows<T, NP, false><<<row_grid, NT, 0, st>>>(q, r);
         z.lse = q.lse;
     }
     if (!grads) return;
@@ -1252,7 +1318,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
             x.nM = (int)(round_up(p.rows, BM) / BM), x.nN = nbn, x.S = (n + L.dx_ks - 1) / L.dx_ks;
             x.K = n, x.Ks = L.dx_ks;
             if (L.dx_whole)
-                x.dst = p.dx, x.dst_stride = p.dx_stride, x.g = r.g, x.kw_dev = r.kw;
+                x.dst = p.dx, x.dst_stride = p.dx_stride, x.g = r.g, x.h = r.h, x.kw_dev = r.kw;
             else
                 x.part = (float *)(ws + L.dx_part), x.part_ld = p.d, x.add = v0 > 0;
             x.out_rows = p.rows, x.out_cols = p.d;
@@ -1282,7 +1348,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     Join j{};
     j.part = (float *)(ws + L.dx_part), j.S = L.dx_split, j.rows = p.rows, j.d = p.d, j.dst = p.dx, j.stride = p.dx_stride;
     j.vec = join_vec(j, eb);
-    j.g = r.g, j.kw = r.kw, j.n_blocks = join_dx ? join_blocks((long)p.rows * p.d / (j.vec ? 4 : 1)) : 0;
+    j.g = r.g, j.h = r.h, j.kw = r.kw, j.n_blocks = join_dx ? join_blocks((long)p.rows * p.d / (j.vec ? 4 : 1)) : 0;
     j.db_part = z.db_part, j.db_tiles = z.nN, j.db_ld = z.db_ld, j.vocab = p.vocab, j.db = p.db;
     k_loss_join<T><<<j.n_blocks + (p.db ? (p.vocab + 63) / 64 : 0), NT, 0, st>>>(j);
 }
