@@ -25,6 +25,15 @@
 // behind its product, so that g_i does not matter to another row's dx either; dW sums over the rows, its
 // planes of x hold x_i c_i m_i 2^(e_i + F), one F for all, by the largest |x_i| 2^e_i.  All sums are fp32.
 //
+// fp16's smallest step leaves a small probability few bits (2^-39 under the scale of 2^14: 1e-10 to 2 %), which
+// is nothing in dx_i, a sum over all entries, and everything in dW's row of a rare entry.  So the logits' epilogue
+// takes each entry's maximum over its rows (32 to 128), and where one of 256 entries is that small stores the
+// tile's dz for dW apart, each entry times a power of two of its own (MAX_D).  dW's product takes such blocks to
+// the entry's largest over its rows on the way to the MFMA, and its sums back at the end; the other blocks are
+// dx's, so that a head without rare entries pays for the maxima alone (8192 x 512 fp32 0.5 %, 4096 x 2048 bf16
+// 2 %, 531 x 1024 bf16 3 %; 8, 6 and 9 % where every block is stored twice).  dx has planes that no other row
+// matters to.
+//
 // Layout.  Every plane is stored as blocks of 32 rows x 16 columns, 1 KB each, the blocks of 32 rows
 // one after another along the columns; rows and columns are padded with zeros.  A block is what one
 // direct global->LDS load of a wave moves.  The one image serves a product over the columns (a lane
@@ -77,6 +86,14 @@ __device__ __forceinline__ void load_lds(const void *base, unsigned off, unsigne
                  : "memory", "m0");
 }
 
+// The same with 4 bytes a lane, to `lds` + 4 lane.
+__device__ __forceinline__ void load_lds4(const void *base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+
 // e of |g| = m 2^e, m in [1, 2); 0 for zero and what is not finite
 __device__ __forceinline__ int exp_of(float g) {
     const float a = fabsf(g);
@@ -100,10 +117,16 @@ __device__ __forceinline__ float mantissa(float v) {
     return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & 0x007fffffu) | 0x3f800000u);
 }
 // c_i of a row: of its softmax at the target, less one
-__device__ __forceinline__ float row_unit(float z_target, float lse) { return mantissa(__builtin_amdgcn_exp2f(z_target - lse) - 1.0f); }
+__device__ __forceinline__ float row_unit(float z_target, float lse) {
+    return mantissa(__builtin_amdgcn_exp2f(z_target - lse) - 1.0f);
+}
 // c_i m_i
 __device__ __forceinline__ float row_factor(float g, float c) { return ldexpf(g, -exp_of(g)) * c; }
 constexpr int DZ_EXP = 14;  // (softmax - onehot) / c is stored times 2^14, at most 2^14
+// For dW an entry's values of a tile of rows are stored times 2^D more, D > 0 where the largest of them is so
+// small that the planes' smallest step, 2^-39, would cost it bits: below 2^-16 16, below 2^-24 24.
+// Down to 2^-24 the factor is an fp16 value.
+constexpr int MAX_D = 24;
 
 // Exponent that takes a magnitude to [2^14, 2^15); 0 for zero and what is not finite.
 __device__ __forceinline__ int scale_exp(float mx) {
@@ -180,8 +203,13 @@ struct LossGemm {
     float *z;                           // kept logits, a workgroup's registers as they are, or null
     const float *lse, *g, *c, *h;       // per row: lse (in units of log 2), g_i = m_i 2^e_i, c_i, c_i m_i
     float *out_c, *out_h;               // LOGITS_ALL: the last two
-    _Float16 *dz;                       // planes of the piece, blocks of rows x entries
+    _Float16 *dz, *dzw;                 // planes of the piece, blocks of rows x entries: for dx, for dW (or null)
     long dz_plane;
+    _Float16 *fx;                       // of dzw, [group of rows][entries of the piece]: 2^-D
+    int *scaled;                        // [group of rows][TV entries]: dzw is not dz; where it is, dzw is not written
+    long fx_ld;
+    int fx_log;                         // GRAD: rows of a group = 2^fx_log
+    const _Float16 *plain;              // GRAD dW: A's planes of blocks that are not scaled
     int dz_ncb;
     float *db_part;                     // [row tile][entries padded]
     long db_ld;
@@ -212,25 +240,27 @@ struct LossGrads {
 // 16 KB values (24 KB of LDS for either NP at the largest tile: three slices and two workgroups a
 // CU, so that one's epilogue runs under the other's MFMAs).  TRA / TRB: the operand's rows are the
 // product's K.
-template <int NP, int WTM, int WTN, int WGM, int WGN>
+template <int NP, int WTM, int WTN, int WGM, int WGN, int EXTRA = 0>  // EXTRA: halves beside a slice
 struct Tile {
     static constexpr int KB = NP == 2 ? 1 : 2;
     static constexpr int TM = WGM * WTM * 32, TN = WGN * WTN * 32;
     static constexpr int A_BLK = TM / 32 * KB, B_BLK = TN / 32 * KB;  // 1 KB loads a plane and slice
     static constexpr int SLICE = NP * (A_BLK + B_BLK) * 512;           // halves of a k slice
     // slices of the LDS ring: what half of a CU's LDS holds, three to six
-    static constexpr int FIT = 80 * 512 / SLICE, STAGES = FIT < 3 ? 3 : FIT > 6 ? 6 : FIT;
-    static constexpr int RING = STAGES * SLICE;
+    static constexpr int FIT = 80 * 512 / (SLICE + EXTRA), STAGES = FIT < 3 ? 3 : FIT > 6 ? 6 : FIT;
+    static constexpr int RING = STAGES * SLICE, LDS = STAGES * (SLICE + EXTRA);
     static_assert(WGM * WGN == 4, "four waves");
-    static_assert(RING * 2 <= 80 * 1024, "two workgroups a CU");
+    static_assert(LDS * 2 <= 80 * 1024, "two workgroups a CU");
 };
+constexpr int FX = 128;  // factors of a slice of dW's dz: one an entry of the tile
 
 template <int MODE, typename T, int NP, int WTM, int WTN, int WGM, int WGN, bool TRA, bool TRB>
 __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *ring) {
-    typedef Tile<NP, WTM, WTN, WGM, WGN> G;
+    typedef Tile<NP, WTM, WTN, WGM, WGN, MODE == GRAD ? FX : 0> G;
+    constexpr bool FACT = MODE == GRAD && TRA;  // dW: dz's groups of rows have scales of their own
     constexpr int KB = G::KB, TM = G::TM, TN = G::TN, A_BLK = G::A_BLK, B_BLK = G::B_BLK, STAGES = G::STAGES;
     constexpr int A_PW = (A_BLK + NW - 1) / NW, B_PW = (B_BLK + NW - 1) / NW;
-    constexpr int LOADS = NP * (A_PW + B_PW);
+    constexpr int LOADS = NP * (A_PW + B_PW) + FACT;
     constexpr int A_SZ = A_BLK * 512, B_SZ = B_BLK * 512;      // halves a plane and slice
     constexpr int SLICE = G::SLICE;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -294,11 +324,29 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
     for (int j = 0; j < A_PW; ++j) asrc[j] = src_of(TRA, (wave + NW * j) % A_BLK, p.a_row0 + mt * TM, p.A);
 #pragma unroll
     for (int j = 0; j < B_PW; ++j) bsrc[j] = src_of(TRB, (wave + NW * j) % B_BLK, nt * TN, p.B);
+    // FACT: which of 64 groups of rows are scaled, from the share's on; of the slices issued last
+    const int g1 = FACT ? (k0 + nk * 16 * KB - 1) >> p.fx_log : 0;
+    auto scaled_groups = [&](int g0) -> unsigned long long {
+        const int g = g0 + lane;
+        return __ballot(g <= g1 && p.scaled[(long)min(g, g1) * (p.fx_ld / TV) + mt / (TV / TM)]);
+    };
+    int mask_g0 = FACT ? k0 >> p.fx_log : 0;
+    unsigned long long mask = FACT ? scaled_groups(mask_g0) : 0;
+    unsigned bits = 0;
     const unsigned aoff = lane_off(TRA), boff = lane_off(TRB);
     const unsigned ring0 = (unsigned)(uintptr_t)(lds_void *)ring;
     auto issue = [&](int kt) {
         const unsigned base = ring0 + (kt % STAGES) * (SLICE * 2);
-        const _Float16 *Ap = p.A.p + step_of(TRA, kt, p.A), *Bp = p.B.p + step_of(TRB, kt, p.B);
+        const _Float16 *Ap = p.A.p;
+        if constexpr (FACT) {
+            const int g = (k0 + kt * 16 * KB) >> p.fx_log;
+            if (g - mask_g0 >= 64) mask = scaled_groups(mask_g0 += 64);
+            const unsigned bit = (unsigned)(mask >> (g - mask_g0)) & 1;
+            if (!bit) Ap = p.plain;
+            bits = bits << 1 | bit;
+        }
+        Ap += step_of(TRA, kt, p.A);
+        const _Float16 *Bp = p.B.p + step_of(TRB, kt, p.B);
         if constexpr (RAW) {
 #pragma unroll
             for (int j = 0; j < R_PW; ++j) load_lds(rbase + kt * 64, roff[j], base + (wave + NW * j) * 1024);
@@ -312,6 +360,11 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             for (int j = 0; j < B_PW; ++j)
                 load_lds(Bp + q * p.B.plane + bsrc[j], boff,
                          base + (NP * A_SZ + q * B_SZ + ((wave + NW * j) % B_BLK) * 512) * 2);
+        }
+        if constexpr (FACT) {
+            static_assert(TM == FX, "a factor an entry");
+            load_lds4(p.fx + (long)((k0 + kt * 16 * KB) >> p.fx_log) * p.fx_ld + mt * TM, lane * 4,
+                      ring0 + (G::RING + kt % STAGES * FX) * 2);
         }
     };
     // MFMA operand of 32 rows (columns) `t` of the tile, k block kb of the slice
@@ -359,6 +412,8 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
+    float fmost[WTM], fless[WTM];  // FACT: a lane's entries' largest factor, and its inverse
+    unsigned long long any = 0;    // FACT: a block of the share's is scaled
     // KEPT: this tile's logits, 16 bytes a lane side by side
     const auto kept = [&](int i, int j, int e4) -> floatx4 * {
         const long tile = (long)(p.a_row0 / TV + mt) * p.nN + nt;
@@ -379,6 +434,19 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 #pragma unroll
         for (int t = 0; t < STAGES - 1; ++t)
             if (t < nk) issue(t);
+        // the largest factor 2^-D of a lane's entries over the share's rows: scaled blocks are taken to its scale
+        for (int g = k0 >> p.fx_log; FACT && g <= g1; g += 64) any |= g == mask_g0 ? mask : scaled_groups(g);
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < WTM; ++i) fmost[i] = 0.0f;
+            const _Float16 *f = p.fx + mt * TM + wm * WTM * 32 + r;
+#pragma unroll 8
+            for (int g = k0 >> p.fx_log; g <= g1; ++g)
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) fmost[i] = fmaxf(fmost[i], (float)f[g * p.fx_ld + i * 32]);
+#pragma unroll
+            for (int i = 0; i < WTM; ++i) fless[i] = 1.0f / fmost[i];
+        }
         for (int kt = 0; kt < nk; ++kt) {
             // slice kt is in LDS once this wave's later loads are all that is in flight; the barrier
             // covers the other waves' loads, and their reads of the slot that is loaded next
@@ -389,6 +457,12 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             lds_barrier();
             if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1);
             const _Float16 *base = ring + (kt % STAGES) * SLICE;
+            const bool scaled = FACT && (bits >> (min(kt + STAGES - 1, nk - 1) - kt) & 1);
+            _Float16 fac[WTM];
+            if (scaled)
+#pragma unroll
+                for (int i = 0; i < WTM; ++i)
+                    fac[i] = (_Float16)((float)ring[G::RING + kt % STAGES * FX + (wm * WTM + i) * 32 + r] * fless[i]);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 half8 a[NP][WTM];
@@ -406,6 +480,11 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 for (int j = 0; j < WTN; ++j)
 #pragma unroll
                     for (int q = 0; q < NP; ++q) b[q][j] = frag(base + NP * A_SZ + q * B_SZ, TRB, wn * WTN + j, kb);
+                if (scaled)
+#pragma unroll
+                    for (int q = 0; q < NP; ++q)
+#pragma unroll
+                        for (int i = 0; i < WTM; ++i) a[q][i] *= fac[i];
                 // all of a k block's reads before its first MFMA: left to itself the compiler reads the last
                 // columns halfway and waits there (8192 x 512 fp32 4600 us for 4505, 4096 x 2048 bf16 3285 for 3218)
                 __builtin_amdgcn_sched_barrier(0);
@@ -433,6 +512,24 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
 
     // Output layout of a 32x32 tile: lane holds column r; register e row 8 (e / 4) + 4 hh + e % 4.
     if constexpr (MODE == GRAD) {
+        if (any) {  // the entries' scales, by way of LDS from a lane an entry to the sums' registers
+            float *own = reinterpret_cast<float *>(ring) + wave * (WTM * 32);
+            if (hh == 0)
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) own[i * 32 + r] = fmost[i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < WTM; ++i)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4) {
+                    const floatx4 t = *reinterpret_cast<const floatx4 *>(own + i * 32 + 8 * e4 + 4 * hh);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int j = 0; j < WTN; ++j) acc[i][j][4 * e4 + e] *= t[e];
+                }
+        }
         const int ec = p.e_all ? *p.e_all : p.g ? *p.kw_dev : 0;  // g: dx, a row's own exponent
         const long r0 = (long)mt * TM + wm * WTM * 32 + 4 * hh;
         const int c0 = nt * TN + wn * WTN * 32 + r;
@@ -556,7 +653,8 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                     for (int i = 0; i < WTM; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) *(MODE == LOGITS_ALL ? zt + j * 32 + r : p.ztgt + m) = acc[i][j][e];
+                            if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) 
+                                *(MODE == LOGITS_ALL ? zt + j * 32 + r : p.ztgt + m) = acc[i][j][e];
             }
             lds_barrier();
             for (int c = tid; MODE != LOGITS_ALL && c < TN; c += NT) {
@@ -574,8 +672,41 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
             }
         }
         if constexpr (MODE == LOGITS_DZ || MODE == LOGITS_ALL || KEPT) {
-            float *colsum = zt + TN + wave * (32 * WTM * 33);              // db: [WTM * 32 entries][32 + 1]
-            float bsum[WTM][16];
+            const bool grads = p.dz || p.dzw || p.db_part;
+            float *any_l = zt + TN, *scale = any_l + 4 + wave * (WTM * 32);     // dzw: [wave]; [WTM * 32 entries]
+            float *colsum = any_l + 4 + 4 * (WTM * 32) + wave * (32 * WTM * 33);  // db: [WTM * 32 entries][32 + 1]
+            float unit_l[WTN];  // LOGITS_ALL: c
+            // 32 rows x 32 entries of a lane's values as blocks: a register pair of 8 values becomes the two
+            // 16-byte chunks of a block's row (columns 0-7 in the lower half of the wave, 8-15 in the upper one)
+            auto put = [&](_Float16 *dst, int i, int j, auto value) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    unsigned pk[NP][4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        unsigned w[NP] = {};
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            const float x = value(8 * h + 2 * u + v);  // (a power of two times a value: rounded once)
+                            const _Float16 hi = (_Float16)x;
+                            w[0] |= (unsigned)__builtin_bit_cast(unsigned short, hi) << (16 * v);
+                            if constexpr (NP == 2)
+                                w[1] |= (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(x - (float)hi)) << (16 * v);
+                        }
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) pk[q][u] = w[q];
+                    }
+                    const long blk = (long)(nt * (TN / 32) + j) * p.dz_ncb + (long)mt * (TM / 16) + (wm * WTM + i) * 2 + h;
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) {
+                        const auto x0 = __builtin_amdgcn_permlane32_swap(pk[q][0], pk[q][2], false, false);
+                        const auto x1 = __builtin_amdgcn_permlane32_swap(pk[q][1], pk[q][3], false, false);
+                        const uint4v o = {x0[0], x1[0], x0[1], x1[1]};
+                        *reinterpret_cast<uint4v *>(dst + q * p.dz_plane + blk * 512 + r * 16 + hh * 8) = o;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // one pair after the other: 128 values are held besides
+                }
+            };
 #pragma unroll
             for (int j = 0; j < WTN; ++j) {
                 const long m = (long)nt * TN + j * 32 + r;
@@ -597,14 +728,15 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                     if (wave == 0 && hh == 0) {
                         if (p.out_lse && m < p.rows) p.out_lse[m] = tm >= 0 ? lse * LN2 : 0.0f;
                         if (p.out_loss && m < p.rows) p.out_loss[m] = tm >= 0 ? (lse - z) * LN2 : 0.0f;
-                        if (p.dz) p.out_c[m] = cm, p.out_h[m] = row_factor(gm, cm);
+                        if (grads) p.out_c[m] = cm, p.out_h[m] = row_factor(gm, cm);
                     }
-                    if (!p.dz) continue;
+                    unit_l[j] = cm;
+                    if (!grads) continue;
                 } else {
                     lse = p.lse[m];
                     cm = p.c[m];
                 }
-                const float qm = (1 << DZ_EXP) / cm;
+                const float unit = 1.0f / cm;
                 const bool off = gm == 0.0f;  // no target, or nothing from upstream: exactly zero
 #pragma unroll
                 for (int i = 0; i < WTM; ++i)
@@ -619,49 +751,92 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                             if (t == i * 32 + 8 * (e / 4) + 4 * hh + e % 4) acc[i][j][e] -= 1.0f;
 #pragma unroll
                 for (int i = 0; i < WTM; ++i) {
-                    // a register pair of 8 values becomes the two 16-byte chunks of a block's row
-                    // (columns 0-7 in the lower half of the wave, 8-15 in the upper one)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        unsigned pk[NP][4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            unsigned w[NP] = {};
-#pragma unroll
-                            for (int v = 0; v < 2; ++v) {
-                                const int e = 8 * h + 2 * u + v;
-                                const float x = off ? 0.0f : rounded(acc[i][j][e] * qm);
-                                if (p.db_part) bsum[i][e] = (j ? bsum[i][e] : 0.0f) + (off ? 0.0f : acc[i][j][e] * gm);
-                                const _Float16 hi = (_Float16)x;
-                                w[0] |= (unsigned)__builtin_bit_cast(unsigned short, hi) << (16 * v);
-                                if constexpr (NP == 2)
-                                    w[1] |= (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(x - (float)hi)) << (16 * v);
-                            }
-#pragma unroll
-                            for (int q = 0; q < NP; ++q) pk[q][u] = w[q];
-                        }
-                        const long blk = (long)(nt * (TN / 32) + j) * p.dz_ncb + (long)mt * (TM / 16) + (wm * WTM + i) * 2 + h;
-#pragma unroll
-                        for (int q = 0; q < NP; ++q) {
-                            const auto x0 = __builtin_amdgcn_permlane32_swap(pk[q][0], pk[q][2], false, false);
-                            const auto x1 = __builtin_amdgcn_permlane32_swap(pk[q][1], pk[q][3], false, false);
-                            const uint4v o = {x0[0], x1[0], x0[1], x1[1]};
-                            *reinterpret_cast<uint4v *>(p.dz + q * p.dz_plane + blk * 512 + r * 16 + hh * 8) = o;
-                        }
-                    }
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] = off ? 0.0f : rounded(acc[i][j][e] * unit);
+                    if (p.dz) put(p.dz, i, j, [&](int e) { return acc[i][j][e] * (float)(1 << DZ_EXP); });
                 }
             }
-            if (p.dz && p.db_part) {  // each entry's sum over the tile's rows, lanes in order
+            if (grads && p.db_part) {  // each entry's sum over the tile's rows, lanes in order
+                float gm[WTN], cm[WTN];
+#pragma unroll
+                for (int j = 0; j < WTN; ++j) {
+                    const long m = (long)nt * TN + j * 32 + r;
+                    gm[j] = p.g[m];
+                    if constexpr (MODE == LOGITS_ALL)
+                        cm[j] = unit_l[j];
+                    else
+                        cm[j] = p.c[m];
+                }
 #pragma unroll
                 for (int i = 0; i < WTM; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) colsum[(i * 32 + 8 * (e / 4) + 4 * hh + e % 4) * 33 + r] = bsum[i][e];
+                    for (int e = 0; e < 16; ++e) {
+                        float t = acc[i][0][e] * gm[0] * cm[0];
+#pragma unroll
+                        for (int j = 1; j < WTN; ++j) t += acc[i][j][e] * gm[j] * cm[j];
+                        colsum[(i * 32 + 8 * (e / 4) + 4 * hh + e % 4) * 33 + r] = t;
+                    }
                 lds_barrier();
                 if (lane < WTM * 32) {
                     float t = 0.0f;
 #pragma unroll
                     for (int c = 0; c < 32; ++c) t += colsum[lane * 33 + c];
                     p.db_part[(long)nt * p.db_ld + v0 + wm * WTM * 32 + lane] = t;
+                }
+            }
+            if (p.dzw) {
+                // an entry's largest value over the tile's rows: those of a lane, then over the 32 lanes of a half wave,
+                // which divide the 32 values a lane holds between them a bit at a time, so that lane r ends with value r
+                static_assert(WTM == 2, "32 values a lane");
+                float top[32];
+#pragma unroll
+                for (int q = 0; q < 32; ++q) {
+                    top[q] = fabsf(acc[q / 16][0][q % 16]);
+#pragma unroll
+                    for (int j = 1; j < WTN; ++j) top[q] = fmaxf(top[q], fabsf(acc[q / 16][j][q % 16]));
+                }
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    const auto x = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, top[q]),
+                                                                    __builtin_bit_cast(unsigned, top[q + 16]), false, false);
+                    top[q] = fmaxf(__builtin_bit_cast(float, (unsigned)x[0]), __builtin_bit_cast(float, (unsigned)x[1]));
+                }
+                auto halve = [&](auto n, auto ctrl) {  // lanes that differ in bit n, for n = 4 in all three lower bits
+                    constexpr int N = decltype(n)::value, C = decltype(ctrl)::value;
+#pragma unroll
+                    for (int q = 0; q < N; ++q) {
+                        const float mine = lane & N ? top[q + N] : top[q], other = lane & N ? top[q] : top[q + N];
+                        const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, other), C, 0xF, 0xF, true);
+                        top[q] = fmaxf(mine, __builtin_bit_cast(float, moved));
+                    }
+                };
+                using std::integral_constant;
+                halve(integral_constant<int, 8>{}, integral_constant<int, 0x128>{});  // row_ror 8
+                halve(integral_constant<int, 4>{}, integral_constant<int, 0x141>{});  // row_half_mirror
+                halve(integral_constant<int, 2>{}, integral_constant<int, 0x4E>{});   // quad_perm 2 3 0 1
+                halve(integral_constant<int, 1>{}, integral_constant<int, 0xB1>{});   // quad_perm 1 0 3 2
+                const float most = top[0];
+                const int D = most < 0x1p-24f ? MAX_D : most < 0x1p-16f ? 16 : 0;
+                const int at = (r >> 4) * 32 + 8 * ((r & 15) >> 2) + 4 * hh + (r & 3);
+                scale[at] = ldexpf(1.0f, DZ_EXP + D);
+                p.fx[(long)nt * p.fx_ld + mt * TM + wm * (WTM * 32) + at] = (_Float16)ldexpf(1.0f, -D);
+                const bool any_here = __any(D > 0 && most > 0.0f);
+                if (lane == 0) any_l[wave] = any_here ? 1.0f : 0.0f;
+                lds_barrier();
+                const bool any = any_l[0] + any_l[1] + any_l[2] + any_l[3] > 0.0f;
+                if (tid == 0) p.scaled[(long)nt * (p.fx_ld / TV) + mt] = any;
+                if (p.dz && !any) return;  // dz serves dW too
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) {
+                    float f[16];
+#pragma unroll
+                    for (int e4 = 0; e4 < 4; ++e4) {
+                        const floatx4 t = *reinterpret_cast<const floatx4 *>(scale + i * 32 + 8 * e4 + 4 * hh);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[4 * e4 + e] = t[e];
+                    }
+#pragma unroll
+                    for (int j = 0; j < WTN; ++j) put(p.dzw, i, j, [&](int e) { return acc[i][j][e] * f[e]; });
                 }
             }
         }
@@ -676,7 +851,7 @@ __global__ __launch_bounds__(NT, 2) void k_loss_logits(LossGemm p) {
 
 template <typename T, int NP, int WTM, int WTN, int WGM, int WGN>
 __global__ __launch_bounds__(NT, 2) void k_loss_grads(LossGrads p) {
-    __shared__ __attribute__((aligned(1024))) _Float16 ring[Tile<NP, WTM, WTN, WGM, WGN>::RING];
+    __shared__ __attribute__((aligned(1024))) _Float16 ring[Tile<NP, WTM, WTN, WGM, WGN, FX>::LDS];
     const int b = blockIdx.x;
     if ((b < p.first) == (p.dx_first != 0))
         loss_tile<GRAD, T, NP, WTM, WTN, WGM, WGN, false, true>(p.dx, p.dx_first ? b : b - p.first, ring);
@@ -1032,7 +1207,7 @@ struct LossPlan {
     int w_blocks, w_sample, w_step, w_head;
     int bn;                  // columns of a gradient tile
     int dx_split, dx_ks, dw_split, dw_ks;
-    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, w_max, part_m, part_s, ztgt, lse, c, h, e_dw, z, dz, dx_part, dw_part, db_part, bytes;
+    size_t xp, x2p, wp, w_part, f, tgt, g, gmax, kw, w_max, part_m, part_s, ztgt, lse, c, h, e_dw, z, dz, dzw, fx, scaled, dx_part, dw_part, db_part, bytes;
 };
 
 // K of `len` (a multiple of 32) in at most `want` shares of whole 32s, each not empty
@@ -1168,7 +1343,12 @@ LossPlan loss_plan(const LossParams &p) {
     }
     L.z = take(L.keep ? (size_t)round_up(p.rows, L.tn) * L.v_pad * 4 : 0);
     if (grads) {
-        L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
+        if (p.dx) L.dz = take((size_t)L.rows_pad * L.piece * 2 * L.np);
+        if (p.dw) {
+            L.dzw = take((size_t)L.rows_pad * L.piece * 2 * L.np);
+            L.fx = take((size_t)(L.rows_pad / L.tn) * L.piece * 2);
+            L.scaled = take((size_t)(L.rows_pad / L.tn) * (L.piece / TV) * 4);
+        }
         GradSizes g{L.np, p.d};
         if (p.dx) g.dx_rows = round_up(p.rows, BM) / BM, g.dx_k = L.piece, g.dx_elems = (long)p.rows * p.d;
         if (p.dw) {
@@ -1267,7 +1447,9 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     z.g = r.g, z.c = z.out_c = r.c, z.h = z.out_h = r.h;
     const unsigned row_grid = (unsigned)(round_up(p.rows, L.tn) / XR);
     if (grads) {
-        z.dz = (_Float16 *)(ws + L.dz), z.dz_plane = L.rows_pad * L.piece, z.dz_ncb = L.piece / 16;
+        z.dz = p.dx ? (_Float16 *)(ws + L.dz) : nullptr, z.dzw = p.dw ? (_Float16 *)(ws + L.dzw) : nullptr;
+        z.dz_plane = L.rows_pad * L.piece, z.dz_ncb = L.piece / 16;
+        z.fx = (_Float16 *)(ws + L.fx), z.fx_ld = L.piece, z.scaled = (int *)(ws + L.scaled);
         z.db_part = p.db ? (float *)(ws + L.db_part) : nullptr, z.db_ld = L.v_pad;
     }
     const bool all = L.v_tiles == 1;  // one tile holds the vocabulary: one pass
@@ -1301,7 +1483,6 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
     const int nbn = (p.d + L.bn - 1) / L.bn;
     for (long v0 = 0; v0 < L.v_pad; v0 += L.piece) {
         const int n = (int)std::min<long>(L.piece, L.v_pad - v0);  // entries of the piece, padded
-        const Planes DZ{z.dz, z.dz_plane, z.dz_ncb};
         z.a_row0 = (int)v0;
         z.nM = n / TV;
         if (L.keep)
@@ -1313,7 +1494,7 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         LossGrads g{};
         if (p.dx) {
             LossGemm &x = g.dx;
-            x.A = DZ, x.B = W;
+            x.A = Planes{z.dz, z.dz_plane, z.dz_ncb}, x.B = W;
             x.B.p += v0 / 32 * (long)W.ncb * 512;
             x.nM = (int)(round_up(p.rows, BM) / BM), x.nN = nbn, x.S = (n + L.dx_ks - 1) / L.dx_ks;
             x.K = n, x.Ks = L.dx_ks;
@@ -1325,7 +1506,9 @@ void run_loss(const LossParams &p, const LossPlan &L, char *ws, hipStream_t st) 
         }
         if (p.dw) {
             LossGemm &w = g.dw;
-            w.A = DZ, w.B = X2;
+            w.A = Planes{z.dzw, z.dz_plane, z.dz_ncb}, w.B = X2;
+            w.plain = p.dx ? z.dz : z.dzw;
+            w.scaled = z.scaled, w.fx = z.fx, w.fx_ld = z.fx_ld, w.fx_log = L.tn == 128 ? 7 : L.tn == 64 ? 6 : 5;
             w.nM = (live + BM - 1) / BM, w.nN = nbn, w.S = L.dw_split;
             w.K = (int)round_up(p.rows, 32), w.Ks = L.dw_ks;
             w.out_rows = live, w.out_cols = p.d;
