@@ -30,9 +30,9 @@
 // takes each entry's maximum over its rows (32 to 128), and where one of 256 entries is that small stores the
 // tile's dz for dW apart, each entry times a power of two of its own (MAX_D).  dW's product takes such blocks to
 // the entry's largest over its rows on the way to the MFMA, and its sums back at the end; the other blocks are
-// dx's, so that a head without rare entries pays for the maxima alone (8192 x 512 fp32 0.5 %, 4096 x 2048 bf16
-// 2 %, 531 x 1024 bf16 3 %; 8, 6 and 9 % where every block is stored twice).  dx has planes that no other row
-// matters to.
+// dx's, so that a head with few rare entries pays for the maxima and some shares of dW (8192 x 512 fp32 1 %,
+// 4096 x 2048 bf16 nothing, 531 x 1024 bf16 2 %, calls of 50 us 2 us; with rare entries everywhere 8, 4 and 9 %).
+// dx has planes that no other row matters to.
 //
 // Layout.  Every plane is stored as blocks of 32 rows x 16 columns, 1 KB each, the blocks of 32 rows
 // one after another along the columns; rows and columns are padded with zeros.  A block is what one
@@ -124,8 +124,8 @@ __device__ __forceinline__ float row_unit(float z_target, float lse) {
 __device__ __forceinline__ float row_factor(float g, float c) { return ldexpf(g, -exp_of(g)) * c; }
 constexpr int DZ_EXP = 14;  // (softmax - onehot) / c is stored times 2^14, at most 2^14
 // For dW an entry's values of a tile of rows are stored times 2^D more, D > 0 where the largest of them is so
-// small that the planes' smallest step, 2^-39, would cost it bits: below 2^-16 16, below 2^-24 24.
-// Down to 2^-24 the factor is an fp16 value.
+// small that the planes' smallest step, 2^-39, would cost it bits: with two planes (22 bits) 16 below 2^-16, and
+// with either number 24 below 2^-24.  Down to 2^-24 the factor is an fp16 value.
 constexpr int MAX_D = 24;
 
 // Exponent that takes a magnitude to [2^14, 2^15); 0 for zero and what is not finite.
@@ -260,7 +260,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
     constexpr bool FACT = MODE == GRAD && TRA;  // dW: dz's groups of rows have scales of their own
     constexpr int KB = G::KB, TM = G::TM, TN = G::TN, A_BLK = G::A_BLK, B_BLK = G::B_BLK, STAGES = G::STAGES;
     constexpr int A_PW = (A_BLK + NW - 1) / NW, B_PW = (B_BLK + NW - 1) / NW;
-    constexpr int LOADS = NP * (A_PW + B_PW) + FACT;
+    constexpr int LOADS = NP * (A_PW + B_PW);
     constexpr int A_SZ = A_BLK * 512, B_SZ = B_BLK * 512;      // halves a plane and slice
     constexpr int SLICE = G::SLICE;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -335,10 +335,12 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
     unsigned bits = 0;
     const unsigned aoff = lane_off(TRA), boff = lane_off(TRB);
     const unsigned ring0 = (unsigned)(uintptr_t)(lds_void *)ring;
-    auto issue = [&](int kt) {
+    // sc (dW): scaled blocks and their factors are looked out for
+    auto issue = [&](int kt, auto sc) {
+        constexpr bool SC = decltype(sc)::value;
         const unsigned base = ring0 + (kt % STAGES) * (SLICE * 2);
-        const _Float16 *Ap = p.A.p;
-        if constexpr (FACT) {
+        const _Float16 *Ap = FACT && !SC ? p.plain : p.A.p;
+        if constexpr (SC) {
             const int g = (k0 + kt * 16 * KB) >> p.fx_log;
             if (g - mask_g0 >= 64) mask = scaled_groups(mask_g0 += 64);
             const unsigned bit = (unsigned)(mask >> (g - mask_g0)) & 1;
@@ -361,7 +363,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 load_lds(Bp + q * p.B.plane + bsrc[j], boff,
                          base + (NP * A_SZ + q * B_SZ + ((wave + NW * j) % B_BLK) * 512) * 2);
         }
-        if constexpr (FACT) {
+        if constexpr (SC) {
             static_assert(TM == FX, "a factor an entry");
             load_lds4(p.fx + (long)((k0 + kt * 16 * KB) >> p.fx_log) * p.fx_ld + mt * TM, lane * 4,
                       ring0 + (G::RING + kt % STAGES * FX) * 2);
@@ -431,76 +433,87 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                     for (int e = 0; e < 4; ++e) acc[i][j][4 * e4 + e] = t[e];
                 }
     } else {
+        auto product = [&](auto sc) {
+            constexpr bool SC = decltype(sc)::value;
+            constexpr int IN_FLIGHT = (STAGES - 2) * (LOADS + SC);
 #pragma unroll
-        for (int t = 0; t < STAGES - 1; ++t)
-            if (t < nk) issue(t);
-        // the largest factor 2^-D of a lane's entries over the share's rows: scaled blocks are taken to its scale
-        for (int g = k0 >> p.fx_log; FACT && g <= g1; g += 64) any |= g == mask_g0 ? mask : scaled_groups(g);
-        if (any) {
-#pragma unroll
-            for (int i = 0; i < WTM; ++i) fmost[i] = 0.0f;
-            const _Float16 *f = p.fx + mt * TM + wm * WTM * 32 + r;
-#pragma unroll 8
-            for (int g = k0 >> p.fx_log; g <= g1; ++g)
-#pragma unroll
-                for (int i = 0; i < WTM; ++i) fmost[i] = fmaxf(fmost[i], (float)f[g * p.fx_ld + i * 32]);
-#pragma unroll
-            for (int i = 0; i < WTM; ++i) fless[i] = 1.0f / fmost[i];
-        }
-        for (int kt = 0; kt < nk; ++kt) {
-            // slice kt is in LDS once this wave's later loads are all that is in flight; the barrier
-            // covers the other waves' loads, and their reads of the slot that is loaded next
-            if (kt + STAGES - 2 < nk)
-                wait_vmcnt<(STAGES - 2) * LOADS>();
-            else
-                wait_vmcnt<0>();
-            lds_barrier();
-            if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1);
-            const _Float16 *base = ring + (kt % STAGES) * SLICE;
-            const bool scaled = FACT && (bits >> (min(kt + STAGES - 1, nk - 1) - kt) & 1);
-            _Float16 fac[WTM];
-            if (scaled)
-#pragma unroll
-                for (int i = 0; i < WTM; ++i)
-                    fac[i] = (_Float16)((float)ring[G::RING + kt % STAGES * FX + (wm * WTM + i) * 32 + r] * fless[i]);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                half8 a[NP][WTM];
-                if constexpr (RAW) {
-#pragma unroll
-                    for (int i = 0; i < WTM; ++i) raw_frag(base, wm * WTM + i, kb, a[0][i], a[NP - 1][i]);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < NP; ++q)
-#pragma unroll
-                        for (int i = 0; i < WTM; ++i) a[q][i] = frag(base + q * A_SZ, TRA, wm * WTM + i, kb);
-                }
-                half8 b[NP][WTN];
-#pragma unroll
-                for (int j = 0; j < WTN; ++j)
-#pragma unroll
-                    for (int q = 0; q < NP; ++q) b[q][j] = frag(base + NP * A_SZ + q * B_SZ, TRB, wn * WTN + j, kb);
+            for (int t = 0; t < STAGES - 1; ++t)
+                if (t < nk) issue(t, sc);
+            for (int kt = 0; kt < nk; ++kt) {
+                // slice kt is in LDS once this wave's later loads are all that is in flight; the barrier
+                // covers the other waves' loads, and their reads of the slot that is loaded next
+                if (kt + STAGES - 2 < nk)
+                    wait_vmcnt<IN_FLIGHT>();
+                else
+                    wait_vmcnt<0>();
+                lds_barrier();
+                if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1, sc);
+                const _Float16 *base = ring + (kt % STAGES) * SLICE;
+                const bool scaled = SC && (bits >> (min(kt + STAGES - 1, nk - 1) - kt) & 1);
+                _Float16 fac[WTM];
                 if (scaled)
 #pragma unroll
-                    for (int q = 0; q < NP; ++q)
+                    for (int i = 0; i < WTM; ++i)
+                        fac[i] = (_Float16)((float)ring[G::RING + kt % STAGES * FX + (wm * WTM + i) * 32 + r] * fless[i]);
 #pragma unroll
-                        for (int i = 0; i < WTM; ++i) a[q][i] *= fac[i];
-                // all of a k block's reads before its first MFMA: left to itself the compiler reads the last
-                // columns halfway and waits there (8192 x 512 fp32 4600 us for 4505, 4096 x 2048 bf16 3285 for 3218)
-                __builtin_amdgcn_sched_barrier(0);
+                for (int kb = 0; kb < KB; ++kb) {
+                    half8 a[NP][WTM];
+                    if constexpr (RAW) {
 #pragma unroll
-                for (int j = 0; j < WTN; ++j) {
+                        for (int i = 0; i < WTM; ++i) raw_frag(base, wm * WTM + i, kb, a[0][i], a[NP - 1][i]);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < WTM; ++i) {
-                        if constexpr (NP == 2) {
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
+                        for (int q = 0; q < NP; ++q)
+#pragma unroll
+                            for (int i = 0; i < WTM; ++i) a[q][i] = frag(base + q * A_SZ, TRA, wm * WTM + i, kb);
+                    }
+                    half8 b[NP][WTN];
+#pragma unroll
+                    for (int j = 0; j < WTN; ++j)
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) b[q][j] = frag(base + NP * A_SZ + q * B_SZ, TRB, wn * WTN + j, kb);
+                    if (scaled)
+#pragma unroll
+                        for (int q = 0; q < NP; ++q)
+#pragma unroll
+                            for (int i = 0; i < WTM; ++i) a[q][i] *= fac[i];
+                    // all of a k block's reads before its first MFMA: left to itself the compiler reads the last
+                    // columns halfway and waits there (8192 x 512 fp32 4600 us for 4505, 4096 x 2048 bf16 3285 for 3218)
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < WTN; ++j) {
+#pragma unroll
+                        for (int i = 0; i < WTM; ++i) {
+                            if constexpr (NP == 2) {
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
+                            }
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
                         }
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
                     }
                 }
             }
-        }
+        };
+        // dW: the marks of the share's blocks.  The product that looks out for scaled ones costs 10 % more
+        // whether there are any or not, so that shares without one take the other.
+        for (int g = k0 >> p.fx_log; FACT && g <= g1; g += 64) any |= g == mask_g0 ? mask : scaled_groups(g);
+        if constexpr (FACT)
+            if (any) {
+                // the largest factor 2^-D of a lane's entries over the share's rows: scaled blocks are taken to its scale
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) fmost[i] = 0.0f;
+                const _Float16 *f = p.fx + mt * TM + wm * WTM * 32 + r;
+#pragma unroll 16
+                for (int g = mask_g0 + hh; g <= g1; g += 2)
+#pragma unroll
+                    for (int i = 0; i < WTM; ++i) fmost[i] = fmaxf(fmost[i], (float)f[g * p.fx_ld + i * 32]);
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) fmost[i] = fmaxf(fmost[i], __shfl_xor(fmost[i], 32, 64));
+#pragma unroll
+                for (int i = 0; i < WTM; ++i) fless[i] = 1.0f / fmost[i];
+                product(std::true_type{});
+            }
+        if (!any) product(std::false_type{});
     }
     if constexpr (RAW) {
         if (p.w_head && !p.w_redo && nt == 0) {
@@ -816,7 +829,7 @@ __device__ __forceinline__ void loss_tile(const LossGemm &p, int bid, _Float16 *
                 halve(integral_constant<int, 2>{}, integral_constant<int, 0x4E>{});   // quad_perm 2 3 0 1
                 halve(integral_constant<int, 1>{}, integral_constant<int, 0xB1>{});   // quad_perm 1 0 3 2
                 const float most = top[0];
-                const int D = most < 0x1p-24f ? MAX_D : most < 0x1p-16f ? 16 : 0;
+                const int D = most < 0x1p-24f ? MAX_D : NP == 2 && most < 0x1p-16f ? 16 : 0;
                 const int at = (r >> 4) * 32 + 8 * ((r & 15) >> 2) + 4 * hh + (r & 3);
                 scale[at] = ldexpf(1.0f, DZ_EXP + D);
                 p.fx[(long)nt * p.fx_ld + mt * TM + wm * (WTM * 32) + at] = (_Float16)ldexpf(1.0f, -D);
@@ -914,12 +927,11 @@ struct Prep {
     int32_t *kw, *e_dw;          // exponent of W's scale; of dW's results
 };
 
-// The planes of XR rows of x, row r times 2^ex[r] f[r] (zeros where live[r] < 0): chunk (column block, row,
+// The planes of XR rows of x, row r times 2^ex[r] (zeros where live[r] < 0): chunk (column block, row,
 // half) by chunk, neighbouring threads side by side.  XR = 8: four blocks share a block row of 32, so
 // that 4096 rows fill the chip.
 template <typename T, int NP, bool VECX>
-__device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb, const int *live, const int *ex,
-                                           const float *f) {
+__device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb, const int *live, const int *ex) {
     const long row0 = rb * XR;
     dst += row0 / 32 * p.dcb * 512 + row0 % 32 * 16;
 #pragma unroll 4
@@ -927,27 +939,54 @@ __device__ __forceinline__ void split_rows(const Prep &p, _Float16 *dst, long rb
         const int cb = ch / (2 * XR), rl = (ch >> 1) % XR, c = cb * 16 + (ch & 1) * 8;
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (live[rl] >= 0) load8<T, VECX>((const T *)p.x + (row0 + rl) * p.x_stride, c, p.d, x);
-        store_planes<NP>(dst + (long)cb * 512 + rl * 16 + (ch & 1) * 8, p.x_plane, x, ex[rl], f ? f[rl] : 1.0f);
+        store_planes<NP>(dst + (long)cb * 512 + rl * 16 + (ch & 1) * 8, p.x_plane, x, ex[rl]);
     }
 }
 
-// The planes of x for dW, rows [rb XR, + XR), whose c_i m_i are f: from k_loss_prep's maxima.
-template <typename T, int NP, bool VECX>
-__device__ __forceinline__ void split_x2(const Prep &p, long rb, const float *f) {
-    __shared__ float red[4];
-    __shared__ int ex[XR], live[XR];
-    const int tid = threadIdx.x;
-    float m = 0.0f;
+// The planes of x for dW, rows [rb XR, + XR), from k_loss_prep's maxima.  factors(f) writes the rows' c_i m_i; what
+// does not depend on them is loaded before.
+template <typename T, int NP, bool VECX, typename F>
+__device__ __forceinline__ void split_x2(const Prep &p, long rb, F &&factors) {
+    constexpr int AHEAD = 2;  // chunks of x a thread loads ahead
+    __shared__ float top[NT / 64], f[XR];
+    __shared__ int live[XR], ex[XR];
+    const int tid = threadIdx.x, total = p.dcb * 2 * XR;
+    float m = 0.0f, x[AHEAD][8];
     for (int i = tid; i < p.row_blocks; i += NT) m = fmaxf(m, p.gmax[i]);
-    const int e = scale_exp(block_max256(m, red)) - 2;  // c_i m_i < 4
-    if (rb == 0 && tid == 0) *p.e_dw = -DZ_EXP - e;
+    const auto row_of = [&](int ch) { return (const T *)p.x + min(rb * XR + (ch >> 1) % XR, (long)p.rows - 1) * p.x_stride; };
+    const auto col_of = [&](int ch) { return ch / (2 * XR) * 16 + (ch & 1) * 8; };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+        if (tid + u * NT < total) load8<T, VECX>(row_of(tid + u * NT), col_of(tid + u * NT), p.d, x[u]);
+    const float g = tid < XR ? p.g[rb * XR + tid] : 0.0f;
+    factors(f);
+    m = wave_max(m);
+    if ((tid & 63) == 0) top[tid >> 6] = m;
     if (tid < XR) {
-        const float g = p.g[rb * XR + tid];
-        ex[tid] = exp_of(g) + e;
+        ex[tid] = exp_of(g);
         live[tid] = g == 0.0f ? -1 : 0;  // a row that gives nothing is not in the scale's range
     }
     __syncthreads();
-    split_rows<T, NP, VECX>(p, p.x2p, rb, live, ex, f);
+    const int e = scale_exp(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) - 2;  // c_i m_i < 4
+    if (rb == 0 && tid == 0) *p.e_dw = -DZ_EXP - e;
+    const long row0 = rb * XR;
+    _Float16 *dst = p.x2p + row0 / 32 * p.dcb * 512 + row0 % 32 * 16;
+    auto put = [&](int ch, float (&v)[8]) {
+        const int rl = (ch >> 1) % XR;
+        if (live[rl] < 0)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        store_planes<NP>(dst + (long)(ch / (2 * XR)) * 512 + rl * 16 + (ch & 1) * 8, p.x_plane, v, ex[rl] + e, f[rl]);
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+        if (tid + u * NT < total) put(tid + u * NT, x[u]);
+#pragma unroll 4
+    for (int ch = tid + AHEAD * NT; ch < total; ch += NT) {
+        float v[8];
+        load8<T, VECX>(row_of(ch), col_of(ch), p.d, v);
+        put(ch, v);
+    }
 }
 
 // The first row_blocks blocks: XR rows of x each, split into planes with a scale of their own; rows
@@ -1019,7 +1058,7 @@ __global__ __launch_bounds__(NT) void k_loss_prep(Prep p) {
         for (int r = 1; r < XR; ++r) m = fmaxf(m, rmax[r]);
         p.gmax[rb] = m;
     }
-    split_rows<T, NP, VECX>(p, p.xp, rb, tg, fx, nullptr);
+    split_rows<T, NP, VECX>(p, p.xp, rb, tg, fx);
 }
 
 // W's planes, from k_loss_prep's maxima: each block those of every so many-th block of 32 rows, of a share
@@ -1061,67 +1100,77 @@ struct Rows {
     float *out_loss, *out_lse;
 };
 
-// XR rows a block; 32 threads share a row's tiles, eight loads in flight each.  Where dW is wanted, then
-// the rows' planes of x for it.
+// XR rows a block; 32 threads share a row's tiles, eight loads in flight each: a row's 8 in a wave, the waves then.
+// Where dW is wanted, then the rows' planes of x for it.
 template <typename T, int NP, bool VECX>
 __global__ __launch_bounds__(NT) void k_loss_rows(Rows p, Prep pr) {
     constexpr int PARTS = NT / XR;
-    __shared__ float sm[PARTS][XR + 1], ss[PARTS][XR + 1], f[XR];
-    const int rl = threadIdx.x % XR, part = threadIdx.x / XR;
+    __shared__ float sm[NT / 64][XR], ss[NT / 64][XR];
+    const int rl = threadIdx.x % XR, part = threadIdx.x / XR, wave = threadIdx.x >> 6;
     const long i = (long)blockIdx.x * XR + rl;
-    float mx = -INFINITY, s = 0.0f;
-    for (int t0 = part; t0 < p.tiles; t0 += PARTS * 8) {
-        float m[8], v[8];
+    auto stats = [&](float *f) {
+        const bool there = p.tgt[i] >= 0;
+        const float zt = p.ztgt[i], g = pr.g[i];
+        float mx = -INFINITY, s = 0.0f;
+        for (int t0 = part; t0 < p.tiles; t0 += PARTS * 8) {
+            float m[8], v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int t = t0 + PARTS * u;
-            const long o = (long)min(t, p.tiles - 1) * p.rows_pad + i;
-            m[u] = p.part_m[o];
-            v[u] = p.part_s[o];
-            if (t >= p.tiles) m[u] = -INFINITY, v[u] = 0.0f;
+            for (int u = 0; u < 8; ++u) {
+                const int t = t0 + PARTS * u;
+                const long o = (long)min(t, p.tiles - 1) * p.rows_pad + i;
+                m[u] = p.part_m[o];
+                v[u] = p.part_s[o];
+                if (t >= p.tiles) m[u] = -INFINITY, v[u] = 0.0f;
+            }
+            float nm = mx;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) nm = fmaxf(nm, m[u]);
+            const float ref = nm == -INFINITY ? 0.0f : nm;
+            s *= __builtin_amdgcn_exp2f(mx - ref);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u] * __builtin_amdgcn_exp2f(m[u] - ref);
+            mx = nm;
         }
-        float nm = mx;
+        float top = mx;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) nm = fmaxf(nm, m[u]);
-        const float ref = nm == -INFINITY ? 0.0f : nm;
-        s *= __builtin_amdgcn_exp2f(mx - ref);
+        for (int off = XR; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        s *= __builtin_amdgcn_exp2f(mx - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
-        for (int u = 0; u < 8; ++u) s += v[u] * __builtin_amdgcn_exp2f(m[u] - ref);
-        mx = nm;
-    }
-    sm[part][rl] = mx;
-    ss[part][rl] = s;
-    __syncthreads();
-    if (part == 0) {
-#pragma unroll
-        for (int q = 1; q < PARTS; ++q) mx = fmaxf(mx, sm[q][rl]);
+        for (int off = XR; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
+        if (part % (64 / XR) == 0) {
+            sm[wave][rl] = top;
+            ss[wave][rl] = s;
+        }
+        __syncthreads();
+        if (part) return;
+        mx = fmaxf(fmaxf(sm[0][rl], sm[1][rl]), fmaxf(sm[2][rl], sm[3][rl]));
         const float ref = mx == -INFINITY ? 0.0f : mx;
         s = 0.0f;
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) s += ss[q][rl] * __builtin_amdgcn_exp2f(sm[q][rl] - ref);
+        for (int q = 0; q < NT / 64; ++q) s += ss[q][rl] * __builtin_amdgcn_exp2f(sm[q][rl] - ref);
         const float lse = ref + log2f(s);
-        const bool there = p.tgt[i] >= 0;
-        const float z = there ? p.ztgt[i] : lse, c = row_unit(z, lse);
+        const float z = there ? zt : lse, c = row_unit(z, lse);
         p.lse[i] = lse;
         pr.c[i] = c;
-        pr.h[i] = f[rl] = row_factor(pr.g[i], c);
+        pr.h[i] = row_factor(g, c);
+        if (f) f[rl] = row_factor(g, c);
         if (i < p.rows) {
             if (p.out_lse) p.out_lse[i] = there ? lse * LN2 : 0.0f;
             if (p.out_loss) p.out_loss[i] = there ? (lse - z) * LN2 : 0.0f;
         }
-    }
-    if (!pr.x2p) return;
-    __syncthreads();
-    split_x2<T, NP, VECX>(pr, blockIdx.x, f);
+    };
+    if (pr.x2p)
+        split_x2<T, NP, VECX>(pr, blockIdx.x, stats);
+    else
+        stats(nullptr);
 }
 
 // Those planes by themselves, where one tile of the logits' product was the whole vocabulary.
 template <typename T, int NP, bool VECX>
 __global__ __launch_bounds__(NT) void k_loss_x2(Prep p) {
-    __shared__ float f[XR];
-    if (threadIdx.x < XR) f[threadIdx.x] = p.h[(long)blockIdx.x * XR + threadIdx.x];
-    __syncthreads();
-    split_x2<T, NP, VECX>(p, blockIdx.x, f);
+    split_x2<T, NP, VECX>(p, blockIdx.x, [&](float *f) {
+        if (threadIdx.x < XR) f[threadIdx.x] = p.h[(long)blockIdx.x * XR + threadIdx.x];
+    });
 }
 
 // ---- shares of the gradients ---------------------------------------------------------------

@@ -333,9 +333,9 @@ int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const flo
  * row whose logits are all -inf, or not a number, has a loss, a dx and a share of dw that are not
  * numbers.  Precision: fp32 operands keep at least 21 bits in the products and bf16 ones all of
  * theirs, dz 21 and 11; w's entries are resolved to 2^-36 of its largest, dz for dx to 2^-38 of its
- * dloss, dz for dw too, where an entry's largest |dz / dloss| of 32 to 128 rows is below 2^-16 to
- * 2^-54 and below 2^-24 to 2^-62, so that a row of dw keeps its bits however rare its entry is (db is
- * formed from dz in fp32).  Calls that need no planes of dz (few rows, small sizes) have no such step. */
+ * dloss, dz for dw too, but where an entry's largest |dz / dloss| of 32 to 128 rows is below 2^-16
+ * (fp32 calls) to 2^-54, and below 2^-24 to 2^-62, so that a row of dw keeps its bits however rare
+ * its entry is (db is formed from dz in fp32).  Calls that need no planes of dz (few rows, small sizes) have no such step. */
 typedef struct adn_lm_loss_args {
     int32_t rows, d, vocab;     /* rows in [0, 2^20], d in [1, 8192], vocab in [1, 2^24] */
     uint32_t dtype;             /* ADN_T_*: x, w, dx and dw                               */

@@ -8,7 +8,7 @@ Tolerances, with u = 2^-24, A_iv = sum_k |x_ik w_vk|:
          the exponentials themselves, 3 u |lse|;
   dz     rounded to 21 bits (fp32 calls) or 11 (bf16 calls, half a step 2^-12); half the smallest step, of dloss: fp16's 2^-24
          under a scale of 2^14, times at most 2 (dz / dloss is stored over a factor in [1, 2)), 2^-38, and 2^-16 of that for an
-         entry whose largest value is below 2^-16, 2^-24 of that below 2^-24;
+         entry whose largest value is below 2^-16 (fp32 calls), 2^-24 of that below 2^-24;
   dW     sum over the rows of that error times |x|, operands 2^-20 and x's own planes 2^-35 of the largest |x dloss| (bf16 calls:
          x dloss rounded to 11 bits), a chain of at most `rows` fp32 additions; the output's half step.
 """
@@ -86,7 +86,7 @@ def test_gradients_of_rare_entries(be, rows, d, V, dtype):
     bf = dtype == BF16
     e = p * (tz + tz.amax(1, keepdim=True) + 2.0 ** -16 + 3 * U * lse.abs()) + (2.0 ** -12 if bf else 2.0 ** -21) * dz.abs()
     top = dz.abs().amax(0, keepdim=True)
-    e += torch.where(top >= 2.0 ** -16, 2.0 ** -38, torch.where(top >= 2.0 ** -24, 2.0 ** -54, 2.0 ** -62))
+    e += torch.where(top >= (2.0 ** -24 if bf else 2.0 ** -16), 2.0 ** -38, torch.where(top >= 2.0 ** -24, 2.0 ** -54, 2.0 ** -62))
     xg = (x * g).abs()
     wide = xg * ((2.0 ** -12 if bf else 0.0) + 2.0 ** -20 + rows * U) + 2.0 ** -35 * xg.max()
     ref = torch.mm((dz * g).t().contiguous(), x)
