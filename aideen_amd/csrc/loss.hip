@@ -1416,15 +1416,25 @@ LossPlan loss_plan(const LossParams &p) {
     return L;
 }
 
+// A launch has less than 2^32 threads: the pass over the whole vocabulary (2^20 rows against 2^19 entries are 2^24
+// workgroups) is launched a range of its tiles at a time.  A piece's tiles are fewer.
+constexpr long MOST_BLOCKS = (1L << 32) / NT - 1;
+
 template <int MODE, typename T, int NP>
-void launch_logits(const LossGemm &g, int tn, hipStream_t st) {
-    const unsigned grid = (unsigned)(g.nM * g.nN);
-    if (tn == 128)
-        k_loss_logits<MODE, T, NP, 4><<<grid, NT, 0, st>>>(g);
-    else if (tn == 64)
-        k_loss_logits<MODE, T, NP, 2><<<grid, NT, 0, st>>>(g);
-    else
-        k_loss_logits<MODE, T, NP, 1><<<grid, NT, 0, st>>>(g);
+void launch_logits(LossGemm g, int tn, hipStream_t st) {
+    const int tiles = g.nM, most = (int)std::min<long>(tiles, MOST_BLOCKS / g.nN);
+    for (int m = 0; m < tiles; m += most) {
+        g.nM = std::min(most, tiles - m);
+        const unsigned grid = (unsigned)(g.nM * g.nN);
+        if (tn == 128)
+            k_loss_logits<MODE, T, NP, 4><<<grid, NT, 0, st>>>(g);
+        else if (tn == 64)
+            k_loss_logits<MODE, T, NP, 2><<<grid, NT, 0, st>>>(g);
+        else
+            k_loss_logits<MODE, T, NP, 1><<<grid, NT, 0, st>>>(g);
+        g.a_row0 += most * TV;
+        g.part_m += most * g.rows_pad, g.part_s += most * g.rows_pad;
+    }
 }
 
 template <typename T, int NP>
