@@ -9,6 +9,8 @@
 // pass a team walks its share of the rows and keeps the gain's gradient of its columns in
 // registers; the teams' sums are written as partials and added in a fixed order, so the result
 // does not depend on the schedule.
+#include <algorithm>
+
 #include "train.h"
 
 namespace adn {
@@ -236,17 +238,24 @@ void launch_norm(const NormParams &p, hipStream_t st) {
     if (p.rows == 0) return;
     const int eb = elem_bytes(p.dtype);
     const bool vec = rows_vec16(p.x, p.x_stride, p.d, eb) && rows_vec16(p.y, p.y_stride, p.d, eb);
-    dispatch_type(p.dtype, [&](auto t) {
-        typedef decltype(t) T;
-        dispatch_row(p.d, [&](auto team, auto e) {
-            constexpr int TEAM = decltype(team)::value, E = decltype(e)::value;
-            const dim3 grid((unsigned)(((long)p.rows * TEAM + NB - 1) / NB));
-            if (vec)
-                k_rms_norm<T, TEAM, E, true><<<grid, NB, 0, st>>>(p);
-            else
-                k_rms_norm<T, TEAM, E, false><<<grid, NB, 0, st>>>(p);
+    // a launch has less than 2^32 threads: 2^23 rows at a time, a block a row at most
+    NormParams q = p;
+    for (int row = 0; row < p.rows; row += 1 << 23) {
+        q.rows = std::min(p.rows - row, 1 << 23);
+        q.x = (const char *)p.x + row * p.x_stride * eb;
+        q.y = (char *)p.y + row * p.y_stride * eb;
+        dispatch_type(p.dtype, [&](auto t) {
+            typedef decltype(t) T;
+            dispatch_row(p.d, [&](auto team, auto e) {
+                constexpr int TEAM = decltype(team)::value, E = decltype(e)::value;
+                const dim3 grid((unsigned)(((long)q.rows * TEAM + NB - 1) / NB));
+                if (vec)
+                    k_rms_norm<T, TEAM, E, true><<<grid, NB, 0, st>>>(q);
+                else
+                    k_rms_norm<T, TEAM, E, false><<<grid, NB, 0, st>>>(q);
+            });
         });
-    });
+    }
 }
 
 size_t norm_backward_workspace_bytes(const NormParams &p) {

@@ -2,7 +2,7 @@
 
 Tolerances.  Losses: logits of at most 32 exact products (bf16) with partial sums below 2^4, 32 x 2^-24 x 2^4 = 2^-15, and the
 conversion to units of log 2, 3 x 2^-24 x 2^4; a sum of exponentials is at most 2^9 additions deep, 2^-15; lse (below 2^5) is
-rounded twice, 2^-18."""
+rounded twice, 2^-18.  Norm: bf16 outputs by half a step, 2^-8, the fp32 sum of 2049 squares before by 2^-13 at most."""
 import pytest
 import torch
 
@@ -47,3 +47,24 @@ def test_losses_of_many_rows_and_entries(be, d):
     ref = lse - z.gather(1, t[at].long()[:, None])[:, 0]
     assert ((out["loss"][at].double() - ref).abs() <= 2 * tol).all(), float((out["loss"][at].double() - ref).abs().max())
     assert torch.isfinite(out["loss"]).all() and (out["lse"] > 8).all()
+
+
+def test_norm_of_many_long_rows(be):
+    """2^24 rows of a block each."""
+    rows, d = 1 << 24, 2049
+    print(f"norm {rows} x {d}", flush=True)
+    x, y = torch.empty((rows, d), device="cuda", dtype=BF16), torch.empty((rows, d), device="cuda", dtype=BF16)
+    part = torch.randn((1 << 18, d), device="cuda", dtype=BF16)
+    for i in range(0, rows, 1 << 18):
+        x[i:i + (1 << 18)] = part * (1 + i / rows)
+    y[::4099].fill_(7)
+    torch.cuda.synchronize()
+    be.rms_norm_async(x, y)
+    be.synchronize()
+    for i in (0, (1 << 23) - 300, 1 << 23, rows - 300):
+        X = x[i:i + 300].double()
+        ref = X / torch.sqrt((X * X).mean(1, keepdim=True) + 1e-5)
+        assert ((y[i:i + 300].double() - ref).abs() <= (2.0 ** -8 + 2.0 ** -12) * ref.abs() + 1e-30).all(), i
+    X = x[::4099].double()
+    ref = X / torch.sqrt((X * X).mean(1, keepdim=True) + 1e-5)
+    assert ((y[::4099].double() - ref).abs() <= (2.0 ** -8 + 2.0 ** -12) * ref.abs() + 1e-30).all()
