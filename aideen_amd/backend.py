@@ -272,6 +272,11 @@ class GpuDeqBackend:
     # training operators (device memory, enqueue only) --------------------------------------
     # Arguments are torch tensors on the context's GPU; matrices float32 or bfloat16 (all of one
     # call alike) with adjacent elements in a row and any row stride, vectors float32, ids int32.
+    # A call returns before its kernels have run.  They run on the context's stream, a stream of its own
+    # that is not ordered with torch's unless `set_stream` has handed it one of those (not the default
+    # one, whose handle is null): otherwise the caller lets it wait for what fills the tensors, and lets
+    # what reads them wait for it.  Tensors stay alive until the stream has passed the call; one that
+    # torch may free before needs `record_stream`.
     def _matrix(self, t, name: str, rows: int, d: int, dtype=None):
         """(pointer, row stride) of a [rows][d] tensor."""
         if t.shape != (rows, d):
@@ -316,7 +321,8 @@ class GpuDeqBackend:
         """Softmax cross entropy of the rows x [rows][d] against targets [rows] through the head w
         [vocab][d] (+ bias [vocab]; w None: the uploaded lm_w and lm_b), with its gradients for the
         upstream gradient dloss [rows] (None = 1).  ``outputs`` names the wanted results: loss [rows],
-        lse [rows], dx [rows][d], dw [vocab][d], db [vocab].  A target < 0 leaves its row out."""
+        lse [rows], dx [rows][d], dw [vocab][d], db [vocab].  A target < 0 leaves its row out.  Runs on the context's stream; the
+        caller orders it with the streams that fill and read the tensors, and keeps them until then."""
         unknown = set(outputs) - {"loss", "lse", "dx", "dw", "db"}
         if unknown:
             raise _invalid(f"unknown outputs {sorted(unknown)}")
@@ -345,7 +351,9 @@ class GpuDeqBackend:
         check(lib().adn_lm_loss_async(self._ctx, C.byref(a)))
 
     def rms_norm_async(self, x, y, *, gain=None, eps: float = 1e-5) -> None:
-        """y = x / sqrt(mean(x^2) + eps) * gain per row (the LM head's norm); gain [d] float32 or None."""
+        """y = x / sqrt(mean(x^2) + eps) * gain per row (the LM head's norm); gain [d] float32 or None.  Runs on
+        the context's stream; the caller orders it with the streams that fill and read the tensors, and
+        keeps them until then."""
         if x.dim() != 2:
             raise _invalid("x must be a matrix")
         rows, d = x.shape
@@ -356,7 +364,8 @@ class GpuDeqBackend:
 
     def rms_norm_backward_async(self, x, dy, *, outputs: Dict[str, object], gain=None, eps: float = 1e-5) -> None:
         """Gradients of rms_norm_async for the upstream gradient dy: ``outputs`` names dx [rows][d]
-        and/or dg [d] (float32)."""
+        and/or dg [d] (float32).  Runs on the context's stream; the caller orders it with the streams that
+        fill and read the tensors, and keeps them until then."""
         unknown = set(outputs) - {"dx", "dg"}
         if unknown:
             raise _invalid(f"unknown outputs {sorted(unknown)}")
@@ -374,7 +383,9 @@ class GpuDeqBackend:
 
     def embed_lookup_async(self, tokens, out, *, table=None, scale: float = 1.0) -> None:
         """out[i] = scale * table[tokens[i]] (``Tokenizer::embed_sequence``, tokenizer.rs:151-159, with a
-        factor); table None: the uploaded embedding.  A token < 0 gives a row of zeros."""
+        factor); table None: the uploaded embedding.  A token < 0 gives a row of zeros.
+        Runs on the context's stream; the caller orders it with the streams that fill and read the tensors,
+        and keeps them until then."""
         if out.dim() != 2 or (table is not None and table.dim() != 2):
             raise _invalid("out and table must be matrices")
         n, d = out.shape
@@ -386,7 +397,8 @@ class GpuDeqBackend:
 
     def embed_grad_async(self, dout, tokens, dtable, *, scale: float = 1.0) -> None:
         """The table's gradient: dtable[v] = scale * sum of the rows dout[i] with tokens[i] = v, always added
-        in the same order; every row of dtable is written."""
+        in the same order; every row of dtable is written.  Runs on the context's stream; the caller orders
+        it with the streams that fill and read the tensors, and keeps them until then."""
         if dout.dim() != 2 or dtable.dim() != 2:
             raise _invalid("dout and dtable must be matrices")
         n, d = dout.shape

@@ -1,5 +1,5 @@
-// Softmax cross entropy of the LM head over the whole vocabulary, with its gradients, without
-// keeping the logits:
+// Softmax cross entropy of the LM head over the whole vocabulary, with its gradients, keeping the
+// logits only where they are few:
 //
 //   z = x W^T + b,  lse_i = log sum_v exp(z_iv),  loss_i = lse_i - z_i,t(i)
 //   dz_iv = g_i (exp(z_iv - lse_i) - [v = t(i)])
@@ -8,9 +8,12 @@
 // Four products on the fp16 MFMA, 2 n V d operations each (n rows, V entries, width d): the logits
 // for lse (stored nowhere: their epilogue leaves each row's maximum and sum of exponentials per 256
 // entries), then a piece of the vocabulary at a time the logits again, whose epilogue stores the
-// piece's dz, and dz W and dz^T x from it.  The piece holds at most PIECE_BYTES, so the workspace
-// does not grow with n V.  Forming the logits twice costs a third more operations than keeping them,
-// n V values of 4 bytes, which is done where they are few (loss_plan).
+// piece's dz, and dz W and dz^T x from it.  A piece's dz takes at most PIECE_BYTES, or 256 entries of
+// every row where those are more (beyond 2^18 rows of fp32), and is there twice, for dx and for dW.
+// What grows with n V in the workspace is the statistics, 8 bytes a row and 256 entries, and db's
+// partial sums, 4 bytes an entry and tile of rows.  Forming the logits twice costs a third more
+// operations than keeping them, n V values of 4 bytes, which is done up to PIECE_BYTES where it
+// saves time (loss_plan).
 //
 // Operands are fp16 planes.  fp32 tensors: two planes, hi = f16(s x) and lo = f16(s x - hi), three
 // products hi hi + hi lo + lo hi (the split of the forward's products: 2^-22 of a product is lost).

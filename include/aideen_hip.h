@@ -310,8 +310,9 @@ int adn_adjoint_async(adn_ctx *ctx, int32_t ntok, const float *h_star, const flo
  * What lies between a forward's pooled rows and adn_adjoint's dl, and behind its source gradient:
  * the head's RMS norm (lm_head.rs:35-54), the softmax cross entropy over the whole vocabulary with
  * its gradients, and the embedding rows (tokenizer.rs:117-119, 151-159) with the table's gradient.
- * All take device memory of the context's GPU and only enqueue on the context's stream; the tensors
- * must not overlap.  Sizes are the call's own (the context's configuration bounds them only where
+ * All take device memory of the context's GPU and only enqueue on the context's stream: the caller
+ * orders that stream with others that use the tensors, which stay alive until it has passed the call
+ * and must not overlap.  Sizes are the call's own (the context's configuration bounds them only where
  * its weights are used).  Matrices are rows of d elements at a stride in elements (>= d) of the type
  * dtype; any alignment of whole elements is served (16-byte aligned rows at the full rate).  Sums
  * are taken in fp32 in an order that the call's sizes, ids and alignment decide, never the schedule,
