@@ -15,6 +15,7 @@ BF16 = torch.bfloat16
 
 @pytest.fixture()
 def be():
+    torch.cuda.empty_cache()
     if torch.cuda.mem_get_info()[0] < 150 << 30:
         pytest.skip("less than 150 GB of the GPU's memory are free")
     b = GpuDeqBackend(synth.ModelConfig(d=64, H=2, V=300, N=1, flags=0), 1, 1)
