@@ -100,6 +100,25 @@ def test_gradients_of_rare_entries(be, rows, d, V, dtype):
     assert ((loss(be, s, ("dw",))["dw"].double() - ref_dw).abs() <= tol_dw).all()  # by itself
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,d,V", [(300, 64, 2000), (300, 192, 250), (5000, 64, 9000)])
+def test_rows_and_calls_apart(be, rows, d, V, dtype):
+    """Beside rare entries too: equal calls give equal bits, and a row matters to no other row's loss and dx."""
+    s, _ = peaked(rows, d, V, dtype, rows)
+    out = loss(be, s)
+    again = loss(be, s)
+    assert all(torch.equal(out[k], again[k]) for k in out)
+    s["x"][7] = float("nan")  # takes its values out of its entries' largest
+    s["x"][rows - 2] *= 30
+    s["dloss"][40] = 1e6
+    s["targets"][60] = V - 2
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[[7, 40, 60, rows - 2]] = False
+    other = loss(be, s)
+    for k in ("loss", "lse", "dx"):
+        assert torch.equal(other[k][rest], out[k][rest]), k
+
+
 @pytest.mark.parametrize("counted,V,spread", [(425, 3000, 1.0), (600, 1500, 0.05), (531, 5003, 0.02), (425, 100, 0.02), (130, 2500, 0.05)])
 def test_roundings_have_no_common_sign(be, counted, V, spread):
     """bf16 gradients of a mean over the rows (dloss = 1 / n, alike for all), probabilities nearly alike too: their error has no
