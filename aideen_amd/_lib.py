@@ -77,6 +77,40 @@ class AdnLmLossArgs(C.Structure):
                 ("dw_stride", C.c_int64), ("db", C.c_void_p)]
 
 
+class AdnResidualNormArgs(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("d", C.c_int32), ("dtype", C.c_uint32), ("gate_kind", C.c_uint32),
+                ("gate_sigmoid", C.c_int32), ("post_norm", C.c_int32), ("keep", C.c_float), ("scale", C.c_float),
+                ("eps", C.c_float), ("reserved", C.c_uint32), ("x", C.c_void_p), ("x_stride", C.c_int64),
+                ("f", C.c_void_p), ("f_stride", C.c_int64), ("post_gain", C.c_void_p), ("gate", C.c_void_p),
+                ("gate_stride", C.c_int64), ("pre_gain", C.c_void_p), ("z", C.c_void_p), ("z_stride", C.c_int64),
+                ("y", C.c_void_p), ("y_stride", C.c_int64), ("dz", C.c_void_p), ("dz_stride", C.c_int64),
+                ("dy", C.c_void_p), ("dy_stride", C.c_int64), ("dx", C.c_void_p), ("dx_stride", C.c_int64),
+                ("df", C.c_void_p), ("df_stride", C.c_int64), ("dgate", C.c_void_p), ("dgate_stride", C.c_int64),
+                ("dpost_gain", C.c_void_p), ("dpre_gain", C.c_void_p)]
+
+
+GATES = {"none": 0, "channel": 1, "row": 2, "element": 3}
+
+
+class AdnAdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("copy", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n", C.c_int64), ("lr_scale", C.c_float),
+                ("weight_decay", C.c_float), ("grad_dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class AdnAdamwConfig(C.Structure):
+    _fields_ = [("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("seed", C.c_uint64),
+                ("step", C.c_void_p), ("state_bits", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class AdnAdamwStep(C.Structure):
+    _fields_ = [("lr", C.c_double), ("lr_device", C.c_void_p), ("grad_norm", C.c_void_p), ("max_norm", C.c_float),
+                ("grad_scale", C.c_float)]
+
+
+ADAMW_BLOCK = 256  # values of an 8-bit state that share a scale
+
+
 class AdnError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"[{code}] {msg}")
@@ -162,6 +196,13 @@ def lib():
                                              C.c_void_p, C.c_int64, C.c_float, C.c_void_p, C.c_int64]),
         "adn_embed_grad_async": (C.c_int, [ctx_p, C.c_int32, C.c_int32, C.c_int32, C.c_uint32, C.c_void_p, C.c_void_p,
                                            C.c_int64, C.c_float, C.c_void_p, C.c_int64]),
+        "adn_residual_norm_async": (C.c_int, [ctx_p, C.POINTER(AdnResidualNormArgs)]),
+        "adn_residual_norm_backward_async": (C.c_int, [ctx_p, C.POINTER(AdnResidualNormArgs)]),
+        "adn_adamw_create": (C.c_int, [ctx_p, C.POINTER(AdnAdamwConfig), C.c_int64, C.POINTER(AdnAdamwTensor),
+                                       C.POINTER(C.c_void_p)]),
+        "adn_adamw_destroy": (None, [C.c_void_p]),
+        "adn_adamw_grad_norm_async": (C.c_int, [C.c_void_p, C.c_void_p]),
+        "adn_adamw_step_async": (C.c_int, [C.c_void_p, C.POINTER(AdnAdamwStep)]),
         "adn_profile_forward": (C.c_int, [ctx_p, C.POINTER(AdnRun), C.POINTER(AdnOutputs),
                                           C.POINTER(AdnProfile)]),
     }

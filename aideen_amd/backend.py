@@ -18,12 +18,15 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-from typing import Dict, Optional
+from typing import TYPE_CHECKING, Dict, Optional
 
 import numpy as np
 
 from . import _lib
 from ._lib import AdnConfig, AdnOutputs, AdnRun, AdnWeights, check, lib
+
+if TYPE_CHECKING:
+    from .optimizer import AdamW
 
 _F32P = _lib.F32P
 _I32P = _lib.I32P
@@ -380,6 +383,93 @@ class GpuDeqBackend:
             return
         check(lib().adn_rms_norm_backward_async(self._ctx, rows, d, self._dtype(x), xp, xs,
                                                 self._vector(gain, "gain", d), eps, dyp, dys, dxp, dxs, dgp))
+
+    def _residual_args(self, f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps):
+        if f.dim() != 2:
+            raise _invalid("f must be a matrix")
+        rows, d = f.shape
+        a = _lib.AdnResidualNormArgs(rows=rows, d=d, dtype=self._dtype(f), gate_sigmoid=bool(gate_sigmoid),
+                                     post_norm=bool(post_norm), keep=keep, scale=scale, eps=eps)
+        a.f, a.f_stride = self._matrix(f, "f", rows, d)
+        a.post_gain, a.pre_gain = self._vector(post_gain, "post_gain", d), self._vector(pre_gain, "pre_gain", d)
+        kind = "none"
+        if gate is not None:
+            kind = "channel" if gate.dim() == 1 else "row" if gate.shape == (rows, 1) and _dtype_code(gate.dtype) == 0 else "element"
+        a.gate_kind = _lib.GATES[kind]
+        a.gate, a.gate_stride = self._gate(kind, gate, "gate", rows, d, f.dtype)
+        return a, kind
+
+    def _gate(self, kind, t, name, rows, d, dtype):
+        """(pointer, row stride) of a gate or its gradient, as the gate is shared."""
+        if t is None:
+            return None, 0
+        if kind == "element":
+            return self._matrix(t, name, rows, d, dtype)
+        if kind == "row":
+            if t.shape != (rows, 1):
+                raise _invalid(f"{name} must have the shape ({rows}, 1), got {tuple(t.shape)}")
+            t = t[:, 0]
+        return self._vector(t, name, rows if kind == "row" else d), 0
+
+    def residual_norm_async(self, x, f, *, outputs: Dict[str, object], gate=None, gate_sigmoid: bool = False,
+                            post_norm: bool = True, post_gain=None, pre_gain=None, keep: float = 1.0,
+                            scale: float = 1.0, eps: float = 1e-6) -> None:
+        """The norms around a residual block: z = keep x + scale gate n, n = f / sqrt(mean(f^2) + eps) *
+        post_gain (post_norm False: f), y = z / sqrt(mean(z^2) + eps) * pre_gain, the input of the next block
+        or the head.  x, f [rows][d]; ``outputs`` names z and/or y [rows][d]; z may be x.  The gate is [d]
+        float32 (a scale a channel), [rows, 1] float32 (one a row) or [rows][d] of f's type; gate_sigmoid: it
+        is given as logits.  keep = 1 - damping and scale = damping make it the solver's damped update.
+        Runs on the context's stream; the caller orders it with the streams that fill and read the
+        tensors, and keeps them until then."""
+        unknown = set(outputs) - {"z", "y"}
+        if unknown:
+            raise _invalid(f"unknown outputs {sorted(unknown)}")
+        a, _ = self._residual_args(f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps)
+        a.x, a.x_stride = self._matrix(x, "x", a.rows, a.d, f.dtype)
+        for k in ("z", "y"):
+            t = outputs.get(k)
+            if t is not None:
+                p, stride = self._matrix(t, k, a.rows, a.d, f.dtype)
+                setattr(a, k, p), setattr(a, k + "_stride", stride)
+        if a.rows == 0 and outputs.keys():
+            return
+        check(lib().adn_residual_norm_async(self._ctx, C.byref(a)))
+
+    def residual_norm_backward_async(self, z, f, *, outputs: Dict[str, object], dz=None, dy=None, gate=None,
+                                     gate_sigmoid: bool = False, post_norm: bool = True, post_gain=None, pre_gain=None,
+                                     keep: float = 1.0, scale: float = 1.0, eps: float = 1e-6) -> None:
+        """Gradients of residual_norm_async for the gradients dz (that reach z by other ways) and/or dy: ``outputs``
+        names any of dx, df [rows][d], dgate (as the gate), dpost_gain, dpre_gain [d] (float32).  z is the
+        forward's (needed where dy is given, else None will do); dx may be dz.  Runs on the context's
+        stream; the caller orders it with the streams that fill and read the tensors, and keeps them until
+        then."""
+        unknown = set(outputs) - {"dx", "df", "dgate", "dpost_gain", "dpre_gain"}
+        if unknown:
+            raise _invalid(f"unknown outputs {sorted(unknown)}")
+        a, kind = self._residual_args(f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps)
+        rows, d = a.rows, a.d
+        for k, t in (("z", z), ("dz", dz), ("dy", dy), ("dx", outputs.get("dx")), ("df", outputs.get("df"))):
+            if t is not None:
+                p, stride = self._matrix(t, k, rows, d, f.dtype)
+                setattr(a, k, p), setattr(a, k + "_stride", stride)
+        if outputs.get("dgate") is not None:
+            if gate is None:
+                raise _invalid("dgate without a gate")
+            a.dgate, a.dgate_stride = self._gate(kind, outputs["dgate"], "dgate", rows, d, f.dtype)
+        a.dpost_gain = self._vector(outputs.get("dpost_gain"), "dpost_gain", d)
+        a.dpre_gain = self._vector(outputs.get("dpre_gain"), "dpre_gain", d)
+        if rows == 0:
+            a.dx = a.df = None
+            if kind != "channel":
+                a.dgate = None
+            if not (a.dgate or a.dpost_gain or a.dpre_gain):
+                return  # an empty batch, and only row outputs: nothing to write
+        check(lib().adn_residual_norm_backward_async(self._ctx, C.byref(a)))
+
+    def adamw(self, params, grads, **options) -> "AdamW":
+        """An AdamW optimizer over lists of tensors on this context's GPU and stream: see ``AdamW``."""
+        from .optimizer import AdamW
+        return AdamW(self, params, grads, **options)
 
     def embed_lookup_async(self, tokens, out, *, table=None, scale: float = 1.0) -> None:
         """out[i] = scale * table[tokens[i]] (``Tokenizer::embed_sequence``, tokenizer.rs:151-159, with a

@@ -12,6 +12,7 @@
 #include <cstring>
 #include <cmath>
 #include <initializer_list>
+#include <memory>
 #include <utility>
 #include <mutex>
 #include <vector>
@@ -113,6 +114,12 @@ struct adn_ctx {
     // ComputeBackend tensors
     std::vector<DevBuf> tensors;
     std::vector<void *> allocs;
+    std::vector<adn_adamw *> optimizers;  // live handles, told when the context goes
+};
+
+struct adn_adamw {
+    adn_ctx *ctx = nullptr;  // null once the context is destroyed
+    OptPlan plan{};
 };
 
 namespace {
@@ -1000,6 +1007,7 @@ int adn_create(const adn_config *cfg, adn_ctx **out) {
 void adn_destroy(adn_ctx *c) {
     if (!c) return;
     if (c->stream) (void)hipStreamSynchronize(c->stream);
+    for (adn_adamw *o : c->optimizers) o->ctx = nullptr;
     dfree_all(c);
     for (auto &b : c->staging)
         if (b.p) (void)hipFree(b.p);
@@ -2135,6 +2143,236 @@ int adn_embed_grad_async(adn_ctx *c, int32_t n, int32_t d, int32_t vocab, uint32
         if (!msg.empty()) return fail(ADN_E_INVALID, msg);
         TableParams p{n, d, vocab, dtype, tokens, scale, dout, dout_stride, dtable, dtable_stride, c->d_err};
         return train_launch(c, embed_grad_workspace_bytes(p), [&](void *ws) { launch_embed_grad(p, ws, c->stream); });
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+// What both directions of the residual norm check; the launch's arguments but for the gradients.
+std::string residual_params(const adn_residual_norm_args *a, ResidualParams &p) {
+    std::string msg = check_sizes(a->rows, TRAIN_MAX_ROWS, a->d, 1, a->dtype);
+    if (!msg.empty()) return msg;
+    if (a->reserved) return "reserved must be 0";
+    if (a->gate_kind > ADN_GATE_ELEMENT) return "unknown gate_kind";
+    if ((a->gate_sigmoid | a->post_norm) & ~1) return "gate_sigmoid and post_norm are 0 or 1";
+    if (!(a->eps >= 0.0f)) return "eps must be >= 0";
+    const bool none = a->gate_kind == ADN_GATE_NONE, element = a->gate_kind == ADN_GATE_ELEMENT;
+    if (none && (a->gate || a->dgate || a->gate_sigmoid)) return "a gate (or its gradient) with ADN_GATE_NONE";
+    if (!a->post_norm && (a->post_gain || a->dpost_gain)) return "post_gain without post_norm";
+    if (!none && !element && !a->gate && (a->gate_kind == ADN_GATE_CHANNEL || a->rows > 0)) return "null gate";
+    msg = first_of({check_rows("f", a->f, a->f_stride, a->rows, a->d, a->dtype),
+                    element ? check_rows("gate", a->gate, a->gate_stride, a->rows, a->d, a->dtype) : check_words("gate", a->gate),
+                    check_words("post_gain", a->post_gain), check_words("pre_gain", a->pre_gain)});
+    if (!msg.empty()) return msg;
+    p.rows = a->rows, p.d = a->d, p.dtype = a->dtype, p.gate_kind = a->gate_kind;
+    p.sigmoid = a->gate_sigmoid, p.post = a->post_norm;
+    p.keep = a->keep, p.scale = a->scale, p.eps = a->eps;
+    p.f = a->f, p.f_stride = a->f_stride, p.gate = a->gate, p.gate_stride = a->gate_stride;
+    p.post_gain = a->post_gain, p.pre_gain = a->pre_gain;
+    p.z = a->z, p.z_stride = a->z_stride;
+    return "";
+}
+
+// What a list of tensors writes must not meet itself or what it reads.
+struct MemSpan {
+    uintptr_t begin, end;
+    bool written;
+};
+bool spans_meet(std::vector<MemSpan> &s) {
+    std::sort(s.begin(), s.end(), [](const MemSpan &a, const MemSpan &b) { return a.begin < b.begin; });
+    uintptr_t written = 0, any = 0;  // the furthest ends so far
+    for (const MemSpan &x : s) {
+        if (x.begin < written || (x.written && x.begin < any)) return true;
+        any = std::max(any, x.end);
+        if (x.written) written = std::max(written, x.end);
+    }
+    return false;
+}
+
+int check_optimizer(const adn_adamw *o) {
+    if (!o) return fail(ADN_E_INVALID, "null optimizer");
+    if (!o->ctx) return fail(ADN_E_INVALID, "the optimizer's context has been destroyed");
+    return ADN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int adn_residual_norm_async(adn_ctx *c, const adn_residual_norm_args *a) {
+    return train_entry([&]() -> int {
+        if (!c || !a) return fail(ADN_E_INVALID, "null argument");
+        ResidualParams p{};
+        std::string msg = residual_params(a, p);
+        if (msg.empty() && !a->z && !a->y) msg = "no output is wanted";
+        if (msg.empty())
+            msg = first_of({check_rows("x", a->x, a->x_stride, a->rows, a->d, a->dtype),
+                            a->z ? check_rows("z", a->z, a->z_stride, a->rows, a->d, a->dtype) : "",
+                            a->y ? check_rows("y", a->y, a->y_stride, a->rows, a->d, a->dtype) : "",
+                            a->z == a->x && a->z && a->z_stride != a->x_stride ? "z in x's place has another stride" : "",
+                            !a->y && a->pre_gain ? "pre_gain without y" : ""});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        p.x = a->x, p.x_stride = a->x_stride;
+        p.y = a->y, p.y_stride = a->y_stride;
+        return train_launch(c, 0, [&](void *) { launch_residual(p, c->stream); });
+    });
+}
+
+int adn_residual_norm_backward_async(adn_ctx *c, const adn_residual_norm_args *a) {
+    return train_entry([&]() -> int {
+        if (!c || !a) return fail(ADN_E_INVALID, "null argument");
+        ResidualParams p{};
+        std::string msg = residual_params(a, p);
+        const bool element = a->gate_kind == ADN_GATE_ELEMENT;
+        auto rows = [&](const char *what, const void *q, int64_t stride) {
+            return q ? check_rows(what, q, stride, a->rows, a->d, a->dtype) : std::string();
+        };
+        if (msg.empty() && !a->dx && !a->df && !a->dgate && !a->dpost_gain && !a->dpre_gain) msg = "no output is wanted";
+        if (msg.empty() && !a->dz && !a->dy && a->rows > 0) msg = "neither dz nor dy is there";
+        if (msg.empty())
+            msg = first_of({a->dy ? check_rows("z", a->z, a->z_stride, a->rows, a->d, a->dtype) : "",
+                            rows("dz", a->dz, a->dz_stride), rows("dy", a->dy, a->dy_stride), rows("dx", a->dx, a->dx_stride),
+                            rows("df", a->df, a->df_stride),
+                            element ? rows("dgate", a->dgate, a->dgate_stride) : check_words("dgate", a->dgate),
+                            check_words("dpost_gain", a->dpost_gain), check_words("dpre_gain", a->dpre_gain),
+                            a->dx == a->dz && a->dx && a->dx_stride != a->dz_stride ? "dx in dz's place has another stride" : "",
+                            !a->dy && a->rows > 0 && (a->pre_gain || a->dpre_gain) ? "pre_gain or its gradient without dy" : ""});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        p.dz = a->dz, p.dz_stride = a->dz_stride;
+        p.dy = a->dy, p.dy_stride = a->dy_stride;
+        p.dx = a->dx, p.dx_stride = a->dx_stride;
+        p.df = a->df, p.df_stride = a->df_stride;
+        p.dgate = a->dgate, p.dgate_stride = a->dgate_stride;
+        p.dpost = a->dpost_gain, p.dpre = a->dpre_gain;
+        return train_launch(c, residual_backward_workspace_bytes(p), [&](void *ws) { launch_residual_backward(p, ws, c->stream); });
+    });
+}
+
+int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors, const adn_adamw_tensor *tensors, adn_adamw **out) {
+    return train_entry([&]() -> int {
+        if (out) *out = nullptr;
+        if (!c || !cfg || !out || (n_tensors > 0 && !tensors)) return fail(ADN_E_INVALID, "null argument");
+        if (n_tensors < 0 || n_tensors > (1 << 24)) return fail(ADN_E_INVALID, "the number of tensors must be in [0, 2^24]");
+        const bool grads_alone = cfg->state_bits == 0, eight = cfg->state_bits == 8;
+        if (!grads_alone && !eight && cfg->state_bits != 32) return fail(ADN_E_INVALID, "state_bits must be 32, 8 or 0");
+        if (cfg->reserved) return fail(ADN_E_INVALID, "reserved must be 0");
+        if (!grads_alone) {
+            if (!(cfg->beta1 >= 0 && cfg->beta1 < 1 && cfg->beta2 >= 0 && cfg->beta2 < 1))
+                return fail(ADN_E_INVALID, "beta1 and beta2 must be in [0, 1)");
+            if (!(cfg->eps >= 1e-30 && cfg->eps <= 1e30)) return fail(ADN_E_INVALID, "eps must be in [1e-30, 1e30]");
+            if (!cfg->step || (uintptr_t)cfg->step % 4) return fail(ADN_E_INVALID, "step is null or not aligned to its elements");
+        }
+        std::vector<MemSpan> spans;
+        std::vector<OptTensor> recs((size_t)n_tensors);
+        int64_t total = 0, block = 0;
+        for (int64_t i = 0; i < n_tensors; ++i) {
+            const adn_adamw_tensor &t = tensors[i];
+            const std::string at = " of tensor " + std::to_string(i);
+            if (t.n < 0 || t.n > (1ll << 40)) return fail(ADN_E_INVALID, "n must be in [0, 2^40]" + at);
+            if (t.reserved) return fail(ADN_E_INVALID, "reserved must be 0" + at);
+            if (t.grad_dtype != ADN_T_F32 && t.grad_dtype != ADN_T_BF16) return fail(ADN_E_INVALID, "unknown grad_dtype" + at);
+            auto span = [&](const char *what, const void *p, int64_t bytes, int align, bool wanted, bool written) -> std::string {
+                if (wanted && t.n > 0 && !p) return std::string("null ") + what + at;
+                if (!wanted && p) return std::string(what) + at + " does not go with the list's state_bits";
+                if ((uintptr_t)p % align) return std::string(what) + at + " is not aligned to its elements";
+                if (p && bytes) spans.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
+                return "";
+            };
+            const int64_t blocks = (t.n + OPT_BLOCK - 1) / OPT_BLOCK;
+            const int sb = eight ? 1 : 4, gb = elem_bytes(t.grad_dtype);
+            std::string msg = first_of({span("grad", t.grad, t.n * gb, gb, true, false),
+                                        span("param", t.param, t.n * 4, 4, !grads_alone, true),
+                                        span("m", t.m, t.n * sb, sb, !grads_alone, true), span("v", t.v, t.n * sb, sb, !grads_alone, true),
+                                        span("m_scale", t.m_scale, blocks * 4, 4, eight, true),
+                                        span("v_scale", t.v_scale, blocks * 4, 4, eight, true),
+                                        t.copy || grads_alone ? span("copy", t.copy, t.n * 2, 2, !grads_alone, true) : ""});
+            if (msg.empty() && !grads_alone && !(std::isfinite(t.lr_scale) && std::isfinite(t.weight_decay)))
+                msg = "lr_scale and weight_decay must be finite" + at;
+            if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+            OptTensor &r = recs[(size_t)i];
+            r.param = t.param, r.grad = t.grad, r.copy = (__bf16 *)t.copy, r.m = t.m, r.v = t.v;
+            r.m_scale = t.m_scale, r.v_scale = t.v_scale;
+            r.n = t.n, r.block = block, r.lr_scale = t.lr_scale, r.decay = t.weight_decay;
+            r.grad_bf16 = t.grad_dtype == ADN_T_BF16;
+            total += t.n, block += blocks;
+        }
+        if (!grads_alone) spans.push_back({(uintptr_t)cfg->step, (uintptr_t)cfg->step + 4, true});
+        if (spans_meet(spans)) return fail(ADN_E_INVALID, "tensors that the step writes overlap each other or the gradients");
+        const int per = opt_chunk_values(total);
+        std::vector<OptChunk> chunks;
+        for (int64_t i = 0; i < n_tensors; ++i) {
+            const int64_t k = (recs[(size_t)i].n + per - 1) / per;
+            if ((int64_t)chunks.size() + k >= (1 << 24)) return fail(ADN_E_INVALID, "the list needs 2^24 workgroups or more");
+            for (int64_t j = 0; j < k; ++j) chunks.push_back({(int32_t)i, (int32_t)j});
+        }
+        DeviceScope scope(c->device);
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        ADN_HIP(hipStreamIsCapturing(c->stream, &cap));
+        if (cap != hipStreamCaptureStatusNone) return fail(ADN_E_CAPACITY, "an optimizer cannot be created under stream capture");
+        // one block: records, chunks, the step's scalars, the norm's partial sums and counter
+        auto place = [](size_t &at, size_t bytes) {
+            const size_t a = (at + 255) & ~(size_t)255;
+            at = a + bytes;
+            return a;
+        };
+        size_t bytes = 0;
+        const size_t at_recs = place(bytes, recs.size() * sizeof(OptTensor)), at_chunks = place(bytes, chunks.size() * sizeof(OptChunk));
+        const size_t at_scalars = place(bytes, sizeof(OptScalars)), at_partials = place(bytes, OPT_NORM_BLOCKS * sizeof(double));
+        const size_t at_ticket = place(bytes, sizeof(unsigned));
+        std::vector<char> host(bytes, 0);
+        if (!recs.empty()) memcpy(host.data() + at_recs, recs.data(), recs.size() * sizeof(OptTensor));
+        if (!chunks.empty()) memcpy(host.data() + at_chunks, chunks.data(), chunks.size() * sizeof(OptChunk));
+        auto opt = std::make_unique<adn_adamw>();
+        c->optimizers.reserve(c->optimizers.size() + 1);
+        char *dev = (char *)dmalloc(c, bytes);
+        ADN_HIP(hipMemcpyAsync(dev, host.data(), bytes, hipMemcpyHostToDevice, c->stream));
+        ADN_HIP(hipStreamSynchronize(c->stream));
+        OptPlan &p = opt->plan;
+        p.tensors = (const OptTensor *)(dev + at_recs), p.chunks = (const OptChunk *)(dev + at_chunks);
+        p.n_chunks = (int)chunks.size(), p.chunk_values = per, p.state_bits = (int)cfg->state_bits;
+        p.beta1 = cfg->beta1, p.beta2 = cfg->beta2, p.eps = (float)cfg->eps, p.seed = cfg->seed, p.step = cfg->step;
+        p.scalars = (OptScalars *)(dev + at_scalars), p.partials = (double *)(dev + at_partials), p.ticket = (unsigned *)(dev + at_ticket);
+        opt->ctx = c;
+        c->optimizers.push_back(opt.get());
+        *out = opt.release();
+        return ADN_OK;
+    });
+}
+
+void adn_adamw_destroy(adn_adamw *o) {
+    if (!o) return;
+    if (o->ctx) {
+        auto &v = o->ctx->optimizers;
+        v.erase(std::remove(v.begin(), v.end(), o), v.end());
+    }
+    delete o;
+}
+
+int adn_adamw_grad_norm_async(adn_adamw *o, float *norm) {
+    return train_entry([&]() -> int {
+        const int rc = check_optimizer(o);
+        if (rc != ADN_OK) return rc;
+        if (!norm || (uintptr_t)norm % 4) return fail(ADN_E_INVALID, "norm is null or not aligned to its elements");
+        return train_launch(o->ctx, 0, [&](void *) { launch_grad_norm(o->plan, norm, o->ctx->stream); });
+    });
+}
+
+int adn_adamw_step_async(adn_adamw *o, const adn_adamw_step *s) {
+    return train_entry([&]() -> int {
+        const int rc = check_optimizer(o);
+        if (rc != ADN_OK) return rc;
+        if (!s) return fail(ADN_E_INVALID, "null argument");
+        if (o->plan.state_bits == 0) return fail(ADN_E_INVALID, "the list holds gradients alone");
+        std::string msg = first_of({check_words("lr_device", s->lr_device), check_words("grad_norm", s->grad_norm),
+                                    s->lr_device || std::isfinite(s->lr) ? "" : "lr must be finite",
+                                    s->max_norm >= 0.0f && std::isfinite(s->max_norm) ? "" : "max_norm must be finite and >= 0",
+                                    s->max_norm > 0.0f && !s->grad_norm ? "max_norm without grad_norm" : "",
+                                    s->grad_scale > 0.0f && std::isfinite(s->grad_scale) ? "" : "grad_scale must be finite and > 0"});
+        if (!msg.empty()) return fail(ADN_E_INVALID, msg);
+        const OptStep step{s->lr, s->lr_device, s->grad_norm, s->max_norm, s->grad_scale};
+        return train_launch(o->ctx, 0, [&](void *) { launch_adamw(o->plan, step, o->ctx->stream); });
     });
 }
 

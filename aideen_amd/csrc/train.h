@@ -85,6 +85,73 @@ size_t norm_backward_workspace_bytes(const NormParams &p);
 void launch_norm(const NormParams &p, hipStream_t st);
 void launch_norm_backward(const NormParams &p, void *ws, hipStream_t st);
 
+// ---- norms around a residual block (residual.hip) -------------------------------------------
+struct ResidualParams {
+    int rows, d;
+    uint32_t dtype;
+    uint32_t gate_kind;      // ADN_GATE_*
+    bool sigmoid, post;      // the gate is given as logits; f is normed
+    float keep, scale, eps;
+    const void *x, *f, *gate;
+    long x_stride, f_stride, gate_stride;
+    const float *post_gain, *pre_gain;  // [d] or null = 1
+    void *z, *y;             // forward: y null: not wanted; backward: z is read
+    long z_stride, y_stride;
+    const void *dz, *dy;     // backward: one of them may be null = 0
+    long dz_stride, dy_stride;
+    void *dx, *df, *dgate;   // each null: not wanted
+    long dx_stride, df_stride, dgate_stride;
+    float *dpost, *dpre;
+};
+void launch_residual(const ResidualParams &p, hipStream_t st);
+size_t residual_backward_workspace_bytes(const ResidualParams &p);
+void launch_residual_backward(const ResidualParams &p, void *ws, hipStream_t st);
+
+// ---- AdamW over a list of tensors (optim.hip) ----------------------------------------------
+struct OptTensor {  // one tensor of the list
+    float *param;
+    const void *grad;
+    __bf16 *copy;            // or null
+    void *m, *v;             // fp32, or e4m3 codes
+    float *m_scale, *v_scale;
+    int64_t n;
+    int64_t block;           // the list's number of its first block of 256 values
+    float lr_scale, decay;
+    uint32_t grad_bf16;
+    uint32_t pad_;
+};
+struct OptChunk {  // a workgroup's share of a tensor
+    int32_t tensor, chunk;
+};
+struct OptScalars {  // what the step's first kernel leaves for the others
+    double coef;
+    uint64_t key;
+    float lr, inv_bc1, inv_sqrt_bc2;
+    int32_t skip;
+};
+struct OptPlan {  // the list as it stands on the device
+    const OptTensor *tensors;
+    const OptChunk *chunks;
+    int n_chunks, chunk_values, state_bits;
+    double beta1, beta2;
+    float eps;
+    uint64_t seed;
+    int32_t *step;
+    OptScalars *scalars;
+    double *partials;        // [OPT_NORM_BLOCKS]
+    unsigned *ticket;
+};
+struct OptStep {
+    double lr;
+    const float *lr_device, *grad_norm;  // or null
+    float max_norm, grad_scale;
+};
+constexpr int OPT_BLOCK = 256;         // values of an 8-bit state that share a scale
+constexpr int OPT_NORM_BLOCKS = 2048;  // most workgroups of the norm
+int opt_chunk_values(int64_t total);
+void launch_grad_norm(const OptPlan &p, float *norm, hipStream_t st);
+void launch_adamw(const OptPlan &p, const OptStep &s, hipStream_t st);
+
 // ---- embedding table (table.hip) -----------------------------------------------------------
 struct TableParams {
     int n, d, vocab;

@@ -1,0 +1,173 @@
+"""AdamW over a list of tensors, and the norm of the list's gradients, over the C ABI (``adn_adamw_*``).
+
+The reference's trainers step their weights by AdamW (``gpu_lm_head.rs``, ``gpu_embedding.rs:496-670``);
+here one launch serves the whole list, with moments in fp32 or in 8 bits.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib
+from ._lib import check, lib
+
+_TORCH = {}
+
+
+def _torch():
+    """torch, and the types that are met here, looked up once."""
+    if not _TORCH:
+        import torch
+        _TORCH.update(torch=torch, f32=torch.float32, bf16=torch.bfloat16, i32=torch.int32, codes=(torch.float8_e4m3fn, torch.uint8))
+    return _TORCH
+
+
+def _invalid(msg: str) -> "_lib.AdnError":
+    return _lib.AdnError(_lib.ADN_E_INVALID, msg)
+
+
+class AdamW:
+    """The optimizer of lists of tensors: ``params`` (float32), their ``grads`` (float32 or bfloat16, each as
+    it is), each contiguous, of any sizes, on the context's GPU, two of a place in the lists of as many values.
+
+    ``m`` and ``v`` are lists of float32 tensors, or (states of 8 bits) of float8_e4m3fn or uint8 ones, with
+    ``m_scale`` and ``v_scale``, float32 [ceil(n / 256)] each; ``step`` is an int32 tensor of one value, the steps done.
+    They are the caller's to save and restore.  None of them given: new ones, of ``state_bits``, kept as the
+    attributes of those names.  ``copies``: bfloat16 tensors (or None in a place) that receive the new parameters.
+    ``weight_decay`` and ``lr_scale`` are numbers, or lists with one a tensor.  ``params`` None: a list of
+    gradients alone, for ``grad_norm_async``.
+
+    A handle keeps its tensors, and must not outlive what its context's graphs need of them.  Calls only enqueue on
+    the context's stream; the caller orders it with the streams that fill and read the tensors."""
+
+    def __init__(self, backend, params, grads, *, m=None, v=None, m_scale=None, v_scale=None, step=None, copies=None,
+                 state_bits: int = 32, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0, seed: int = 0):
+        self._opt = C.c_void_p()
+        self._backend = backend
+        self._device = backend.device
+        T = _torch()
+        grads = list(grads)
+        k = len(grads)
+        alone = params is None
+        if alone and any(x is not None for x in (m, v, m_scale, v_scale, step, copies)):
+            raise _invalid("a list of gradients alone has no states and no copies")
+        params = [None] * k if alone else list(params)
+        given = [x is not None for x in (m, v, step)]
+        if not alone and any(given) and not all(given):
+            raise _invalid("m, v and step go together")
+        if len(params) != k:
+            raise _invalid(f"as many grads as params expected ({len(params)}), got {k}")
+        for i, (p, g) in enumerate(zip(params, grads)):
+            self._check(g, f"grads[{i}]", (T["f32"], T["bf16"]), None)
+            if not alone:
+                self._check(p, f"params[{i}]", (T["f32"],), g.numel())
+        if not alone and not any(given):
+            if m_scale is not None or v_scale is not None:
+                raise _invalid("scales without states")
+            m, v, m_scale, v_scale, step = self._new_state(params, state_bits)
+        eight = False
+        if not alone:
+            m, v = list(m), list(v)
+            eight = k > 0 and len(m) > 0 and m[0].dtype in T["codes"] or m_scale is not None
+            if eight != (m_scale is not None) or eight != (v_scale is not None):
+                raise _invalid("m_scale and v_scale go with states of 8 bits")
+            m_scale, v_scale = (list(m_scale), list(v_scale)) if eight else ([None] * k, [None] * k)
+            copies = [None] * k if copies is None else list(copies)
+            for name, x in (("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale), ("copies", copies)):
+                if len(x) != k:
+                    raise _invalid(f"{name} must have {k} entries, got {len(x)}")
+            self._check(step, "step", (T["i32"],), 1)
+        decay, scale = self._numbers(weight_decay, "weight_decay", k), self._numbers(lr_scale, "lr_scale", k)
+        recs = (_lib.AdnAdamwTensor * max(k, 1))()
+        kinds = T["codes"] if eight else (T["f32"],)
+        for i, (p, g) in enumerate(zip(params, grads)):
+            r, n = recs[i], g.numel()
+            r.grad, r.n, r.grad_dtype = g.data_ptr(), n, _lib.ADN_T_F32 if g.dtype == T["f32"] else _lib.ADN_T_BF16
+            if alone:
+                continue
+            self._check(m[i], f"m[{i}]", kinds, n), self._check(v[i], f"v[{i}]", kinds, n)
+            r.param, r.m, r.v, r.lr_scale, r.weight_decay = p.data_ptr(), m[i].data_ptr(), v[i].data_ptr(), scale[i], decay[i]
+            if eight:
+                blocks = -(-n // _lib.ADAMW_BLOCK)
+                self._check(m_scale[i], f"m_scale[{i}]", (T["f32"],), blocks)
+                self._check(v_scale[i], f"v_scale[{i}]", (T["f32"],), blocks)
+                r.m_scale, r.v_scale = m_scale[i].data_ptr(), v_scale[i].data_ptr()
+            if copies[i] is not None:
+                self._check(copies[i], f"copies[{i}]", (T["bf16"],), n)
+                r.copy = copies[i].data_ptr()
+        if not 0 <= int(seed) < 1 << 64:
+            raise _invalid("seed must be in [0, 2^64)")
+        cfg = _lib.AdnAdamwConfig(beta1=betas[0], beta2=betas[1], eps=eps, seed=int(seed), state_bits=0 if alone else 8 if eight else 32)
+        cfg.step = None if alone else step.data_ptr()
+        check(lib().adn_adamw_create(backend._ctx, C.byref(cfg), k, recs, C.byref(self._opt)))
+        self.params, self.grads, self.copies = params, grads, copies
+        self.m, self.v, self.m_scale, self.v_scale, self.step = m, v, m_scale, v_scale, step
+
+    def _check(self, t, name, dtypes, n) -> None:
+        if t.dtype not in dtypes or not t.is_contiguous() or (n is not None and t.numel() != n):
+            kinds = " or ".join(str(d) for d in dtypes)
+            raise _invalid(f"{name} must be a contiguous {kinds} tensor" + ("" if n is None else f" of {n} values"))
+        if t.get_device() != self._device:
+            raise _invalid(f"{name} must be on the context's GPU (cuda:{self._device}), got {t.device}")
+
+    @staticmethod
+    def _numbers(x, name, k):
+        if isinstance(x, (int, float)):
+            return [float(x)] * k
+        x = [float(v) for v in x]
+        if len(x) != k:
+            raise _invalid(f"{name} must be a number or {k} of them, got {len(x)}")
+        return x
+
+    def _new_state(self, params, state_bits):
+        if state_bits not in (32, 8):
+            raise _invalid("state_bits must be 32 or 8")
+        T = _torch()
+        torch, dev = T["torch"], f"cuda:{self._device}"
+        eight = state_bits == 8
+
+        def zeros(size):
+            return [torch.zeros(size(p), device=dev, dtype=T["f32"]) for p in params]
+
+        def codes():
+            return [torch.zeros(p.shape, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn) for p in params]
+        blocks = lambda p: -(-p.numel() // _lib.ADAMW_BLOCK)  # noqa: E731
+        m, v = (codes(), codes()) if eight else (zeros(lambda p: p.shape), zeros(lambda p: p.shape))
+        ms, vs = (zeros(blocks), zeros(blocks)) if eight else (None, None)
+        step = torch.zeros(1, device=dev, dtype=T["i32"])
+        torch.cuda.current_stream(self._device).synchronize()  # the context's stream is another one
+        return m, v, ms, vs, step
+
+    def grad_norm_async(self, norm) -> None:
+        """norm [1] float32 = the square root of the sum of the squares of all gradients, summed in 64 bits."""
+        if not self._opt:
+            raise _invalid("the optimizer is closed")
+        check(lib().adn_adamw_grad_norm_async(self._opt, self._backend._vector(norm, "norm", 1)))
+
+    def step_async(self, *, lr=None, grad_norm=None, max_norm: float = 0.0, grad_scale: float = 1.0) -> None:
+        """One step.  lr: a number, or a float32 tensor of one value that the step reads when it runs (a captured
+        step's rate).  grad_norm: ``grad_norm_async``'s result; the step is skipped as a whole where it is not
+        finite, and with max_norm > 0 the gradients are scaled so that their norm is at most max_norm.
+        grad_scale is a factor of every gradient (and so of the norm)."""
+        if not self._opt:
+            raise _invalid("the optimizer is closed")
+        s = _lib.AdnAdamwStep(max_norm=max_norm, grad_scale=grad_scale)
+        vector = self._backend._vector
+        if lr is None:
+            raise _invalid("lr must be a number or a tensor of one value")
+        if isinstance(lr, (int, float)):
+            s.lr = lr
+        else:
+            s.lr_device = vector(lr, "lr", 1)
+        s.grad_norm = vector(grad_norm, "grad_norm", 1)
+        check(lib().adn_adamw_step_async(self._opt, C.byref(s)))
+
+    def close(self) -> None:
+        if self._opt:
+            lib().adn_adamw_destroy(self._opt)
+            self._opt = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

@@ -365,6 +365,115 @@ int adn_rms_norm_backward_async(adn_ctx *ctx, int32_t rows, int32_t d, uint32_t 
                                 int64_t x_stride, const float *gain, float eps, const void *dy, int64_t dy_stride,
                                 void *dx, int64_t dx_stride, float *dg);
 
+/* The norms around a residual block, per row of d elements (rows in [0, 2^24], d in [1, 8192]):
+ *   n = f rf post_gain, rf = 1 / sqrt(mean(f^2) + eps)    (post_norm 0: n = f)
+ *   z = keep x + scale s n                                (s: the gate; gate_sigmoid: the sigmoid of it)
+ *   y = z rz pre_gain,  rz = 1 / sqrt(mean(z^2) + eps)    (the next block's or the head's norm)
+ * With post_norm, keep = 1 - damping and scale = damping this is the damped update of the Picard
+ * iteration (fixed_point_memory_reasoning.rs:1300-1303).  y is formed from z before it is rounded.
+ * Forward reads x, f, the gate and the gains and writes z and/or y.  Backward reads f, the gate, the
+ * gains, the gradients dz (of z by other ways) and/or dy, and, where dy is there, z as the forward
+ * wrote it, and writes any of
+ *   dx = keep D, D = dz + rz (a - z rz^2 mean(a z)), a = dy pre_gain
+ *   df = rf (b - f rf^2 mean(b f)), b = scale s D post_gain   (post_norm 0: b)
+ *   dgate = scale D n (gate_sigmoid: times s (1 - s)), summed over the rows or the row as the gate is shared
+ *   dpost_gain = sum over the rows of scale s D f rf,  dpre_gain = sum over the rows of dy z rz   (fp32)
+ * z may be x itself, and dx dz (the same pointer and stride); nothing else may overlap.  y, dz, dy and
+ * the outputs are each NULL where not wanted or not there. */
+#define ADN_GATE_NONE 0u
+#define ADN_GATE_CHANNEL 1u /* gate, dgate: [d] fp32                                      */
+#define ADN_GATE_ROW 2u     /* gate, dgate: [rows] fp32                                   */
+#define ADN_GATE_ELEMENT 3u /* gate, dgate: [rows] rows of d of dtype, at their strides   */
+typedef struct adn_residual_norm_args {
+    int32_t rows, d;
+    uint32_t dtype;               /* ADN_T_*: x, f, z, y, dz, dy, dx, df, an element gate */
+    uint32_t gate_kind;           /* ADN_GATE_*                                           */
+    int32_t gate_sigmoid;         /* 1: the gate is given as logits                       */
+    int32_t post_norm;            /* 1: f is normed                                       */
+    float keep, scale, eps;
+    uint32_t reserved;            /* 0                                                    */
+    const void *x;
+    int64_t x_stride;
+    const void *f;
+    int64_t f_stride;
+    const float *post_gain;       /* [d], NULL = 1                                        */
+    const void *gate;
+    int64_t gate_stride;          /* ADN_GATE_ELEMENT                                     */
+    const float *pre_gain;        /* [d], NULL = 1                                        */
+    void *z;                      /* backward: read                                       */
+    int64_t z_stride;
+    void *y;
+    int64_t y_stride;
+    const void *dz;               /* from here on backward                                */
+    int64_t dz_stride;
+    const void *dy;
+    int64_t dy_stride;
+    void *dx;
+    int64_t dx_stride;
+    void *df;
+    int64_t df_stride;
+    void *dgate;
+    int64_t dgate_stride;
+    float *dpost_gain, *dpre_gain; /* [d]                                                 */
+} adn_residual_norm_args;
+int adn_residual_norm_async(adn_ctx *ctx, const adn_residual_norm_args *args);
+int adn_residual_norm_backward_async(adn_ctx *ctx, const adn_residual_norm_args *args);
+
+/* AdamW over a list of tensors (the reference's trainers step the head, the embedding and the block by
+ * AdamW, gpu_lm_head.rs, gpu_embedding.rs:496-670).  One step, t = *step + 1:
+ *   g = coef grad,  coef = grad_scale min(1, max_norm / (grad_norm grad_scale + 1e-6))
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   param -= lr lr_scale (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay param)
+ *   copy = param in bf16 (for the products that read the weights so),  *step = t
+ * Everything that changes from step to step is read on the device (the counter, lr_device, grad_norm),
+ * so that a captured step can be replayed.  A grad_norm that is not finite skips the step as a whole:
+ * nothing is written, the counter stays.
+ * States of 32 bits are fp32.  States of 8 bits are e4m3 codes (OCP; v's without a sign) times a scale of
+ * each 256 consecutive values of a tensor, a power of two 2^(E - 7), E the exponent of the largest
+ * magnitude (at least -110): 2 bytes a parameter in the place of 8.  Their moments are formed in 64 bits,
+ * used by the step as they are, and rounded to codes stochastically, by 16 random bits a value that are
+ * a hash of seed, *step, the value's place in the list (blocks of 256, counted from the first tensor's)
+ * and in its block; a v that is not zero keeps a code that is not.  A block whose m or v would hold a value
+ * beyond fp32 or a NaN gets a scale that is not a number.  A new state is zeros: codes, scales and
+ * counter.  Equal states, gradients and lists give equal bits.
+ * The list is laid out on the device when it is created (which blocks), and stays until the context is
+ * destroyed, as captured graphs may use it.  Sizes: up to 2^24 tensors and workgroups, n >= 0 any, any
+ * alignment of whole elements.  What a list writes must not overlap itself or its gradients; that is
+ * checked.  A handle belongs to its context and stream; after adn_destroy only adn_adamw_destroy takes it. */
+typedef struct adn_adamw adn_adamw;
+typedef struct adn_adamw_tensor {
+    float *param;               /* [n]                                                   */
+    const void *grad;           /* [n] of grad_dtype                                     */
+    void *copy;                 /* [n] bf16, NULL: not wanted                            */
+    void *m, *v;                /* [n] fp32, or codes                                    */
+    float *m_scale, *v_scale;   /* [ceil(n / 256)] with 8-bit states, else NULL          */
+    int64_t n;
+    float lr_scale, weight_decay;
+    uint32_t grad_dtype;        /* ADN_T_*                                               */
+    uint32_t reserved;          /* 0                                                     */
+} adn_adamw_tensor;
+typedef struct adn_adamw_config {
+    double beta1, beta2;        /* [0, 1)                                                */
+    double eps;                 /* at least 1e-30                                        */
+    uint64_t seed;              /* of the rounding of 8-bit states                       */
+    int32_t *step;              /* [1] device: steps done                                */
+    uint32_t state_bits;        /* 32 or 8; 0: gradients alone (param, m, v, step NULL)  */
+    uint32_t reserved;          /* 0                                                     */
+} adn_adamw_config;
+typedef struct adn_adamw_step {
+    double lr;
+    const float *lr_device;     /* [1] device: in the place of lr, or NULL               */
+    const float *grad_norm;     /* [1] device: adn_adamw_grad_norm_async's, or NULL      */
+    float max_norm;             /* 0: no clipping; > 0 goes with grad_norm               */
+    float grad_scale;           /* a factor of every gradient, 1 / the loss's scale      */
+} adn_adamw_step;
+int adn_adamw_create(adn_ctx *ctx, const adn_adamw_config *config, int64_t n_tensors, const adn_adamw_tensor *tensors,
+                     adn_adamw **out);
+void adn_adamw_destroy(adn_adamw *opt);
+/* *norm (device) = sqrt(the sum of the squares of all gradients of the list), summed in 64 bits. */
+int adn_adamw_grad_norm_async(adn_adamw *opt, float *norm);
+int adn_adamw_step_async(adn_adamw *opt, const adn_adamw_step *step);
+
 /* out_i = scale * table[tokens_i], i < n (n in [0, 2^24], vocab in [1, 2^24], d in [1, 8192]); rows
  * without a token are 0.  table NULL: the context's embedding (then d = d_r, its vocab, ADN_T_F32).
  * The gradient writes the whole table: dtable[v] = scale * the sum of the dout_i with tokens_i = v
