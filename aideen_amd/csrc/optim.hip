@@ -30,9 +30,6 @@ constexpr int NB = 256;          // threads a block
 constexpr int V = 4;             // values a lane
 constexpr int MIN_EXPONENT = -110;  // of a block: the smallest code times its scale is a normal fp32 number
 
-typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32_any __attribute__((aligned(1)));
 
 // SplitMix64's finaliser (Steele, Lea, Flood 2014)
 __device__ __forceinline__ uint64_t mix64(uint64_t x) {
@@ -50,77 +47,13 @@ __device__ __forceinline__ uint32_t mix32(uint32_t a, uint32_t i) {
     return r ^ (r >> 16);
 }
 
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
-    return v;
-}
-
-// The e4m3 code (without its sign) of a magnitude whose high word is `hi`, in a block of exponent E:
-// `r` in [0, 2^17) is added below the code's last bit before the rest is cut off.
-__device__ __forceinline__ uint32_t code_of(uint32_t hi, int E, uint32_t r) {
-    const int k = (int)hi - ((1023 + E - 14) << 20);  // exponent with e4m3's bias, and 20 bits of mantissa
-    const int below = 1 - (k >> 20);                  // binades below the smallest normal code
-    const uint32_t sub = ((hi & 0xFFFFF) | 0x100000) >> min(below, 31);
-    return ((below > 0 ? sub : (uint32_t)k) + r) >> 17;
-}
-
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, int n, float (&v)[V]) {
-    if (n >= V) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(p);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = x[j];
-        } else {
-            const bf16x4 x = *reinterpret_cast<const bf16x4 *>(p);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = (float)x[j];
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void store4(T *p, int n, const float (&v)[V]) {
-    if (n >= V) {
-        if constexpr (sizeof(T) == 4) {
-            f32x4 x;
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = v[j];
-            *reinterpret_cast<f32x4 *>(p) = x;
-        } else {
-            bf16x4 x;
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = (__bf16)v[j];
-            *reinterpret_cast<bf16x4 *>(p) = x;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < n) p[j] = (T)v[j];
-    }
-}
-
-__device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int n) {
-    if (n >= V) return *reinterpret_cast<const u32_any *>(p);
-    uint32_t w = 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (j < n) w |= (uint32_t)p[j] << (8 * j);
-    return w;
-}
-
-__device__ __forceinline__ void store_codes(uint8_t *p, int n, uint32_t w) {
-    if (n >= V) {
-        *reinterpret_cast<u32_any *>(p) = w;
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (j < n) p[j] = (uint8_t)(w >> (8 * j));
+// The e4m3 code (without its sign) of the magnitude x, whose high word is `hi`, in a block of exponent E:
+// `r` in [0, 2^17) is added below the code's last bit before the rest is cut off.  The high word of a
+// normal code holds it behind a change of bias; below those, x to_steps (2^(33-E)) counts 2^-17 of a step.
+__device__ __forceinline__ uint32_t code_of(double x, uint32_t hi, int E, double to_steps, uint32_t r) {
+    const int k = (int)hi - ((1023 + E - 14) << 20);
+    const uint32_t below = (uint32_t)fmin(fabs(x) * to_steps, 0x1p20);
+    return ((k < 1 << 20 ? below : (uint32_t)k) + r) >> 17;
 }
 
 __device__ __forceinline__ void decode4(uint32_t w, float scale, float (&v)[V]) {
@@ -139,142 +72,306 @@ __device__ __forceinline__ double moment(double b, double old, double g, double 
     return kept + more;
 }
 
-// The step's scalars, one thread: the counter, the bias corrections, the clipping coefficient.
-__global__ void k_adamw_begin(OptPlan p, OptStep s) {
-    OptScalars o;
-    const float norm = s.grad_norm ? *s.grad_norm : 0.0f;
+struct Scalars {
+    double coef;
+    uint64_t key;
+    float lr, inv_bc1, inv_sqrt_bc2;
+    int t;
+    bool skip;
+};
+
+// What a step takes from the device: the counter, the bias corrections, the clipping coefficient.
+__device__ __forceinline__ Scalars scalars(const OptPlan &P, const OptStep &S) {
+    Scalars o;
+    const float norm = S.grad_norm ? *S.grad_norm : 0.0f;
+    const int done = max(*P.step, 0);
+    asm volatile("" ::"s"(done));  // it has arrived: the workgroup may say that it has read the counter
     o.skip = !(fabsf(norm) < INFINITY);
-    const int done = max(*p.step, 0), t = done < INT32_MAX ? done + 1 : done;
-    o.coef = (double)s.grad_scale;
-    if (s.max_norm > 0.0f) o.coef *= fmin(1.0, (double)s.max_norm / ((double)norm * (double)s.grad_scale + 1e-6));
-    o.lr = (float)(s.lr_device ? (double)*s.lr_device : s.lr);
-    o.inv_bc1 = (float)(1.0 / (1.0 - pow(p.beta1, (double)t)));
-    o.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(p.beta2, (double)t)));
-    o.key = mix64(p.seed + (uint64_t)(int64_t)(t - 1) * GOLDEN);
-    *p.scalars = o;
-    if (!o.skip) *p.step = t;
+    o.t = done < INT32_MAX ? done + 1 : done;
+    o.coef = (double)S.grad_scale;
+    if (S.max_norm > 0.0f) o.coef *= fmin(1.0, (double)S.max_norm / ((double)norm * (double)S.grad_scale + 1e-6));
+    o.lr = (float)(S.lr_device ? (double)*S.lr_device : S.lr);
+    // 1 - b^t = -expm1(t log b), as exact in fp32 as its argument
+    o.inv_bc1 = -__builtin_amdgcn_rcpf(expm1f((float)(o.t * P.log_beta1)));
+    o.inv_sqrt_bc2 = __builtin_amdgcn_rsqf(-expm1f((float)(o.t * P.log_beta2)));
+    o.key = mix64(P.seed + (uint64_t)(int64_t)(o.t - 1) * GOLDEN);
+    return o;
 }
 
-// p - lr (m / bc1 / (sqrt(v / bc2) + eps) + decay p)
-__device__ __forceinline__ float stepped(float p, float m, float v, const OptScalars &o, float lr, float decay, float eps) {
-    const float away = m * o.inv_bc1 / (sqrtf(v) * o.inv_sqrt_bc2 + eps);
-    return p - lr * (away + decay * p);
+// True in the last workgroup of the grid that comes here (one thread of each calls it).  One address
+// takes a read-modify-write in about 10 ns from the whole chip (512 workgroups at one: 5 us), so a
+// group of the workgroups counts at a place of its own and its last one at a common place.
+__device__ __forceinline__ bool last_of_grid(unsigned *ticket) {
+    const unsigned group = blockIdx.x % OPT_TICKETS, groups = min((unsigned)OPT_TICKETS, gridDim.x);
+    const unsigned members = (gridDim.x - group + OPT_TICKETS - 1) / OPT_TICKETS;
+    unsigned *mine = ticket + (1 + group) * OPT_TICKET_PITCH;
+    if (__hip_atomic_fetch_add(mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != members - 1) return false;
+    __hip_atomic_store(mine, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != groups - 1) return false;
+    __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
 }
 
-template <bool EIGHT>
-__global__ __launch_bounds__(NB) void k_adamw(OptPlan P) {
-    const OptScalars o = *P.scalars;
-    if (o.skip) return;
-    const OptChunk ck = P.chunks[blockIdx.x];
-    const OptTensor t = P.tensors[ck.tensor];
-    const int lane = threadIdx.x & 63;
-    const int64_t begin = (int64_t)ck.chunk * P.chunk_values;
-    const int64_t end = min(begin + P.chunk_values, t.n);
-    const float lr = o.lr * t.lr_scale;
-    for (int64_t b = begin + (threadIdx.x >> 6) * OPT_BLOCK; b < end; b += (NB / 64) * OPT_BLOCK) {
-        const int64_t i = b + lane * V;
-        const int n = (int)min<int64_t>(max<int64_t>(t.n - i, 0), V);  // this lane's values
-        float p[V], g[V], m[V], v[V];
-        load4(t.param + i, n, p);
-        if (t.grad_bf16)
-            load4((const __bf16 *)t.grad + i, n, g);
-        else
-            load4((const float *)t.grad + i, n, g);
+// p - lr (m / bc1 / (sqrt(v / bc2) + eps) + decay p), the root and the reciprocal to 1 ulp.  The root
+// instruction takes numbers below 2^-126 for zero, which is nothing beside an eps of 1e-10 or more.
+__device__ __forceinline__ void stepped(float (&p)[V], const float (&m)[V], const float (&v)[V], const Scalars &o, float lr,
+                                        float decay, float eps) {
+    float root[V];
+    if (eps >= 1e-10f) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) root[j] = __builtin_amdgcn_sqrtf(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) root[j] = sqrtf(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float away = m[j] * o.inv_bc1 * __builtin_amdgcn_rcpf(root[j] * o.inv_sqrt_bc2 + eps);
+        p[j] -= lr * (away + decay * p[j]);
+    }
+}
+
+// The largest of the wave's values, the same in every lane and known to be so.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#define ADN_DPP_MAX(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, true))
+    ADN_DPP_MAX(0x111, 0xF);  // from the lane one, two, four, eight to the left in a row of 16
+    ADN_DPP_MAX(0x112, 0xF);
+    ADN_DPP_MAX(0x114, 0xF);
+    ADN_DPP_MAX(0x118, 0xF);
+    ADN_DPP_MAX(0x142, 0xA);  // a row's last lane to the next row, then to the upper half
+    ADN_DPP_MAX(0x143, 0xC);
+#undef ADN_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// A pointer that is known to be to global memory (one that was loaded from a record is not).
+template <typename T>
+using global_ptr = __attribute__((address_space(1))) T *;
+
+// A lane's four values (or the n that there are) as they are loaded.
+template <typename T, bool FULL, bool NT>
+struct Four {
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    vec x;
+    __device__ __forceinline__ void load(const T *p, int n) {
+        if constexpr (FULL && NT) {
+            x = __builtin_nontemporal_load((global_ptr<const vec>)p);
+        } else if constexpr (FULL) {
+            x = *(global_ptr<const vec>)p;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = j < n ? p[j] : (T)0;
+        }
+    }
+    __device__ __forceinline__ void store(T *p, int n) const {
+        if constexpr (FULL && NT) {
+            __builtin_nontemporal_store(x, (global_ptr<vec>)p);
+        } else if constexpr (FULL) {
+            *(global_ptr<vec>)p = x;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j < n) p[j] = x[j];
+        }
+    }
+};
+
+// A block of 256 values of a tensor (or what the tensor has left), loaded ahead and stepped.
+template <bool EIGHT, bool BF16, bool FULL, bool NT>
+struct Block {
+    typedef std::conditional_t<EIGHT, uint8_t, float> S;
+    typedef std::conditional_t<BF16, __bf16, float> G;
+    Four<float, FULL, NT> p;
+    Four<G, FULL, NT> g;
+    Four<S, FULL, NT> m, v;
+    float ms, vs;
+
+    __device__ __forceinline__ int count(const OptTensor &t, int64_t blk, int lane) const {
+        return FULL ? V : (int)min<int64_t>(max<int64_t>(t.n - blk * OPT_BLOCK - lane * V, 0), V);
+    }
+
+    __device__ __forceinline__ void load(const OptTensor &t, int64_t blk, int lane) {
+        const int64_t i = blk * OPT_BLOCK + lane * V;
+        const int n = count(t, blk, lane);
+        g.load((const G *)t.grad + i, n);
+        m.load((const S *)t.m + i, n);
+        v.load((const S *)t.v + i, n);
+        p.load(t.param + i, n);
+        if constexpr (EIGHT) ms = ((global_ptr<const float>)t.m_scale)[blk], vs = ((global_ptr<const float>)t.v_scale)[blk];
+    }
+
+    __device__ __forceinline__ void step(const OptPlan &P, const OptTensor &t, const Scalars &o, float lr, int64_t blk, int lane) {
+        const int64_t i = blk * OPT_BLOCK + lane * V;
+        const int n = count(t, blk, lane);
+        float mf[V], vf[V];
         if constexpr (EIGHT) {
-            uint8_t *m8 = (uint8_t *)t.m + i, *v8 = (uint8_t *)t.v + i;
-            const int64_t blk = b / OPT_BLOCK;
-            decode4(load_codes(m8, n), t.m_scale[blk], m);
-            decode4(load_codes(v8, n), t.v_scale[blk], v);
+            decode4(__builtin_bit_cast(uint32_t, m.x), ms, mf);
+            decode4(__builtin_bit_cast(uint32_t, v.x), vs, vf);
             double md[V], vd[V];
             uint32_t mtop = 0, vtop = 0;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const double gd = (double)g[j] * o.coef;
-                md[j] = moment(P.beta1, m[j], gd, 1.0);
-                vd[j] = moment(P.beta2, v[j], gd, gd);
-                if (j >= n) md[j] = vd[j] = 0.0;
+                const double gd = (double)(float)g.x[j] * o.coef;
+                md[j] = moment(P.beta1, mf[j], gd, 1.0);
+                vd[j] = moment(P.beta2, vf[j], gd, gd);
+                if (!FULL && j >= n) md[j] = vd[j] = 0.0;
                 mtop = max(mtop, (uint32_t)__double2hiint(md[j]) & 0x7FFFFFFFu);
                 vtop = max(vtop, (uint32_t)__double2hiint(vd[j]) & 0x7FFFFFFFu);
             }
             mtop = wave_max_u32(mtop), vtop = wave_max_u32(vtop);
             const int me = max((int)(mtop >> 20) - 1023, MIN_EXPONENT), ve = max((int)(vtop >> 20) - 1023, MIN_EXPONENT);
             const uint32_t a = (uint32_t)mix64(o.key + (uint64_t)(t.block + blk + 1) * GOLDEN);
+            const double m_steps = __hiloint2double((1023 + 33 - me) << 20, 0), v_steps = __hiloint2double((1023 + 33 - ve) << 20, 0);
             uint32_t mw = 0, vw = 0;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const uint32_t r = mix32(a, lane * V + j);
                 const uint32_t mh = (uint32_t)__double2hiint(md[j]), vh = (uint32_t)__double2hiint(vd[j]);
-                const uint32_t mc = code_of(mh & 0x7FFFFFFFu, me, (r & 0xFFFFu) << 1) | (mh >> 24 & 0x80u);
-                uint32_t vc = code_of(vh & 0x7FFFFFFFu, ve, (r >> 16) << 1);
-                if (vc == 0 && vd[j] > 0.0) vc = 1;
+                const uint32_t mc = code_of(md[j], mh & 0x7FFFFFFFu, me, m_steps, (r & 0xFFFFu) << 1) | (mh >> 24 & 0x80u);
+                const uint32_t vc = max(code_of(vd[j], vh, ve, v_steps, (r >> 16) << 1), min(vh, 1u));
                 mw |= mc << (8 * j), vw |= vc << (8 * j);
-                m[j] = (float)md[j], v[j] = (float)vd[j];
+                mf[j] = (float)md[j], vf[j] = (float)vd[j];
             }
             // a block that holds a value beyond fp32, an infinity or a NaN is not a number as a whole
             const bool mbad = me > 127, vbad = ve > 127;
-            store_codes(m8, n, mbad ? 0 : mw);
-            store_codes(v8, n, vbad ? 0 : vw);
+            typedef typename Four<S, FULL, NT>::vec codes;
+            m.x = __builtin_bit_cast(codes, mbad ? 0 : mw), v.x = __builtin_bit_cast(codes, vbad ? 0 : vw);
             if (lane == 0) {
-                t.m_scale[blk] = mbad ? NAN : __uint_as_float((uint32_t)(me - 7 + 127) << 23);
-                t.v_scale[blk] = vbad ? NAN : __uint_as_float((uint32_t)(ve - 7 + 127) << 23);
+                ((global_ptr<float>)t.m_scale)[blk] = mbad ? NAN : __uint_as_float((uint32_t)(me - 7 + 127) << 23);
+                ((global_ptr<float>)t.v_scale)[blk] = vbad ? NAN : __uint_as_float((uint32_t)(ve - 7 + 127) << 23);
             }
         } else {
             const float b1 = (float)P.beta1, c1 = (float)(1.0 - P.beta1), b2 = (float)P.beta2, c2 = (float)(1.0 - P.beta2);
             const float coef = (float)o.coef;
-            load4((const float *)t.m + i, n, m);
-            load4((const float *)t.v + i, n, v);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float gj = g[j] * coef;
-                m[j] = b1 * m[j] + c1 * gj;
-                v[j] = b2 * v[j] + c2 * gj * gj;
+                const float gj = (float)g.x[j] * coef;
+                m.x[j] = mf[j] = b1 * m.x[j] + c1 * gj;
+                v.x[j] = vf[j] = b2 * v.x[j] + c2 * gj * gj;
             }
-            store4((float *)t.m + i, n, m);
-            store4((float *)t.v + i, n, v);
         }
+        m.store((S *)t.m + i, n);
+        v.store((S *)t.v + i, n);
+        float pf[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = stepped(p[j], m[j], v[j], o, lr, t.decay, P.eps);
-        store4(t.param + i, n, p);
-        if (t.copy) store4(t.copy + i, n, p);
+        for (int j = 0; j < V; ++j) pf[j] = p.x[j];
+        stepped(pf, mf, vf, o, lr, t.decay, P.eps);
+#pragma unroll
+        for (int j = 0; j < V; ++j) p.x[j] = pf[j];
+        p.store(t.param + i, n);
+        if (t.copy) {
+            Four<__bf16, FULL, NT> c;
+#pragma unroll
+            for (int j = 0; j < V; ++j) c.x[j] = (__bf16)p.x[j];
+            c.store(t.copy + i, n);
+        }
+    }
+};
+
+// A workgroup's chunk: its waves take the chunk's blocks in turn.  The first is loaded before the step's
+// scalars are asked for, so that the two round trips are one (3.1 M parameters in 701 tensors, 8 bits:
+// 18.8 -> 16.3 us).
+template <bool EIGHT, bool BF16, bool NT>
+__device__ __forceinline__ void step_chunk(const OptPlan &P, const OptStep &S, const OptTensor &t, int chunk) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t per = P.step_values / OPT_BLOCK, first = chunk * per, whole = t.n / OPT_BLOCK;
+    const int64_t end = min(first + per, whole);
+    Block<EIGHT, BF16, true, NT> block;
+    int64_t b = first + wave;
+    if (b < end) block.load(t, b, lane);
+    const Scalars o = scalars(P, S);
+    if (o.skip) return;
+    // every workgroup has read the counter once the last one comes here: it sets the next count
+    __syncthreads();
+    if (threadIdx.x == 0 && last_of_grid(P.ticket)) *P.step = o.t;
+    const float lr = o.lr * t.lr_scale;
+    if (b < end) block.step(P, t, o, lr, b, lane);
+    for (b += NB / 64; b < end; b += NB / 64) {
+        block.load(t, b, lane);
+        block.step(P, t, o, lr, b, lane);
+    }
+    // the tensor's last block where it does not fill it, in its last chunk
+    if (whole * OPT_BLOCK < t.n && whole < first + per && wave == (int)((whole - first) % (NB / 64))) {
+        Block<EIGHT, BF16, false, NT> tail;
+        tail.load(t, whole, lane);
+        tail.step(P, t, o, lr, whole, lane);
     }
 }
 
+template <bool EIGHT, bool NT>
+__global__ __launch_bounds__(NB) void k_adamw(OptPlan P, OptStep S) {
+    const OptChunk ck = P.step_chunks[blockIdx.x];
+    const OptTensor t = P.tensors[ck.tensor];
+    if (t.grad_bf16)
+        step_chunk<EIGHT, true, NT>(P, S, t, ck.chunk);
+    else
+        step_chunk<EIGHT, false, NT>(P, S, t, ck.chunk);
+}
+
+// An empty list's step.
+__global__ void k_adamw_count(OptPlan P, OptStep S) {
+    const Scalars o = scalars(P, S);
+    if (!o.skip) *P.step = o.t;
+}
+
+// The squares of R times 64 lanes' 16 bytes, all loaded before the first is used.
+template <typename T, int R>
+__device__ __forceinline__ void add_squares(const T *g, double (&s)[4]) {
+    constexpr int W = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+    vec x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = *reinterpret_cast<const vec *>(g + r * 64 * W);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < W; ++j) s[j & 3] += (double)(float)x[r][j] * (double)(float)x[r][j];
+}
+
+template <typename T>
+__device__ __forceinline__ void add_squares(const T *g, int64_t n, int lane, double (&s)[4]) {
+    constexpr int W = 16 / (int)sizeof(T), R = 4;
+    int64_t i = 0;
+    for (; i + R * 64 * W <= n; i += R * 64 * W) add_squares<T, R>(g + i + lane * W, s);
+    for (; i + 64 * W <= n; i += 64 * W) add_squares<T, 1>(g + i + lane * W, s);
+    for (i += lane; i < n; i += 64) s[0] += (double)(float)g[i] * (double)(float)g[i];
+}
+
 // Sum of the squares of all gradients in 64 bits (no overflow, and no order that matters to fp32): each
-// workgroup's chunks in order, then the workgroups' sums in order by the last one to finish.
+// wave's chunks in order, then the workgroups' sums in order by the last one to finish.  A sum is
+// handed over by a read-modify-write of its place, and the workgroup counted once that has returned,
+// so that no cache has to be written back (with a release of the caches in each of 1850 workgroups the
+// kernel took 47 us for 1.9 M values, now 7).
 __global__ __launch_bounds__(NB) void k_grad_norm(OptPlan P, float *norm) {
     __shared__ double red[NB / 64];
     __shared__ bool last;
-    double s = 0.0;
-    for (int c = blockIdx.x; c < P.n_chunks; c += gridDim.x) {
-        const OptChunk ck = P.chunks[c];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double s4[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int c = blockIdx.x * (NB / 64) + wave; c < P.n_norm_chunks; c += gridDim.x * (NB / 64)) {
+        const OptChunk ck = P.norm_chunks[c];
         const OptTensor &t = P.tensors[ck.tensor];
-        const int64_t begin = (int64_t)ck.chunk * P.chunk_values, n = t.n;
-        const int64_t end = min(begin + P.chunk_values, n);
-        for (int64_t i = begin + threadIdx.x * V; i < end; i += NB * V) {
-            float g[V];
-            const int k = (int)min<int64_t>(n - i, V);
-            if (t.grad_bf16)
-                load4((const __bf16 *)t.grad + i, k, g);
-            else
-                load4((const float *)t.grad + i, k, g);
-#pragma unroll
-            for (int j = 0; j < V; ++j) s += (double)g[j] * (double)g[j];
-        }
+        const int64_t begin = (int64_t)ck.chunk * P.norm_values, n = min((int64_t)P.norm_values, t.n - begin);
+        if (t.grad_bf16)
+            add_squares((const __bf16 *)t.grad + begin, n, lane, s4);
+        else
+            add_squares((const float *)t.grad + begin, n, lane, s4);
     }
     auto block_sum = [&](double x) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+        if (lane == 0) red[wave] = x;
         __syncthreads();
         x = 0.0;
         for (int w = 0; w < NB / 64; ++w) x += red[w];
         return x;
     };
-    s = block_sum(s);
+    double s = block_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
     if (threadIdx.x == 0) {
-        __hip_atomic_store(&P.partials[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = __hip_atomic_fetch_add(P.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        const uint64_t before = __hip_atomic_exchange((uint64_t *)&P.partials[blockIdx.x], (uint64_t)__double_as_longlong(s), __ATOMIC_RELAXED,
+                                                      __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("" ::"v"(before) : "memory");  // the exchange has returned before the counter is raised
+        last = last_of_grid(P.ticket);
     }
     __syncthreads();
     if (!last) return;
@@ -282,33 +379,44 @@ __global__ __launch_bounds__(NB) void k_grad_norm(OptPlan P, float *norm) {
     for (unsigned i = threadIdx.x; i < gridDim.x; i += NB)
         s += __hip_atomic_load(&P.partials[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s = block_sum(s);
-    if (threadIdx.x == 0) {
-        *norm = (float)sqrt(s);
-        __hip_atomic_store(P.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
 }  // namespace
 
-// Values a workgroup: enough workgroups to fill the GPU, and no more than 2^31 of them.
-int opt_chunk_values(int64_t total) {
+// Values of a workgroup's chunk in a step.  With fp32 states one block a wave: more blocks a workgroup, or
+// more workgroups in flight, spread the open pages of seven streams (65 M parameters: 16 blocks a wave 351 us, 4 322, 1
+// 307).  With 8-bit states three where there are enough, as the scalars' arithmetic counts (65 M: 1 block 198 us,
+// 3 178, 8 187; 206 M: 618, 565, 617).
+int opt_step_values(int64_t total, bool eight) {
+    constexpr int LEAST = NB * V;
+    return eight && total >= (int64_t)4096 * 3 * LEAST ? 3 * LEAST : LEAST;
+}
+
+// Values of a wave's chunk in the norm: 2048 waves, up to 16 thousand values at a time.
+int opt_norm_values(int64_t total) {
     constexpr int64_t LEAST = NB * V, MOST = 16 * NB * V;
-    const int64_t per = total / 4096 / LEAST * LEAST;
-    return (int)std::min(std::max(per, LEAST), MOST);
+    return (int)std::min(std::max(total / (OPT_NORM_BLOCKS * (NB / 64)) / LEAST * LEAST, LEAST), MOST);
 }
 
 void launch_grad_norm(const OptPlan &p, float *norm, hipStream_t st) {
-    const int blocks = std::max(1, std::min(p.n_chunks, OPT_NORM_BLOCKS));
+    const int blocks = std::max(1, std::min((p.n_norm_chunks + NB / 64 - 1) / (NB / 64), OPT_NORM_BLOCKS));
     k_grad_norm<<<blocks, NB, 0, st>>>(p, norm);
 }
 
+// A list that streams through the caches (more than they hold) is read and written past them: 65 M parameters
+// 313 -> 301 us, 8 bits 207 -> 205; a list that they hold keeps them (1.9 M: 11.4 us, past them 12.8).  With fp32 states
+// 32 KB of LDS that nothing uses then keep the workgroups at five a CU, for the same reason as the chunks:
+// 65 M 308 -> 287 us (8 a CU; 6: 304, 4: 289, 2: 340), 206 M with bf16 gradients and copies 977 -> 929.
 void launch_adamw(const OptPlan &p, const OptStep &s, hipStream_t st) {
-    k_adamw_begin<<<1, 1, 0, st>>>(p, s);
-    if (p.n_chunks == 0) return;
-    if (p.state_bits == 8)
-        k_adamw<true><<<p.n_chunks, NB, 0, st>>>(p);
+    const int wg = p.n_step_chunks;
+    constexpr int FEWER = 32768;
+    if (wg == 0)
+        k_adamw_count<<<1, 1, 0, st>>>(p, s);
+    else if (p.state_bits == 8)
+        p.streams ? k_adamw<true, true><<<wg, NB, 0, st>>>(p, s) : k_adamw<true, false><<<wg, NB, 0, st>>>(p, s);
     else
-        k_adamw<false><<<p.n_chunks, NB, 0, st>>>(p);
+        p.streams ? k_adamw<false, true><<<wg, NB, FEWER, st>>>(p, s) : k_adamw<false, false><<<wg, NB, 0, st>>>(p, s);
 }
 
 }  // namespace adn

@@ -2300,40 +2300,49 @@ int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors,
         }
         if (!grads_alone) spans.push_back({(uintptr_t)cfg->step, (uintptr_t)cfg->step + 4, true});
         if (spans_meet(spans)) return fail(ADN_E_INVALID, "tensors that the step writes overlap each other or the gradients");
-        const int per = opt_chunk_values(total);
-        std::vector<OptChunk> chunks;
-        for (int64_t i = 0; i < n_tensors; ++i) {
-            const int64_t k = (recs[(size_t)i].n + per - 1) / per;
-            if ((int64_t)chunks.size() + k >= (1 << 24)) return fail(ADN_E_INVALID, "the list needs 2^24 workgroups or more");
-            for (int64_t j = 0; j < k; ++j) chunks.push_back({(int32_t)i, (int32_t)j});
+        const int per[2] = {grads_alone ? 0 : opt_step_values(total, eight), opt_norm_values(total)};
+        std::vector<OptChunk> chunks[2];
+        for (int which = grads_alone ? 1 : 0; which < 2; ++which) {
+            for (int64_t i = 0; i < n_tensors; ++i) {
+                const int64_t k = (recs[(size_t)i].n + per[which] - 1) / per[which];
+                if ((int64_t)chunks[which].size() + k >= (1 << 24)) return fail(ADN_E_INVALID, "the list needs 2^24 workgroups or more");
+                for (int64_t j = 0; j < k; ++j) chunks[which].push_back({(int32_t)i, (int32_t)j});
+            }
         }
         DeviceScope scope(c->device);
         hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
         ADN_HIP(hipStreamIsCapturing(c->stream, &cap));
         if (cap != hipStreamCaptureStatusNone) return fail(ADN_E_CAPACITY, "an optimizer cannot be created under stream capture");
-        // one block: records, chunks, the step's scalars, the norm's partial sums and counter
+        // one block: records, chunks, the norm's partial sums, the counters of workgroups
         auto place = [](size_t &at, size_t bytes) {
             const size_t a = (at + 255) & ~(size_t)255;
             at = a + bytes;
             return a;
         };
         size_t bytes = 0;
-        const size_t at_recs = place(bytes, recs.size() * sizeof(OptTensor)), at_chunks = place(bytes, chunks.size() * sizeof(OptChunk));
-        const size_t at_scalars = place(bytes, sizeof(OptScalars)), at_partials = place(bytes, OPT_NORM_BLOCKS * sizeof(double));
-        const size_t at_ticket = place(bytes, sizeof(unsigned));
+        const size_t at_recs = place(bytes, recs.size() * sizeof(OptTensor));
+        const size_t at_chunks[2] = {place(bytes, chunks[0].size() * sizeof(OptChunk)), place(bytes, chunks[1].size() * sizeof(OptChunk))};
+        const size_t at_partials = place(bytes, OPT_NORM_BLOCKS * sizeof(double));
+        const size_t at_ticket = place(bytes, (1 + OPT_TICKETS) * OPT_TICKET_PITCH * sizeof(unsigned));
         std::vector<char> host(bytes, 0);
         if (!recs.empty()) memcpy(host.data() + at_recs, recs.data(), recs.size() * sizeof(OptTensor));
-        if (!chunks.empty()) memcpy(host.data() + at_chunks, chunks.data(), chunks.size() * sizeof(OptChunk));
+        for (int i = 0; i < 2; ++i)
+            if (!chunks[i].empty()) memcpy(host.data() + at_chunks[i], chunks[i].data(), chunks[i].size() * sizeof(OptChunk));
         auto opt = std::make_unique<adn_adamw>();
         c->optimizers.reserve(c->optimizers.size() + 1);
         char *dev = (char *)dmalloc(c, bytes);
         ADN_HIP(hipMemcpyAsync(dev, host.data(), bytes, hipMemcpyHostToDevice, c->stream));
         ADN_HIP(hipStreamSynchronize(c->stream));
         OptPlan &p = opt->plan;
-        p.tensors = (const OptTensor *)(dev + at_recs), p.chunks = (const OptChunk *)(dev + at_chunks);
-        p.n_chunks = (int)chunks.size(), p.chunk_values = per, p.state_bits = (int)cfg->state_bits;
+        p.tensors = (const OptTensor *)(dev + at_recs);
+        p.step_chunks = (const OptChunk *)(dev + at_chunks[0]), p.norm_chunks = (const OptChunk *)(dev + at_chunks[1]);
+        p.n_step_chunks = (int)chunks[0].size(), p.step_values = per[0];
+        p.n_norm_chunks = (int)chunks[1].size(), p.norm_values = per[1];
+        p.state_bits = (int)cfg->state_bits;
+        p.streams = total > (eight ? 16ll : 8ll) << 20;
         p.beta1 = cfg->beta1, p.beta2 = cfg->beta2, p.eps = (float)cfg->eps, p.seed = cfg->seed, p.step = cfg->step;
-        p.scalars = (OptScalars *)(dev + at_scalars), p.partials = (double *)(dev + at_partials), p.ticket = (unsigned *)(dev + at_ticket);
+        p.log_beta1 = std::log(cfg->beta1), p.log_beta2 = std::log(cfg->beta2);
+        p.partials = (double *)(dev + at_partials), p.ticket = (unsigned *)(dev + at_ticket);
         opt->ctx = c;
         c->optimizers.push_back(opt.get());
         *out = opt.release();

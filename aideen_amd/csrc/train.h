@@ -120,26 +120,21 @@ struct OptTensor {  // one tensor of the list
     uint32_t grad_bf16;
     uint32_t pad_;
 };
-struct OptChunk {  // a workgroup's share of a tensor
+struct OptChunk {  // a share of a tensor
     int32_t tensor, chunk;
-};
-struct OptScalars {  // what the step's first kernel leaves for the others
-    double coef;
-    uint64_t key;
-    float lr, inv_bc1, inv_sqrt_bc2;
-    int32_t skip;
 };
 struct OptPlan {  // the list as it stands on the device
     const OptTensor *tensors;
-    const OptChunk *chunks;
-    int n_chunks, chunk_values, state_bits;
-    double beta1, beta2;
+    const OptChunk *step_chunks, *norm_chunks;  // a workgroup's of the step, a wave's of the norm
+    int n_step_chunks, step_values, n_norm_chunks, norm_values;
+    int state_bits;
+    bool streams;            // a step moves more bytes than the caches hold
+    double beta1, beta2, log_beta1, log_beta2;
     float eps;
     uint64_t seed;
     int32_t *step;
-    OptScalars *scalars;
     double *partials;        // [OPT_NORM_BLOCKS]
-    unsigned *ticket;
+    unsigned *ticket;        // [1 + OPT_TICKETS] at OPT_TICKET_PITCH, zero between calls
 };
 struct OptStep {
     double lr;
@@ -147,8 +142,10 @@ struct OptStep {
     float max_norm, grad_scale;
 };
 constexpr int OPT_BLOCK = 256;         // values of an 8-bit state that share a scale
-constexpr int OPT_NORM_BLOCKS = 2048;  // most workgroups of the norm
-int opt_chunk_values(int64_t total);
+constexpr int OPT_NORM_BLOCKS = 512;   // most workgroups of the norm
+constexpr int OPT_TICKETS = 32, OPT_TICKET_PITCH = 64;  // places at which workgroups count themselves, 256 bytes apart
+int opt_step_values(int64_t total, bool eight);
+int opt_norm_values(int64_t total);
 void launch_grad_norm(const OptPlan &p, float *norm, hipStream_t st);
 void launch_adamw(const OptPlan &p, const OptStep &s, hipStream_t st);
 
