@@ -89,9 +89,6 @@ class AdnResidualNormArgs(C.Structure):
                 ("dpost_gain", C.c_void_p), ("dpre_gain", C.c_void_p)]
 
 
-GATES = {"none": 0, "channel": 1, "row": 2, "element": 3}
-
-
 class AdnAdamwTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("copy", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
                 ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n", C.c_int64), ("lr_scale", C.c_float),

@@ -384,32 +384,26 @@ class GpuDeqBackend:
         check(lib().adn_rms_norm_backward_async(self._ctx, rows, d, self._dtype(x), xp, xs,
                                                 self._vector(gain, "gain", d), eps, dyp, dys, dxp, dxs, dgp))
 
-    def _residual_args(self, f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps):
-        if f.dim() != 2:
-            raise _invalid("f must be a matrix")
-        rows, d = f.shape
-        a = _lib.AdnResidualNormArgs(rows=rows, d=d, dtype=self._dtype(f), gate_sigmoid=bool(gate_sigmoid),
-                                     post_norm=bool(post_norm), keep=keep, scale=scale, eps=eps)
-        a.f, a.f_stride = self._matrix(f, "f", rows, d)
-        a.post_gain, a.pre_gain = self._vector(post_gain, "post_gain", d), self._vector(pre_gain, "pre_gain", d)
-        kind = "none"
-        if gate is not None:
-            kind = "channel" if gate.dim() == 1 else "row" if gate.shape == (rows, 1) and _dtype_code(gate.dtype) == 0 else "element"
-        a.gate_kind = _lib.GATES[kind]
-        a.gate, a.gate_stride = self._gate(kind, gate, "gate", rows, d, f.dtype)
-        return a, kind
+    def _residual_args(self, rows, d, f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps):
+        """The first 16 fields of the arguments, those before x left out: (head, f to pre_gain, the kind of gate)."""
+        dtype = f.dtype
+        kind = 0 if gate is None else 1 if gate.dim() == 1 else 3
+        if kind == 3 and gate.shape[1] == 1 and (d > 1 or dtype != gate.dtype):
+            kind = 2
+        g, gs = (None, 0) if kind == 0 else self._gate(kind, gate, "gate", rows, d, dtype)
+        return ((rows, d, self._dtype(f), kind, 1 if gate_sigmoid else 0, 1 if post_norm else 0, keep, scale, eps, 0),
+                (*self._matrix(f, "f", rows, d), self._vector(post_gain, "post_gain", d), g, gs,
+                 self._vector(pre_gain, "pre_gain", d)), kind)
 
     def _gate(self, kind, t, name, rows, d, dtype):
         """(pointer, row stride) of a gate or its gradient, as the gate is shared."""
-        if t is None:
-            return None, 0
-        if kind == "element":
+        if kind == 3:
             return self._matrix(t, name, rows, d, dtype)
-        if kind == "row":
+        if kind == 2:
             if t.shape != (rows, 1):
                 raise _invalid(f"{name} must have the shape ({rows}, 1), got {tuple(t.shape)}")
             t = t[:, 0]
-        return self._vector(t, name, rows if kind == "row" else d), 0
+        return self._vector(t, name, rows if kind == 2 else d), 0
 
     def residual_norm_async(self, x, f, *, outputs: Dict[str, object], gate=None, gate_sigmoid: bool = False,
                             post_norm: bool = True, post_gain=None, pre_gain=None, keep: float = 1.0,
@@ -421,17 +415,17 @@ class GpuDeqBackend:
         is given as logits.  keep = 1 - damping and scale = damping make it the solver's damped update.
         Runs on the context's stream; the caller orders it with the streams that fill and read the
         tensors, and keeps them until then."""
-        unknown = set(outputs) - {"z", "y"}
-        if unknown:
-            raise _invalid(f"unknown outputs {sorted(unknown)}")
-        a, _ = self._residual_args(f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps)
-        a.x, a.x_stride = self._matrix(x, "x", a.rows, a.d, f.dtype)
-        for k in ("z", "y"):
-            t = outputs.get(k)
-            if t is not None:
-                p, stride = self._matrix(t, k, a.rows, a.d, f.dtype)
-                setattr(a, k, p), setattr(a, k + "_stride", stride)
-        if a.rows == 0 and outputs.keys():
+        if not outputs.keys() <= {"z", "y"}:
+            raise _invalid(f"unknown outputs {sorted(set(outputs) - {'z', 'y'})}")
+        if f.dim() != 2:
+            raise _invalid("f must be a matrix")
+        rows, d = f.shape
+        dtype, z, y = f.dtype, outputs.get("z"), outputs.get("y")
+        head, rest, _ = self._residual_args(rows, d, f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps)
+        a = _lib.AdnResidualNormArgs(*head, *self._matrix(x, "x", rows, d, dtype), *rest,
+                                     *((None, d) if z is None else self._matrix(z, "z", rows, d, dtype)),
+                                     *((None, d) if y is None else self._matrix(y, "y", rows, d, dtype)))
+        if rows == 0:
             return
         check(lib().adn_residual_norm_async(self._ctx, C.byref(a)))
 
@@ -443,24 +437,28 @@ class GpuDeqBackend:
         forward's (needed where dy is given, else None will do); dx may be dz.  Runs on the context's
         stream; the caller orders it with the streams that fill and read the tensors, and keeps them until
         then."""
-        unknown = set(outputs) - {"dx", "df", "dgate", "dpost_gain", "dpre_gain"}
-        if unknown:
-            raise _invalid(f"unknown outputs {sorted(unknown)}")
-        a, kind = self._residual_args(f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps)
-        rows, d = a.rows, a.d
-        for k, t in (("z", z), ("dz", dz), ("dy", dy), ("dx", outputs.get("dx")), ("df", outputs.get("df"))):
-            if t is not None:
-                p, stride = self._matrix(t, k, rows, d, f.dtype)
-                setattr(a, k, p), setattr(a, k + "_stride", stride)
-        if outputs.get("dgate") is not None:
-            if gate is None:
-                raise _invalid("dgate without a gate")
-            a.dgate, a.dgate_stride = self._gate(kind, outputs["dgate"], "dgate", rows, d, f.dtype)
-        a.dpost_gain = self._vector(outputs.get("dpost_gain"), "dpost_gain", d)
-        a.dpre_gain = self._vector(outputs.get("dpre_gain"), "dpre_gain", d)
+        names = {"dx", "df", "dgate", "dpost_gain", "dpre_gain"}
+        if not outputs.keys() <= names:
+            raise _invalid(f"unknown outputs {sorted(set(outputs) - names)}")
+        if f.dim() != 2:
+            raise _invalid("f must be a matrix")
+        rows, d = f.shape
+        dtype = f.dtype
+        head, rest, kind = self._residual_args(rows, d, f, gate, gate_sigmoid, post_norm, post_gain, pre_gain, keep, scale, eps)
+        dgate = outputs.get("dgate")
+        if dgate is not None and kind == 0:
+            raise _invalid("dgate without a gate")
+
+        def matrix(t, name):
+            return (None, d) if t is None else self._matrix(t, name, rows, d, dtype)
+        a = _lib.AdnResidualNormArgs(*head, None, d, *rest, *matrix(z, "z"), None, d, *matrix(dz, "dz"), *matrix(dy, "dy"),
+                                     *matrix(outputs.get("dx"), "dx"), *matrix(outputs.get("df"), "df"),
+                                     *((None, d) if dgate is None else self._gate(kind, dgate, "dgate", rows, d, dtype)),
+                                     self._vector(outputs.get("dpost_gain"), "dpost_gain", d),
+                                     self._vector(outputs.get("dpre_gain"), "dpre_gain", d))
         if rows == 0:
             a.dx = a.df = None
-            if kind != "channel":
+            if kind != 1:
                 a.dgate = None
             if not (a.dgate or a.dpost_gain or a.dpre_gain):
                 return  # an empty batch, and only row outputs: nothing to write

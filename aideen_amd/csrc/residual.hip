@@ -21,7 +21,18 @@ namespace adn {
 
 namespace {
 
+// Blocks of a launch, which walk the rows: two to four a CU.  More rows in flight read no faster and spread the
+// memory's open pages (8192 x 512 fp32 forward: 512 blocks 13.8 us, 1024 15.2, 2048 19.5; 32749 x 2048 bf16: 768
+// blocks 136, 1024 132, 2048 148; backward: 32749 x 2048 bf16 256 blocks 268, 512 217, 1024 239, 2048 243).
+constexpr int ROW_BLOCKS = 512, WIDE_BLOCKS = 768;  // forward: of rows of a wave, and longer ones
+constexpr int MAX_TEAM = 512;     // lanes of the longest rows
 constexpr int COL_BLOCKS = 512;  // most blocks of the backward pass = partial rows of a column sum
+
+// A lane's elements of a row.
+constexpr int elements(int team) { return team < MAX_TEAM ? 8 : 16; }
+
+// A block's threads: four teams of a wave, or one of more waves.
+constexpr int block_threads(int team) { return team > 64 ? team : NB; }
 
 // The gate's value s and ds / dgate.  The exponential is taken of -|g|: it cannot overflow, and
 // s (1 - s) = t / (1 + t)^2 loses nothing where s is near 1.
@@ -35,188 +46,327 @@ __device__ __forceinline__ float gate_value(float g, bool sigmoid, float &slope)
     return g >= 0.0f ? i : t * i;
 }
 
-template <typename T, int TEAM, int E, bool VEC>
-__global__ __launch_bounds__(NB) void k_residual(ResidualParams p) {
-    __shared__ float red[1][NB / 64];
-    typedef Cols<T, TEAM, VEC> C;
-    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
-    const long row = (long)blockIdx.x * (NB / TEAM) + team;
-    if (row >= p.rows) return;  // a whole wave (TEAM 64) or never (a block a row)
-    Row<T, TEAM, E, VEC> x, f, gr;
-    x.load((const T *)p.x + row * p.x_stride, p.d, lane);
-    f.load((const T *)p.f + row * p.f_stride, p.d, lane);
-    if (p.gate_kind == ADN_GATE_ELEMENT) gr.load((const T *)p.gate + row * p.gate_stride, p.d, lane);
-    float slope, row_gate = 1.0f;
-    if (p.gate_kind == ADN_GATE_ROW) row_gate = gate_value(((const float *)p.gate)[row], p.sigmoid, slope);
-    float rf = 1.0f;
-    if (p.post) {
-        float s[1] = {0.0f};
+// Sums of N values over the team, in every lane of it: six steps across a wave's lanes, then (teams of
+// several waves) a place in LDS a wave; `turn` alternates, so that a call needs one barrier and not two.
+template <int TEAM, int N>
+__device__ __forceinline__ void team_add(float (&v)[N], float (*red)[3][MAX_TEAM / 64], int turn) {
+#define ADN_DPP_ADD(ctrl, rows) \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) \
+        v[i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v[i]), ctrl, rows, 0xF, true))
+    ADN_DPP_ADD(0x111, 0xF);  // from the lane one, two, four, eight to the left in a row of 16
+    ADN_DPP_ADD(0x112, 0xF);
+    ADN_DPP_ADD(0x114, 0xF);
+    ADN_DPP_ADD(0x118, 0xF);
+    ADN_DPP_ADD(0x142, 0xA);  // a row's last lane to the next row, then to the upper half
+    ADN_DPP_ADD(0x143, 0xC);
+#undef ADN_DPP_ADD
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[0] += f[e] * f[e];
-        team_sum<TEAM, 1>(s, red);
-        rf = 1.0f / sqrtf(s[0] / (float)p.d + p.eps);
-    }
-    float v[E], s[1] = {0.0f};
+    for (int i = 0; i < N; ++i) v[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[i]), 63));
+    if constexpr (TEAM > 64) {  // the team is the block
+        if ((threadIdx.x & 63) == 0)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = C::col(lane, e);
-        float n = f[e] * rf, g = row_gate;
-        if (p.post_gain && c < p.d) n *= p.post_gain[c];
-        if (p.gate_kind == ADN_GATE_CHANNEL)
-            g = c < p.d ? gate_value(((const float *)p.gate)[c], p.sigmoid, slope) : 0.0f;
-        else if (p.gate_kind == ADN_GATE_ELEMENT)
-            g = gate_value(gr[e], p.sigmoid, slope);
-        v[e] = c < p.d ? p.keep * x[e] + p.scale * g * n : 0.0f;
-        s[0] += v[e] * v[e];
-    }
-    if (p.z) store_row<T, TEAM, E, VEC>((T *)p.z + row * p.z_stride, p.d, lane, v);
-    if (!p.y) return;
-    team_sum<TEAM, 1>(s, red);
-    const float rz = 1.0f / sqrtf(s[0] / (float)p.d + p.eps);
+            for (int i = 0; i < N; ++i) red[turn][i][threadIdx.x >> 6] = v[i];
+        __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = C::col(lane, e);
-        v[e] *= rz;
-        if (p.pre_gain && c < p.d) v[e] *= p.pre_gain[c];
+        for (int i = 0; i < N; ++i) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < TEAM / 64; ++w) s += red[turn][i][w];
+            v[i] = s;
+        }
     }
-    store_row<T, TEAM, E, VEC>((T *)p.y + row * p.y_stride, p.d, lane, v);
+}
+
+// A row's share of a lane, STREAM: past the caches.
+template <bool STREAM, typename T, int TEAM, int E, bool VEC>
+__device__ __forceinline__ void take_row(Row<T, TEAM, E, VEC> &r, const T *row, int d, int lane) {
+    typedef Row<T, TEAM, E, VEC> R;
+    if constexpr (!STREAM) return r.load(row, d, lane);
+#pragma unroll
+    for (int q = 0; q < E / R::C::W; ++q) {
+        const int c = R::C::col(lane, q * R::C::W);
+        r.v[q] = typename R::V{};
+        if (c < d) r.v[q] = __builtin_nontemporal_load(reinterpret_cast<const typename R::V *>(row + c));
+    }
 }
 
 template <typename T, int TEAM, int E, bool VEC>
-__global__ __launch_bounds__(NB) void k_residual_back(ResidualParams p, float *part) {
-    __shared__ float red[2][NB / 64];
+__device__ __forceinline__ void put_row(T *row, int d, int lane, const float (&v)[E]) {
+    typedef Row<T, TEAM, E, VEC> R;
+#pragma unroll
+    for (int q = 0; q < E / R::C::W; ++q) {
+        const int c = R::C::col(lane, q * R::C::W);
+        typename R::V x;
+#pragma unroll
+        for (int j = 0; j < R::C::W; ++j) x[j] = from_f32<T>(v[q * R::C::W + j]);
+        if (c < d) __builtin_nontemporal_store(x, reinterpret_cast<typename R::V *>(row + c));
+    }
+}
+
+// What a lane has of a row's inputs, loaded ahead.
+template <typename T, int TEAM, bool VEC, bool STREAM, bool BACK>
+struct Inputs {
+    static constexpr int E = elements(TEAM);
+    typedef Row<T, TEAM, E, VEC> R;
+    R a, f, g, dz, dy;  // a: x, or z in the backward pass
+    float row_gate;
+    __device__ __forceinline__ void load(const ResidualParams &p, long row, int lane) {
+        auto take = [&](R &r, const void *base, long stride) {
+            take_row<STREAM>(r, (const T *)base + row * stride, p.d, lane);
+        };
+        take(f, p.f, p.f_stride);
+        if constexpr (BACK) {
+            if (p.dy) take(a, p.z, p.z_stride), take(dy, p.dy, p.dy_stride);
+            if (p.dz) take(dz, p.dz, p.dz_stride);
+        } else {
+            take(a, p.x, p.x_stride);
+        }
+        if (p.gate_kind == ADN_GATE_ELEMENT) take(g, p.gate, p.gate_stride);
+        if (p.gate_kind == ADN_GATE_ROW) row_gate = ((const float *)p.gate)[row];
+    }
+};
+
+template <typename T, int TEAM, bool VEC, bool STREAM>
+__global__ __launch_bounds__(block_threads(TEAM)) void k_residual(ResidualParams p) {
+    __shared__ float red[2][3][MAX_TEAM / 64];
     typedef Cols<T, TEAM, VEC> C;
-    constexpr int TEAMS = NB / TEAM;
+    constexpr int E = elements(TEAM), TEAMS = block_threads(TEAM) / TEAM;
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
-    const bool channel = p.gate_kind == ADN_GATE_CHANNEL, element = p.gate_kind == ADN_GATE_ELEMENT;
-    float gp[E], gq[E], gc[E], slope_c[E], dgp[E], dgq[E], dgc[E];
+    const long step = (long)gridDim.x * TEAMS;
+    long row = (long)blockIdx.x * TEAMS + team;
+    if (row >= p.rows) return;  // a whole wave (TEAM 64) or never (a block a row)
+    Inputs<T, TEAM, VEC, STREAM, false> in, next;
+    in.load(p, row, lane);
+    float w[E], gq[E], slope;  // scale, the gain and a gate of the channels
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int c = C::col(lane, e);
-        gp[e] = p.post_gain && c < p.d ? p.post_gain[c] : 1.0f;
-        gq[e] = p.pre_gain && c < p.d ? p.pre_gain[c] : 1.0f;
-        gc[e] = slope_c[e] = 1.0f;
-        if (channel && c < p.d) gc[e] = gate_value(((const float *)p.gate)[c], p.sigmoid, slope_c[e]);
-        dgp[e] = dgq[e] = dgc[e] = 0.0f;
+        w[e] = p.scale;
+        gq[e] = 1.0f;
+        if (c < p.d) {
+            if (p.post_gain) w[e] *= p.post_gain[c];
+            if (p.gate_kind == ADN_GATE_CHANNEL) w[e] *= gate_value(((const float *)p.gate)[c], p.sigmoid, slope);
+            if (p.pre_gain) gq[e] = p.pre_gain[c];
+        }
     }
     const float inv_d = 1.0f / (float)p.d;
-    for (long row = (long)blockIdx.x * TEAMS + team; row < p.rows; row += (long)gridDim.x * TEAMS) {
-        Row<T, TEAM, E, VEC> z, f, dz, dy, gr;
-        z.load((const T *)p.z + row * p.z_stride, p.d, lane);
-        f.load((const T *)p.f + row * p.f_stride, p.d, lane);
-        if (p.dz) dz.load((const T *)p.dz + row * p.dz_stride, p.d, lane);
-        if (p.dy) dy.load((const T *)p.dy + row * p.dy_stride, p.d, lane);
-        if (element) gr.load((const T *)p.gate + row * p.gate_stride, p.d, lane);
-        float slope_r = 1.0f, gate_r = 1.0f;
-        if (p.gate_kind == ADN_GATE_ROW) gate_r = gate_value(((const float *)p.gate)[row], p.sigmoid, slope_r);
-        float D[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) D[e] = p.dz ? dz[e] : 0.0f;
+    for (; row < p.rows; row += step) {
+        if (row + step < p.rows) next.load(p, row + step, lane);
         float rf = 1.0f;
-        if (p.dy) {
-            float s[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                s[0] += z[e] * z[e];
-                s[1] += dy[e] * gq[e] * z[e];
-            }
-            team_sum<TEAM, 2>(s, red);
-            const float rz = 1.0f / sqrtf(s[0] * inv_d + p.eps), k = rz * rz * (s[1] * inv_d);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                dgq[e] += dy[e] * (z[e] * rz);
-                D[e] += rz * (dy[e] * gq[e] - z[e] * k);
-            }
-        }
         if (p.post) {
             float s[1] = {0.0f};
 #pragma unroll
-            for (int e = 0; e < E; ++e) s[0] += f[e] * f[e];
-            team_sum<TEAM, 1>(s, red);
+            for (int e = 0; e < E; ++e) s[0] += in.f[e] * in.f[e];
+            team_add<TEAM, 1>(s, red, 0);
             rf = 1.0f / sqrtf(s[0] * inv_d + p.eps);
+        }
+        if (p.gate_kind == ADN_GATE_ROW) rf *= gate_value(in.row_gate, p.sigmoid, slope);
+        float v[E], s[1] = {0.0f};
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float n = in.f[e] * rf * w[e];
+            if (p.gate_kind == ADN_GATE_ELEMENT) n *= gate_value(in.g[e], p.sigmoid, slope);
+            v[e] = p.keep * in.a[e] + n;
+            s[0] += v[e] * v[e];
+        }
+        if (p.z) put_row<T, TEAM, E, VEC>((T *)p.z + row * p.z_stride, p.d, lane, v);
+        if (p.y) {
+            team_add<TEAM, 1>(s, red, 1);
+            const float rz = 1.0f / sqrtf(s[0] * inv_d + p.eps);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] *= rz * gq[e];
+            put_row<T, TEAM, E, VEC>((T *)p.y + row * p.y_stride, p.d, lane, v);
+        }
+        in = next;
+    }
+}
+
+// The column sums need two accumulators: A, the sum of u f rf (u = scale D, times a row's or an element's gate), which is
+// dgp but for a channel's gate, and that gate's gradient but for dgp's factor; and dgq.
+template <typename T, int TEAM, bool VEC, bool STREAM, uint32_t GATE>
+__global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualParams p, float *part) {
+    __shared__ float red[2][3][MAX_TEAM / 64];
+    typedef Cols<T, TEAM, VEC> C;
+    constexpr int E = elements(TEAM), TEAMS = block_threads(TEAM) / TEAM;
+    p.gate_kind = GATE;
+    const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+    const long step = (long)gridDim.x * TEAMS;
+    long row = (long)blockIdx.x * TEAMS + team;
+    Inputs<T, TEAM, VEC, STREAM, true> in, next;
+    if (row < p.rows) in.load(p, row, lane);
+    float w[E], gq[E], A[E], dgq[E], slope;  // w: the gain, times a gate of the channels
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int c = C::col(lane, e);
+        w[e] = gq[e] = 1.0f;
+        A[e] = dgq[e] = 0.0f;
+        if (c < p.d) {
+            if (p.post_gain) w[e] = p.post_gain[c];
+            if (GATE == ADN_GATE_CHANNEL) w[e] *= gate_value(((const float *)p.gate)[c], p.sigmoid, slope);
+            if (p.pre_gain) gq[e] = p.pre_gain[c];
+        }
+    }
+    const float inv_d = 1.0f / (float)p.d;
+    for (; row < p.rows; row += step) {
+        if (row + step < p.rows) next.load(p, row + step, lane);
+        float s[3] = {0.0f, 0.0f, 0.0f};
+        if (p.dy) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                s[0] += in.a[e] * in.a[e];
+                s[1] += in.dy[e] * gq[e] * in.a[e];
+            }
+        }
+        if (p.post) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[2] += in.f[e] * in.f[e];
+        }
+        team_add<TEAM, 3>(s, red, 0);
+        const float rf = p.post ? 1.0f / sqrtf(s[2] * inv_d + p.eps) : 1.0f;
+        float D[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) D[e] = p.dz ? in.dz[e] : 0.0f;
+        if (p.dy) {
+            const float rz = 1.0f / sqrtf(s[0] * inv_d + p.eps), k = rz * rz * (s[1] * inv_d);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                dgq[e] += in.dy[e] * (in.a[e] * rz);
+                D[e] += rz * (in.dy[e] * gq[e] - in.a[e] * k);
+            }
         }
         if (p.dx) {
             float v[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = p.keep * D[e];
-            store_row<T, TEAM, E, VEC>((T *)p.dx + row * p.dx_stride, p.d, lane, v);
+            put_row<T, TEAM, E, VEC>((T *)p.dx + row * p.dx_stride, p.d, lane, v);
         }
-        // dn, then b = dn gp in D's place; the gate's gradient
-        float dg[E], s[2] = {0.0f, 0.0f};
+        // D becomes b = scale D s gp
+        float slope_r = 1.0f, gate_r = 1.0f, t[2] = {0.0f, 0.0f};
+        if (GATE == ADN_GATE_ROW) gate_r = gate_value(in.row_gate, p.sigmoid, slope_r);
+        float dg[GATE == ADN_GATE_ELEMENT ? E : 1];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            float g = gate_r, slope = slope_r;
-            if (channel) g = gc[e], slope = slope_c[e];
-            if (element) g = gate_value(gr[e], p.sigmoid, slope);
-            const float fr = f[e] * rf, u = p.scale * D[e], dn = u * g;
-            dg[e] = u * (fr * gp[e]) * slope;
-            s[1] += dg[e];
-            dgc[e] += dg[e];
-            dgp[e] += dn * fr;
-            D[e] = dn * gp[e];
-            s[0] += D[e] * f[e];
+            const float fr = in.f[e] * rf;
+            float u = p.scale * D[e];
+            if (GATE == ADN_GATE_ROW) {
+                t[1] += u * fr * w[e];
+                u *= gate_r;
+            }
+            if constexpr (GATE == ADN_GATE_ELEMENT) {
+                const float g = gate_value(in.g[e], p.sigmoid, slope);
+                dg[e] = u * fr * w[e] * slope;
+                u *= g;
+            }
+            A[e] += u * fr;
+            D[e] = u * w[e];
+            t[0] += D[e] * in.f[e];
         }
-        if (p.dgate && element) store_row<T, TEAM, E, VEC>((T *)p.dgate + row * p.dgate_stride, p.d, lane, dg);
-        team_sum<TEAM, 2>(s, red);
-        if (p.dgate && p.gate_kind == ADN_GATE_ROW && lane == 0) ((float *)p.dgate)[row] = s[1];
+        if constexpr (GATE == ADN_GATE_ELEMENT)
+            if (p.dgate) put_row<T, TEAM, E, VEC>((T *)p.dgate + row * p.dgate_stride, p.d, lane, dg);
+        team_add<TEAM, 2>(t, red, 1);
+        if (GATE == ADN_GATE_ROW && p.dgate && lane == 0) ((float *)p.dgate)[row] = t[1] * slope_r;
         if (p.df) {
-            const float k = p.post ? rf * rf * (s[0] * inv_d) : 0.0f;
+            const float k = p.post ? rf * rf * (t[0] * inv_d) : 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) D[e] = rf * (D[e] - f[e] * k);
-            store_row<T, TEAM, E, VEC>((T *)p.df + row * p.df_stride, p.d, lane, D);
+            for (int e = 0; e < E; ++e) D[e] = rf * (D[e] - in.f[e] * k);
+            put_row<T, TEAM, E, VEC>((T *)p.df + row * p.df_stride, p.d, lane, D);
         }
+        in = next;
     }
     if (!part) return;
-    // the block's teams in order, then one partial row a block, for each of the three sums that is wanted
-    __shared__ float sum[TEAMS > 1 ? TEAMS : 1][64][E + 1];
+    // the block's teams in order, then one partial row a block of A and of dgq
+    if constexpr (TEAMS > 1) {
+        __shared__ float sum[TEAMS][64][2 * E + 1];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        if (!(i == 0 ? p.dpost != nullptr : i == 1 ? p.dpre != nullptr : p.dgate && channel)) continue;
-        float t[E];
+        for (int e = 0; e < E; ++e) sum[team][lane][e] = A[e], sum[team][lane][E + e] = dgq[e];
+        __syncthreads();
+        if (team) return;
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[e] = i == 0 ? dgp[e] : i == 1 ? dgq[e] : dgc[e];
-        if constexpr (TEAMS > 1) {
-            __syncthreads();
+        for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum[team][lane][e] = t[e];
-            __syncthreads();
-            if (team == 0) {
+            for (int q = 1; q < TEAMS; ++q) A[e] += sum[q][lane][e], dgq[e] += sum[q][lane][E + e];
+    }
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    t[e] = sum[0][lane][e];
-#pragma unroll
-                    for (int q = 1; q < TEAMS; ++q) t[e] += sum[q][lane][e];
-                }
-            }
+    for (int e = 0; e < E; ++e) {
+        const int c = C::col(lane, e);
+        if (c < p.d) {
+            part[(long)blockIdx.x * p.d + c] = A[e];
+            part[((long)gridDim.x + blockIdx.x) * p.d + c] = dgq[e];
         }
-        if (team == 0)
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int c = C::col(lane, e);
-                if (c < p.d) part[((long)i * gridDim.x + blockIdx.x) * p.d + c] = t[e];
-            }
     }
 }
 
-// f(TEAM, E): the smallest team and share that hold a row (E a multiple of 8: whole 16-byte pieces)
+// The column sums: 64 threads a column each take every 64th of its n partial sums in order, then a tree.  Behind
+// them A's factors: dgp = A times a channel's gate, that gate's gradient = A times the gain (and the slope).
+__global__ __launch_bounds__(1024) void k_residual_join(ResidualParams p, const float *part, int n) {
+    constexpr int COLS = 16, GROUPS = 64;
+    __shared__ float red[GROUPS][COLS + 1];
+    const int col = threadIdx.x % COLS, g = threadIdx.x / COLS, c = blockIdx.x * COLS + col;
+    const bool second = blockIdx.y;
+    const float *src = part + (second ? (long)n * p.d : 0);
+    float s = 0.0f;
+    if (c < p.d) {
+#pragma unroll 8
+        for (int i = g; i < n; i += GROUPS) s += src[(long)i * p.d + c];
+    }
+    red[g][col] = s;
+#pragma unroll
+    for (int k = GROUPS / 2; k; k >>= 1) {
+        __syncthreads();
+        if (g < k) red[g][col] += red[g + k][col];
+    }
+    if (g || c >= p.d) return;
+    s = red[0][col];
+    if (second) {
+        if (p.dpre) p.dpre[c] = s;
+        return;
+    }
+    float gate = 1.0f, slope = 1.0f;
+    const bool channel = p.gate_kind == ADN_GATE_CHANNEL;
+    if (channel) gate = gate_value(((const float *)p.gate)[c], p.sigmoid, slope);
+    if (p.dpost) p.dpost[c] = s * gate;
+    if (p.dgate && channel) ((float *)p.dgate)[c] = s * (p.post_gain ? p.post_gain[c] : 1.0f) * slope;
+}
+
+// f(TEAM): the smallest team that holds a row
 template <typename F>
 void dispatch_row(int d, F &&f) {
     using std::integral_constant;
-    if (d <= 512)
-        f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
-    else if (d <= 1024)
-        f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
-    else if (d <= 2048)
-        f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+    if (d <= 64 * elements(64))
+        f(integral_constant<int, 64>{});
+    else if (d <= 128 * elements(128))
+        f(integral_constant<int, 128>{});
+    else if (d <= 256 * elements(256))
+        f(integral_constant<int, 256>{});
     else
-        f(integral_constant<int, 256>{}, integral_constant<int, 32>{});
+        f(integral_constant<int, MAX_TEAM>{});
 }
 
 bool column_sums(const ResidualParams &p) { return p.dpost || p.dpre || (p.dgate && p.gate_kind == ADN_GATE_CHANNEL); }
 
+// A call whose matrices are more than the caches hold reads past them (backward of 32749 x 2048 bf16, 1.07 GB: 220 -> 200 us; of
+// 8192 x 512 fp32, 101 MB: 23.5 through them, 26.7 past them).
+bool streams(const ResidualParams &p, int matrices) {
+    return (double)p.rows * p.d * elem_bytes(p.dtype) * matrices > 256e6;
+}
+
 int back_blocks(const ResidualParams &p) {
-    const int teams = p.d <= 1024 ? NB / 64 : 1;
+    const int teams = p.d <= 64 * elements(64) ? NB / 64 : 1;
     return (int)std::min<long>(COL_BLOCKS, ((long)p.rows + teams - 1) / teams);
+}
+
+// f(GATE) for the kind of gate
+template <typename F>
+void dispatch_gate(uint32_t kind, F &&f) {
+    using std::integral_constant;
+    if (kind == ADN_GATE_NONE)
+        f(integral_constant<uint32_t, ADN_GATE_NONE>{});
+    else if (kind == ADN_GATE_CHANNEL)
+        f(integral_constant<uint32_t, ADN_GATE_CHANNEL>{});
+    else if (kind == ADN_GATE_ROW)
+        f(integral_constant<uint32_t, ADN_GATE_ROW>{});
+    else
+        f(integral_constant<uint32_t, ADN_GATE_ELEMENT>{});
 }
 
 }  // namespace
@@ -228,32 +378,23 @@ void launch_residual(const ResidualParams &p, hipStream_t st) {
     const bool vec = rows_vec16(p.x, p.x_stride, p.d, eb) && rows_vec16(p.f, p.f_stride, p.d, eb) &&
                      (!p.z || rows_vec16(p.z, p.z_stride, p.d, eb)) && (!p.y || rows_vec16(p.y, p.y_stride, p.d, eb)) &&
                      (!element || rows_vec16(p.gate, p.gate_stride, p.d, eb));
-    // a launch has less than 2^32 threads: 2^23 rows at a time, a block a row at most
-    ResidualParams q = p;
-    for (int row = 0; row < p.rows; row += 1 << 23) {
-        q.rows = std::min(p.rows - row, 1 << 23);
-        q.x = (const char *)p.x + row * p.x_stride * eb;
-        q.f = (const char *)p.f + row * p.f_stride * eb;
-        if (p.z) q.z = (char *)p.z + row * p.z_stride * eb;
-        if (p.y) q.y = (char *)p.y + row * p.y_stride * eb;
-        if (element) q.gate = (const char *)p.gate + row * p.gate_stride * eb;
-        if (p.gate_kind == ADN_GATE_ROW) q.gate = (const float *)p.gate + row;
-        dispatch_type(p.dtype, [&](auto t) {
-            typedef decltype(t) T;
-            dispatch_row(p.d, [&](auto team, auto e) {
-                constexpr int TEAM = decltype(team)::value, E = decltype(e)::value;
-                const dim3 grid((unsigned)(((long)q.rows * TEAM + NB - 1) / NB));
-                if (vec)
-                    k_residual<T, TEAM, E, true><<<grid, NB, 0, st>>>(q);
-                else
-                    k_residual<T, TEAM, E, false><<<grid, NB, 0, st>>>(q);
-            });
+    dispatch_type(p.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        dispatch_row(p.d, [&](auto team) {
+            constexpr int TEAM = decltype(team)::value, BLOCK = block_threads(TEAM);
+            const unsigned grid = (unsigned)std::min<long>(((long)p.rows * TEAM + BLOCK - 1) / BLOCK, TEAM > 64 ? WIDE_BLOCKS : ROW_BLOCKS);
+            if (vec && streams(p, 3))
+                k_residual<T, TEAM, true, true><<<grid, BLOCK, 0, st>>>(p);
+            else if (vec)
+                k_residual<T, TEAM, true, false><<<grid, BLOCK, 0, st>>>(p);
+            else
+                k_residual<T, TEAM, false, false><<<grid, BLOCK, 0, st>>>(p);
         });
-    }
+    });
 }
 
 size_t residual_backward_workspace_bytes(const ResidualParams &p) {
-    return column_sums(p) ? (size_t)3 * back_blocks(p) * p.d * sizeof(float) : 0;
+    return column_sums(p) ? (size_t)2 * back_blocks(p) * p.d * sizeof(float) : 0;
 }
 
 void launch_residual_backward(const ResidualParams &p, void *ws, hipStream_t st) {
@@ -267,17 +408,20 @@ void launch_residual_backward(const ResidualParams &p, void *ws, hipStream_t st)
     if (blocks)
         dispatch_type(p.dtype, [&](auto t) {
             typedef decltype(t) T;
-            dispatch_row(p.d, [&](auto team, auto e) {
-                constexpr int TEAM = decltype(team)::value, E = decltype(e)::value;
-                if (vec)
-                    k_residual_back<T, TEAM, E, true><<<blocks, NB, 0, st>>>(p, part);
-                else
-                    k_residual_back<T, TEAM, E, false><<<blocks, NB, 0, st>>>(p, part);
+            dispatch_row(p.d, [&](auto team) {
+                constexpr int TEAM = decltype(team)::value, BLOCK = block_threads(TEAM);
+                dispatch_gate(p.gate_kind, [&](auto gate) {
+                    constexpr uint32_t GATE = decltype(gate)::value;
+                    if (vec && streams(p, 6))
+                        k_residual_back<T, TEAM, true, true, GATE><<<blocks, BLOCK, 0, st>>>(p, part);
+                    else if (vec)
+                        k_residual_back<T, TEAM, true, false, GATE><<<blocks, BLOCK, 0, st>>>(p, part);
+                    else
+                        k_residual_back<T, TEAM, false, false, GATE><<<blocks, BLOCK, 0, st>>>(p, part);
+                });
             });
         });
-    if (part)
-        launch_sum_rows(part, blocks, p.d, SumRows{{p.dpost, p.dpre, p.gate_kind == ADN_GATE_CHANNEL ? (float *)p.dgate : nullptr}},
-                        3, st);
+    if (part) k_residual_join<<<dim3((p.d + 15) / 16, 2), 1024, 0, st>>>(p, part, blocks);
 }
 
 }  // namespace adn
