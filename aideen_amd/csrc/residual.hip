@@ -421,7 +421,7 @@ void launch_residual_backward(const ResidualParams &p, void *ws, hipStream_t st)
                 });
             });
         });
-    if (part) k_residual_join<<<dim3((p.d + 15) / 16, 2), 1024, 0, st>>>(p, part, blocks);
+    if (column_sums(p)) k_residual_join<<<dim3((p.d + 15) / 16, 2), 1024, 0, st>>>(p, part, blocks);
 }
 
 }  // namespace adn
