@@ -47,9 +47,11 @@ __device__ __forceinline__ float gate_value(float g, bool sigmoid, float &slope)
 }
 
 // Sums of N values over the team, in every lane of it: six steps across a wave's lanes, then (teams of
-// several waves) a place in LDS a wave; `turn` alternates, so that a call needs one barrier and not two.
+// several waves) a place in LDS a wave.  `turn` alternates from call to call, so that one barrier a call is
+// enough: a place is written again two calls later, behind the barrier of the call between, which a
+// wave reaches when it has read what stood there.
 template <int TEAM, int N>
-__device__ __forceinline__ void team_add(float (&v)[N], float (*red)[3][MAX_TEAM / 64], int turn) {
+__device__ __forceinline__ void team_add(float (&v)[N], float (*red)[3][MAX_TEAM / 64], int &turn) {
 #define ADN_DPP_ADD(ctrl, rows) \
     _Pragma("unroll") for (int i = 0; i < N; ++i) \
         v[i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v[i]), ctrl, rows, 0xF, true))
@@ -74,6 +76,7 @@ __device__ __forceinline__ void team_add(float (&v)[N], float (*red)[3][MAX_TEAM
             for (int w = 0; w < TEAM / 64; ++w) s += red[turn][i][w];
             v[i] = s;
         }
+        turn ^= 1;
     }
 }
 
@@ -150,6 +153,7 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual(ResidualParams
         }
     }
     const float inv_d = 1.0f / (float)p.d;
+    int turn = 0;
     for (; row < p.rows; row += step) {
         if (row + step < p.rows) next.load(p, row + step, lane);
         float rf = 1.0f;
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual(ResidualParams
             float s[1] = {0.0f};
 #pragma unroll
             for (int e = 0; e < E; ++e) s[0] += in.f[e] * in.f[e];
-            team_add<TEAM, 1>(s, red, 0);
+            team_add<TEAM, 1>(s, red, turn);
             rf = 1.0f / sqrtf(s[0] * inv_d + p.eps);
         }
         if (p.gate_kind == ADN_GATE_ROW) rf *= gate_value(in.row_gate, p.sigmoid, slope);
@@ -171,7 +175,7 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual(ResidualParams
         }
         if (p.z) put_row<T, TEAM, E, VEC>((T *)p.z + row * p.z_stride, p.d, lane, v);
         if (p.y) {
-            team_add<TEAM, 1>(s, red, 1);
+            team_add<TEAM, 1>(s, red, turn);
             const float rz = 1.0f / sqrtf(s[0] * inv_d + p.eps);
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] *= rz * gq[e];
@@ -207,6 +211,7 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualP
         }
     }
     const float inv_d = 1.0f / (float)p.d;
+    int turn = 0;
     for (; row < p.rows; row += step) {
         if (row + step < p.rows) next.load(p, row + step, lane);
         float s[3] = {0.0f, 0.0f, 0.0f};
@@ -221,7 +226,7 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualP
 #pragma unroll
             for (int e = 0; e < E; ++e) s[2] += in.f[e] * in.f[e];
         }
-        team_add<TEAM, 3>(s, red, 0);
+        team_add<TEAM, 3>(s, red, turn);
         const float rf = p.post ? 1.0f / sqrtf(s[2] * inv_d + p.eps) : 1.0f;
         float D[E];
 #pragma unroll
@@ -263,7 +268,7 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualP
         }
         if constexpr (GATE == ADN_GATE_ELEMENT)
             if (p.dgate) put_row<T, TEAM, E, VEC>((T *)p.dgate + row * p.dgate_stride, p.d, lane, dg);
-        team_add<TEAM, 2>(t, red, 1);
+        team_add<TEAM, 2>(t, red, turn);
         if (GATE == ADN_GATE_ROW && p.dgate && lane == 0) ((float *)p.dgate)[row] = t[1] * slope_r;
         if (p.df) {
             const float k = p.post ? rf * rf * (t[0] * inv_d) : 0.0f;

@@ -2269,14 +2269,14 @@ int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors,
         int64_t total = 0, block = 0;
         for (int64_t i = 0; i < n_tensors; ++i) {
             const adn_adamw_tensor &t = tensors[i];
-            const std::string at = " of tensor " + std::to_string(i);
-            if (t.n < 0 || t.n > (1ll << 40)) return fail(ADN_E_INVALID, "n must be in [0, 2^40]" + at);
-            if (t.reserved) return fail(ADN_E_INVALID, "reserved must be 0" + at);
-            if (t.grad_dtype != ADN_T_F32 && t.grad_dtype != ADN_T_BF16) return fail(ADN_E_INVALID, "unknown grad_dtype" + at);
+            auto at = [&](const char *what) { return std::string(what) + " of tensor " + std::to_string(i); };
+            if (t.n < 0 || t.n > (1ll << 40)) return fail(ADN_E_INVALID, at("n") + " must be in [0, 2^40]");
+            if (t.reserved) return fail(ADN_E_INVALID, at("reserved") + " must be 0");
+            if (t.grad_dtype != ADN_T_F32 && t.grad_dtype != ADN_T_BF16) return fail(ADN_E_INVALID, "unknown " + at("grad_dtype"));
             auto span = [&](const char *what, const void *p, int64_t bytes, int align, bool wanted, bool written) -> std::string {
-                if (wanted && t.n > 0 && !p) return std::string("null ") + what + at;
-                if (!wanted && p) return std::string(what) + at + " does not go with the list's state_bits";
-                if ((uintptr_t)p % align) return std::string(what) + at + " is not aligned to its elements";
+                if (wanted && t.n > 0 && !p) return "null " + at(what);
+                if (!wanted && p) return at(what) + " does not go with the list's state_bits";
+                if ((uintptr_t)p % align) return at(what) + " is not aligned to its elements";
                 if (p && bytes) spans.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
                 return "";
             };
@@ -2289,7 +2289,7 @@ int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors,
                                         span("v_scale", t.v_scale, blocks * 4, 4, eight, true),
                                         t.copy || grads_alone ? span("copy", t.copy, t.n * 2, 2, !grads_alone, true) : ""});
             if (msg.empty() && !grads_alone && !(std::isfinite(t.lr_scale) && std::isfinite(t.weight_decay)))
-                msg = "lr_scale and weight_decay must be finite" + at;
+                msg = at("lr_scale or weight_decay") + " is not finite";
             if (!msg.empty()) return fail(ADN_E_INVALID, msg);
             OptTensor &r = recs[(size_t)i];
             r.param = t.param, r.grad = t.grad, r.copy = (__bf16 *)t.copy, r.m = t.m, r.v = t.v;

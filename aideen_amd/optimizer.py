@@ -56,10 +56,11 @@ class AdamW:
             raise _invalid("m, v and step go together")
         if len(params) != k:
             raise _invalid(f"as many grads as params expected ({len(params)}), got {k}")
+        either, single = (T["f32"], T["bf16"]), (T["f32"],)
         for i, (p, g) in enumerate(zip(params, grads)):
-            self._check(g, f"grads[{i}]", (T["f32"], T["bf16"]), None)
+            self._check(g, "grads", i, either, None)
             if not alone:
-                self._check(p, f"params[{i}]", (T["f32"],), g.numel())
+                self._check(p, "params", i, single, g.numel())
         if not alone and not any(given):
             if m_scale is not None or v_scale is not None:
                 raise _invalid("scales without states")
@@ -75,25 +76,23 @@ class AdamW:
             for name, x in (("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale), ("copies", copies)):
                 if len(x) != k:
                     raise _invalid(f"{name} must have {k} entries, got {len(x)}")
-            self._check(step, "step", (T["i32"],), 1)
+            self._check(step, "step", None, (T["i32"],), 1)
         decay, scale = self._numbers(weight_decay, "weight_decay", k), self._numbers(lr_scale, "lr_scale", k)
+        kinds, f32, block = T["codes"] if eight else (T["f32"],), T["f32"], _lib.ADAMW_BLOCK
         recs = (_lib.AdnAdamwTensor * max(k, 1))()
-        kinds = T["codes"] if eight else (T["f32"],)
-        for i, (p, g) in enumerate(zip(params, grads)):
-            r, n = recs[i], g.numel()
-            r.grad, r.n, r.grad_dtype = g.data_ptr(), n, _lib.ADN_T_F32 if g.dtype == T["f32"] else _lib.ADN_T_BF16
+        for i, g in enumerate(grads):
+            n, dtype = g.numel(), _lib.ADN_T_F32 if g.dtype is f32 else _lib.ADN_T_BF16
             if alone:
+                recs[i] = (None, g.data_ptr(), None, None, None, None, None, n, 1.0, 0.0, dtype, 0)
                 continue
-            self._check(m[i], f"m[{i}]", kinds, n), self._check(v[i], f"v[{i}]", kinds, n)
-            r.param, r.m, r.v, r.lr_scale, r.weight_decay = p.data_ptr(), m[i].data_ptr(), v[i].data_ptr(), scale[i], decay[i]
+            mp, vp, cp = self._check(m[i], "m", i, kinds, n), self._check(v[i], "v", i, kinds, n), None
+            ms = vs = None
             if eight:
-                blocks = -(-n // _lib.ADAMW_BLOCK)
-                self._check(m_scale[i], f"m_scale[{i}]", (T["f32"],), blocks)
-                self._check(v_scale[i], f"v_scale[{i}]", (T["f32"],), blocks)
-                r.m_scale, r.v_scale = m_scale[i].data_ptr(), v_scale[i].data_ptr()
+                blocks = -(-n // block)
+                ms, vs = self._check(m_scale[i], "m_scale", i, (f32,), blocks), self._check(v_scale[i], "v_scale", i, (f32,), blocks)
             if copies[i] is not None:
-                self._check(copies[i], f"copies[{i}]", (T["bf16"],), n)
-                r.copy = copies[i].data_ptr()
+                cp = self._check(copies[i], "copies", i, (T["bf16"],), n)
+            recs[i] = (params[i].data_ptr(), g.data_ptr(), cp, mp, vp, ms, vs, n, scale[i], decay[i], dtype, 0)
         if not 0 <= int(seed) < 1 << 64:
             raise _invalid("seed must be in [0, 2^64)")
         cfg = _lib.AdnAdamwConfig(beta1=betas[0], beta2=betas[1], eps=eps, seed=int(seed), state_bits=0 if alone else 8 if eight else 32)
@@ -102,12 +101,15 @@ class AdamW:
         self.params, self.grads, self.copies = params, grads, copies
         self.m, self.v, self.m_scale, self.v_scale, self.step = m, v, m_scale, v_scale, step
 
-    def _check(self, t, name, dtypes, n) -> None:
-        if t.dtype not in dtypes or not t.is_contiguous() or (n is not None and t.numel() != n):
+    def _check(self, t, name, i, dtypes, n):
+        """The pointer of a contiguous tensor of n values (None: any number) on the context's GPU."""
+        if t.dtype not in dtypes or not t.is_contiguous() or (n is not None and t.numel() != n) or t.get_device() != self._device:
+            name = name if i is None else f"{name}[{i}]"
+            if t.dtype in dtypes and t.is_contiguous() and (n is None or t.numel() == n):
+                raise _invalid(f"{name} must be on the context's GPU (cuda:{self._device}), got {t.device}")
             kinds = " or ".join(str(d) for d in dtypes)
             raise _invalid(f"{name} must be a contiguous {kinds} tensor" + ("" if n is None else f" of {n} values"))
-        if t.get_device() != self._device:
-            raise _invalid(f"{name} must be on the context's GPU (cuda:{self._device}), got {t.device}")
+        return t.data_ptr()
 
     @staticmethod
     def _numbers(x, name, k):

@@ -166,6 +166,16 @@ def test_parts(be, gate, post, pre, dz, dtype):
     check(run(be, t, *names_of(t, pre)), ref, tol)
 
 
+@pytest.mark.parametrize("d", [1000, 2048, 5000])
+@pytest.mark.parametrize("post,pre", [(True, False), (False, True), (False, False)])
+def test_wide_rows_with_one_sum_each(be, d, post, pre):
+    """Rows of several waves, many a block, with one reduction a row (or none): the waves' sums have places of their own from row to row."""
+    t = make(6000, d, F32, "none", False, post, pre)
+    if not pre:
+        t["z"] = None
+    check(run(be, t, *names_of(t, pre)), *reference(t, F32))
+
+
 @pytest.mark.parametrize("gate", GATES)
 def test_outputs_apart(be, gate):
     t = make(77, 320, F32, gate, True and gate != "none")
