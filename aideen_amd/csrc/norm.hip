@@ -11,13 +11,99 @@
 // does not depend on the schedule.
 #include <algorithm>
 
-#include "rows.h"
+#include "train.h"
 
 namespace adn {
 
 namespace {
 
+constexpr int NB = 256;          // threads a block
 constexpr int DG_BLOCKS = 512;   // most blocks of the backward pass = partial rows of dg
+
+template <typename T, int W>
+struct VecOf {
+    typedef T type __attribute__((ext_vector_type(W)));
+};
+
+// Where a lane's element e of a row stands: whole 16-byte pieces (VEC: 4 fp32 or 8 bf16 values
+// each) or single elements, `TEAM` lanes side by side in both.
+template <typename T, int TEAM, bool VEC>
+struct Cols {
+    static constexpr int W = VEC ? 16 / (int)sizeof(T) : 1;
+    __device__ __forceinline__ static int col(int lane, int e) { return ((e / W) * TEAM + lane) * W + e % W; }
+};
+
+// A lane's share of a row as it is loaded: E elements in pieces of W.
+template <typename T, int TEAM, int E, bool VEC>
+struct Row {
+    typedef Cols<T, TEAM, VEC> C;
+    typedef typename VecOf<T, C::W>::type V;
+    V v[E / C::W];
+    __device__ __forceinline__ void load(const T *row, int d, int lane) {
+#pragma unroll
+        for (int q = 0; q < E / C::W; ++q) {
+            const int c = C::col(lane, q * C::W);
+            v[q] = V{};
+            if (c < d) v[q] = *reinterpret_cast<const V *>(row + c);
+        }
+    }
+    __device__ __forceinline__ float operator[](int e) const { return to_f32<T>(v[e / C::W][e % C::W]); }
+};
+
+template <typename T, int TEAM, int E, bool VEC>
+__device__ __forceinline__ void store_row(T *row, int d, int lane, const float (&v)[E]) {
+    typedef Cols<T, TEAM, VEC> C;
+    if constexpr (VEC) {
+        typedef typename VecOf<T, C::W>::type V;
+#pragma unroll
+        for (int e = 0; e < E; e += C::W) {
+            const int c = C::col(lane, e);
+            if (c < d) {
+                V x;
+#pragma unroll
+                for (int j = 0; j < C::W; ++j) x[j] = from_f32<T>(v[e + j]);
+                *reinterpret_cast<V *>(row + c) = x;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int c = C::col(lane, e);
+            if (c < d) row[c] = from_f32<T>(v[e]);
+        }
+    }
+}
+
+// The gain of a lane's columns (1 where there is none; 0 beyond the row is never used).
+template <typename T, int TEAM, int E, bool VEC>
+__device__ __forceinline__ void load_gain(const float *gain, int d, int lane, float (&g)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int c = Cols<T, TEAM, VEC>::col(lane, e);
+        g[e] = gain && c < d ? gain[c] : 1.0f;
+    }
+}
+
+// Sums of N values over the team; every lane of it gets them.
+template <int TEAM, int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float (*red)[NB / 64]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if constexpr (TEAM > 64) {
+        __syncthreads();  // the last row's sums have been read
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) red[i][threadIdx.x >> 6] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < TEAM / 64; ++w) s += red[i][w];
+            v[i] = s;
+        }
+    }
+}
 
 template <typename T, int TEAM, int E, bool VEC>
 __global__ __launch_bounds__(NB) void k_rms_norm(NormParams p) {
@@ -104,12 +190,9 @@ __global__ __launch_bounds__(NB) void k_rms_norm_back(NormParams p, float *part)
     }
 }
 
-// A vector's sum over its n partial rows: 16 waves of a block each take a share of the rows of 64 columns
+// dst[c] = sum over the n partial rows: 16 waves of a block each take a share of the rows of 64 columns
 // in order, then the shares in order.
-__global__ __launch_bounds__(1024) void k_sum_rows(const float *part, int n, int d, SumRows to) {
-    float *const dst = to.dst[blockIdx.y];
-    if (!dst) return;
-    part += (long)blockIdx.y * n * d;
+__global__ __launch_bounds__(1024) void k_sum_rows(const float *part, int n, int d, float *dst) {
     constexpr int WAVES = 16;
     __shared__ float red[WAVES][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -150,10 +233,6 @@ int back_blocks(const NormParams &p) {
 }
 
 }  // namespace
-
-void launch_sum_rows(const float *part, int n, int d, const SumRows &to, int vectors, hipStream_t st) {
-    k_sum_rows<<<dim3((d + 63) / 64, vectors), 1024, 0, st>>>(part, n, d, to);
-}
 
 void launch_norm(const NormParams &p, hipStream_t st) {
     if (p.rows == 0) return;
@@ -199,7 +278,7 @@ void launch_norm_backward(const NormParams &p, void *ws, hipStream_t st) {
                     k_rms_norm_back<T, TEAM, E, false><<<blocks, NB, 0, st>>>(p, part);
             });
         });
-    if (p.dg) launch_sum_rows(part, blocks, p.d, SumRows{{p.dg}}, 1, st);
+    if (p.dg) k_sum_rows<<<(p.d + 63) / 64, 1024, 0, st>>>(part, blocks, p.d, p.dg);
 }
 
 }  // namespace adn

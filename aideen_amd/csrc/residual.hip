@@ -9,13 +9,13 @@
 //   df = rf (b - f rf^2 mean(b f)),  b = dn gp;   dgp = sum over the rows of dn f rf;  dgq of dy z rz
 //
 // A team of lanes owns a row and keeps all of its tensors in registers between the reductions, so
-// that each is read or written once and HBM is the bound.  Sums in fp32.  Rows of up to 1024
-// elements are a wave's (no barriers), longer ones a block's.  In the backward pass a team walks its
-// share of the rows and keeps the column sums in registers; the blocks' sums are written as partials
-// and added in a fixed order.
+// that each is read or written once and HBM is the bound.  Sums in fp32.  Rows of up to 512
+// elements are a wave's (no barriers), longer ones a block's of 2, 4 or 8 waves.  A team walks its share of
+// the rows, the next one loaded while one is used; in the backward pass it keeps the column sums in
+// registers, the blocks' sums are written as partials and added in a fixed order.
 #include <algorithm>
 
-#include "rows.h"
+#include "train.h"
 
 namespace adn {
 
@@ -25,6 +25,7 @@ namespace {
 // memory's open pages (8192 x 512 fp32 forward: 512 blocks 13.8 us, 1024 15.2, 2048 19.5; 32749 x 2048 bf16: 768
 // blocks 136, 1024 132, 2048 148; backward: 32749 x 2048 bf16 256 blocks 268, 512 217, 1024 239, 2048 243).
 constexpr int ROW_BLOCKS = 512, WIDE_BLOCKS = 768;  // forward: of rows of a wave, and longer ones
+constexpr int NB = 256;           // threads of a block of four waves' teams
 constexpr int MAX_TEAM = 512;     // lanes of the longest rows
 constexpr int COL_BLOCKS = 512;  // most blocks of the backward pass = partial rows of a column sum
 
@@ -80,42 +81,56 @@ __device__ __forceinline__ void team_add(float (&v)[N], float (*red)[3][MAX_TEAM
     }
 }
 
-// A row's share of a lane, STREAM: past the caches.
-template <bool STREAM, typename T, int TEAM, int E, bool VEC>
-__device__ __forceinline__ void take_row(Row<T, TEAM, E, VEC> &r, const T *row, int d, int lane) {
-    typedef Row<T, TEAM, E, VEC> R;
-    if constexpr (!STREAM) return r.load(row, d, lane);
+// A lane's share of a row: E elements, TEAM lanes side by side, in whole aligned pieces of 16 bytes (VEC) or by single elements.
+// Pieces that are not aligned cost more than elements do (8191 x 777 fp32 backward 45 us by elements, 82 by pieces at any address; 20000 x 1535
+// bf16 133 and 405).  STREAM: past the caches, as all stores of pieces go.
+template <typename T, int TEAM, bool VEC>
+struct Row {
+    static constexpr int E = elements(TEAM), W = VEC ? 16 / (int)sizeof(T) : 1;
+    typedef T V __attribute__((ext_vector_type(W)));
+    V v[E / W];
+    __device__ __forceinline__ static int col(int lane, int e) { return ((e / W) * TEAM + lane) * W + e % W; }
+    __device__ __forceinline__ float operator[](int e) const { return to_f32<T>(v[e / W][e % W]); }
+    template <bool STREAM>
+    __device__ __forceinline__ void load(const T *row, int d, int lane) {
 #pragma unroll
-    for (int q = 0; q < E / R::C::W; ++q) {
-        const int c = R::C::col(lane, q * R::C::W);
-        r.v[q] = typename R::V{};
-        if (c < d) r.v[q] = __builtin_nontemporal_load(reinterpret_cast<const typename R::V *>(row + c));
+        for (int q = 0; q < E / W; ++q) {
+            const int c = col(lane, q * W);
+            v[q] = V{};
+            if (c < d) {
+                if constexpr (STREAM)
+                    v[q] = __builtin_nontemporal_load(reinterpret_cast<const V *>(row + c));
+                else
+                    v[q] = *reinterpret_cast<const V *>(row + c);
+            }
+        }
     }
-}
-
-template <typename T, int TEAM, int E, bool VEC>
-__device__ __forceinline__ void put_row(T *row, int d, int lane, const float (&v)[E]) {
-    typedef Row<T, TEAM, E, VEC> R;
+    __device__ __forceinline__ static void store(T *row, int d, int lane, const float (&x)[E]) {
 #pragma unroll
-    for (int q = 0; q < E / R::C::W; ++q) {
-        const int c = R::C::col(lane, q * R::C::W);
-        typename R::V x;
+        for (int q = 0; q < E / W; ++q) {
+            const int c = col(lane, q * W);
+            V y;
 #pragma unroll
-        for (int j = 0; j < R::C::W; ++j) x[j] = from_f32<T>(v[q * R::C::W + j]);
-        if (c < d) __builtin_nontemporal_store(x, reinterpret_cast<typename R::V *>(row + c));
+            for (int j = 0; j < W; ++j) y[j] = from_f32<T>(x[q * W + j]);
+            if (c < d) {
+                if constexpr (VEC)
+                    __builtin_nontemporal_store(y, reinterpret_cast<V *>(row + c));
+                else
+                    *reinterpret_cast<V *>(row + c) = y;
+            }
+        }
     }
-}
+};
 
 // What a lane has of a row's inputs, loaded ahead.
 template <typename T, int TEAM, bool VEC, bool STREAM, bool BACK>
 struct Inputs {
-    static constexpr int E = elements(TEAM);
-    typedef Row<T, TEAM, E, VEC> R;
+    typedef Row<T, TEAM, VEC> R;
     R a, f, g, dz, dy;  // a: x, or z in the backward pass
     float row_gate;
     __device__ __forceinline__ void load(const ResidualParams &p, long row, int lane) {
         auto take = [&](R &r, const void *base, long stride) {
-            take_row<STREAM>(r, (const T *)base + row * stride, p.d, lane);
+            r.template load<STREAM>((const T *)base + row * stride, p.d, lane);
         };
         take(f, p.f, p.f_stride);
         if constexpr (BACK) {
@@ -132,7 +147,7 @@ struct Inputs {
 template <typename T, int TEAM, bool VEC, bool STREAM>
 __global__ __launch_bounds__(block_threads(TEAM)) void k_residual(ResidualParams p) {
     __shared__ float red[2][3][MAX_TEAM / 64];
-    typedef Cols<T, TEAM, VEC> C;
+    typedef Row<T, TEAM, VEC> C;
     constexpr int E = elements(TEAM), TEAMS = block_threads(TEAM) / TEAM;
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
     const long step = (long)gridDim.x * TEAMS;
@@ -173,13 +188,13 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual(ResidualParams
             v[e] = p.keep * in.a[e] + n;
             s[0] += v[e] * v[e];
         }
-        if (p.z) put_row<T, TEAM, E, VEC>((T *)p.z + row * p.z_stride, p.d, lane, v);
+        if (p.z) C::store((T *)p.z + row * p.z_stride, p.d, lane, v);
         if (p.y) {
             team_add<TEAM, 1>(s, red, turn);
             const float rz = 1.0f / sqrtf(s[0] * inv_d + p.eps);
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] *= rz * gq[e];
-            put_row<T, TEAM, E, VEC>((T *)p.y + row * p.y_stride, p.d, lane, v);
+            C::store((T *)p.y + row * p.y_stride, p.d, lane, v);
         }
         in = next;
     }
@@ -190,14 +205,15 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual(ResidualParams
 template <typename T, int TEAM, bool VEC, bool STREAM, uint32_t GATE>
 __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualParams p, float *part) {
     __shared__ float red[2][3][MAX_TEAM / 64];
-    typedef Cols<T, TEAM, VEC> C;
+    typedef Row<T, TEAM, VEC> C;
     constexpr int E = elements(TEAM), TEAMS = block_threads(TEAM) / TEAM;
     p.gate_kind = GATE;
     const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
     const long step = (long)gridDim.x * TEAMS;
     long row = (long)blockIdx.x * TEAMS + team;
+    constexpr bool AHEAD = TEAM < MAX_TEAM;  // the next row is loaded while this one is used, where there are registers
     Inputs<T, TEAM, VEC, STREAM, true> in, next;
-    if (row < p.rows) in.load(p, row, lane);
+    if (AHEAD && row < p.rows) in.load(p, row, lane);
     float w[E], gq[E], A[E], dgq[E], slope;  // w: the gain, times a gate of the channels
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -213,7 +229,10 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualP
     const float inv_d = 1.0f / (float)p.d;
     int turn = 0;
     for (; row < p.rows; row += step) {
-        if (row + step < p.rows) next.load(p, row + step, lane);
+        if (!AHEAD)
+            in.load(p, row, lane);
+        else if (row + step < p.rows)
+            next.load(p, row + step, lane);
         float s[3] = {0.0f, 0.0f, 0.0f};
         if (p.dy) {
 #pragma unroll
@@ -243,7 +262,7 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualP
             float v[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = p.keep * D[e];
-            put_row<T, TEAM, E, VEC>((T *)p.dx + row * p.dx_stride, p.d, lane, v);
+            C::store((T *)p.dx + row * p.dx_stride, p.d, lane, v);
         }
         // D becomes b = scale D s gp
         float slope_r = 1.0f, gate_r = 1.0f, t[2] = {0.0f, 0.0f};
@@ -267,16 +286,16 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualP
             t[0] += D[e] * in.f[e];
         }
         if constexpr (GATE == ADN_GATE_ELEMENT)
-            if (p.dgate) put_row<T, TEAM, E, VEC>((T *)p.dgate + row * p.dgate_stride, p.d, lane, dg);
+            if (p.dgate) C::store((T *)p.dgate + row * p.dgate_stride, p.d, lane, dg);
         team_add<TEAM, 2>(t, red, turn);
         if (GATE == ADN_GATE_ROW && p.dgate && lane == 0) ((float *)p.dgate)[row] = t[1] * slope_r;
         if (p.df) {
             const float k = p.post ? rf * rf * (t[0] * inv_d) : 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) D[e] = rf * (D[e] - in.f[e] * k);
-            put_row<T, TEAM, E, VEC>((T *)p.df + row * p.df_stride, p.d, lane, D);
+            C::store((T *)p.df + row * p.df_stride, p.d, lane, D);
         }
-        in = next;
+        if (AHEAD) in = next;
     }
     if (!part) return;
     // the block's teams in order, then one partial row a block of A and of dgq
@@ -379,10 +398,9 @@ void dispatch_gate(uint32_t kind, F &&f) {
 void launch_residual(const ResidualParams &p, hipStream_t st) {
     if (p.rows == 0) return;
     const int eb = elem_bytes(p.dtype);
-    const bool element = p.gate_kind == ADN_GATE_ELEMENT;
-    const bool vec = rows_vec16(p.x, p.x_stride, p.d, eb) && rows_vec16(p.f, p.f_stride, p.d, eb) &&
-                     (!p.z || rows_vec16(p.z, p.z_stride, p.d, eb)) && (!p.y || rows_vec16(p.y, p.y_stride, p.d, eb)) &&
-                     (!element || rows_vec16(p.gate, p.gate_stride, p.d, eb));
+    auto ok = [&](const void *q, long stride) { return !q || rows_vec16(q, stride, p.d, eb); };
+    const bool vec = ok(p.x, p.x_stride) && ok(p.f, p.f_stride) && ok(p.z, p.z_stride) && ok(p.y, p.y_stride) &&
+                     (p.gate_kind != ADN_GATE_ELEMENT || ok(p.gate, p.gate_stride));
     dispatch_type(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         dispatch_row(p.d, [&](auto team) {
@@ -403,12 +421,10 @@ size_t residual_backward_workspace_bytes(const ResidualParams &p) {
 }
 
 void launch_residual_backward(const ResidualParams &p, void *ws, hipStream_t st) {
-    const int eb = elem_bytes(p.dtype), blocks = back_blocks(p);
-    const bool element = p.gate_kind == ADN_GATE_ELEMENT;
+    const int blocks = back_blocks(p), eb = elem_bytes(p.dtype);
     auto ok = [&](const void *q, long stride) { return !q || rows_vec16(q, stride, p.d, eb); };
-    const bool vec = ok(p.z, p.z_stride) && ok(p.f, p.f_stride) && ok(p.dz, p.dz_stride) && ok(p.dy, p.dy_stride) &&
-                     ok(p.dx, p.dx_stride) && ok(p.df, p.df_stride) &&
-                     (!element || (ok(p.gate, p.gate_stride) && ok(p.dgate, p.dgate_stride)));
+    const bool vec = ok(p.z, p.z_stride) && ok(p.f, p.f_stride) && ok(p.dz, p.dz_stride) && ok(p.dy, p.dy_stride) && ok(p.dx, p.dx_stride) &&
+                     ok(p.df, p.df_stride) && (p.gate_kind != ADN_GATE_ELEMENT || (ok(p.gate, p.gate_stride) && ok(p.dgate, p.dgate_stride)));
     float *part = column_sums(p) ? (float *)ws : nullptr;
     if (blocks)
         dispatch_type(p.dtype, [&](auto t) {

@@ -118,7 +118,7 @@ struct OptTensor {  // one tensor of the list
     int64_t block;           // the list's number of its first block of 256 values
     float lr_scale, decay;
     uint32_t grad_bf16;
-    uint32_t pad_;
+    uint32_t pad;
 };
 struct OptChunk {  // a share of a tensor
     int32_t tensor, chunk;
