@@ -388,6 +388,8 @@ class GpuDeqBackend:
         """The first 16 fields of the arguments, those before x left out: (head, f to pre_gain, the kind of gate)."""
         dtype = f.dtype
         kind = 0 if gate is None else 1 if gate.dim() == 1 else 3
+        if kind == 3 and gate.dim() != 2:
+            raise _invalid("the gate must be a vector or a matrix")
         if kind == 3 and gate.shape[1] == 1 and (d > 1 or dtype != gate.dtype):
             kind = 2
         g, gs = (None, 0) if kind == 0 else self._gate(kind, gate, "gate", rows, d, dtype)

@@ -36,13 +36,17 @@ constexpr int elements(int team) { return team < MAX_TEAM ? 8 : 16; }
 constexpr int block_threads(int team) { return team > 64 ? team : NB; }
 
 // The gate's value s and ds / dgate.  The exponential is taken of -|g|: it cannot overflow, and
-// s (1 - s) = t / (1 + t)^2 loses nothing where s is near 1.
+// s (1 - s) = t / (1 + t)^2 loses nothing where s is near 1.  exp(a) = 2^e (1 + ln 2 r), e the rounded and r what the
+// rounding of a log2(e) leaves; 2^e and the reciprocal to 1 ulp.
 __device__ __forceinline__ float gate_value(float g, bool sigmoid, float &slope) {
     if (!sigmoid) {
         slope = 1.0f;
         return g;
     }
-    const float t = expf(-fabsf(g)), i = 1.0f / (1.0f + t);
+    constexpr float LOG2E = 1.44269502f, REST = 1.92596303e-8f, LN2 = 0.693147182f;
+    const float a = -fabsf(g) < -150.0f ? -150.0f : -fabsf(g);  // below, the exponential is 0 (and a NaN stays)
+    const float e = a * LOG2E, r = fmaf(a, REST, fmaf(a, LOG2E, -e));
+    const float p = __builtin_amdgcn_exp2f(e), t = fmaf(p, LN2 * r, p), i = __builtin_amdgcn_rcpf(1.0f + t);
     slope = t * i * i;
     return g >= 0.0f ? i : t * i;
 }

@@ -154,12 +154,13 @@ class AdamW:
             raise _invalid("the optimizer is closed")
         s = _lib.AdnAdamwStep(max_norm=max_norm, grad_scale=grad_scale)
         vector = self._backend._vector
-        if lr is None:
-            raise _invalid("lr must be a number or a tensor of one value")
-        if isinstance(lr, (int, float)):
-            s.lr = lr
-        else:
+        if hasattr(lr, "data_ptr"):
             s.lr_device = vector(lr, "lr", 1)
+        else:
+            try:
+                s.lr = float(lr)
+            except (TypeError, ValueError):
+                raise _invalid("lr must be a number or a tensor of one value") from None
         s.grad_norm = vector(grad_norm, "grad_norm", 1)
         check(lib().adn_adamw_step_async(self._opt, C.byref(s)))
 

@@ -535,7 +535,7 @@ def test_refused_lists(be, kw):
 def test_refused_steps(be):
     opt, alone = be.adamw([torch.zeros(9, device="cuda")], [torch.zeros(9, device="cuda")]), be.adamw(None, [torch.zeros(9, device="cuda")])
     norm = torch.zeros(1, device="cuda")
-    for kw in (dict(), dict(lr=float("nan")), dict(lr=1.0, max_norm=1.0), dict(lr=1.0, max_norm=-1.0, grad_norm=norm), dict(lr=1.0, grad_scale=0.0),
+    for kw in (dict(), dict(lr="fast"), dict(lr=float("nan")), dict(lr=1.0, max_norm=1.0), dict(lr=1.0, max_norm=-1.0, grad_norm=norm), dict(lr=1.0, grad_scale=0.0),
                dict(lr=1.0, grad_scale=float("inf")), dict(lr=1.0, max_norm=float("nan"), grad_norm=norm), dict(lr=torch.zeros(2, device="cuda")),
                dict(lr=1.0, grad_norm=torch.zeros(1))):
         with pytest.raises(AdnError) as ei:
@@ -545,6 +545,8 @@ def test_refused_steps(be):
         alone.step_async(lr=1.0)
     with pytest.raises(AdnError):
         opt.grad_norm_async(torch.zeros(2, device="cuda"))
+    opt.step_async(lr=np.float32(1e-3))  # any number
+    be.synchronize()
     opt.close()
     for f in (lambda: opt.step_async(lr=1.0), lambda: opt.grad_norm_async(norm)):
         with pytest.raises(AdnError):

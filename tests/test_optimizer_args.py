@@ -53,6 +53,8 @@ def test_structs_match_the_header(name, mirror, size):
     lambda b, m, v: b.residual_norm_async(m, m, outputs=dict(z=m), gate=v),
     lambda b, m, v: b.residual_norm_async(m, m, outputs=dict(z=m), gate=m[:2]),
     lambda b, m, v: b.residual_norm_async(m, m, outputs=dict(z=m), gate=m[:3, :1]),
+    lambda b, m, v: b.residual_norm_async(m, m, outputs=dict(z=m), gate=v.sum()),
+    lambda b, m, v: b.residual_norm_async(m, m, outputs=dict(z=m), gate=m[None]),
     lambda b, m, v: b.residual_norm_backward_async(m, m, outputs=dict(dz=m)),
     lambda b, m, v: b.residual_norm_backward_async(m, m, dy=m, outputs=dict(dgate=m)),
     lambda b, m, v: b.residual_norm_backward_async(m, m, dy=m[:1], outputs=dict(dx=m)),
