@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 import torch
 
-from aideen_amd import synth
+from aideen_amd import _lib, synth
 from aideen_amd._lib import ADN_E_INVALID, AdnError
 from aideen_amd.backend import GpuDeqBackend
 
@@ -324,6 +324,18 @@ def test_a_gradient_that_is_not_a_number(be, bits, bad):
         assert torch.equal(a[0][same].float(), b[0][same].float())
 
 
+def test_moments_at_the_end_of_fp32(be):
+    """m of 2^127 and more could be rounded to 2^128: its block is not a number; half of that is."""
+    for g, bad in ((3.0e38, True), (1.6e38, False)):
+        lst = List([256], 8)
+        lst.g[0].fill_(0)
+        lst.g[0][3] = g
+        one_step(be, lst, betas=(0.0, 0.999))
+        assert bool(torch.isnan(lst.ms[0][0])) == bad and bool(torch.isnan(lst.vs[0][0]))
+        if not bad:
+            assert bool(torch.isfinite(lst.m[0].float() * lst.ms[0]).all())
+
+
 def test_v_beyond_fp32(be):
     lst = List([256], 8)
     lst.g[0][3] = 1e21
@@ -551,6 +563,58 @@ def test_refused_steps(be):
     for f in (lambda: opt.step_async(lr=1.0), lambda: opt.grad_norm_async(norm)):
         with pytest.raises(AdnError):
             f()
+
+
+@pytest.mark.parametrize("bits", [32, 8, 0])
+@pytest.mark.parametrize("what", ["null grad", "null param", "null m", "odd grad", "odd param", "odd copy", "grad_dtype", "reserved", "negative n", "scale", "step",
+                                  "config", "bits", "count", "list"])
+def test_refused_by_the_library(be, bits, what):
+    import ctypes as C
+    t = {k: torch.zeros(600, device="cuda") for k in ("p", "g", "m", "v", "ms", "vs", "c")}
+    step = torch.zeros(1, device="cuda", dtype=torch.int32)
+    a = {k: v.data_ptr() for k, v in t.items()}
+    r = (_lib.AdnAdamwTensor * 1)()
+    r[0] = ((None, a["g"], None, None, None, None, None, 512, 1.0, 0.0, 0, 0) if bits == 0 else
+            (a["p"], a["g"], a["c"], a["m"], a["v"], a["ms"] if bits == 8 else None, a["vs"] if bits == 8 else None, 512, 1.0, 0.0, 0, 0))
+    cfg = _lib.AdnAdamwConfig(0.9, 0.999, 1e-8, 0, step.data_ptr() if bits else None, bits, 0)
+    n, recs, opt = 1, r, C.c_void_p()
+    L = _lib.lib()
+    assert L.adn_adamw_create(be._ctx, C.byref(cfg), n, recs, C.byref(opt)) == 0
+    L.adn_adamw_destroy(opt)
+    if what == "null grad":
+        r[0].grad = None
+    elif what == "null param":  # or one that does not belong there
+        r[0].param = None if bits else a["p"]
+    elif what == "null m":
+        r[0].m = None if bits else a["m"]
+    elif what == "odd grad":
+        r[0].grad = a["g"] + 2
+    elif what == "odd param":
+        r[0].param = a["p"] + 1
+    elif what == "odd copy":
+        r[0].copy = a["c"] + 1
+    elif what == "grad_dtype":
+        r[0].grad_dtype = 2
+    elif what == "reserved":
+        r[0].reserved = 1
+    elif what == "negative n":
+        r[0].n = -1
+    elif what == "scale":
+        r[0].m_scale = None if bits == 8 else a["ms"]
+    elif what == "step":
+        cfg.step = step.data_ptr() + 1 if bits else None
+        cfg.state_bits = bits or 32
+    elif what == "config":
+        cfg.reserved = 1
+    elif what == "bits":
+        cfg.state_bits = 16
+    elif what == "count":
+        n = -1
+    elif what == "list":
+        recs = None
+    opt = C.c_void_p(5)
+    assert L.adn_adamw_create(be._ctx, C.byref(cfg), n, recs, C.byref(opt)) == ADN_E_INVALID
+    assert L.adn_last_error().decode() and not opt.value
 
 
 def test_a_context_that_goes_first():
