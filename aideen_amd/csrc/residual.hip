@@ -294,9 +294,11 @@ __global__ __launch_bounds__(block_threads(TEAM)) void k_residual_back(ResidualP
         team_add<TEAM, 2>(t, red, turn);
         if (GATE == ADN_GATE_ROW && p.dgate && lane == 0) ((float *)p.dgate)[row] = t[1] * slope_r;
         if (p.df) {
-            const float k = p.post ? rf * rf * (t[0] * inv_d) : 0.0f;
+            if (p.post) {  // without the norm df is b, whatever f holds
+                const float k = rf * rf * (t[0] * inv_d);
 #pragma unroll
-            for (int e = 0; e < E; ++e) D[e] = rf * (D[e] - in.f[e] * k);
+                for (int e = 0; e < E; ++e) D[e] = rf * (D[e] - in.f[e] * k);
+            }
             C::store((T *)p.df + row * p.df_stride, p.d, lane, D);
         }
         if (AHEAD) in = next;
