@@ -245,10 +245,12 @@ struct Block {
             }
         } else {
             const float b1 = (float)P.beta1, c1 = (float)(1.0 - P.beta1), b2 = (float)P.beta2, c2 = (float)(1.0 - P.beta2);
-            const float coef = (float)o.coef;
+            // a coefficient below fp32's normal numbers would lose bits: its power of two is a factor of its own
+            const bool below = o.coef < 0x1p-126;
+            const float low = below ? 0x1p-126f : 1.0f, coef = (float)(below ? o.coef * 0x1p126 : o.coef);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float gj = (float)g.x[j] * coef;
+                const float gj = (float)g.x[j] * coef * low;
                 // fused as written: a block's bits do not depend on how it is loaded
                 m.x[j] = mf[j] = fmaf(b1, m.x[j], c1 * gj);
                 v.x[j] = vf[j] = fmaf(b2, v.x[j], c2 * gj * gj);
