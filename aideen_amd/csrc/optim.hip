@@ -112,11 +112,12 @@ __device__ __forceinline__ bool last_of_grid(unsigned *ticket) {
 }
 
 // p - lr (m / bc1 / (sqrt(v / bc2) + eps) + decay p), the root and the reciprocal to 1 ulp.  The root
-// instruction takes numbers below 2^-126 for zero, which is nothing beside an eps of 1e-10 or more.
+// instruction takes numbers below 2^-126 for zero: what is lost, less than 2^-63 / sqrt(bc2), is nothing
+// beside an eps of 2^25 times that.
 __device__ __forceinline__ void stepped(float (&p)[V], const float (&m)[V], const float (&v)[V], const Scalars &o, float lr,
                                         float decay, float eps) {
     float root[V];
-    if (eps >= 1e-10f) {
+    if (eps >= 0x1p-38f * o.inv_sqrt_bc2) {
 #pragma unroll
         for (int j = 0; j < V; ++j) root[j] = __builtin_amdgcn_sqrtf(v[j]);
     } else {

@@ -6,7 +6,7 @@ import torch
 from aideen_amd import synth
 from aideen_amd._lib import ADN_E_INVALID, AdnError
 from aideen_amd.backend import GpuDeqBackend
-from test_gpu_adamw import List, cfg_of, log
+from test_gpu_adamw import List, cfg_of, log, one_step
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -44,4 +44,20 @@ def test_a_coefficient_below_the_normal_numbers(be, bits, max_norm, grad_scale):
     cfg, before = cfg_of(lst, coef=coef, eps=1e-15), lst.host()
     opt.step_async(lr=1e-3, grad_norm=norm, max_norm=max_norm, grad_scale=grad_scale)
     be.synchronize()
+    lst.check(before, cfg)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_second_moments_below_the_normal_numbers(be, bits):
+    """v' in [2^-127.5, 2^-126], which a bias correction of 2^-30 makes 2^-15 of eps under the root: 512 u of the way, where 36 u are allowed.
+    v' itself is rounded to 2^-150, 1.4 u of its root, which is 2^-15 of the denominator."""
+    lst = List([700, 3], bits)
+    fresh(lst)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for t, p in zip(lst.g, lst.p):
+        t.copy_(2.0 ** -48 * (0.6 + 0.4 * torch.rand(t.shape, device="cuda", generator=g)))
+        t[1::2].neg_()
+        p.zero_()
+    lst.step.zero_()
+    cfg, before, _ = one_step(be, lst, betas=(0.9, 1 - 2.0 ** -30), eps=2.0 ** -33)
     lst.check(before, cfg)
