@@ -117,9 +117,15 @@ struct adn_ctx {
     std::vector<adn_adamw *> optimizers;  // live handles, told when the context goes
 };
 
+struct MemSpan {
+    uintptr_t begin, end;
+    bool written;
+};
+
 struct adn_adamw {
     adn_ctx *ctx = nullptr;  // null once the context is destroyed
     OptPlan plan{};
+    std::vector<MemSpan> written, grads;  // what a step writes, and reads only
 };
 
 namespace {
@@ -2176,10 +2182,6 @@ std::string residual_params(const adn_residual_norm_args *a, ResidualParams &p) 
 }
 
 // What a list of tensors writes must not meet itself or what it reads.
-struct MemSpan {
-    uintptr_t begin, end;
-    bool written;
-};
 bool spans_meet(std::vector<MemSpan> &s) {
     std::sort(s.begin(), s.end(), [](const MemSpan &a, const MemSpan &b) { return a.begin < b.begin; });
     uintptr_t written = 0, any = 0;  // the furthest ends so far
@@ -2189,6 +2191,20 @@ bool spans_meet(std::vector<MemSpan> &s) {
         if (x.written) written = std::max(written, x.end);
     }
     return false;
+}
+
+// Of spans in the order of their beginnings the ones that are written, and those that are only read where
+// they are not within one before; both end in the order of their beginnings, so that they can be searched.
+void keep_spans(adn_adamw *o, const std::vector<MemSpan> &s) {
+    for (const MemSpan &x : s) {
+        auto &v = x.written ? o->written : o->grads;
+        if (v.empty() || x.end > v.back().end) v.push_back(x);
+    }
+}
+bool word_within(const std::vector<MemSpan> &v, const void *p) {
+    const uintptr_t at = (uintptr_t)p;
+    auto x = std::upper_bound(v.begin(), v.end(), at, [](uintptr_t a, const MemSpan &b) { return a < b.end; });  // the first that ends behind it
+    return p && x != v.end() && x->begin < at + 4;
 }
 
 int check_optimizer(const adn_adamw *o) {
@@ -2345,6 +2361,7 @@ int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors,
         p.log_beta1 = std::log(cfg->beta1), p.log_beta2 = std::log(cfg->beta2);
         p.partials = (double *)(dev + at_partials), p.ticket = (unsigned *)(dev + at_ticket);
         opt->ctx = c;
+        keep_spans(opt.get(), spans);
         c->optimizers.push_back(opt.get());
         *out = opt.release();
         return ADN_OK;
@@ -2365,6 +2382,7 @@ int adn_adamw_grad_norm_async(adn_adamw *o, float *norm) {
         const int rc = check_optimizer(o);
         if (rc != ADN_OK) return rc;
         if (!norm || (uintptr_t)norm % 4) return fail(ADN_E_INVALID, "norm is null or not aligned to its elements");
+        if (word_within(o->written, norm) || word_within(o->grads, norm)) return fail(ADN_E_INVALID, "norm overlaps a tensor of the list");
         return train_launch(o->ctx, 0, [&](void *) { launch_grad_norm(o->plan, norm, o->ctx->stream); });
     });
 }
@@ -2379,7 +2397,9 @@ int adn_adamw_step_async(adn_adamw *o, const adn_adamw_step *s) {
                                     s->lr_device || std::isfinite(s->lr) ? "" : "lr must be finite",
                                     s->max_norm >= 0.0f && std::isfinite(s->max_norm) ? "" : "max_norm must be finite and >= 0",
                                     s->max_norm > 0.0f && !s->grad_norm ? "max_norm without grad_norm" : "",
-                                    s->grad_scale > 0.0f && std::isfinite(s->grad_scale) ? "" : "grad_scale must be finite and > 0"});
+                                    s->grad_scale > 0.0f && std::isfinite(s->grad_scale) ? "" : "grad_scale must be finite and > 0",
+                                    word_within(o->written, s->lr_device) || word_within(o->written, s->grad_norm)
+                                        ? "lr_device or grad_norm overlaps what the step writes" : ""});
         if (!msg.empty()) return fail(ADN_E_INVALID, msg);
         const OptStep step{s->lr, s->lr_device, s->grad_norm, s->max_norm, s->grad_scale};
         return train_launch(o->ctx, 0, [&](void *) { launch_adamw(o->plan, step, o->ctx->stream); });

@@ -438,8 +438,9 @@ int adn_residual_norm_backward_async(adn_ctx *ctx, const adn_residual_norm_args 
  * counter.  Equal states, gradients and lists give equal bits.
  * The list is laid out on the device when it is created (which blocks), and stays until the context is
  * destroyed, as captured graphs may use it.  Sizes: up to 2^24 tensors and workgroups, n >= 0 any, any
- * alignment of whole elements.  What a list writes must not overlap itself or its gradients; that is
- * checked.  A handle belongs to its context and stream; after adn_destroy only adn_adamw_destroy takes it. */
+ * alignment of whole elements.  What a step writes must not overlap itself, the gradients, lr_device or
+ * grad_norm, and a norm that is written none of the list's tensors; that is checked.  A handle belongs
+ * to its context and stream; after adn_destroy only adn_adamw_destroy takes it. */
 typedef struct adn_adamw adn_adamw;
 typedef struct adn_adamw_tensor {
     float *param;               /* [n]                                                   */

@@ -1,4 +1,5 @@
-"""AdamW at the ends of its documented range: coefficients and second moments below the normal numbers of fp32 (needs an MI355X).
+"""AdamW at the ends of its documented range: coefficients and second moments below the normal numbers of fp32, arguments within
+the list's own tensors (needs an MI355X).
 Definition and tolerances are those of the optimizer's own tests."""
 import pytest
 import torch
@@ -60,4 +61,38 @@ def test_second_moments_below_the_normal_numbers(be, bits):
         p.zero_()
     lst.step.zero_()
     cfg, before, _ = one_step(be, lst, betas=(0.9, 1 - 2.0 ** -30), eps=2.0 ** -33)
+    lst.check(before, cfg)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_words_of_a_step_within_its_tensors_are_refused(be, bits):
+    """The rate and the norm are read by all workgroups of a step: not from what some of them have written.  The norm is not
+    written over a gradient or a state either; beside them is fine."""
+    flat, norm = torch.zeros(1000, device="cuda"), torch.zeros(1, device="cuda")
+    lst = List([300, 40], bits, copy=lambda i: True)
+    lst.p[1] = flat[500:540]
+    lst.g[1] = flat[600:640]
+    opt = lst.optimizer(be)
+    word = lambda t: t.view(-1).view(torch.uint8)[:4].view(F32)  # noqa: E731
+    written = [lst.p[0][:1], lst.p[0][299:], flat[500:501], flat[539:540], word(lst.m[0]), word(lst.v[1]), opt.step.view(F32)]
+    written += [lst.copy[0][2:4].view(F32)] + ([lst.ms[0][1:], lst.vs[1][:1]] if bits == 8 else [])
+    for w in written:
+        for kw in (dict(lr=w), dict(lr=1.0, grad_norm=w)):
+            with pytest.raises(AdnError) as ei:
+                opt.step_async(**kw)
+            assert ei.value.code == ADN_E_INVALID and "overlap" in str(ei.value)
+    for w in written + [lst.g[0][5:6], flat[600:601], flat[639:640]]:
+        with pytest.raises(AdnError) as ei:
+            opt.grad_norm_async(w)
+        assert ei.value.code == ADN_E_INVALID and "overlap" in str(ei.value)
+    torch.cuda.synchronize()
+    before, cfg = lst.host(), cfg_of(lst)
+    flat[499:500].fill_(1e-3)
+    torch.cuda.synchronize()
+    opt.grad_norm_async(flat[540:541])
+    opt.grad_norm_async(norm)
+    opt.step_async(lr=flat[499:500], grad_norm=flat[540:541])
+    be.synchronize()
+    assert torch.equal(flat[540:541], norm)
+    cfg["lr"] = float(flat[499])
     lst.check(before, cfg)
