@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <cfloat>
 #include <cmath>
 #include <initializer_list>
 #include <memory>
@@ -2394,7 +2395,7 @@ int adn_adamw_step_async(adn_adamw *o, const adn_adamw_step *s) {
         if (!s) return fail(ADN_E_INVALID, "null argument");
         if (o->plan.state_bits == 0) return fail(ADN_E_INVALID, "the list holds gradients alone");
         std::string msg = first_of({check_words("lr_device", s->lr_device), check_words("grad_norm", s->grad_norm),
-                                    s->lr_device || std::isfinite(s->lr) ? "" : "lr must be finite",
+                                    s->lr_device || std::fabs(s->lr) <= FLT_MAX ? "" : "lr must be finite in fp32",
                                     s->max_norm >= 0.0f && std::isfinite(s->max_norm) ? "" : "max_norm must be finite and >= 0",
                                     s->max_norm > 0.0f && !s->grad_norm ? "max_norm without grad_norm" : "",
                                     s->grad_scale > 0.0f && std::isfinite(s->grad_scale) ? "" : "grad_scale must be finite and > 0",

@@ -462,7 +462,7 @@ typedef struct adn_adamw_config {
     uint32_t reserved;          /* 0                                                     */
 } adn_adamw_config;
 typedef struct adn_adamw_step {
-    double lr;
+    double lr;                  /* finite in fp32                                        */
     const float *lr_device;     /* [1] device: in the place of lr, or NULL               */
     const float *grad_norm;     /* [1] device: adn_adamw_grad_norm_async's, or NULL      */
     float max_norm;             /* 0: no clipping; > 0 goes with grad_norm               */

@@ -96,3 +96,20 @@ def test_words_of_a_step_within_its_tensors_are_refused(be, bits):
     assert torch.equal(flat[540:541], norm)
     cfg["lr"] = float(flat[499])
     lst.check(before, cfg)
+
+
+def test_a_rate_beyond_fp32_is_refused(be):
+    lst = List([40], 32)
+    opt = lst.optimizer(be)
+    for lr in (3.5e38, -1e39, 1e300):
+        with pytest.raises(AdnError) as ei:
+            opt.step_async(lr=lr)
+        assert ei.value.code == ADN_E_INVALID
+    for t in lst.g + lst.m:
+        t.zero_()
+    before = lst.p[0].clone()
+    torch.cuda.synchronize()
+    lst.wd = [0.0]
+    lst.optimizer(be).step_async(lr=3.4e38)
+    be.synchronize()
+    assert torch.equal(lst.p[0], before)
