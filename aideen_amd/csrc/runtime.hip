@@ -116,6 +116,7 @@ struct adn_ctx {
     std::vector<DevBuf> tensors;
     std::vector<void *> allocs;
     std::vector<adn_adamw *> optimizers;  // live handles, told when the context goes
+    std::vector<DevBuf> free_tables;      // of optimizers that are gone, for the next ones
 };
 
 struct MemSpan {
@@ -126,6 +127,8 @@ struct MemSpan {
 struct adn_adamw {
     adn_ctx *ctx = nullptr;  // null once the context is destroyed
     OptPlan plan{};
+    DevBuf tables;           // what the plan's pointers are to
+    bool captured = false;   // a graph may read the tables after the handle is gone
     std::vector<MemSpan> written, grads;  // what a step writes, and reads only
 };
 
@@ -2208,6 +2211,31 @@ bool word_within(const std::vector<MemSpan> &v, const void *p) {
     return p && x != v.end() && x->begin < at + 4;
 }
 
+// Device memory of a list's tables: an earlier list's, or new.  In powers of two, so that lists of all sizes leave few
+// kinds behind.  The earlier list's work stands before this one's copy on the stream (adn_set_stream
+// waits for the stream that it leaves).
+DevBuf list_tables(adn_ctx *c, size_t bytes) {
+    size_t size = 64 << 10;
+    while (size < bytes) size *= 2;
+    auto &v = c->free_tables;
+    v.reserve(v.size() + c->optimizers.size() + 1);  // all that can come back
+    for (DevBuf &b : v)
+        if (b.bytes == size) {
+            const DevBuf found = b;
+            b = v.back();
+            v.pop_back();
+            return found;
+        }
+    return {dmalloc(c, size), size};
+}
+
+// Before a launch: one that is captured leaves its tables to the graph.
+void note_capture(adn_adamw *o) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (!o->captured) ADN_HIP(hipStreamIsCapturing(o->ctx->stream, &cap));
+    o->captured |= cap != hipStreamCaptureStatusNone;
+}
+
 int check_optimizer(const adn_adamw *o) {
     if (!o) return fail(ADN_E_INVALID, "null optimizer");
     if (!o->ctx) return fail(ADN_E_INVALID, "the optimizer's context has been destroyed");
@@ -2345,9 +2373,12 @@ int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors,
         if (!recs.empty()) memcpy(host.data() + at_recs, recs.data(), recs.size() * sizeof(OptTensor));
         for (int i = 0; i < 2; ++i)
             if (!chunks[i].empty()) memcpy(host.data() + at_chunks[i], chunks[i].data(), chunks[i].size() * sizeof(OptChunk));
-        auto opt = std::make_unique<adn_adamw>();
+        std::unique_ptr<adn_adamw, void (*)(adn_adamw *)> opt(new adn_adamw, adn_adamw_destroy);
+        keep_spans(opt.get(), spans);
         c->optimizers.reserve(c->optimizers.size() + 1);
-        char *dev = (char *)dmalloc(c, bytes);
+        opt->tables = list_tables(c, bytes);
+        opt->ctx = c;  // from here on the tables go back with the handle
+        char *dev = (char *)opt->tables.p;
         ADN_HIP(hipMemcpyAsync(dev, host.data(), bytes, hipMemcpyHostToDevice, c->stream));
         ADN_HIP(hipStreamSynchronize(c->stream));
         OptPlan &p = opt->plan;
@@ -2361,8 +2392,6 @@ int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors,
         p.beta1 = cfg->beta1, p.beta2 = cfg->beta2, p.eps = (float)cfg->eps, p.seed = cfg->seed, p.step = cfg->step;
         p.log_beta1 = std::log(cfg->beta1), p.log_beta2 = std::log(cfg->beta2);
         p.partials = (double *)(dev + at_partials), p.ticket = (unsigned *)(dev + at_ticket);
-        opt->ctx = c;
-        keep_spans(opt.get(), spans);
         c->optimizers.push_back(opt.get());
         *out = opt.release();
         return ADN_OK;
@@ -2374,6 +2403,7 @@ void adn_adamw_destroy(adn_adamw *o) {
     if (o->ctx) {
         auto &v = o->ctx->optimizers;
         v.erase(std::remove(v.begin(), v.end(), o), v.end());
+        if (!o->captured) o->ctx->free_tables.push_back(o->tables);
     }
     delete o;
 }
@@ -2384,6 +2414,7 @@ int adn_adamw_grad_norm_async(adn_adamw *o, float *norm) {
         if (rc != ADN_OK) return rc;
         if (!norm || (uintptr_t)norm % 4) return fail(ADN_E_INVALID, "norm is null or not aligned to its elements");
         if (word_within(o->written, norm) || word_within(o->grads, norm)) return fail(ADN_E_INVALID, "norm overlaps a tensor of the list");
+        note_capture(o);
         return train_launch(o->ctx, 0, [&](void *) { launch_grad_norm(o->plan, norm, o->ctx->stream); });
     });
 }
@@ -2403,6 +2434,7 @@ int adn_adamw_step_async(adn_adamw *o, const adn_adamw_step *s) {
                                         ? "lr_device or grad_norm overlaps what the step writes" : ""});
         if (!msg.empty()) return fail(ADN_E_INVALID, msg);
         const OptStep step{s->lr, s->lr_device, s->grad_norm, s->max_norm, s->grad_scale};
+        note_capture(o);
         return train_launch(o->ctx, 0, [&](void *) { launch_adamw(o->plan, step, o->ctx->stream); });
     });
 }

@@ -36,7 +36,8 @@ class AdamW:
     ``weight_decay`` and ``lr_scale`` are numbers, or lists with one a tensor.  ``params`` None: a list of
     gradients alone, for ``grad_norm_async``.
 
-    A handle keeps its tensors, and must not outlive what its context's graphs need of them.  Calls only enqueue on
+    A handle keeps its tensors; ``close`` (or its end) gives its device tables to the context's next lists, but for
+    those that a captured call has left to its graph, and a graph's tensors are the caller's to keep.  Calls only enqueue on
     the context's stream; the caller orders it with the streams that fill and read the tensors."""
 
     def __init__(self, backend, params, grads, *, m=None, v=None, m_scale=None, v_scale=None, step=None, copies=None,
