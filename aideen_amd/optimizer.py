@@ -11,6 +11,7 @@ from . import _lib
 from ._lib import check, lib
 
 _TORCH = {}
+_NO_NUMBER = (TypeError, ValueError, RuntimeError, OverflowError)  # what float() and the structures' fields raise
 
 
 def _torch():
@@ -94,9 +95,17 @@ class AdamW:
             if copies[i] is not None:
                 cp = self._check(copies[i], "copies", i, (T["bf16"],), n)
             recs[i] = (params[i].data_ptr(), g.data_ptr(), cp, mp, vp, ms, vs, n, scale[i], decay[i], dtype, 0)
-        if not 0 <= int(seed) < 1 << 64:
-            raise _invalid("seed must be in [0, 2^64)")
-        cfg = _lib.AdnAdamwConfig(beta1=betas[0], beta2=betas[1], eps=eps, seed=int(seed), state_bits=0 if alone else 8 if eight else 32)
+        try:
+            seed = int(seed)
+        except _NO_NUMBER:
+            seed = -1
+        if not 0 <= seed < 1 << 64:
+            raise _invalid("seed must be a number in [0, 2^64)")
+        try:
+            beta1, beta2 = betas
+            cfg = _lib.AdnAdamwConfig(beta1=beta1, beta2=beta2, eps=eps, seed=seed, state_bits=0 if alone else 8 if eight else 32)
+        except _NO_NUMBER:
+            raise _invalid("betas must be two numbers and eps one") from None
         cfg.step = None if alone else step.data_ptr()
         check(lib().adn_adamw_create(backend._ctx, C.byref(cfg), k, recs, C.byref(self._opt)))
         self.params, self.grads, self.copies = params, grads, copies
@@ -114,9 +123,13 @@ class AdamW:
 
     @staticmethod
     def _numbers(x, name, k):
-        if isinstance(x, (int, float)):
-            return [float(x)] * k
-        x = [float(v) for v in x]
+        """[k] floats: a number (of Python, numpy or torch) for all tensors, or one a tensor."""
+        try:
+            if isinstance(x, (int, float)) or getattr(x, "ndim", 1) == 0:
+                return [float(x)] * k
+            x = [float(v) for v in x]
+        except _NO_NUMBER:
+            raise _invalid(f"{name} must be a number or {k} of them") from None
         if len(x) != k:
             raise _invalid(f"{name} must be a number or {k} of them, got {len(x)}")
         return x
@@ -153,14 +166,17 @@ class AdamW:
         grad_scale is a factor of every gradient (and so of the norm)."""
         if not self._opt:
             raise _invalid("the optimizer is closed")
-        s = _lib.AdnAdamwStep(max_norm=max_norm, grad_scale=grad_scale)
+        try:
+            s = _lib.AdnAdamwStep(max_norm=max_norm, grad_scale=grad_scale)
+        except _NO_NUMBER:
+            raise _invalid("max_norm and grad_scale must be numbers") from None
         vector = self._backend._vector
         if hasattr(lr, "data_ptr"):
             s.lr_device = vector(lr, "lr", 1)
         else:
             try:
                 s.lr = float(lr)
-            except (TypeError, ValueError):
+            except _NO_NUMBER:
                 raise _invalid("lr must be a number or a tensor of one value") from None
         s.grad_norm = vector(grad_norm, "grad_norm", 1)
         check(lib().adn_adamw_step_async(self._opt, C.byref(s)))
