@@ -18,7 +18,7 @@ def _torch():
     """torch, and the types that are met here, looked up once."""
     if not _TORCH:
         import torch
-        _TORCH.update(torch=torch, f32=torch.float32, bf16=torch.bfloat16, i32=torch.int32, codes=(torch.float8_e4m3fn, torch.uint8))
+        _TORCH.update(torch=torch, tensor=torch.Tensor, f32=torch.float32, bf16=torch.bfloat16, i32=torch.int32, codes=(torch.float8_e4m3fn, torch.uint8))
     return _TORCH
 
 
@@ -70,7 +70,7 @@ class AdamW:
         eight = False
         if not alone:
             m, v = list(m), list(v)
-            eight = k > 0 and len(m) > 0 and m[0].dtype in T["codes"] or m_scale is not None
+            eight = k > 0 and len(m) > 0 and getattr(m[0], "dtype", None) in T["codes"] or m_scale is not None
             if eight != (m_scale is not None) or eight != (v_scale is not None):
                 raise _invalid("m_scale and v_scale go with states of 8 bits")
             m_scale, v_scale = (list(m_scale), list(v_scale)) if eight else ([None] * k, [None] * k)
@@ -113,6 +113,8 @@ class AdamW:
 
     def _check(self, t, name, i, dtypes, n):
         """The pointer of a contiguous tensor of n values (None: any number) on the context's GPU."""
+        if not isinstance(t, _TORCH["tensor"]):
+            raise _invalid(f"{name if i is None else f'{name}[{i}]'} must be a tensor, got {type(t).__name__}")
         if t.dtype not in dtypes or not t.is_contiguous() or (n is not None and t.numel() != n) or t.get_device() != self._device:
             name = name if i is None else f"{name}[{i}]"
             if t.dtype in dtypes and t.is_contiguous() and (n is None or t.numel() == n):
