@@ -433,9 +433,11 @@ int adn_residual_norm_backward_async(adn_ctx *ctx, const adn_residual_norm_args 
  * magnitude (at least -110): 2 bytes a parameter in the place of 8.  Their moments are formed in 64 bits,
  * used by the step as they are, and rounded to codes stochastically, by 16 random bits a value that are
  * a hash of seed, *step, the value's place in the list (blocks of 256, counted from the first tensor's)
- * and in its block; a v that is not zero keeps a code that is not.  A block whose m or v would hold 2^127
- * or more in magnitude or a NaN gets a scale that is not a number.  A new state is zeros: codes, scales and
- * counter.  Equal states, gradients and lists give equal bits.
+ * and in its block; a v that is not zero keeps a code that is not.  The smallest is about 2^-16 of the
+ * block's largest v: a value whose gradients are less than about 2^-8 of its block's largest takes shorter
+ * steps than with 32 bits.  A block whose m or v would hold 2^127 or more in magnitude or a NaN gets a
+ * scale that is not a number.  A new state is zeros: codes, scales and counter.  Equal states, gradients
+ * and lists give equal bits.
  * The list is laid out on the device when it is created (which blocks).  Destroyed, its tables serve the
  * context's next lists, work in flight notwithstanding; those of a list whose calls have been captured stay
  * until the context is destroyed, as the graphs read them.  Sizes: up to 2^24 tensors and workgroups, n >= 0 any, any
