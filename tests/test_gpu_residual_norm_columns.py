@@ -97,3 +97,21 @@ def test_a_lost_row_would_show(lost):
     short = expected({k: torch.cat([v[:lost], v[lost + 1:]]) if v.dim() == 2 else v for k, v in t.items()}, 0.5, 2.0)
     for k in ("dgate", "dpost_gain", "dpre_gain"):
         assert float((whole[k] != short[k]).float().mean()) > 0.5
+
+
+def test_exact_at_the_most_rows(be):
+    """2^24 rows, of which one in 64 has a gradient: sums of at most 2^20."""
+    rows, d = 1 << 24, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    f = (torch.randint(0, 2, (rows, d), device="cuda", generator=g) * 2 - 1).float()
+    dz = torch.zeros((rows, d), device="cuda")
+    dz[5::64] = torch.randint(1, 3, (rows // 64, d), device="cuda", generator=g).float()
+    gate, gain = torch.full((rows, 1), 0.5, device="cuda"), torch.ones(d, device="cuda")
+    out = dict(dpost_gain=torch.full((d,), 7.0, device="cuda"), df=torch.full_like(f, 7.0), dgate=torch.full_like(gate, 7.0))
+    torch.cuda.synchronize()
+    be.residual_norm_backward_async(None, f, dz=dz, gate=gate, post_gain=gain, scale=2.0, eps=0.0, outputs=out)
+    be.synchronize()
+    D, h = dz.double(), f.double()
+    assert torch.equal(out["dpost_gain"].double(), (D * h).sum(0))
+    assert torch.equal(out["dgate"].double(), 2 * (D * h).sum(1, keepdim=True))
+    assert torch.equal(out["df"].double(), D - h * (D * h).mean(1, keepdim=True))
