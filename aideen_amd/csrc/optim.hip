@@ -38,7 +38,8 @@ __device__ __forceinline__ uint64_t mix64(uint64_t x) {
 }
 constexpr uint64_t GOLDEN = 0x9E3779B97F4A7C15ull;
 
-// 32 random bits of place i of a block whose hash is a (two multiplications, shifts of 16, 15, 16)
+// 32 random bits of place i of a block whose hash is a: a bijection of two multiplications between shifts of 16, 15 and 16, with the
+// constants that C. Wellons found by a search for the least bias (Prospecting for hash functions, 2018)
 __device__ __forceinline__ uint32_t mix32(uint32_t a, uint32_t i) {
     uint32_t r = a + i * 0x9E3779B9u;
     r = (r ^ (r >> 16)) * 0x7FEB352Du;
@@ -347,7 +348,9 @@ __device__ __forceinline__ void add_squares(const T *g, int64_t n, int lane, dou
 // wave's chunks in order, then the workgroups' sums in order by the last one to finish.  A sum is
 // handed over by a read-modify-write of its place, and the workgroup counted once that has returned,
 // so that no cache has to be written back (with a release of the caches in each of 1850 workgroups the
-// kernel took 47 us for 1.9 M values, now 5).
+// kernel took 47 us for 1.9 M values, now 5).  The order is the hardware's, not the memory model's, which knows no order of
+// relaxed operations on two places: an agent-scope read-modify-write is carried out where all XCDs see it before
+// it returns its old value, the use of that value keeps the count behind it, and the sums are read by agent-scope loads.
 __global__ __launch_bounds__(NB) void k_grad_norm(OptPlan P, float *norm) {
     __shared__ double red[NB / 64];
     __shared__ bool last;
@@ -410,8 +413,9 @@ void launch_grad_norm(const OptPlan &p, float *norm, hipStream_t st) {
     k_grad_norm<<<blocks, NB, 0, st>>>(p, norm);
 }
 
-// A list that streams through the caches (more than they hold) is read and written past them: 65 M parameters
-// 313 -> 301 us, 8 bits 207 -> 205; a list that they hold keeps them (1.9 M: 11.4 us, past them 12.8).  With fp32 states
+// A list of more than 8 M parameters (16 M with 8 bits) is read and written past the caches: with lists that take turns, us
+// through them and past them, fp32 states 6 M 31 and 32, 8 M 44 and 41, 12 M 68 and 61, 48 M 262 and 224; 8 bits 8 M 30 and 30, 12 M 44
+// and 40, 20 M 68 and 61; 1.9 M behind a step of its own 11.4 and 12.8.  With fp32 states
 // 32 KB of LDS that nothing uses then keep the workgroups at five a CU, for the same reason as the chunks:
 // 65 M 308 -> 287 us (8 a CU; 6: 304, 4: 289, 2: 340), 206 M with bf16 gradients and copies 977 -> 929.
 void launch_adamw(const OptPlan &p, const OptStep &s, hipStream_t st) {

@@ -21,9 +21,11 @@ namespace adn {
 
 namespace {
 
-// Blocks of a launch, which walk the rows: two to four a CU.  More rows in flight read no faster and spread the
-// memory's open pages (8192 x 512 fp32 forward: 512 blocks 13.8 us, 1024 15.2, 2048 19.5; 32749 x 2048 bf16: 768
-// blocks 136, 1024 132, 2048 148; backward: 32749 x 2048 bf16 256 blocks 268, 512 217, 1024 239, 2048 243).
+// Blocks of a launch, which walk the rows: two a CU, or three in the forward pass of longer rows.  More rows in flight
+// read no faster and spread the memory's open pages (8192 x 512 fp32 forward: 512 blocks 13.8 us, 1024 15.2, 2048 19.5;
+// 32749 x 2048 bf16, a gate an element and without one: 512 blocks 138 and 114, 768 123 and 94, 1024 125 and 97; backward: 256
+// blocks 268, 512 217, 1024 239, 2048 243).  Rows by single elements alone would have more: 20000 x 1535 bf16 forward 65,
+// with 1024 blocks 58.
 constexpr int ROW_BLOCKS = 512, WIDE_BLOCKS = 768;  // forward: of rows of a wave, and longer ones
 constexpr int NB = 256;           // threads of a block of four waves' teams
 constexpr int MAX_TEAM = 512;     // lanes of the longest rows
@@ -37,7 +39,7 @@ constexpr int block_threads(int team) { return team > 64 ? team : NB; }
 
 // The gate's value s and ds / dgate.  The exponential is taken of -|g|: it cannot overflow, and
 // s (1 - s) = t / (1 + t)^2 loses nothing where s is near 1.  exp(a) = 2^e (1 + ln 2 r), e the rounded and r what the
-// rounding of a log2(e) leaves; 2^e and the reciprocal to 1 ulp.
+// rounding of a log2(e) leaves; 2^e and the reciprocal to 1 ulp (a gate below 2^-126 is 0).
 __device__ __forceinline__ float gate_value(float g, bool sigmoid, float &slope) {
     if (!sigmoid) {
         slope = 1.0f;
@@ -374,8 +376,10 @@ void dispatch_row(int d, F &&f) {
 
 bool column_sums(const ResidualParams &p) { return p.dpost || p.dpre || (p.dgate && p.gate_kind == ADN_GATE_CHANNEL); }
 
-// A call whose matrices are more than the caches hold reads past them (backward of 32749 x 2048 bf16, 1.07 GB: 220 -> 200 us; of
-// 8192 x 512 fp32, 101 MB: 23.5 through them, 26.7 past them).
+// A call reads past the caches where three of its matrices (backward six) are more than their 256 MB; it has up to five (up to
+// eight).  What is best depends on what the call finds there: rows of 512 fp32, forward with z alone, us through the caches and past
+// them, 84 MB a matrix: 38 and 41 behind a call on the same tensors, 47 and 42 behind one on others; 101 MB: 45 and 49, 56 and 51;
+// 17 MB: 9.0 and 9.6, 10.1 and 11.3.  Backward, 42 MB: 42 and 48, 52 and 49; 50 MB: 49 and 56, 61 and 57.
 bool streams(const ResidualParams &p, int matrices) {
     return (double)p.rows * p.d * elem_bytes(p.dtype) * matrices > 256e6;
 }

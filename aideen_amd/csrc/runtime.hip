@@ -2387,7 +2387,7 @@ int adn_adamw_create(adn_ctx *c, const adn_adamw_config *cfg, int64_t n_tensors,
         p.n_step_chunks = (int)chunks[0].size(), p.step_values = per[0];
         p.n_norm_chunks = (int)chunks[1].size(), p.norm_values = per[1];
         p.state_bits = (int)cfg->state_bits;
-        // 16 or 10 bytes a parameter against 256 MB of cache beside what else a program has there
+        // 28 or 16 bytes a parameter: more than the caches' 256 MB hold beside what else a program has there (launch_adamw has both sides)
         p.streams = total > (eight ? 16ll : 8ll) << 20;
         p.beta1 = cfg->beta1, p.beta2 = cfg->beta2, p.eps = (float)cfg->eps, p.seed = cfg->seed, p.step = cfg->step;
         p.log_beta1 = std::log(cfg->beta1), p.log_beta2 = std::log(cfg->beta2);

@@ -1,5 +1,6 @@
-// Launch interfaces of the training operators (loss.hip, norm.hip, table.hip): the vocabulary
-// cross entropy, the head's RMS norm and the embedding table, all on caller-owned device tensors.
+// Launch interfaces of the training operators: the vocabulary cross entropy (loss.hip, loss_mid.hip, loss_few.hip), the
+// head's RMS norm (norm.hip), the norms around a residual block (residual.hip), AdamW and the gradients' norm
+// (optim.hip) and the embedding table (table.hip), all on caller-owned device tensors.
 #pragma once
 
 #include "common.h"
@@ -128,7 +129,7 @@ struct OptPlan {  // the list as it stands on the device
     const OptChunk *step_chunks, *norm_chunks;  // a workgroup's of the step, a wave's of the norm
     int n_step_chunks, step_values, n_norm_chunks, norm_values;
     int state_bits;
-    bool streams;            // a step moves more bytes than the caches hold
+    bool streams;            // a step reads and writes past the caches
     double beta1, beta2, log_beta1, log_beta2;
     float eps;
     uint64_t seed;

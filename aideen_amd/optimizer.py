@@ -39,7 +39,8 @@ class AdamW:
 
     A handle keeps its tensors; ``close`` (or its end) gives its device tables to the context's next lists, but for
     those that a captured call has left to its graph, and a graph's tensors are the caller's to keep.  Calls only enqueue on
-    the context's stream; the caller orders it with the streams that fill and read the tensors."""
+    the context's stream; the caller orders it with the streams that fill and read the tensors, and keeps ``lr``, ``grad_norm`` and
+    ``norm`` until then."""
 
     def __init__(self, backend, params, grads, *, m=None, v=None, m_scale=None, v_scale=None, step=None, copies=None,
                  state_bits: int = 32, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, lr_scale=1.0, seed: int = 0):

@@ -371,6 +371,8 @@ int adn_rms_norm_backward_async(adn_ctx *ctx, int32_t rows, int32_t d, uint32_t 
  *   y = z rz pre_gain,  rz = 1 / sqrt(mean(z^2) + eps)    (the next block's or the head's norm)
  * With post_norm, keep = 1 - damping and scale = damping this is the damped update of the Picard
  * iteration (fixed_point_memory_reasoning.rs:1300-1303).  y is formed from z before it is rounded.
+ * Squares are summed in fp32: a row whose sum of them passes it (elements of 2^64 / sqrt(d) and more) has
+ * a norm of 0 in the place of its own.
  * Forward reads x, f, the gate and the gains and writes z and/or y.  Backward reads f, the gate, the
  * gains, the gradients dz (of z by other ways) and/or dy, and, where dy is there, z as the forward
  * wrote it, and writes any of
