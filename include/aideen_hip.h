@@ -442,8 +442,9 @@ int adn_residual_norm_backward_async(adn_ctx *ctx, const adn_residual_norm_args 
  * and lists give equal bits.
  * The list is laid out on the device when it is created (which blocks).  Destroyed, its tables serve the
  * context's next lists, work in flight notwithstanding; those of a list whose calls have been captured stay
- * until the context is destroyed, as the graphs read them.  Sizes: up to 2^24 tensors and workgroups, n >= 0 any, any
- * alignment of whole elements.  What a step writes must not overlap itself, the gradients, lr_device or
+ * until the context is destroyed, as the graphs read them.  Sizes: up to 2^24 tensors, fewer than 2^24
+ * workgroups (a tensor's have at least 1024 values each, but for its last), n >= 0 any, any alignment
+ * of whole elements.  What a step writes must not overlap itself, the gradients, lr_device or
  * grad_norm, and a norm that is written none of the list's tensors; that is checked.  A handle belongs
  * to its context and stream; after adn_destroy only adn_adamw_destroy takes it. */
 typedef struct adn_adamw adn_adamw;

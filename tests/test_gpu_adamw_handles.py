@@ -91,3 +91,28 @@ def test_a_captured_list_keeps_its_tables(be):
     finally:
         torch.cuda.synchronize()
         be.set_stream(None)
+
+
+def test_a_list_closed_behind_many_steps(be):
+    """Some milliseconds of steps in flight when the handle goes and others take their tables in its place: all of the steps are its own."""
+    n, steps = 8 << 20, 100
+    g = torch.randn(n, device="cuda")
+    got = []
+    for kept in (True, False):
+        p, step = torch.zeros(n, device="cuda"), torch.zeros(1, device="cuda", dtype=torch.int32)
+        m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+        q, h = torch.ones(n - 5000, device="cuda"), torch.ones(n - 5000, device="cuda")
+        torch.cuda.synchronize()
+        opt = be.adamw([p], [g], m=[m], v=[v], step=step)
+        for _ in range(steps):
+            opt.step_async(lr=1e-3)
+        if not kept:
+            opt.close()
+        r = be.adamw([q], [h], m=[torch.zeros_like(q)], v=[torch.zeros_like(q)], step=torch.zeros_like(step))
+        torch.cuda.synchronize()
+        r.step_async(lr=1e-3)
+        be.synchronize()
+        got.append([p, m, v, step, q, r.m[0], r.v[0]])
+        opt.close(), r.close()
+    assert int(got[1][3]) == steps
+    assert all(torch.equal(a, b) for a, b in zip(*got))
