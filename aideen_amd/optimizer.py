@@ -175,7 +175,7 @@ class AdamW:
             raise _invalid("max_norm and grad_scale must be numbers") from None
         vector = self._backend._vector
         if hasattr(lr, "data_ptr"):
-            s.lr_device = vector(lr, "lr", 1)
+            s.lr_device = vector(lr.reshape(1) if lr.numel() == 1 else lr, "lr", 1)
         else:
             try:
                 s.lr = float(lr)

@@ -113,3 +113,18 @@ def test_a_rate_beyond_fp32_is_refused(be):
     lst.optimizer(be).step_async(lr=3.4e38)
     be.synchronize()
     assert torch.equal(lst.p[0], before)
+
+
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1)])
+def test_a_rate_on_the_device_of_any_shape(be, shape):
+    """A tensor of one value is one whatever its dimensions."""
+    lst, rate = List([300], 32), torch.full(shape, 2e-3, device="cuda")
+    opt, cfg, before = lst.optimizer(be), cfg_of(lst, float(rate)), lst.host()
+    torch.cuda.synchronize()
+    opt.step_async(lr=rate)
+    be.synchronize()
+    lst.check(before, cfg)
+    for bad in (torch.zeros(shape, device="cuda", dtype=torch.float64), torch.zeros(shape), torch.zeros((0,), device="cuda"), torch.zeros((2, 1), device="cuda")):
+        with pytest.raises(AdnError) as ei:
+            opt.step_async(lr=bad)
+        assert ei.value.code == ADN_E_INVALID
